@@ -14,6 +14,7 @@
 #include "gemm.cuh"
 #include "kernels.cuh"
 #include "model.h"
+#include "operators.cuh"
 #include "runtime.h"
 
 struct msst_model {
@@ -155,6 +156,29 @@ int device_of(const void* p) {
   int cur = 0;
   MSST_CUDA(cudaGetDevice(&cur));
   return cur;
+}
+
+// A tensor operand of the conditioned-block operators: `align` > 1 wants its base on
+// 16 bytes and every stride that is walked (extent > 1) a multiple of `align` elements.
+msst::HeadsView heads_view(const msst_heads* t, int batch, int seq, int align, const char* what) {
+  const std::string name(what);
+  MSST_REQUIRE(t && t->heads > 0, name + " needs at least one head");
+  MSST_REQUIRE(t->data || batch == 0 || seq == 0, name + " is null");
+  MSST_REQUIRE(t->batch_stride >= 0 && t->seq_stride >= 0 && t->head_stride >= 0, name + " has a negative stride");
+  msst::HeadsView v{t->data, t->heads, batch > 1 ? t->batch_stride : 0, seq > 1 ? t->seq_stride : 0,
+                    t->heads > 1 ? t->head_stride : 0};
+  if (align > 1) {
+    check_align(t->data, what);
+    MSST_REQUIRE(v.batch_stride % align == 0 && v.seq_stride % align == 0 && v.head_stride % align == 0,
+                 name + " needs strides that are multiples of " + std::to_string(align) + " elements");
+  }
+  return v;
+}
+
+void check_workspace(const void* p, long long have, long long need) {
+  MSST_REQUIRE(need == 0 || (p && have >= need), "the workspace holds " + std::to_string(have) + " bytes, " +
+                                                     std::to_string(need) + " are needed");
+  if (need) check_align(p, "workspace");
 }
 
 }  // namespace
@@ -404,6 +428,137 @@ int msst_sdpa(const void* q, const void* k, const void* v, int B, int H, int Nq,
     };
     const CUtensorMap mq = seq_map(q, Nq), mk = seq_map(k, Nk), mv = seq_map(v, Nk);
     MSST_CUDA(msst::launch_sdpa(mq, mk, mv, a, dtype, sm_count(), as_stream(stream)));
+  });
+}
+
+int msst_qk_norm_rope(const msst_heads* q, const msst_heads* k, int batch, int seq, int head_dim,
+                      const float* q_gamma, const float* k_gamma, float eps, const float* cos_tab,
+                      const float* sin_tab, int num_pos, int rot_dim, const int* positions, int pairing, int dtype,
+                      const msst_heads* q_out, const msst_heads* k_out, void* stream) {
+  return guarded([&] {
+    check_dtype(dtype);
+    MSST_REQUIRE(batch >= 0 && seq >= 0, "bad shape");
+    MSST_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0, "head_dim must be even and <= 256");
+    MSST_REQUIRE(rot_dim >= 0 && rot_dim <= head_dim && rot_dim % 2 == 0, "rot_dim must be even and <= head_dim");
+    MSST_REQUIRE(rot_dim == 0 || (cos_tab && sin_tab && num_pos > 0), "the rotation needs cos and sin tables");
+    MSST_REQUIRE(rot_dim == 0 || positions || seq <= num_pos, "the sequence is longer than the tables");
+    MSST_REQUIRE(pairing == MSST_PAIRS_INTERLEAVED || pairing == MSST_PAIRS_HALVES, "bad pairing");
+    MSST_REQUIRE(eps >= 0.f, "eps must be >= 0");
+    msst::QkNormParams p{};
+    p.x[0] = heads_view(q, batch, seq, 1, "q");
+    p.out[0] = heads_view(q_out, batch, seq, 1, "q_out");
+    MSST_REQUIRE(p.x[0].heads == p.out[0].heads, "q_out must have q's heads");
+    if (k) {
+      p.x[1] = heads_view(k, batch, seq, 1, "k");
+      p.out[1] = heads_view(k_out, batch, seq, 1, "k_out");
+      MSST_REQUIRE(p.x[1].heads == p.out[1].heads, "k_out must have k's heads");
+    }
+    MSST_REQUIRE((long long)batch * seq <= (1LL << 31) / (p.x[0].heads + p.x[1].heads), "too many head vectors");
+    if (batch == 0 || seq == 0) return;
+    p.gamma[0] = q_gamma;
+    p.gamma[1] = k_gamma;
+    p.eps = eps;
+    p.batch = batch;
+    p.seq = seq;
+    p.head_dim = head_dim;
+    p.rot_dim = rot_dim;
+    p.halves = pairing == MSST_PAIRS_HALVES;
+    p.cos_tab = cos_tab;
+    p.sin_tab = sin_tab;
+    p.num_pos = num_pos;
+    p.positions = positions;
+    DeviceScope dev_scope(device_of(q->data));
+    MSST_CUDA(msst::launch_qk_norm(p, dtype, as_stream(stream)));
+  });
+}
+
+int msst_cross_attention_workspace(int batch, int q_len, int k_len, int q_heads, int kv_heads, int head_dim,
+                                   long long* bytes) {
+  return guarded([&] {
+    MSST_REQUIRE(bytes && batch >= 0 && q_len >= 0 && k_len >= 0 && q_heads > 0 && kv_heads > 0 && head_dim > 0,
+                 "bad shape");
+    *bytes = 0;
+  });
+}
+
+int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_heads* v, int batch, int q_len, int k_len,
+                         int head_dim, float scale, const int* key_lens, const unsigned char* key_mask, int dtype,
+                         const msst_heads* out, void* workspace, long long workspace_bytes, void* stream) {
+  return guarded([&] {
+    check_dtype(dtype);
+    MSST_REQUIRE(batch >= 0 && q_len >= 0 && k_len >= 0, "bad shape");
+    MSST_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "head_dim must be a multiple of 8, <= 128");
+    MSST_REQUIRE(std::isfinite(scale), "scale must be finite");
+    msst::CrossAttnParams p{};
+    p.q = heads_view(q, batch, q_len, 8, "q");
+    p.k = heads_view(k, batch, k_len, 8, "k");
+    p.v = heads_view(v, batch, k_len, 8, "v");
+    p.out = heads_view(out, batch, q_len, 8, "out");
+    MSST_REQUIRE(p.out.heads == p.q.heads, "out must have q's heads");
+    MSST_REQUIRE(p.k.heads == p.v.heads && p.q.heads % p.k.heads == 0,
+                 "k and v need the same number of heads, and q a multiple of it");
+    MSST_REQUIRE((long long)batch * q_len <= (1LL << 31) / p.q.heads, "too many query rows");
+    if (batch == 0 || q_len == 0) return;
+    p.batch = batch;
+    p.q_len = q_len;
+    p.k_len = k_len;
+    p.head_dim = head_dim;
+    const float s = scale == 0.f ? 1.0f / std::sqrt((float)head_dim) : scale;
+    p.scale_log2 = s * 1.4426950408889634f;
+    p.key_lens = key_lens;
+    p.key_mask = key_mask;
+    DeviceScope dev_scope(device_of(q->data));
+    check_workspace(workspace, workspace_bytes, 0);
+    MSST_CUDA(msst::launch_cross_attention(p, dtype, as_stream(stream)));
+  });
+}
+
+int msst_adapter_gemm_workspace(long long rows, int K, int N, int adapters, int rank, long long* bytes) {
+  return guarded([&] {
+    MSST_REQUIRE(bytes && rows >= 0 && rows < (1LL << 31) && K > 0 && N > 0 && adapters >= 0 && rank > 0, "bad shape");
+    *bytes = rows * rank * 4;
+  });
+}
+
+int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const void* w, int N, const float* bias,
+                      const void* lora_a, const void* lora_b, const float* scales, int adapters, int rank,
+                      const int* row_adapter, int dtype, void* out, long long ldo, void* workspace,
+                      long long workspace_bytes, void* stream) {
+  return guarded([&] {
+    check_dtype(dtype);
+    MSST_REQUIRE(rows >= 0 && rows < (1LL << 31), "bad rows");
+    MSST_REQUIRE(K > 0 && K % 8 == 0 && N > 0 && N % 8 == 0, "K and N must be positive multiples of 8");
+    MSST_REQUIRE(rank > 0 && rank <= 256 && rank % 8 == 0, "rank must be a multiple of 8, <= 256");
+    MSST_REQUIRE(adapters >= 0, "adapters must be >= 0");
+    MSST_REQUIRE(ldx >= K && ldx % 8 == 0 && ldo >= N && ldo % 8 == 0,
+                 "ldx / ldo must cover a row and be multiples of 8 elements");
+    if (rows == 0) return;
+    MSST_REQUIRE(x && w && out && row_adapter && (adapters == 0 || (lora_a && lora_b)), "null argument");
+    check_align(x, "x");
+    check_align(w, "w");
+    check_align(out, "out");
+    check_align(lora_a, "lora_a");
+    check_align(lora_b, "lora_b");
+    DeviceScope dev_scope(device_of(x));
+    check_workspace(workspace, workspace_bytes, rows * rank * 4);
+    msst::AdapterGemmParams p{};
+    p.x = x;
+    p.w = w;
+    p.bias = bias;
+    p.lora_a = lora_a;
+    p.lora_b = lora_b;
+    p.scales = scales;
+    p.row_adapter = row_adapter;
+    p.out = out;
+    p.u = static_cast<float*>(workspace);
+    p.ldx = ldx;
+    p.ldo = ldo;
+    p.rows = (int)rows;
+    p.K = K;
+    p.N = N;
+    p.adapters = adapters;
+    p.rank = rank;
+    MSST_CUDA(msst::launch_adapter_gemm(p, dtype, as_stream(stream)));
   });
 }
 

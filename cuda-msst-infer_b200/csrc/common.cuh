@@ -34,6 +34,9 @@ enum DeviceError : unsigned {
   kErrTimeoutFfnP = 11,
   kErrTimeoutFfnO = 12,
   kErrTimeoutFfnFlag = 13,
+  // not a wait: data of the call outside its documented range (see the operator)
+  kErrPosition = 14,
+  kErrAdapter = 15,
 };
 
 // One flag per translation unit; each .cu exposes a host accessor (see
@@ -523,6 +526,17 @@ template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   auto h = Half2Of<T>::pack(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
 }
 
 template <typename T>

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import wave
 
 import numpy as np
@@ -23,12 +24,14 @@ F16, BF16, F32 = 0, 1, 2
 EPI = {"store16": 0, "resid32": 1, "store32": 2, "glu32": 3}
 ACT = {"none": 0, "gelu": 1, "tanh": 2, "sigmoid": 3}
 AXIS = {"time": 0, "band": 1}
+PAIRING = {"interleaved": 0, "halves": 1}
 SEPARATE_FIX_TAIL_PADDING = 1
 
 EXPORTS = [
     "msst_last_error", "msst_device_error", "msst_version", "msst_kernel_launches", "msst_kernel_timing",
     "msst_kernel_timing_report", "msst_rmsnorm", "msst_gemm", "msst_gemm_qkv_rope",
-    "msst_attention", "msst_layernorm", "msst_sdpa", "msst_grouped_gemm", "msst_band_gather", "msst_mask_apply", "msst_model_band_tables",
+    "msst_attention", "msst_layernorm", "msst_sdpa", "msst_qk_norm_rope", "msst_cross_attention_workspace",
+    "msst_cross_attention", "msst_adapter_gemm_workspace", "msst_adapter_gemm", "msst_grouped_gemm", "msst_band_gather", "msst_mask_apply", "msst_model_band_tables",
     "msst_roformer_attn_block", "msst_roformer_ffn_block", "msst_model_load", "msst_model_free", "msst_model_get_info", "msst_model_forward",
     "msst_model_masks", "msst_model_transformer", "msst_model_transformer_noalloc", "msst_model_separate", "msst_model_separate_host",
     "msst_model_chunk_plan", "msst_model_forward_chunks", "msst_model_stitch",
@@ -93,6 +96,14 @@ def lib():
     L.msst_attention.argtypes = [vp, c_int, c_int, c_int, c_int, c_int, c_float, vp, c_int, vp, vp]
     L.msst_layernorm.argtypes = [vp, i64, c_int, vp, vp, c_float, c_int, vp, vp]
     L.msst_sdpa.argtypes = [vp, vp, vp, c_int, c_int, c_int, c_int, c_int, c_float, c_int, vp, vp]
+    pi64 = ctypes.POINTER(i64)
+    L.msst_qk_norm_rope.argtypes = [vp, vp, c_int, c_int, c_int, vp, vp, c_float, vp, vp, c_int, c_int, vp, c_int,
+                                    c_int, vp, vp, vp]
+    L.msst_cross_attention_workspace.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int, pi64]
+    L.msst_cross_attention.argtypes = [vp, vp, vp, c_int, c_int, c_int, c_int, c_float, vp, vp, c_int, vp, vp, i64, vp]
+    L.msst_adapter_gemm_workspace.argtypes = [i64, c_int, c_int, c_int, c_int, pi64]
+    L.msst_adapter_gemm.argtypes = [vp, i64, c_int, i64, vp, c_int, vp, vp, vp, vp, c_int, c_int, vp, c_int, vp, i64,
+                                    vp, i64, vp]
     L.msst_grouped_gemm.argtypes = [c_int, ctypes.POINTER(GemmGroupC), vp, i64, i64, vp, i64, i64, c_int, c_int,
                                     c_int, vp, i64, i64, vp]
     L.msst_band_gather.argtypes = [vp, c_int, c_int, ctypes.POINTER(BandTables), c_int, vp, i64, vp]
@@ -117,7 +128,6 @@ def lib():
     L.msst_model_forward_chunks_strided.argtypes = [vp, vp, c_int, i64, c_float, c_int, c_int, c_int, c_int, c_int,
                                                     vp, vp]
     L.msst_model_stitch_range.argtypes = [vp, vp, c_int, c_int, c_int, i64, c_float, i64, i64, vp, vp]
-    pi64 = ctypes.POINTER(i64)
     L.msst_model_chunk_span.argtypes = [vp, i64, c_float, c_int, c_int, pi64, pi64, pi64]
     _lib = L
     return L
@@ -181,6 +191,40 @@ def _dtype_code(dt) -> int:
     if dt == torch.bfloat16:
         return BF16
     raise ValueError(f"16-bit dtype expected, got {dt}")
+
+
+# msst_heads: pointer, heads, strides of batch, sequence and head in elements
+_HEADS = struct.Struct("Pi4xqqq")
+
+
+def _heads(t):
+    """The msst_heads of a [batch, sequence, heads, head_dim] tensor (unit last stride)."""
+    sb, sn, sh, _ = t.stride()
+    return _HEADS.pack(t.data_ptr(), t.shape[2], sb, sn, sh)
+
+
+def _need(ok, msg):
+    if not ok:
+        raise ValueError(msg)
+
+
+def _unit(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _aligned_heads(t):
+    """`t` itself where 16-byte loads can walk it, else a contiguous copy."""
+    sb, sn, sh, s1 = t.stride()
+    b, n, h, _ = t.shape
+    ok = s1 == 1 and not t.data_ptr() & 15 and (b < 2 or not sb & 7) and (n < 2 or not sn & 7) and (h < 2 or not sh & 7)
+    return t if ok else t.clone(memory_format=_torch().contiguous_format)
+
+
+def _f32(t, device, what):
+    if t is None:
+        return None
+    _need(t.dtype == _torch().float32 and t.device == device, f"{what} must be float32 on the operands' device")
+    return t.contiguous()
 
 
 class ops:
@@ -273,6 +317,137 @@ class ops:
         out = torch.empty((B, H, Nq, d), dtype=q.dtype, device=q.device)
         check(lib().msst_sdpa(_ptr(q.contiguous()), _ptr(k.contiguous()), _ptr(v.contiguous()), B, H, Nq, Nk, d,
                               float(scale), _dtype_code(q.dtype), _ptr(out), _stream(None, q.device)))
+        return out
+
+    @staticmethod
+    def qk_norm_rope(q, k=None, q_gamma=None, k_gamma=None, cos=None, sin=None, positions=None, eps=1e-6,
+                     pairing="interleaved", out_q=None, out_k=None):
+        """Norms of queries and keys for each head with the position rotation in the same pass.
+
+        q [B, N, Hq, d] and k [B, N, Hk, d] (or None), 16-bit, any order and strides of the first
+        three dimensions (views into a packed QKV buffer included), d even and <= 256; gammas
+        float32 [d] or None; cos / sin float32 [P, rot / 2] (None: no rotation) rotate the first
+        `rot` columns, pairs (2i, 2i + 1) for "interleaved", (i, i + rot / 2) for "halves";
+        positions int32 [B, N] (None: the index in the sequence).  Returns (q, k) as new
+        contiguous tensors, or out_q / out_k (which may be q / k themselves); k is None without one."""
+        torch = _torch()
+        code = _dtype_code(q.dtype)
+        _need(q.dim() == 4, "q must be [B, N, heads, head_dim]")
+        B, N, _, d = q.shape
+        q = _unit(q)
+        out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is None else out_q
+        _need(out_q.shape == q.shape and out_q.dtype == q.dtype and out_q.device == q.device and
+              (out_q.stride(-1) == 1 or d == 1), "out_q must have q's shape, type and device, and unit last stride")
+        kh = ko = None
+        if k is not None:
+            _need(k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == d and k.dtype == q.dtype and
+                  k.device == q.device, "k must be [B, N, heads, head_dim] with q's B, N, head_dim, type and device")
+            k = _unit(k)
+            out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device) if out_k is None else out_k
+            _need(out_k.shape == k.shape and out_k.dtype == k.dtype and out_k.device == k.device and
+                  (out_k.stride(-1) == 1 or d == 1),
+                  "out_k must have k's shape, type and device, and unit last stride")
+            kh, ko = _heads(k), _heads(out_k)
+        else:
+            out_k = None
+        q_gamma, k_gamma = _f32(q_gamma, q.device, "q_gamma"), _f32(k_gamma, q.device, "k_gamma")
+        _need(all(g is None or g.numel() == d for g in (q_gamma, k_gamma)), "gammas must hold head_dim values")
+        cos, sin = _f32(cos, q.device, "cos"), _f32(sin, q.device, "sin")
+        _need((cos is None) == (sin is None) and (cos is None or (cos.dim() == 2 and cos.shape == sin.shape)),
+              "cos and sin must both be [positions, rot / 2]")
+        rot, num_pos = (2 * cos.shape[1], cos.shape[0]) if cos is not None else (0, 0)
+        if positions is not None:
+            _need(positions.dtype == torch.int32 and positions.device == q.device and
+                  positions.shape == q.shape[:2], "positions must be int32 [B, N] on q's device")
+            positions = positions.contiguous()
+        check(lib().msst_qk_norm_rope(_heads(q), kh, B, N, d, _ptr(q_gamma), _ptr(k_gamma), eps, _ptr(cos), _ptr(sin),
+                                      num_pos, rot, _ptr(positions), PAIRING[pairing], code, _heads(out_q), ko,
+                                      _stream(None, q.device)))
+        return out_q, out_k
+
+    @staticmethod
+    def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=0.0, out=None):
+        """Cross attention to an encoder's states of another length.
+
+        q [B, Nq, Hq, d], k / v [B, Nk, Hk, d], 16-bit, Hq a multiple of Hk, d a multiple of 8 and
+        <= 128, any order of the first three dimensions (a tensor whose strides or base do not
+        allow 16-byte loads is copied first).  key_lens int32 [B] keeps the first keys of each
+        batch entry, key_mask bool [B, Nk] single ones; keys that are not kept may hold anything.
+        A row without a kept key gives zeros.  Returns [B, Nq, Hq, d]."""
+        torch = _torch()
+        code = _dtype_code(q.dtype)
+        _need(q.dim() == 4 and k.dim() == 4, "q, k and v must be [B, N, heads, head_dim]")
+        B, Nq, Hq, d = q.shape
+        Nk, Hk = k.shape[1], k.shape[2]
+        _need(k.shape[0] == B and k.shape[3] == d and v.shape == k.shape,
+              "k and v must be [B, Nk, heads, head_dim] with q's B and head_dim")
+        _need(k.dtype == q.dtype and v.dtype == q.dtype and k.device == q.device and v.device == q.device,
+              "q, k and v must share one 16-bit dtype and one device")
+        q, k, v = _aligned_heads(q), _aligned_heads(k), _aligned_heads(v)
+        if out is None:
+            out = torch.empty((B, Nq, Hq, d), dtype=q.dtype, device=q.device)
+        else:
+            _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.stride(-1) == 1,
+                  "out must have q's shape, type and device, and unit last stride")
+        if key_lens is not None:
+            _need(key_lens.dtype == torch.int32 and key_lens.device == q.device and key_lens.shape == (B,),
+                  "key_lens must be int32 [B] on q's device")
+            key_lens = key_lens.contiguous()
+        if key_mask is not None:
+            _need(key_mask.dtype == torch.bool and key_mask.device == q.device and key_mask.shape == (B, Nk),
+                  "key_mask must be bool [B, Nk] on q's device")
+            key_mask = key_mask.contiguous()
+        need = ctypes.c_longlong()
+        check(lib().msst_cross_attention_workspace(B, Nq, Nk, Hq, Hk, d, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+        check(lib().msst_cross_attention(_heads(q), _heads(k), _heads(v), B, Nq, Nk, d, scale, _ptr(key_lens),
+                                         _ptr(key_mask), code, _heads(out), _ptr(ws), need.value,
+                                         _stream(None, q.device)))
+        return out
+
+    @staticmethod
+    def adapter_gemm(x, w, lora_a, lora_b, row_adapter, scales=None, bias=None, out=None):
+        """A shared projection with the low-rank adapters of many requests beside it:
+        y[t] = W x[t] + bias + scales[a] B_a (A_a x[t]) with a = row_adapter[t], -1 for none.
+
+        x [..., K], W [N, K], lora_a [adapters, rank, K], lora_b [adapters, N, rank], one 16-bit
+        type; row_adapter int32 with one entry per row of x; scales float32 [adapters], bias
+        float32 [N]; K, N and rank multiples of 8, rank <= 256.  Returns [..., N]."""
+        torch = _torch()
+        code = _dtype_code(x.dtype)
+        K, (N, Kw) = x.shape[-1], w.shape
+        count, rank = lora_a.shape[0], lora_a.shape[1]
+        _need(Kw == K and lora_a.shape == (count, rank, K) and lora_b.shape == (count, N, rank),
+              "w must be [N, K], lora_a [adapters, rank, K] and lora_b [adapters, N, rank]")
+        _need(w.dtype == lora_a.dtype == lora_b.dtype == x.dtype and
+              w.device == lora_a.device == lora_b.device == row_adapter.device == x.device,
+              "x, w, lora_a and lora_b must share one 16-bit dtype, and with row_adapter one device")
+        _need(K > 0, "x must have columns")
+        rows = x.numel() // K
+        if x.dim() != 2 or x.stride(1) != 1 or (rows > 1 and (x.stride(0) & 7 or x.stride(0) < K)):
+            x = x.contiguous()
+        if x.data_ptr() & 15:
+            x = x.clone(memory_format=torch.contiguous_format)
+        ldx = x.stride(0) if x.dim() == 2 and rows > 1 else K
+        _need(row_adapter.dtype == torch.int32 and row_adapter.numel() == rows,
+              "row_adapter must be int32 with one entry per row")
+        bias, scales = _f32(bias, x.device, "bias"), _f32(scales, x.device, "scales")
+        _need((bias is None or bias.numel() == N) and (scales is None or scales.numel() == count),
+              "bias must hold N values and scales one per adapter")
+        if out is None:
+            out = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+        else:
+            _need(out.shape == x.shape[:-1] + (N,) and out.dtype == x.dtype and out.device == x.device and
+                  (out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1)),
+                  "out must be [..., N] with x's type and device, and unit last stride")
+        need = ctypes.c_longlong()
+        check(lib().msst_adapter_gemm_workspace(rows, K, N, count, rank, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
+        check(lib().msst_adapter_gemm(_ptr(x), rows, K, ldx, _ptr(w.contiguous()), N,
+                                      _ptr(bias), _ptr(lora_a.contiguous()), _ptr(lora_b.contiguous()), _ptr(scales),
+                                      count, rank, _ptr(row_adapter.contiguous()), code, _ptr(out),
+                                      out.stride(0) if out.dim() == 2 and rows > 1 else N, _ptr(ws), need.value,
+                                      _stream(None, x.device)))
         return out
 
     @staticmethod

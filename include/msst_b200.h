@@ -76,7 +76,8 @@ typedef struct msst_model_info {
 } msst_model_info;
 
 const char* msst_last_error(void);
-/* Code recorded by a kernel whose bounded wait gave up (0 = none); clear != 0 resets it. */
+/* Code recorded by a kernel whose bounded wait gave up, or that met a position or an
+ * adapter index outside the range its operator documents (0 = none); clear != 0 resets it. */
 unsigned msst_device_error(int clear);
 int msst_version(void);
 /* Number of kernels this library has launched (process-wide); reset != 0 returns and zeroes it. */
@@ -150,6 +151,72 @@ int msst_layernorm(const float* x, long long rows, int D, const float* gamma, co
  * src/ops_attention.cu:522-599, including its cross-attention form Nq != Nk). */
 int msst_sdpa(const void* q, const void* k, const void* v, int B, int H, int Nq, int Nk, int head_dim, float scale,
               int dtype, void* out, void* stream);
+
+/* ---- operators of conditioned blocks: a block that attends to an encoder's states
+ * and serves the fine-tunes of many requests from one set of weights.  The
+ * reference has no counterpart of them. */
+
+/* A 16-bit tensor [batch, sequence, heads, head_dim] in any order of its first three
+ * dimensions: element (b, n, h, i) at data + b*batch_stride + n*seq_stride +
+ * h*head_stride + i, strides in elements and >= 0.  Batch, sequence and head_dim
+ * are arguments of the call. */
+typedef struct msst_heads {
+  void* data;
+  int heads;
+  long long batch_stride, seq_stride, head_stride;
+} msst_heads;
+
+#define MSST_PAIRS_INTERLEAVED 0 /* pairs (2i, 2i + 1), as msst_gemm_qkv_rope         */
+#define MSST_PAIRS_HALVES 1      /* pairs (i, i + rot_dim / 2)                        */
+
+/* Norms of queries and keys for each head with the position rotation in the same
+ * pass: every head vector x of q and k becomes
+ *   y = x * rsqrt(mean(x^2) + eps) * gamma
+ * and each pair (a, b) of y's first rot_dim columns (a cos - b sin, b cos + a sin),
+ * cos and sin from row positions[b*seq + n] (row n when positions is NULL) of the
+ * tables [num_pos, rot_dim / 2]; fp32 inside, one rounding at the end.  k may be
+ * NULL; gammas fp32 [head_dim] or NULL (ones).  head_dim is even and <= 256,
+ * rot_dim even and <= head_dim (0: no rotation, tables may be NULL).  q_out / k_out
+ * may be q / k themselves (same strides), and otherwise must not overlap them.
+ * A token whose position lies outside the tables is normed but not rotated, and
+ * msst_device_error reports it. */
+int msst_qk_norm_rope(const msst_heads* q, const msst_heads* k, int batch, int seq, int head_dim,
+                      const float* q_gamma, const float* k_gamma, float eps, const float* cos_tab,
+                      const float* sin_tab, int num_pos, int rot_dim, const int* positions, int pairing, int dtype,
+                      const msst_heads* q_out, const msst_heads* k_out, void* stream);
+
+/* Cross attention to an encoder's states: out = softmax(scale * q k^T) v over the
+ * keys that are kept, q and out [batch, q_len, q.heads, head_dim], k and v [batch,
+ * k_len, k.heads, head_dim], q.heads a multiple of k.heads (query head h reads
+ * key head h / (q.heads / k.heads)).  head_dim is a multiple of 8 and <= 128, scale 0
+ * selects 1/sqrt(head_dim).  Kept are the first key_lens[b] keys (int32, taken into
+ * [0, k_len]; NULL: all k_len) whose key_mask[b*k_len + j] is nonzero (NULL: all).
+ * What the others hold, infinities and NaN included, has no influence.  A row
+ * without a kept key gives zeros.  Data pointers are 16-byte aligned and strides
+ * multiples of 8 elements.  `workspace` holds at least the bytes that
+ * msst_cross_attention_workspace gives for the call's sizes (16-byte aligned; may be
+ * NULL when that is 0); calls that may overlap need workspaces of their own. */
+int msst_cross_attention_workspace(int batch, int q_len, int k_len, int q_heads, int kv_heads, int head_dim,
+                                   long long* bytes);
+int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_heads* v, int batch, int q_len, int k_len,
+                         int head_dim, float scale, const int* key_lens, const unsigned char* key_mask, int dtype,
+                         const msst_heads* out, void* workspace, long long workspace_bytes, void* stream);
+
+/* A shared projection with the low-rank adapters of many requests beside it:
+ *   out16[t] = W x[t] + bias + scales[a] * B_a (A_a x[t]),   a = row_adapter[t],
+ * without the last term where a is -1.  x 16-bit [rows, K] (row stride ldx), W 16-bit
+ * [N, K], bias fp32 [N] or NULL, lora_a 16-bit [adapters, rank, K] (the A_a), lora_b
+ * 16-bit [adapters, N, rank] (the B_a), scales fp32 [adapters] or NULL (ones),
+ * row_adapter int32 [rows], out row stride ldo.  K, N, rank, ldx and ldo are
+ * multiples of 8, rank <= 256; rows of one request need not be adjacent.  An index
+ * outside [-1, adapters) counts as -1, and msst_device_error reports it.  A row's
+ * result does not depend on the other rows of the call beyond the order of sums.
+ * `workspace` as in msst_cross_attention. */
+int msst_adapter_gemm_workspace(long long rows, int K, int N, int adapters, int rank, long long* bytes);
+int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const void* w, int N, const float* bias,
+                      const void* lora_a, const void* lora_b, const float* scales, int adapters, int rank,
+                      const int* row_adapter, int dtype, void* out, long long ldo, void* workspace,
+                      long long workspace_bytes, void* stream);
 
 /* One problem of msst_grouped_gemm: rows [a_row0, a_row0 + m) and columns
  * [a_col0, a_col0 + k) of x times rows [b_row0, b_row0 + n) (same k columns from
