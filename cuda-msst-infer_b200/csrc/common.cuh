@@ -528,6 +528,19 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// the two values packed in a 32-bit word
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
+  const auto h = *reinterpret_cast<const typename Half2Of<T>::type*>(&w);
+  if constexpr (std::is_same<T, __half>::value) {
+    const float2 f = __half22float2(h);
+    a = f.x, b = f.y;
+  } else {
+    const float2 f = __bfloat1622float2(h);
+    a = f.x, b = f.y;
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
 template <>

@@ -168,9 +168,15 @@ def kernel_timing_report() -> dict:
 
 
 # --------------------------------------------------------------------------- torch helpers
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def _ptr(t):
@@ -193,14 +199,22 @@ def _dtype_code(dt) -> int:
     raise ValueError(f"16-bit dtype expected, got {dt}")
 
 
+# ---- plumbing of the conditioned-block operators.  Their smallest calls last a few
+# microseconds on the GPU, so the host side is kept short: addresses and streams travel as
+# plain integers, devices are compared by index, and no attribute is fetched twice.
+
 # msst_heads: pointer, heads, strides of batch, sequence and head in elements
-_HEADS = struct.Struct("Pi4xqqq")
+_HEADS = struct.Struct("Pi4xqqq").pack
 
 
-def _heads(t):
-    """The msst_heads of a [batch, sequence, heads, head_dim] tensor (unit last stride)."""
-    sb, sn, sh, _ = t.stride()
-    return _HEADS.pack(t.data_ptr(), t.shape[2], sb, sn, sh)
+def _heads(t, heads, strides):
+    """The msst_heads of a [batch, sequence, heads, head_dim] tensor."""
+    return _HEADS(t.data_ptr(), heads, strides[0], strides[1], strides[2])
+
+
+def _current_stream(device: int) -> int:
+    """The current stream's handle on GPU `device`."""
+    return _torch()._C._cuda_getCurrentRawStream(device)
 
 
 def _need(ok, msg):
@@ -208,23 +222,26 @@ def _need(ok, msg):
         raise ValueError(msg)
 
 
-def _unit(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+def _aligned_heads(t, shape):
+    """(tensor, strides): `t` itself where 16-byte loads can walk it, else a contiguous copy."""
+    st = t.stride()
+    if (st[3] == 1 and not t.data_ptr() & 15 and (not st[0] & 7 or shape[0] < 2) and (not st[1] & 7 or shape[1] < 2)
+            and (not st[2] & 7 or shape[2] < 2)):
+        return t, st
+    t = t.clone(memory_format=_torch().contiguous_format)
+    return t, t.stride()
 
 
-def _aligned_heads(t):
-    """`t` itself where 16-byte loads can walk it, else a contiguous copy."""
-    sb, sn, sh, s1 = t.stride()
-    b, n, h, _ = t.shape
-    ok = s1 == 1 and not t.data_ptr() & 15 and (b < 2 or not sb & 7) and (n < 2 or not sn & 7) and (h < 2 or not sh & 7)
-    return t if ok else t.clone(memory_format=_torch().contiguous_format)
-
-
-def _f32(t, device, what):
+def _f32_ptr(t, n, device, keep, what):
+    """Address of an optional float32 tensor of n values (a contiguous copy is kept alive in `keep`)."""
     if t is None:
         return None
-    _need(t.dtype == _torch().float32 and t.device == device, f"{what} must be float32 on the operands' device")
-    return t.contiguous()
+    _need(t.dtype is _torch().float32 and t.get_device() == device and t.numel() == n,
+          f"{what} must be float32 on the operands' device, {n} values")
+    if not t.is_contiguous():
+        t = t.contiguous()
+        keep.append(t)
+    return t.data_ptr()
 
 
 class ops:
@@ -331,38 +348,49 @@ class ops:
         positions int32 [B, N] (None: the index in the sequence).  Returns (q, k) as new
         contiguous tensors, or out_q / out_k (which may be q / k themselves); k is None without one."""
         torch = _torch()
-        code = _dtype_code(q.dtype)
-        _need(q.dim() == 4, "q must be [B, N, heads, head_dim]")
-        B, N, _, d = q.shape
-        q = _unit(q)
-        out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is None else out_q
-        _need(out_q.shape == q.shape and out_q.dtype == q.dtype and out_q.device == q.device and
-              (out_q.stride(-1) == 1 or d == 1), "out_q must have q's shape, type and device, and unit last stride")
-        kh = ko = None
+        dt, dev, shape, keep = q.dtype, q.get_device(), q.shape, []
+        code = _dtype_code(dt)
+        _need(len(shape) == 4, "q must be [B, N, heads, head_dim]")
+        B, N, Hq, d = shape
+
+        def side(x, xshape, out, what):
+            st = x.stride()
+            if st[3] != 1 and d > 1:
+                x = x.contiguous()
+                keep.append(x)
+                st = x.stride()
+            if out is None:
+                out = torch.empty_like(x, memory_format=torch.contiguous_format)
+                ost = out.stride()
+            else:
+                ost = out.stride()
+                _need(out.shape == xshape and out.dtype is dt and out.get_device() == dev and (ost[3] == 1 or d == 1),
+                      f"out_{what} must have {what}'s shape, type and device, and unit last stride")
+            return out, _heads(x, xshape[2], st), _heads(out, xshape[2], ost)
+
+        out_q, hq, ho = side(q, shape, out_q, "q")
+        hk = hko = None
         if k is not None:
-            _need(k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == d and k.dtype == q.dtype and
-                  k.device == q.device, "k must be [B, N, heads, head_dim] with q's B, N, head_dim, type and device")
-            k = _unit(k)
-            out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device) if out_k is None else out_k
-            _need(out_k.shape == k.shape and out_k.dtype == k.dtype and out_k.device == k.device and
-                  (out_k.stride(-1) == 1 or d == 1),
-                  "out_k must have k's shape, type and device, and unit last stride")
-            kh, ko = _heads(k), _heads(out_k)
+            ks = k.shape
+            _need(len(ks) == 4 and ks[0] == B and ks[1] == N and ks[3] == d and k.dtype is dt and k.get_device() == dev,
+                  "k must be [B, N, heads, head_dim] with q's B, N, head_dim, type and device")
+            out_k, hk, hko = side(k, ks, out_k, "k")
         else:
             out_k = None
-        q_gamma, k_gamma = _f32(q_gamma, q.device, "q_gamma"), _f32(k_gamma, q.device, "k_gamma")
-        _need(all(g is None or g.numel() == d for g in (q_gamma, k_gamma)), "gammas must hold head_dim values")
-        cos, sin = _f32(cos, q.device, "cos"), _f32(sin, q.device, "sin")
-        _need((cos is None) == (sin is None) and (cos is None or (cos.dim() == 2 and cos.shape == sin.shape)),
+        num_pos, half = (0, 0) if cos is None else cos.shape
+        _need((cos is None) == (sin is None) and (sin is None or sin.shape == cos.shape),
               "cos and sin must both be [positions, rot / 2]")
-        rot, num_pos = (2 * cos.shape[1], cos.shape[0]) if cos is not None else (0, 0)
+        pos = None
         if positions is not None:
-            _need(positions.dtype == torch.int32 and positions.device == q.device and
-                  positions.shape == q.shape[:2], "positions must be int32 [B, N] on q's device")
+            ps = positions.shape
+            _need(positions.dtype is torch.int32 and positions.get_device() == dev and len(ps) == 2 and ps[0] == B and
+                  ps[1] == N, "positions must be int32 [B, N] on q's device")
             positions = positions.contiguous()
-        check(lib().msst_qk_norm_rope(_heads(q), kh, B, N, d, _ptr(q_gamma), _ptr(k_gamma), eps, _ptr(cos), _ptr(sin),
-                                      num_pos, rot, _ptr(positions), PAIRING[pairing], code, _heads(out_q), ko,
-                                      _stream(None, q.device)))
+            pos = positions.data_ptr()
+        check(lib().msst_qk_norm_rope(
+            hq, hk, B, N, d, _f32_ptr(q_gamma, d, dev, keep, "q_gamma"), _f32_ptr(k_gamma, d, dev, keep, "k_gamma"),
+            eps, _f32_ptr(cos, num_pos * half, dev, keep, "cos"), _f32_ptr(sin, num_pos * half, dev, keep, "sin"),
+            num_pos, 2 * half, pos, PAIRING[pairing], code, ho, hko, _current_stream(dev)))
         return out_q, out_k
 
     @staticmethod
@@ -375,34 +403,42 @@ class ops:
         batch entry, key_mask bool [B, Nk] single ones; keys that are not kept may hold anything.
         A row without a kept key gives zeros.  Returns [B, Nq, Hq, d]."""
         torch = _torch()
-        code = _dtype_code(q.dtype)
-        _need(q.dim() == 4 and k.dim() == 4, "q, k and v must be [B, N, heads, head_dim]")
-        B, Nq, Hq, d = q.shape
-        Nk, Hk = k.shape[1], k.shape[2]
-        _need(k.shape[0] == B and k.shape[3] == d and v.shape == k.shape,
+        dt, dev, shape, ks = q.dtype, q.get_device(), q.shape, k.shape
+        code = _dtype_code(dt)
+        _need(len(shape) == 4 and len(ks) == 4, "q, k and v must be [B, N, heads, head_dim]")
+        B, Nq, Hq, d = shape
+        _, Nk, Hk, _ = ks
+        _need(ks[0] == B and ks[3] == d and v.shape == ks,
               "k and v must be [B, Nk, heads, head_dim] with q's B and head_dim")
-        _need(k.dtype == q.dtype and v.dtype == q.dtype and k.device == q.device and v.device == q.device,
+        _need(k.dtype is dt and v.dtype is dt and k.get_device() == dev and v.get_device() == dev,
               "q, k and v must share one 16-bit dtype and one device")
-        q, k, v = _aligned_heads(q), _aligned_heads(k), _aligned_heads(v)
+        (q, sq), (k, sk), (v, sv) = _aligned_heads(q, shape), _aligned_heads(k, ks), _aligned_heads(v, ks)
         if out is None:
-            out = torch.empty((B, Nq, Hq, d), dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            so = out.stride()
         else:
-            _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.stride(-1) == 1,
+            so = out.stride()
+            _need(out.shape == shape and out.dtype is dt and out.get_device() == dev and so[3] == 1,
                   "out must have q's shape, type and device, and unit last stride")
+        lens = mask = ws = None
         if key_lens is not None:
-            _need(key_lens.dtype == torch.int32 and key_lens.device == q.device and key_lens.shape == (B,),
+            _need(key_lens.dtype is torch.int32 and key_lens.get_device() == dev and key_lens.shape == (B,),
                   "key_lens must be int32 [B] on q's device")
             key_lens = key_lens.contiguous()
+            lens = key_lens.data_ptr()
         if key_mask is not None:
-            _need(key_mask.dtype == torch.bool and key_mask.device == q.device and key_mask.shape == (B, Nk),
+            _need(key_mask.dtype is torch.bool and key_mask.get_device() == dev and key_mask.shape == (B, Nk),
                   "key_mask must be bool [B, Nk] on q's device")
             key_mask = key_mask.contiguous()
-        need = ctypes.c_longlong()
-        check(lib().msst_cross_attention_workspace(B, Nq, Nk, Hq, Hk, d, ctypes.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-        check(lib().msst_cross_attention(_heads(q), _heads(k), _heads(v), B, Nq, Nk, d, scale, _ptr(key_lens),
-                                         _ptr(key_mask), code, _heads(out), _ptr(ws), need.value,
-                                         _stream(None, q.device)))
+            mask = key_mask.data_ptr()
+        L, need = lib(), ctypes.c_longlong()
+        check(L.msst_cross_attention_workspace(B, Nq, Nk, Hq, Hk, d, ctypes.byref(need)))
+        need = need.value
+        if need:
+            space = torch.empty(need, dtype=torch.uint8, device=q.device)
+            ws = space.data_ptr()
+        check(L.msst_cross_attention(_heads(q, Hq, sq), _heads(k, Hk, sk), _heads(v, Hk, sv), B, Nq, Nk, d, scale, lens,
+                                     mask, code, _heads(out, Hq, so), ws, need, _current_stream(dev)))
         return out
 
     @staticmethod
@@ -414,40 +450,49 @@ class ops:
         type; row_adapter int32 with one entry per row of x; scales float32 [adapters], bias
         float32 [N]; K, N and rank multiples of 8, rank <= 256.  Returns [..., N]."""
         torch = _torch()
-        code = _dtype_code(x.dtype)
-        K, (N, Kw) = x.shape[-1], w.shape
-        count, rank = lora_a.shape[0], lora_a.shape[1]
-        _need(Kw == K and lora_a.shape == (count, rank, K) and lora_b.shape == (count, N, rank),
+        dt, dev, shape, keep = x.dtype, x.get_device(), x.shape, []
+        code = _dtype_code(dt)
+        (N, K), (count, rank, Ka), lbs = w.shape, lora_a.shape, lora_b.shape
+        _need(shape[-1] == K and Ka == K and lbs == (count, N, rank) and K > 0,
               "w must be [N, K], lora_a [adapters, rank, K] and lora_b [adapters, N, rank]")
-        _need(w.dtype == lora_a.dtype == lora_b.dtype == x.dtype and
-              w.device == lora_a.device == lora_b.device == row_adapter.device == x.device,
+        _need(w.dtype is dt and lora_a.dtype is dt and lora_b.dtype is dt and w.get_device() == dev and
+              lora_a.get_device() == dev and lora_b.get_device() == dev and row_adapter.get_device() == dev,
               "x, w, lora_a and lora_b must share one 16-bit dtype, and with row_adapter one device")
-        _need(K > 0, "x must have columns")
         rows = x.numel() // K
-        if x.dim() != 2 or x.stride(1) != 1 or (rows > 1 and (x.stride(0) & 7 or x.stride(0) < K)):
+        ldx = K
+        if len(shape) == 2 and rows > 1 and x.stride(1) == 1 and x.stride(0) >= K and not x.stride(0) & 7:
+            ldx = x.stride(0)
+        elif not x.is_contiguous():
             x = x.contiguous()
         if x.data_ptr() & 15:
-            x = x.clone(memory_format=torch.contiguous_format)
-        ldx = x.stride(0) if x.dim() == 2 and rows > 1 else K
-        _need(row_adapter.dtype == torch.int32 and row_adapter.numel() == rows,
+            x, ldx = x.clone(memory_format=torch.contiguous_format), K
+        _need(row_adapter.dtype is torch.int32 and row_adapter.numel() == rows,
               "row_adapter must be int32 with one entry per row")
-        bias, scales = _f32(bias, x.device, "bias"), _f32(scales, x.device, "scales")
-        _need((bias is None or bias.numel() == N) and (scales is None or scales.numel() == count),
-              "bias must hold N values and scales one per adapter")
+        ldo = N
         if out is None:
-            out = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+            out = torch.empty(shape[:-1] + (N,), dtype=dt, device=x.device)
         else:
-            _need(out.shape == x.shape[:-1] + (N,) and out.dtype == x.dtype and out.device == x.device and
+            _need(out.shape == shape[:-1] + (N,) and out.dtype is dt and out.get_device() == dev and
                   (out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1)),
                   "out must be [..., N] with x's type and device, and unit last stride")
-        need = ctypes.c_longlong()
-        check(lib().msst_adapter_gemm_workspace(rows, K, N, count, rank, ctypes.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
-        check(lib().msst_adapter_gemm(_ptr(x), rows, K, ldx, _ptr(w.contiguous()), N,
-                                      _ptr(bias), _ptr(lora_a.contiguous()), _ptr(lora_b.contiguous()), _ptr(scales),
-                                      count, rank, _ptr(row_adapter.contiguous()), code, _ptr(out),
-                                      out.stride(0) if out.dim() == 2 and rows > 1 else N, _ptr(ws), need.value,
-                                      _stream(None, x.device)))
+            if out.dim() == 2 and rows > 1:
+                ldo = out.stride(0)
+
+        def ptr(t):
+            if not t.is_contiguous():
+                t = t.contiguous()
+                keep.append(t)
+            return t.data_ptr()
+
+        L, need, ws = lib(), ctypes.c_longlong(), None
+        check(L.msst_adapter_gemm_workspace(rows, K, N, count, rank, ctypes.byref(need)))
+        need = need.value
+        if need:
+            space = torch.empty(need, dtype=torch.uint8, device=x.device)
+            ws = space.data_ptr()
+        check(L.msst_adapter_gemm(x.data_ptr(), rows, K, ldx, ptr(w), N, _f32_ptr(bias, N, dev, keep, "bias"),
+                                  ptr(lora_a), ptr(lora_b), _f32_ptr(scales, count, dev, keep, "scales"), count, rank,
+                                  ptr(row_adapter), code, out.data_ptr(), ldo, ws, need, _current_stream(dev)))
         return out
 
     @staticmethod

@@ -131,6 +131,8 @@ def test_qk_norm_rope(cuda, case, pairing, prec):
     if layout == "packed":
         buf = allh.transpose(0, 1).clone().transpose(0, 1)
         q2, k2 = buf[:, :, :Hq], buf[:, :, Hq:Hq + Hk]
+    elif layout == "odd":
+        q2, k2 = make(Hq).copy_(q), make(Hk).copy_(k)
     iq, ik = ops.qk_norm_rope(q2, k2, qg, kg, cos, sin, positions=pos, eps=1e-5, pairing=pairing, out_q=q2, out_k=k2)
     assert iq is q2 and ik is k2 and torch.equal(q2, yq) and torch.equal(k2, yk)
     if layout == "packed":
