@@ -477,7 +477,7 @@ int msst_cross_attention_workspace(int batch, int q_len, int k_len, int q_heads,
   return guarded([&] {
     MSST_REQUIRE(bytes && batch >= 0 && q_len >= 0 && k_len >= 0 && q_heads > 0 && kv_heads > 0 && head_dim > 0,
                  "bad shape");
-    *bytes = 0;
+    *bytes = msst::cross_attention_workspace(batch, q_len, k_len, q_heads, kv_heads, head_dim, sm_count());
   });
 }
 
@@ -499,6 +499,9 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
                  "k and v need the same number of heads, and q a multiple of it");
     MSST_REQUIRE((long long)batch * q_len <= (1LL << 31) / p.q.heads, "too many query rows");
     if (batch == 0 || q_len == 0) return;
+    MSST_REQUIRE((q_len == 1 || p.q.seq_stride > 0) && (p.q.heads == 1 || p.q.head_stride > 0) &&
+                     (k_len <= 1 || (p.k.seq_stride > 0 && p.v.seq_stride > 0)),
+                 "q's sequence and head strides and the sequence strides of k and v must not be 0");
     p.batch = batch;
     p.q_len = q_len;
     p.k_len = k_len;
@@ -508,8 +511,10 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
     p.key_lens = key_lens;
     p.key_mask = key_mask;
     DeviceScope dev_scope(device_of(q->data));
-    check_workspace(workspace, workspace_bytes, 0);
-    MSST_CUDA(msst::launch_cross_attention(p, dtype, as_stream(stream)));
+    check_workspace(workspace, workspace_bytes,
+                    msst::cross_attention_workspace(batch, q_len, k_len, p.q.heads, p.k.heads, head_dim, sm_count()));
+    p.ws = static_cast<float*>(workspace);
+    MSST_CUDA(msst::launch_cross_attention(p, dtype, sm_count(), as_stream(stream)));
   });
 }
 

@@ -1,4 +1,37 @@
-// cross_attn.cu — cross attention to an encoder's states of another length.
+// cross_attn.cu — cross attention to an encoder's states of another length:
+// out = softmax(scale q k^T) v over the kept keys, grouped heads, head_dim <= 128.
+//
+// The query rows of one key head (its group of G query heads times q_len tokens) are
+// packed into 128-row tiles: row r of a tile is token n0 + r / gt, head g0 + r % gt
+// with gt = min(G, 128), so one K/V tile serves all heads of the group.  A CTA works
+// on a PAIR of row tiles that share every K/V tile; a lone last tile (or the only
+// one, when there are few rows) runs as a pair of itself with the K/V tiles dealt to
+// its two halves in turn, which are merged at the end.
+//
+// Work is cut into units (one K/V tile for a pair, two for a lone tile) and every CTA
+// takes an equal contiguous run of all units, over items of any length; the two
+// items a run may share with its neighbours leave partial results (O, running
+// reference and sum, fp32) in the workspace, which cross_combine_kernel joins in CTA
+// order.  So few rows against a long encoder and ragged batches fill the GPU alike.
+//
+// CTA = 384 threads:
+//   warp 0      TMA producer: Q tiles, K and V tiles through one ring of slots
+//   warp 1      MMA issuer: S_w = Q_w K^T (SS) and O_w += P_w V (P from TMEM), per
+//               tile PV_w(j - 1) then S_w(j); owns TMEM
+//   warp 2      once a V tile has landed: rows of keys that are not kept are zeroed
+//               (0 * NaN would reach the sum otherwise), the tile's mask words published
+//   warps 4-11  softmax, tile (warp - 4) / 4, one query row per thread
+// TMEM: S_0 [0,128) S_1 [128,256) (P_w over S_w's first 64 columns), O_0 at 256, O_1 at
+// 256 + DP.  S_w(j) overwrites P_w(j-1) only after PV_w(j-1), issued before it by the
+// same thread, has read it.
+//
+// Softmax: the reference a row is exponentiated against starts at the maximum of its
+// first 32 kept scores and moves lazily: a tile is taken in one pass without a
+// maximum, and only a row sum above kSumLimit (or not finite) sends the warp through
+// the exact two passes, which move the reference and rescale O.  Statistics are fp32;
+// P is rounded to the operands' 16 bits for the tensor cores.
+#include <algorithm>
+
 #include "common.cuh"
 #include "operators.cuh"
 #include "runtime.h"
@@ -7,79 +40,829 @@ namespace msst {
 
 namespace {
 
-// One warp per query row and head: 32 keys at a time, one score per lane, running
-// maximum and sum; each lane owns head_dim / 32 columns of the output.
-template <typename T>
-__global__ void __launch_bounds__(128) cross_attention_simple_kernel(const __grid_constant__ CrossAttnParams p) {
-  __shared__ float sq[4][128];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long rows = (long long)p.batch * p.q_len * p.q.heads;
-  const long long r = (long long)blockIdx.x * 4 + warp;
-  if (r >= rows) return;
-  const int h = (int)(r % p.q.heads);
-  const long long bn = r / p.q.heads;
-  const int b = (int)(bn / p.q_len), n = (int)(bn - (long long)b * p.q_len);
-  const int hk = h / (p.q.heads / p.k.heads);
-  const int d = p.head_dim;
-  const T* q = static_cast<const T*>(p.q.data) + b * p.q.batch_stride + n * p.q.seq_stride + h * p.q.head_stride;
-  const T* k = static_cast<const T*>(p.k.data) + b * p.k.batch_stride + hk * p.k.head_stride;
-  const T* v = static_cast<const T*>(p.v.data) + b * p.v.batch_stride + hk * p.v.head_stride;
-  T* out = static_cast<T*>(p.out.data) + b * p.out.batch_stride + n * p.out.seq_stride + h * p.out.head_stride;
-  for (int i = lane; i < d; i += 32) sq[warp][i] = to_f32(q[i]);
-  __syncwarp();
-  int len = p.k_len;
-  if (p.key_lens) len = min(max(__ldg(p.key_lens + b), 0), len);
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = 0; j0 < len; j0 += 32) {
-    const int j = j0 + lane;
-    const bool keep = j < len && (!p.key_mask || p.key_mask[(size_t)b * p.k_len + j]);
-    float s = -INFINITY;
-    if (keep) {
-      s = 0.f;
-      for (int i = 0; i < d; ++i) s += sq[warp][i] * to_f32(k[(long long)j * p.k.seq_stride + i]);
-      s *= p.scale_log2;
+constexpr int kThreads = 384;
+constexpr int kSoftmaxWarp0 = 4;
+constexpr float kSumLimit = 4096.0f;
+constexpr uint32_t kHalfBytes = 128 * 64 * 2;  // 128 rows x 64 columns
+
+template <int DP>
+struct Cfg {
+  static constexpr int kHalves = DP / 64;
+  static constexpr uint32_t kTile = kHalves * kHalfBytes;      // one Q, K or V tile
+  static constexpr int kSlots = DP == 128 ? 5 : 8;             // ring of K and V tiles
+  static constexpr size_t kSmem = 2 * kTile + kSlots * kTile + 2560;
+  static constexpr uint32_t kColO = 256;
+};
+
+// Geometry of a launch.
+struct Geom {
+  int kv_heads, group;       // G query heads a key head
+  int gt, nt;                // heads and tokens of a tile
+  int g_tiles, n_tiles;      // tiles along heads and tokens
+  int full, lone;            // per key head: pairs, and 1 if a lone tile is left
+  int q_batched;             // 0: shared by the batch through stride 0
+  int k_batched, k_headed;
+  int v_batched, v_headed;
+  int ksteps;                // ceil(head_dim / 16)
+  int contribs;              // CTAs of the attention launch
+};
+
+__device__ __forceinline__ int key_count(const CrossAttnParams& p, int b) {
+  return p.key_lens ? min(max(__ldg(p.key_lens + b), 0), p.k_len) : p.k_len;
+}
+// K/V tiles of a batch entry (one masked tile where no key is left, so that every item
+// has a unit that writes its rows)
+__device__ __forceinline__ int key_tiles(const CrossAttnParams& p, int b) {
+  return max(1, (key_count(p, b) + 127) >> 7);
+}
+__device__ __forceinline__ long long batch_units(const Geom& g, int tiles) {
+  return (long long)g.kv_heads * ((long long)g.full * tiles + g.lone * ((tiles + 1) >> 1));
+}
+
+// A position in the list of units: batch entry, key head, item of the key head, unit.
+struct Spot {
+  int b, hk, t, j;
+};
+// Spot of unit u < batch_units(tiles of b), counted from batch entry b's first.
+__device__ __forceinline__ Spot spot_in_batch(const Geom& g, int b, int tiles, long long u) {
+  const long long per_head = batch_units(g, tiles) / g.kv_heads;
+  Spot s;
+  s.b = b;
+  s.hk = (int)(u / per_head);
+  const long long r = u - s.hk * per_head;
+  if (r < (long long)g.full * tiles) {
+    s.t = (int)(r / tiles);
+    s.j = (int)(r - (long long)s.t * tiles);
+  } else {
+    s.t = g.full;
+    s.j = (int)(r - (long long)g.full * tiles);
+  }
+  return s;
+}
+
+// One warp: total units of the launch, and for `want` < 2 unit indices their spots.
+// Ragged batches are summed 32 entries at a time.
+__device__ long long total_units(const CrossAttnParams& p, const Geom& g, int lane) {
+  if (!p.key_lens) return p.batch * batch_units(g, key_tiles(p, 0));
+  long long sum = 0;
+  for (int b = lane; b < p.batch; b += 32) sum += batch_units(g, key_tiles(p, b));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+// One warp: the spot of unit u and the units before its batch entry.
+__device__ Spot find_spot(const CrossAttnParams& p, const Geom& g, long long u, int lane) {
+  if (!p.key_lens) {
+    const int tiles = key_tiles(p, 0);
+    const long long per = batch_units(g, tiles);
+    const int b = (int)(u / per);
+    return spot_in_batch(g, b, tiles, u - b * per);
+  }
+  long long before = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const int tiles = b < p.batch ? key_tiles(p, b) : 0;
+    const long long mine = b < p.batch ? batch_units(g, tiles) : 0;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
     }
-    float mx = s;
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const long long start = before + __shfl_sync(0xffffffffu, incl - mine, src);
+      return spot_in_batch(g, b0 + src, __shfl_sync(0xffffffffu, tiles, src), u - start);
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return Spot{p.batch - 1, 0, 0, 0};  // u past the end: not reached
+}
+
+// Walks the segments (one item each) of a CTA's run.
+struct Walk {
+  Spot s;
+  long long left;
+  int seg;
+  // of the current segment: K/V tiles of the batch entry, its key count, units [j0, j1)
+  int tiles, keys, j0, j1, units;
+  bool lone;
+  __device__ Walk(const Spot& s0, long long n) : s(s0), left(n), seg(-1) {}
+  __device__ __forceinline__ bool next(const CrossAttnParams& p, const Geom& g) {
+    if (seg >= 0) {
+      s.j = 0;
+      if (++s.t == g.full + g.lone) {
+        s.t = 0;
+        if (++s.hk == g.kv_heads) {
+          s.hk = 0;
+          ++s.b;
+        }
+      }
+    }
+    if (left <= 0) return false;
+    ++seg;
+    keys = key_count(p, s.b);
+    tiles = max(1, (keys + 127) >> 7);
+    lone = s.t == g.full;
+    units = lone ? (tiles + 1) >> 1 : tiles;
+    j0 = s.j;
+    j1 = (int)min((long long)units, j0 + left);
+    left -= j1 - j0;
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == units; }
+  // K/V tile of query tile w in unit j, and whether it has one
+  __device__ __forceinline__ int kv_tile(int w, int j) const { return lone ? 2 * j + w : j; }
+  __device__ __forceinline__ bool uses(int w, int j) const { return kv_tile(w, j) < tiles; }
+  // ring slots that unit j takes
+  __device__ __forceinline__ int slots(int j) const { return lone ? (uses(1, j) ? 4 : 2) : 2; }
+};
+
+// First token and head of row tile w of the current segment.
+__device__ __forceinline__ void tile_origin(const Walk& k, const Geom& g, int w, int& n0, int& g0) {
+  const int tile = k.lone ? 2 * g.full : 2 * k.s.t + w;
+  const int gi = tile / g.n_tiles;
+  n0 = (tile - gi * g.n_tiles) * g.nt;
+  g0 = gi * g.gt;
+}
+
+// Kept keys among the 32 of chunk ch of a tile that has khi valid keys.
+__device__ __forceinline__ uint32_t len_word(int khi, int ch) {
+  const int n = khi - 32 * ch;
+  return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
+}
+
+// Maximum of s c over the kept scores of a chunk.
+__device__ __forceinline__ float chunk_max(const uint32_t (&r)[32], uint32_t word, float c) {
+  float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    if (mx == -INFINITY) continue;
-    const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
-    const float e = keep ? exp2f(s - mn) : 0.f;
-    float sum = e;
+  for (int i = 0; i < 32; i += 2) {
+    if (word >> i & 1) m0 = fmaxf(m0, __uint_as_float(r[i]) * c);
+    if (word >> (i + 1) & 1) m1 = fmaxf(m1, __uint_as_float(r[i + 1]) * c);
+  }
+  return fmaxf(m0, m1);
+}
+
+// P of one 32-column chunk against the reference: 2^(s c - ref), packed into pk.
+template <typename T>
+__device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], uint32_t word, float2 c2, float2 nref2, float2& sum2,
+                                          uint32_t* pk) {
+  if (word == 0xffffffffu) {
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    l = l * alpha + sum;
-    m = mn;
+    for (int i = 0; i < 16; ++i) {
+      const float2 a = __ffma2_rn(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), c2, nref2);
+      const float2 e = make_float2(fast_exp2(a.x), fast_exp2(a.y));
+      sum2 = __fadd2_rn(sum2, e);
+      pk[i] = pack2<T>(e.x, e.y);
+    }
+  } else if (word == 0u) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] *= alpha;
-    for (int t = 0; t < 32; ++t) {
-      const float pt = __shfl_sync(0xffffffffu, e, t);
-      if (!__shfl_sync(0xffffffffu, (int)keep, t)) continue;
+    for (int i = 0; i < 16; ++i) pk[i] = 0u;
+  } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (lane + 32 * c < d) o[c] += pt * to_f32(v[(long long)(j0 + t) * p.v.seq_stride + lane + 32 * c]);
+    for (int i = 0; i < 16; ++i) {
+      const float2 a = __ffma2_rn(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), c2, nref2);
+      const float e0 = word >> (2 * i) & 1 ? fast_exp2(a.x) : 0.f;
+      const float e1 = word >> (2 * i + 1) & 1 ? fast_exp2(a.y) : 0.f;
+      sum2 = __fadd2_rn(sum2, make_float2(e0, e1));
+      pk[i] = pack2<T>(e0, e1);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+}
+
+// P and the row sum of a whole 128-column row; the next chunk's load is in flight
+// while one is processed.
+template <typename T>
+__device__ __forceinline__ float row_exp(uint32_t sAddr, const uint32_t (&words)[4], float c, float ref,
+                                         uint32_t (&pk)[64]) {
+  const float2 c2 = make_float2(c, c), nref2 = make_float2(-ref, -ref);
+  float2 sum2 = make_float2(0.f, 0.f);
+  uint32_t ra[32], rb[32];
+  tmem_ld32(sAddr, ra);
+  tmem_ld_wait(ra);
+  tmem_ld32(sAddr + 32, rb);
+  chunk_exp<T>(ra, words[0], c2, nref2, sum2, pk);
+  tmem_ld_wait(rb);
+  tmem_ld32(sAddr + 64, ra);
+  chunk_exp<T>(rb, words[1], c2, nref2, sum2, pk + 16);
+  tmem_ld_wait(ra);
+  tmem_ld32(sAddr + 96, rb);
+  chunk_exp<T>(ra, words[2], c2, nref2, sum2, pk + 32);
+  tmem_ld_wait(rb);
+  chunk_exp<T>(rb, words[3], c2, nref2, sum2, pk + 48);
+  return sum2.x + sum2.y;
+}
+
+template <typename T, int DP, bool kMask>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                           const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CrossAttnParams p,
+                           const __grid_constant__ Geom g) {
+  using C = Cfg<DP>;
+  constexpr uint32_t kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  extern __shared__ __align__(1024) uint8_t smem[];  // the swizzled tiles start on 1024 bytes
+  uint8_t* sQ = smem;
+  uint8_t* sKV = sQ + 2 * C::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::kSlots * C::kTile);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* s_full = bars + 2;   // [2]
+  uint64_t* p_full = bars + 4;   // [2]
+  uint64_t* o_done = bars + 6;   // [2]
+  uint64_t* meet = bars + 8;     // [4 lane quarters]: the two halves of a lone tile
+  uint64_t* full = bars + 12;    // [slots] landed
+  uint64_t* ready = full + C::kSlots;   // [slots] fit for the MMA
+  uint64_t* empty = ready + C::kSlots;  // [slots]
+  Spot* s_spot = reinterpret_cast<Spot*>(empty + C::kSlots);
+  long long* s_count = reinterpret_cast<long long*>(s_spot + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_count + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* s_words = tmem_slot + 4;                                 // [slots][4] kept keys of a V slot
+  float* s_ml = reinterpret_cast<float*>(s_words + C::kSlots * 4);   // [2 halves][ref, l][128]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], 128);
+      mbar_init(&o_done[w], 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&ready[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&qmap);
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+  }
+  if (warp == 2) {
+    const long long U = total_units(p, g, lane);
+    const long long u0 = U * blockIdx.x / gridDim.x, u1 = U * (blockIdx.x + 1) / gridDim.x;
+    const Spot s = find_spot(p, g, u0, lane);
+    if (lane == 0) {
+      *s_spot = s;
+      *s_count = u1 - u0;
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Walk k(*s_spot, *s_count);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      uint32_t slot = 0, phase = 0;  // ring position
+      bool ok = true;
+      while (ok && k.next(p, g)) {
+        if (!mbar_wait<false>(q_empty, (k.seg & 1) ^ 1, kErrTimeoutAttnQ, abort_flag)) break;
+        const int nq = k.lone ? 1 : 2;
+        mbar_arrive_expect_tx(q_full, nq * C::kHalves * (uint32_t)(g.gt * g.nt) * 128u);
+        for (int w = 0; w < nq; ++w) {
+          int n0, g0;
+          tile_origin(k, g, w, n0, g0);
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_5d(sQ + w * C::kTile + h * kHalfBytes, &qmap, q_full, h * 64, g0, n0, k.s.hk, k.s.b * g.q_batched);
+        }
+        const int kh = k.s.hk * g.k_headed, kb = k.s.b * g.k_batched;
+        const int vh = k.s.hk * g.v_headed, vb = k.s.b * g.v_batched;
+        for (int j = k.j0; ok && j < k.j1; ++j) {
+          const int n = k.slots(j);
+          for (int i = 0; i < n; ++i) {
+            if (!mbar_wait<false>(&empty[slot], phase ^ 1, kErrTimeoutAttnKV, abort_flag)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&full[slot], C::kTile);
+            const int row = k.kv_tile(i >> 1, j) * 128;
+            for (int h = 0; h < C::kHalves; ++h) {
+              uint8_t* dst = sKV + slot * C::kTile + h * kHalfBytes;
+              if (i & 1)
+                tma_load_4d(dst, &vmap, &full[slot], h * 64, row, vh, vb);
+              else
+                tma_load_4d(dst, &kmap, &full[slot], h * 64, row, kh, kb);
+            }
+            if (++slot == C::kSlots) slot = 0, phase ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t idesc_s = umma_idesc_f16(kIsBf16, 128, 0);
+      const uint32_t idesc_o = umma_idesc_f16(kIsBf16, (uint32_t)g.ksteps * 16, 1);
+      const uint64_t dq0 = sw128_desc(smem_u32(sQ), 16, 1024);
+      const uint64_t dk0 = sw128_desc(smem_u32(sKV), 16, 1024);
+      const uint64_t dv0 = sw128_desc(smem_u32(sKV), kHalfBytes, 1024);
+      uint32_t slot = 0, phase = 0;
+      uint32_t pcnt[2] = {0, 0};
+      bool ok = true;
+      auto issue_s = [&](int w, int tile, uint32_t st) {
+        const uint64_t dq = dq0 + (uint64_t)((tile * C::kTile) >> 4);
+        const uint64_t dk = dk0 + (uint64_t)((st * C::kTile) >> 4);
+        const uint32_t dS = tmem + (uint32_t)(w * 128);
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + 32 * c < d) out[lane + 32 * c] = from_f32<T>(o[c] * inv);
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          if (kk >= g.ksteps) break;
+          const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
+          umma_f16_ss(dS, dq + off, dk + off, idesc_s, kk != 0);
+        }
+        umma_commit(&s_full[w]);
+      };
+      auto issue_pv = [&](int w, uint32_t st, bool first) -> bool {
+        if (!mbar_wait<false>(&p_full[w], pcnt[w] & 1, kErrTimeoutAttnP, abort_flag)) return false;
+        ++pcnt[w];
+        tc_fence_after();
+        const uint64_t dv = dv0 + (uint64_t)((st * C::kTile) >> 4);
+        const uint32_t pa = tmem + (uint32_t)(w * 128), dO = tmem + C::kColO + (uint32_t)(w * DP);
+        umma_f16_ts(dO, pa, dv, idesc_o, first ? 0u : 1u);
+#pragma unroll
+        for (int kk = 1; kk < 8; ++kk) umma_f16_ts(dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
+        return true;
+      };
+      while (ok && k.next(p, g)) {
+        if (!mbar_wait<false>(q_full, k.seg & 1, kErrTimeoutAttnQ, abort_flag)) break;
+        tc_fence_after();
+        uint32_t vslot[2] = {0, 0};      // V slot of each tile's last unit
+        int count[2] = {0, 0};           // units of each tile so far
+        for (int j = k.j0; ok && j < k.j1; ++j) {
+          uint32_t kslot = 0, vs = 0;
+          for (int w = 0; w < 2; ++w) {
+            if (!k.uses(w, j)) continue;
+            if (w == 0 || k.lone) {
+              kslot = slot;
+              if (!mbar_wait<false>(&ready[slot], phase, kErrTimeoutAttnKV, abort_flag)) {
+                ok = false;
+                break;
+              }
+              if (++slot == C::kSlots) slot = 0, phase ^= 1;
+            }
+            tc_fence_after();
+            if (count[w] > 0) {
+              if (!issue_pv(w, vslot[w], count[w] == 1)) {
+                ok = false;
+                break;
+              }
+              if (w == 1 || k.lone) umma_commit(&empty[vslot[w]]);
+            }
+            issue_s(w, k.lone ? 0 : w, kslot);
+            if (w == 1 || k.lone) umma_commit(&empty[kslot]);
+            if (w == 0 || k.lone) {
+              vs = slot;
+              if (!mbar_wait<false>(&ready[slot], phase, kErrTimeoutAttnKV, abort_flag)) {
+                ok = false;
+                break;
+              }
+              if (++slot == C::kSlots) slot = 0, phase ^= 1;
+            }
+            vslot[w] = vs;
+            ++count[w];
+          }
+        }
+        if (!ok) break;
+        umma_commit(q_empty);
+        for (int w = 0; w < 2; ++w) {
+          if (count[w] > 0) {
+            if (!issue_pv(w, vslot[w], count[w] == 1)) {
+              ok = false;
+              break;
+            }
+            if (w == 1 || k.lone) umma_commit(&empty[vslot[w]]);
+          }
+          umma_commit(&o_done[w]);
+        }
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ rows that are not kept
+    uint32_t slot = 0, phase = 0;
+    bool ok = true;
+    while (ok && k.next(p, g)) {
+      for (int j = k.j0; ok && j < k.j1; ++j) {
+        const int n = k.slots(j);
+        for (int i = 0; i < n; ++i) {
+          if (!mbar_wait<false>(&full[slot], phase, kErrTimeoutAttnKV, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (i & 1) {
+            const int key0 = k.kv_tile(i >> 1, j) * 128, khi = k.keys - key0;
+            if (kMask || khi < 128) {
+              bool touched = false;
+#pragma unroll
+              for (int ch = 0; ch < 4; ++ch) {
+                bool keep = ch * 32 + lane < khi;
+                if (kMask && keep) keep = p.key_mask[(size_t)k.s.b * p.k_len + key0 + ch * 32 + lane] != 0;
+                const uint32_t word = __ballot_sync(0xffffffffu, keep);
+                if (kMask && lane == 0) s_words[slot * 4 + ch] = word;
+                for (uint32_t out = ~word; out; out &= out - 1) {
+                  const int row = ch * 32 + __ffs(out) - 1;
+                  if (lane < 8 * C::kHalves)
+                    *reinterpret_cast<uint4*>(sKV + slot * C::kTile + (lane >> 3) * kHalfBytes + row * 128 +
+                                              (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                  touched = true;
+                }
+              }
+              if (touched) fence_proxy_async_smem();
+              __syncwarp();
+            }
+          }
+          if (lane == 0) mbar_arrive(&ready[slot]);
+          if (++slot == C::kSlots) slot = 0, phase ^= 1;
+        }
+      }
+    }
+  } else if (warp >= kSoftmaxWarp0) {
+    // ------------------------------------------------------------ softmax + epilogue
+    const int w = (warp - kSoftmaxWarp0) >> 2, q = warp & 3;
+    const int row = q * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+    const uint32_t sAddr = tmem + lane_off + (uint32_t)(w * 128);
+    const uint32_t oAddr = tmem + lane_off + C::kColO + (uint32_t)(w * DP);
+    const float c = p.scale_log2;
+    uint32_t slot = 0, phase = 0;       // ring position (masks are read at V slots)
+    uint32_t scnt = 0, meets = 0;
+    bool ok = true;
+    while (ok && k.next(p, g)) {
+      int n0, g0;
+      tile_origin(k, g, w, n0, g0);
+      const int rn = row / g.gt, n = n0 + rn, head = g0 + row - rn * g.gt;
+      const bool valid = rn < g.nt && n < p.q_len && head < g.group;
+      const bool warp_active = __any_sync(0xffffffffu, valid);
+      float ref = 0.f, l = 0.f;
+      bool have = false;  // the reference is set
+      int used = 0;
+      for (int j = k.j0; j < k.j1; ++j) {
+        // the V slot of this tile's unit
+        const int ns = k.slots(j);
+        uint32_t vs = slot + (k.lone ? 2 * w : 0) + 1, vphase = phase;
+        if (vs >= C::kSlots) vs -= C::kSlots, vphase ^= 1;
+        slot += ns;
+        if (slot >= C::kSlots) slot -= C::kSlots, phase ^= 1;
+        if (!k.uses(w, j)) continue;
+        if (!mbar_wait<false>(&s_full[w], scnt & 1, kErrTimeoutAttnS, abort_flag)) {
+          ok = false;
+          break;
+        }
+        ++scnt;
+        uint32_t words[4];
+        if constexpr (kMask) {
+          if (!mbar_wait<false>(&ready[vs], vphase, kErrTimeoutAttnKV, abort_flag)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) words[ch] = s_words[vs * 4 + ch];
+        } else {
+          const int khi = k.keys - k.kv_tile(w, j) * 128;
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) words[ch] = len_word(khi, ch);
+        }
+        tc_fence_after();
+        if (warp_active) {
+          uint32_t pk[64];
+          const bool any = (words[0] | words[1] | words[2] | words[3]) != 0u;
+          float sum = 0.f;
+          if (!have && any) {
+            const int ch = words[0] ? 0 : (words[1] ? 1 : (words[2] ? 2 : 3));
+            uint32_t r[32];
+            tmem_ld32(sAddr + ch * 32, r);
+            tmem_ld_wait(r);
+            const float m = chunk_max(r, words[ch], c);
+            ref = m == -INFINITY ? 0.f : m;
+            have = true;
+          }
+          if (any) {
+            sum = row_exp<T>(sAddr, words, c, ref, pk);
+            if (__any_sync(0xffffffffu, valid && !(sum <= kSumLimit))) {
+              // exact passes: the reference moves to the row's maximum, O and l with it
+              float m = -INFINITY;
+#pragma unroll 1
+              for (int ch = 0; ch < 4; ++ch) {
+                uint32_t r[32];
+                tmem_ld32(sAddr + ch * 32, r);
+                tmem_ld_wait(r);
+                m = fmaxf(m, chunk_max(r, words[ch], c));
+              }
+              const float moved = fmaxf(ref, m);
+              const float alpha = fast_exp2(ref - moved);
+              if (used > 0) {
+#pragma unroll 1
+                for (int h = 0; h < DP / 32; ++h) {
+                  uint32_t r[32];
+                  tmem_ld32(oAddr + h * 32, r);
+                  tmem_ld_wait(r);
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                  tmem_st32(oAddr + h * 32, r);
+                }
+                tmem_st_wait();
+              }
+              l *= alpha;
+              ref = moved;
+              sum = row_exp<T>(sAddr, words, c, ref, pk);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) pk[i] = 0u;
+          }
+          l += sum;
+          tmem_st32(sAddr, *reinterpret_cast<const uint32_t(*)[32]>(pk));
+          tmem_st32(sAddr + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
+          tmem_st_wait();
+        }
+        ++used;
+        tc_fence_before();
+        mbar_arrive(&p_full[w]);
+      }
+      if (!ok) break;
+      if (!mbar_wait<false>(&o_done[w], k.seg & 1, kErrTimeoutAttnO, abort_flag)) break;
+      tc_fence_after();
+      // a lone tile: the two halves meet, weigh each other in and write half the columns each
+      float a0 = 1.f, a1 = 0.f;
+      int c_lo = 0, c_hi = p.head_dim;
+      uint32_t src0 = oAddr, src1 = oAddr;
+      if (k.lone) {
+        float* ml = s_ml;
+        ml[w * 256 + row] = ref;
+        ml[w * 256 + 128 + row] = used > 0 ? l : -1.f;  // -1: no O
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&meet[q]);
+        if (!mbar_wait<false>(&meet[q], meets & 1, kErrTimeoutAttnO, abort_flag)) break;
+        ++meets;
+        tc_fence_after();
+        const float r0 = ml[row], r1 = ml[256 + row], l0 = ml[128 + row], l1 = ml[256 + 128 + row];
+        const bool has1 = l1 != -1.f;
+        if (has1) {
+          // a half without a kept key has l = 0 and no reference of its own
+          ref = l0 == 0.f ? r1 : (l1 == 0.f ? r0 : fmaxf(r0, r1));
+          a0 = l0 == 0.f ? 0.f : fast_exp2(r0 - ref);
+          a1 = l1 == 0.f ? 0.f : fast_exp2(r1 - ref);
+          l = l0 * a0 + l1 * a1;
+        } else {
+          ref = r0;
+          l = l0;
+        }
+        src0 = tmem + lane_off + C::kColO;
+        src1 = has1 ? src0 + DP : src0;
+        // 16-column pieces, the first half of them to w = 0
+        const int mid = ((p.head_dim + 31) >> 5) * 16;
+        if (w == 0)
+          c_hi = min(mid, p.head_dim);
+        else
+          c_lo = min(mid, p.head_dim);
+      }
+      const bool whole = k.whole();
+      const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+      const float f0 = a0 * inv, f1 = a1 * inv;
+      if (warp_active) {
+        T* out = static_cast<T*>(p.out.data) + (long long)k.s.b * p.out.batch_stride +
+                 (long long)n * p.out.seq_stride + (long long)(k.s.hk * g.group + head) * p.out.head_stride;
+        const size_t part = (size_t)(2 * blockIdx.x + (k.seg > 0)) * 256 + (k.lone ? 0 : w * 128) + row;
+        float* po = p.ws + part * (size_t)(p.head_dim + 2);
+        for (int c0 = c_lo; c0 < c_hi; c0 += 16) {
+          uint32_t r0[16], r1[16];
+          tmem_ld16(src0 + c0, r0);
+          tmem_ld16(src1 + c0, r1);
+          tmem_ld_wait(r0, r1);
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v[i] = f0 != 0.f ? __uint_as_float(r0[i]) * f0 : 0.f;
+            if (f1 != 0.f) v[i] += __uint_as_float(r1[i]) * f1;
+          }
+          if (valid) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              if (c0 + 8 * u >= c_hi) break;
+              if (whole) {
+                *reinterpret_cast<uint4*>(out + c0 + 8 * u) =
+                    make_uint4(pack2<T>(v[8 * u], v[8 * u + 1]), pack2<T>(v[8 * u + 2], v[8 * u + 3]),
+                               pack2<T>(v[8 * u + 4], v[8 * u + 5]), pack2<T>(v[8 * u + 6], v[8 * u + 7]));
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2)
+                  *reinterpret_cast<float2*>(po + c0 + 8 * u + i) = make_float2(v[8 * u + i], v[8 * u + i + 1]);
+              }
+            }
+          }
+        }
+        if (!whole && valid && (!k.lone || w == 0))
+          *reinterpret_cast<float2*>(po + p.head_dim) = make_float2(ref, l);
+      }
+      tc_fence_before();
+      if (k.lone) {
+        // neither half may go on (and overwrite O or the exchange) before both have read
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&meet[q]);
+        if (!mbar_wait<false>(&meet[q], meets & 1, kErrTimeoutAttnO, abort_flag)) break;
+        ++meets;
+      }
+    }
+  }
+
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the partial results of the items that span CTAs.  Block (x, y): the item that
+// the boundary between CTAs x and x + 1 cuts, if it is that item's first cut; rows
+// [8 y, 8 y + 8) of its 256.  Up to 8 contributors: a warp per row; more: the warps
+// share the contributors out, row by row, and are joined in warp order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    cross_combine_kernel(const __grid_constant__ CrossAttnParams p, const __grid_constant__ Geom g) {
+  __shared__ float s_o[8][128], s_m[8], s_l[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long G = g.contribs;
+  const long long U = total_units(p, g, lane);
+  const long long cut = U * (blockIdx.x + 1) / G;
+  if (cut >= U) return;
+  const Spot s = find_spot(p, g, cut, lane);
+  const long long start = cut - s.j;
+  if (s.j == 0 || U * blockIdx.x / G > start) return;  // no cut, or not its first
+  const int tiles = key_tiles(p, s.b);
+  const bool lone = s.t == g.full;
+  const long long last = start + (lone ? (tiles + 1) >> 1 : tiles) - 1;
+  const int c0 = (int)(((start + 1) * G - 1) / U), c1 = (int)(((last + 1) * G - 1) / U);
+  const int d = p.head_dim, ld = d + 2, count = c1 - c0 + 1;
+  auto part = [&](int c, int row) {
+    const int second = U * c / G < start;  // the item is the last of CTA c's run, not its first
+    return p.ws + ((size_t)(2 * c + second) * 256 + row) * (size_t)ld;
+  };
+  for (int i = 0; i < 8; ++i) {
+    const bool shared_out = count > 8;
+    if (!shared_out && i > 0) break;
+    const int row = blockIdx.y * 8 + (shared_out ? i : warp);
+    const int tile = lone ? 2 * g.full : 2 * s.t + (row >> 7), r = row & 127;
+    const int gi = tile / g.n_tiles, rn = r / g.gt;
+    const int n = (tile - gi * g.n_tiles) * g.nt + rn, head = gi * g.gt + r - rn * g.gt;
+    const bool valid = rn < g.nt && n < p.q_len && head < g.group && !(lone && row >= 128);
+    if (!valid) {
+      if (shared_out) continue;
+      return;
+    }
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = c0 + (shared_out ? warp : 0); c <= c1; c += shared_out ? 8 : 1) {
+      const float* x = part(c, row);
+      if (U * c / G == U * (c + 1) / G) continue;  // a CTA without units
+      const float2 ml = *reinterpret_cast<const float2*>(x + d);
+      if (ml.y == 0.f) continue;
+      const float mn = fmaxf(m, ml.x), a = fast_exp2(m - mn), e = fast_exp2(ml.x - mn);
+      l = l * a + ml.y * e;
+      m = mn;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (lane + 32 * t < d) o[t] = o[t] * a + x[lane + 32 * t] * e;
+    }
+    if (shared_out) {
+      __syncthreads();  // the previous row's exchange has been read
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s_o[warp][lane + 32 * t] = o[t];
+      if (lane == 0) {
+        s_m[warp] = m;
+        s_l[warp] = l;
+      }
+      __syncthreads();
+      if (warp != 0) continue;
+      m = -INFINITY;
+      for (int x = 0; x < 8; ++x) m = fmaxf(m, s_l[x] == 0.f ? -INFINITY : s_m[x]);
+      l = 0.f;
+      o[0] = o[1] = o[2] = o[3] = 0.f;
+      for (int x = 0; x < 8; ++x) {
+        if (s_l[x] == 0.f) continue;
+        const float e = fast_exp2(s_m[x] - m);
+        l += s_l[x] * e;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) o[t] += s_o[x][lane + 32 * t] * e;
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    T* out = static_cast<T*>(p.out.data) + (long long)s.b * p.out.batch_stride + (long long)n * p.out.seq_stride +
+             (long long)(s.hk * g.group + head) * p.out.head_stride;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (lane + 32 * t < d) out[lane + 32 * t] = from_f32<T>(o[t] * inv);
+  }
+}
+
+// No key at all: every row is zero.
+template <typename T>
+__global__ void cross_zero_kernel(const __grid_constant__ CrossAttnParams p) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int pieces = p.head_dim / 8;
+  if (i >= (long long)p.batch * p.q_len * p.q.heads * pieces) return;
+  const int c = (int)(i % pieces);
+  const long long r = i / pieces;
+  const int h = (int)(r % p.q.heads);
+  const long long bn = r / p.q.heads;
+  const int b = (int)(bn / p.q_len), n = (int)(bn % p.q_len);
+  *reinterpret_cast<uint4*>(static_cast<T*>(p.out.data) + b * p.out.batch_stride + n * p.out.seq_stride +
+                            h * p.out.head_stride + c * 8) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+Geom make_geom(int batch, int q_len, int k_len, int q_heads, int kv_heads, int head_dim, int num_sms) {
+  Geom g{};
+  g.kv_heads = kv_heads;
+  g.group = q_heads / kv_heads;
+  g.gt = std::min(g.group, 128);
+  g.nt = 128 / g.gt;
+  g.g_tiles = (g.group + g.gt - 1) / g.gt;
+  g.n_tiles = (q_len + g.nt - 1) / g.nt;
+  const int tiles = g.g_tiles * g.n_tiles;
+  g.full = tiles / 2;
+  g.lone = tiles & 1;
+  g.ksteps = (head_dim + 15) / 16;
+  const long long kt = (k_len + 127) / 128;
+  const long long units = (long long)batch * kv_heads * (g.full * kt + g.lone * ((kt + 1) / 2));
+  g.contribs = (int)std::min<long long>(num_sms, std::max<long long>(units, 1));
+  return g;
+}
+
+CUtensorMap seq_map(const HeadsView& v, int batch, int seq, int d, int rank5_group, int box_g, int box_n, int& batched,
+                    int& headed) {
+  // K / V: {d, seq, heads, batch}, boxes of 64 columns x 128 rows; Q: {d, group, seq, key
+  // heads, batch}, boxes of 64 x gt x nt.  A dimension walked with stride 0 is left out
+  // (extent 1, coordinate 0); a stride that is never walked only has to be a legal one.
+  batched = v.batch_stride != 0;
+  headed = v.head_stride != 0;
+  auto st = [](long long s) { return (uint64_t)(s ? s * 2 : 16); };
+  if (rank5_group) {
+    const uint64_t dims[5] = {(uint64_t)d, (uint64_t)rank5_group, (uint64_t)seq, (uint64_t)(v.heads / rank5_group),
+                              batched ? (uint64_t)batch : 1};
+    const uint64_t str[4] = {st(v.head_stride), st(v.seq_stride), st(v.head_stride * rank5_group), st(v.batch_stride)};
+    const uint32_t box[5] = {64, (uint32_t)box_g, (uint32_t)box_n, 1, 1};
+    return make_tensor_map(v.data, 5, dims, str, box);
+  }
+  const uint64_t dims[4] = {(uint64_t)d, (uint64_t)seq, headed ? (uint64_t)v.heads : 1, batched ? (uint64_t)batch : 1};
+  const uint64_t str[3] = {st(v.seq_stride), st(v.head_stride), st(v.batch_stride)};
+  const uint32_t box[4] = {64, 128, 1, 1};
+  return make_tensor_map(v.data, 4, dims, str, box);
+}
+
+template <typename T, int DP, bool kMask>
+cudaError_t launch_k(const CrossAttnParams& p, Geom g, cudaStream_t s) {
+  static std::atomic<unsigned long long> configured;
+  cudaError_t e = ensure_smem_limit(cross_attention_kernel<T, DP, kMask>, (int)Cfg<DP>::kSmem, configured);
+  if (e != cudaSuccess) return e;
+  int headed;
+  const CUtensorMap mq = seq_map(p.q, p.batch, p.q_len, p.head_dim, g.group, g.gt, g.nt, g.q_batched, headed);
+  const CUtensorMap mk = seq_map(p.k, p.batch, p.k_len, p.head_dim, 0, 0, 0, g.k_batched, g.k_headed);
+  const CUtensorMap mv = seq_map(p.v, p.batch, p.k_len, p.head_dim, 0, 0, 0, g.v_batched, g.v_headed);
+  const double rows = (double)p.batch * p.q_len * p.q.heads, keys = (double)p.batch * p.k_len * p.k.heads;
+  {
+    LaunchScope scope("cross_attention", 4.0 * rows * p.k_len * p.head_dim, 4.0 * (rows + keys) * p.head_dim, s);
+    cross_attention_kernel<T, DP, kMask><<<g.contribs, kThreads, Cfg<DP>::kSmem, s>>>(mq, mk, mv, p, g);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
+  if (g.contribs > 1) {
+    const int rows_max = g.full ? 256 : (int)std::min<long long>(128, (long long)g.gt * g.nt);
+    LaunchScope scope("cross_combine", 0.0, 0.0, s);
+    cross_combine_kernel<T><<<dim3(g.contribs - 1, (rows_max + 7) / 8), 256, 0, s>>>(p, g);
+  }
+  return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t launch_t(const CrossAttnParams& p, cudaStream_t s) {
-  const long long rows = (long long)p.batch * p.q_len * p.q.heads;
-  if (rows == 0) return cudaSuccess;
-  const double d = p.head_dim, keys = (double)p.batch * p.k_len;
-  LaunchScope scope("cross_attention", 4.0 * rows * p.k_len * d, 4.0 * rows * d + 4.0 * keys * p.k.heads * d, s);
-  cross_attention_simple_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_t(const CrossAttnParams& p, int num_sms, cudaStream_t s) {
+  if (p.k_len == 0) {
+    const long long n = (long long)p.batch * p.q_len * p.q.heads * (p.head_dim / 8);
+    LaunchScope scope("cross_zero", 0.0, 16.0 * n, s);
+    cross_zero_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p);
+    return cudaGetLastError();
+  }
+  const Geom g = make_geom(p.batch, p.q_len, p.k_len, p.q.heads, p.k.heads, p.head_dim, num_sms);
+  if (p.head_dim <= 64) return p.key_mask ? launch_k<T, 64, true>(p, g, s) : launch_k<T, 64, false>(p, g, s);
+  return p.key_mask ? launch_k<T, 128, true>(p, g, s) : launch_k<T, 128, false>(p, g, s);
 }
 
 }  // namespace
 
-cudaError_t launch_cross_attention(const CrossAttnParams& p, int bf16, cudaStream_t stream) {
-  return bf16 ? launch_t<__nv_bfloat16>(p, stream) : launch_t<__half>(p, stream);
+long long cross_attention_workspace(int batch, int q_len, int k_len, int q_heads, int kv_heads, int head_dim,
+                                    int num_sms) {
+  if (batch == 0 || q_len == 0 || k_len == 0) return 0;
+  const Geom g = make_geom(batch, q_len, k_len, q_heads, kv_heads, head_dim, num_sms);
+  return g.contribs > 1 ? 2LL * g.contribs * 256 * (head_dim + 2) * 4 : 0;
+}
+
+cudaError_t launch_cross_attention(const CrossAttnParams& p, int bf16, int num_sms, cudaStream_t stream) {
+  return bf16 ? launch_t<__nv_bfloat16>(p, num_sms, stream) : launch_t<__half>(p, num_sms, stream);
 }
 
 MSST_DEFINE_ERROR_ACCESSOR(cross_attn_device_error)

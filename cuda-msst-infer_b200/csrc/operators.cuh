@@ -38,8 +38,11 @@ struct CrossAttnParams {
   float scale_log2;                 // softmax scale * log2(e)
   const int* key_lens;              // [batch] or nullptr
   const unsigned char* key_mask;    // [batch, k_len], nonzero = kept, or nullptr
+  float* ws;                        // cross_attention_workspace() bytes
 };
-cudaError_t launch_cross_attention(const CrossAttnParams& p, int bf16, cudaStream_t stream);
+long long cross_attention_workspace(int batch, int q_len, int k_len, int q_heads, int kv_heads, int head_dim,
+                                    int num_sms);
+cudaError_t launch_cross_attention(const CrossAttnParams& p, int bf16, int num_sms, cudaStream_t stream);
 
 struct AdapterGemmParams {
   const void* x;             // [rows, K], row stride ldx

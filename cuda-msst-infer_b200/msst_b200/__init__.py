@@ -222,11 +222,13 @@ def _need(ok, msg):
         raise ValueError(msg)
 
 
-def _aligned_heads(t, shape):
-    """(tensor, strides): `t` itself where 16-byte loads can walk it, else a contiguous copy."""
+def _aligned_heads(t, shape, shared=False):
+    """(tensor, strides): `t` itself where 16-byte loads can walk it, else a contiguous copy.
+    `shared`: batch and heads may have stride 0 (an expanded tensor)."""
     st = t.stride()
-    if (st[3] == 1 and not t.data_ptr() & 15 and (not st[0] & 7 or shape[0] < 2) and (not st[1] & 7 or shape[1] < 2)
-            and (not st[2] & 7 or shape[2] < 2)):
+    if (st[3] == 1 and not t.data_ptr() & 15 and (not st[0] & 7 or shape[0] < 2)
+            and (st[1] and not st[1] & 7 or shape[1] < 2)
+            and ((st[2] or shared) and not st[2] & 7 or shape[2] < 2)):
         return t, st
     t = t.clone(memory_format=_torch().contiguous_format)
     return t, t.stride()
@@ -412,7 +414,7 @@ class ops:
               "k and v must be [B, Nk, heads, head_dim] with q's B and head_dim")
         _need(k.dtype is dt and v.dtype is dt and k.get_device() == dev and v.get_device() == dev,
               "q, k and v must share one 16-bit dtype and one device")
-        (q, sq), (k, sk), (v, sv) = _aligned_heads(q, shape), _aligned_heads(k, ks), _aligned_heads(v, ks)
+        (q, sq), (k, sk), (v, sv) = _aligned_heads(q, shape), _aligned_heads(k, ks, True), _aligned_heads(v, ks, True)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
             so = out.stride()

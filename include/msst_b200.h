@@ -193,7 +193,8 @@ int msst_qk_norm_rope(const msst_heads* q, const msst_heads* k, int batch, int s
  * [0, k_len]; NULL: all k_len) whose key_mask[b*k_len + j] is nonzero (NULL: all).
  * What the others hold, infinities and NaN included, has no influence.  A row
  * without a kept key gives zeros.  Data pointers are 16-byte aligned and strides
- * multiples of 8 elements.  `workspace` holds at least the bytes that
+ * multiples of 8 elements; batch and head strides of k and v may be 0 (states shared
+ * by the whole batch).  `workspace` holds at least the bytes that
  * msst_cross_attention_workspace gives for the call's sizes (16-byte aligned; may be
  * NULL when that is 0); calls that may overlap need workspaces of their own. */
 int msst_cross_attention_workspace(int batch, int q_len, int k_len, int q_heads, int kv_heads, int head_dim,
