@@ -1,5 +1,27 @@
-// adapter_gemm.cu — a shared projection with the low-rank adapters of many
-// requests beside it.
+// adapter_gemm.cu — a shared projection with the low-rank adapters of many requests
+// beside it: y[t] = W x[t] + bias + s_a B_a (A_a x[t]), a = row_adapter[t].
+//
+// Two launches.  adapter_down_kernel computes u[t] = A_a x[t] for every row that has an
+// adapter; adapter_gemm_kernel computes W x and adds B_a (s_a u) as a few more K steps
+// of the same accumulators, so the low-rank term costs no pass over the output.
+//
+// Both work on tiles of BT rows (32 to 256) and on the list of the distinct adapters
+// of a tile.  An adapter's part of the extra K steps is a slice of 16 rank values
+// (ceil(rank / 16) slices an adapter): B_a's columns on one side, on the other U', which
+// holds s_a u for the rows whose adapter is a and zeros for all others.  So requests
+// may be mixed row by row: a tile costs as many slices as it has adapters.
+//
+// The weights are the MMA's M side (128 of their rows) and the rows of x its N side: with
+// few rows the instruction then still covers 4 KB of weights, where an M side of rows
+// would be padded to 128 and the one issuing thread, at about 60 cycles an MMA, would
+// bound the pass (K = N = 4096: 8 us of issue for 32 columns a CTA, against the 5.2 us
+// that reading W takes).  Few tiles are split along K over a cluster, whose CTAs add
+// their parts through distributed shared memory in rank order.
+//
+// u is rounded to the operands' 16 bits once, as U' feeds the tensor cores; it is summed
+// in fp32 before that (split-K parts of the first launch in order).
+#include <algorithm>
+
 #include "common.cuh"
 #include "operators.cuh"
 #include "runtime.h"
@@ -8,82 +30,637 @@ namespace msst {
 
 namespace {
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+constexpr uint32_t kWTile = 128 * 128;       // 128 weight rows x 64 columns of 16 bits
+constexpr int kSliceRows = 16;               // rank values of a slice
+constexpr int kDownBlocks = 4;               // 128-slice-row accumulators of a pass of the first launch
+constexpr int kMaxDownSplit = 16;
+
+// The plan of a call, the same for both launches.
+struct Plan {
+  int bt;           // rows of x a tile
+  int tiles;        // ceil(rows / bt)
+  int n_tiles;      // ceil(N / 128)
+  int kblocks;      // ceil(K / 64)
+  int chunks;       // slices an adapter
+  int down_split;   // K splits of the first launch
+  int split;        // CTAs of a cluster along K in the second launch
+  int x_box;        // rows of x a TMA box brings (bt, fewer when there are fewer rows)
+  int list_ld;      // ints of a tile's list
+};
+
+// A tile's list: [0] distinct adapters, [1] whether the tile's rows differ, [2 ..] the adapters.
+__host__ __device__ inline size_t list_offset(const AdapterGemmParams& p, const Plan& pl) {
+  return (size_t)pl.down_split * p.rows * p.rank * sizeof(float);
 }
 
-// u[t, r] = s_a (A_a x[t])_r, one warp per value.
-template <typename T>
-__global__ void __launch_bounds__(256) adapter_down_simple_kernel(const __grid_constant__ AdapterGemmParams p) {
-  const long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (i >= (long long)p.rows * p.rank) return;
-  const int t = (int)(i / p.rank), r = (int)(i - (long long)t * p.rank);
+__device__ __forceinline__ int row_id(const AdapterGemmParams& p, long long t) {
+  if (t >= p.rows) return -1;
   const int a = __ldg(p.row_adapter + t);
-  float s = 0.f;
-  if (a >= 0 && a < p.adapters) {
-    const T* x = static_cast<const T*>(p.x) + t * p.ldx;
-    const T* w = static_cast<const T*>(p.lora_a) + ((size_t)a * p.rank + r) * p.K;
-    for (int k = lane; k < p.K; k += 32) s += to_f32(x[k]) * to_f32(w[k]);
-    s = warp_sum(s) * (p.scales ? __ldg(p.scales + a) : 1.f);
-  }
-  if (lane == 0) p.u[i] = s;
+  return a >= 0 && a < p.adapters ? a : -1;
 }
 
-// y[t, n], 16 x 16 outputs per block, x and W through shared memory.
-template <typename T>
-__global__ void __launch_bounds__(256) adapter_gemm_simple_kernel(const __grid_constant__ AdapterGemmParams p) {
-  __shared__ float sx[16][33], sw[16][33];
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  const long long t0 = (long long)blockIdx.y * 16;
-  const int n0 = blockIdx.x * 16;
-  const long long t = t0 + ty;
-  const int n = n0 + tx;
-  float acc = 0.f;
-  for (int k0 = 0; k0 < p.K; k0 += 32) {
-    for (int i = threadIdx.x; i < 512; i += 256) {
-      const int rr = i >> 5, kk = i & 31;
-      const bool in = k0 + kk < p.K;
-      sx[rr][kk] = in && t0 + rr < p.rows ? to_f32(static_cast<const T*>(p.x)[(t0 + rr) * p.ldx + k0 + kk]) : 0.f;
-      sw[rr][kk] = in && n0 + rr < p.N ? to_f32(static_cast<const T*>(p.w)[(size_t)(n0 + rr) * p.K + k0 + kk]) : 0.f;
+// ---------------------------------------------------------------------------
+// First launch: u[t] = A_a x[t], CTA = (row tile, K split).  The M side holds 8 slices of 16
+// rows of the tile's adapters, the N side the tile's rows; of the 128 x BT products each
+// row keeps the ones with its own adapter.  Bound: reading x once.
+// 192 threads: warp 0 TMA, warp 1 MMA, warps 2-5 the tile's list, then the results.
+// ---------------------------------------------------------------------------
+template <int BT>
+struct DownCfg {
+  static constexpr uint32_t kX = BT * 128;
+  static constexpr int kBlocks = 512 / BT < kDownBlocks ? 512 / BT : kDownBlocks;
+  static constexpr uint32_t kStage = kX + kBlocks * kWTile;
+  static constexpr int kStages = BT == 128 ? 2 : 3;
+  static constexpr size_t kSmem = kStages * kStage + 256 + 2 * BT * 4;
+  static constexpr uint32_t kTmem = kBlocks * BT < 32 ? 32 : kBlocks * BT;
+};
+
+template <typename T, int BT>
+__global__ void __launch_bounds__(192, 1)
+    adapter_down_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap amap,
+                        const __grid_constant__ AdapterGemmParams p, const __grid_constant__ Plan pl) {
+  using C = DownCfg<BT>;
+  constexpr uint32_t kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStage);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* acc_full = empty + C::kStages;
+  uint64_t* acc_empty = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_count = reinterpret_cast<int*>(tmem_slot + 2);  // distinct adapters per warp
+  int* s_mixed = s_count + 4;
+  int* s_id = reinterpret_cast<int*>(smem + C::kStages * C::kStage + 256);
+  int* s_list = s_id + BT;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = blockIdx.x / pl.down_split, ks = blockIdx.x - tile * pl.down_split;
+  const long long t0 = (long long)tile * BT;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
-    __syncthreads();
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 128);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&xmap);
+    tma_prefetch_desc(&amap);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kTmem);
+    tc_fence_before();
+  }
+  // the tile's adapters in order of first appearance
+  if (warp >= 2) {
+    const int i = threadIdx.x - 64;
+    for (int r = i; r < BT; r += 128) {
+      s_id[r] = row_id(p, t0 + r);
+      if (t0 + r < p.rows && ks == 0 && s_id[r] < 0 && __ldg(p.row_adapter + t0 + r) != -1) record_error(kErrAdapter);
+    }
+    if (i == 0) *s_mixed = 0;
+  }
+  __syncthreads();
+  constexpr int kPer = BT <= 128 ? 1 : BT / 128;  // rows a thread, consecutive
+  bool first[kPer];
+  if (warp >= 2) {
+    const int i = threadIdx.x - 64;
+    int mine = 0;
 #pragma unroll
-    for (int kk = 0; kk < 32; ++kk) acc += sx[ty][kk] * sw[tx][kk];
-    __syncthreads();
+    for (int e = 0; e < kPer; ++e) {
+      const int r = i * kPer + e;
+      first[e] = r < BT && s_id[r] >= 0;
+      if (r < BT) {
+        for (int x = 0; x < r && first[e]; ++x) first[e] = s_id[x] != s_id[r];
+        if (t0 + r < p.rows && s_id[r] != s_id[0]) *s_mixed = 1;
+      }
+      mine += first[e];
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) s_count[warp - 2] = incl;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    int at = incl - mine;
+    for (int x = 0; x < warp - 2; ++x) at += s_count[x];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (first[e]) s_list[at++] = s_id[i * kPer + e];
   }
-  if (t >= p.rows || n >= p.N) return;
-  if (p.bias) acc += __ldg(p.bias + n);
-  const int a = __ldg(p.row_adapter + t);
-  if (a >= 0 && a < p.adapters) {
-    const T* bw = static_cast<const T*>(p.lora_b) + ((size_t)a * p.N + n) * p.rank;
-    for (int r = 0; r < p.rank; ++r) acc += p.u[(size_t)t * p.rank + r] * to_f32(bw[r]);
-  } else if (a != -1 && n == 0) {
-    record_error(kErrAdapter);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int count = s_count[0] + s_count[1] + s_count[2] + s_count[3];
+  const int slices = count * pl.chunks;
+  const int kb0 = pl.kblocks * ks / pl.down_split, kb1 = pl.kblocks * (ks + 1) / pl.down_split;
+  const int passes = (slices + 8 * C::kBlocks - 1) / (8 * C::kBlocks);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int pass = 0; ok && pass < passes; ++pass) {
+        const int s0 = pass * 8 * C::kBlocks, s1 = min(slices, s0 + 8 * C::kBlocks);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % C::kStages;
+          if (!mbar_wait(&empty[st], ((it / C::kStages) & 1) ^ 1, kErrTimeoutSmemEmpty, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = smem + st * C::kStage;
+          mbar_arrive_expect_tx(&full[st], (uint32_t)pl.x_box * 128u + (uint32_t)(s1 - s0) * 2048u);
+          tma_load_2d(dst, &xmap, &full[st], kb * 64, (int)t0);
+          for (int s = s0; s < s1; ++s)
+            tma_load_3d(dst + C::kX + (s - s0) * 2048, &amap, &full[st], kb * 64, (s % pl.chunks) * kSliceRows,
+                        s_list[s / pl.chunks]);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_f16(kIsBf16, BT, 0);
+      int it = 0;
+      bool ok = true;
+      for (int pass = 0; ok && pass < passes; ++pass) {
+        const int blocks = (min(slices - pass * 8 * C::kBlocks, 8 * C::kBlocks) + 7) / 8;
+        if (!mbar_wait(acc_empty, (pass & 1) ^ 1, kErrTimeoutTmemEmpty, abort_flag)) break;
+        tc_fence_after();
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % C::kStages;
+          if (!mbar_wait(&full[st], (it / C::kStages) & 1, kErrTimeoutTmaFull, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t dx = sw128_desc(smem_u32(smem + st * C::kStage), 16, 1024);
+          const uint64_t da = sw128_desc(smem_u32(smem + st * C::kStage + C::kX), 16, 1024);
+          for (int b = 0; b < blocks; ++b)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16_ss(tmem + (uint32_t)(b * BT), da + (uint64_t)(b * (kWTile >> 4) + 2 * kk), dx + 2 * kk, idesc,
+                          kb > kb0 || kk > 0);
+          umma_commit(&empty[st]);
+        }
+        umma_commit(acc_full);
+      }
+    }
+  } else {
+    const int q = warp & 3;
+    const int lrow = q * 32 + lane;
+    float* u = static_cast<float*>(p.ws) + ((size_t)ks * p.rows + t0) * p.rank;
+    if (ks == 0) {
+      int* list = reinterpret_cast<int*>(static_cast<uint8_t*>(p.ws) + list_offset(p, pl)) + (size_t)tile * pl.list_ld;
+      for (int i = threadIdx.x - 64; i < count + 2; i += 128)
+        list[i] = i == 0 ? count : (i == 1 ? *s_mixed : s_list[i - 2]);
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+      const int s0 = pass * 8 * C::kBlocks, s1 = min(slices, s0 + 8 * C::kBlocks);
+      if (!mbar_wait(acc_full, pass & 1, kErrTimeoutTmemFull, abort_flag)) break;
+      tc_fence_after();
+      for (int b = 0; 8 * b < s1 - s0; ++b) {
+        const int s = s0 + 8 * b + lrow / kSliceRows;
+        const int r = (s % pl.chunks) * kSliceRows + lrow % kSliceRows;
+        const int a = s < s1 && r < p.rank ? s_list[s / pl.chunks] : -2;
+        for (int c = 0; c < BT; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BT + c), v);
+          tmem_ld_wait(v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (s_id[c + i] == a) u[(size_t)(c + i) * p.rank + r] = __uint_as_float(v[i]);
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(acc_empty);
+    }
   }
-  static_cast<T*>(p.out)[t * p.ldo + n] = from_f32<T>(acc);
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmem);
+  }
 }
 
+// ---------------------------------------------------------------------------
+// Second launch: tiles of 128 weight rows x BT rows of x.  448 threads: warp 0 TMA, warp 1
+// MMA, warps 2-5 U' of the slices, warps 6-13 epilogue (lane = weight row, so that 32 lanes
+// write 64 consecutive bytes of an output row).  Up to one tile a CTA the accumulators
+// are single, else double: the epilogue of a tile overlaps the next one's main loop.
+// A ring stage holds 64 columns of W and x, or 4 slices of B_a and U'.
+// ---------------------------------------------------------------------------
+template <int BT>
+struct GemmCfgA {
+  static constexpr uint32_t kX = BT * 128;
+  static constexpr uint32_t kStage = kWTile + kX;
+  static constexpr int kStages = BT == 256 ? 4 : (BT == 128 ? 6 : (BT == 64 ? 8 : 9));
+  static constexpr size_t kSmem = kStages * kStage + 512;
+  static constexpr uint32_t kTmem = 2 * BT;
+  static_assert(4 * kStages * 8 + 48 + 16 * 4 <= 512, "barriers");
+  static_assert(kStages * kStage >= BT * 128 * 4, "the split-K exchange reuses the ring");
+};
+constexpr int kThreadsA = 448;
+
+// Non-finite values of a 16-byte piece of B_a, which would reach every row of the tile as
+// 0 * Inf: replaced by zeros here; the epilogue adds them to their own rows.
 template <typename T>
-cudaError_t launch_t(const AdapterGemmParams& p, cudaStream_t s) {
-  if (p.rows == 0) return cudaSuccess;
+__device__ __forceinline__ bool drop_nonfinite(uint4& v) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & kExp) == kExp) w[i] &= 0xffff0000u, found = true;
+    if ((w[i] >> 16 & kExp) == kExp) w[i] &= 0x0000ffffu, found = true;
+  }
+  return found;
+}
+
+template <typename T, int BT>
+__global__ void __launch_bounds__(kThreadsA, 1)
+    adapter_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+                        const __grid_constant__ CUtensorMap bmap, const __grid_constant__ AdapterGemmParams p,
+                        const __grid_constant__ Plan pl) {
+  using C = GemmCfgA<BT>;
+  constexpr uint32_t kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStage);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* u_go = empty + C::kStages;    // [stages] the stage is free for U' (producer)
+  uint64_t* u_full = u_go + C::kStages;   // [stages] U' written, B_a's slices landed
+  uint64_t* acc_full = u_full + C::kStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;     // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  // [tile count % 16] = tile count + 1 where values of B_a were left out (U' runs ahead of
+  // the epilogue by fewer tiles than the ring has stages, plus the two accumulators)
+  volatile int* s_dropped = reinterpret_cast<volatile int*>(tmem_slot + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = pl.split > 1 ? (int)cluster_ctarank() : 0;
+  const int tile0 = pl.split > 1 ? blockIdx.x / pl.split : blockIdx.x;
+  const int step = pl.split > 1 ? pl.tiles * pl.n_tiles : gridDim.x;
+  const int total = pl.tiles * pl.n_tiles;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+      mbar_init(&u_go[i], 1);
+      mbar_init(&u_full[i], 128);
+    }
+    for (int i = 0; i < 16; ++i) s_dropped[i] = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 256);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&xmap);
+    tma_prefetch_desc(&wmap);
+    tma_prefetch_desc(&bmap);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kTmem);
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int* lists = reinterpret_cast<const int*>(static_cast<const uint8_t*>(p.ws) + list_offset(p, pl));
+  const int kb0 = pl.kblocks * rank / pl.split, kb1 = pl.kblocks * (rank + 1) / pl.split;
+  // this CTA's slices of a tile whose list is `list`
+  auto slice_range = [&](const int* list, int& s0, int& s1) {
+    const int n = list[0] * pl.chunks;
+    s0 = n * rank / pl.split;
+    s1 = n * (rank + 1) / pl.split;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int tile = tile0; ok && tile < total; tile += step) {
+        const int tt = tile / pl.n_tiles, n0 = (tile - tt * pl.n_tiles) * 128;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % C::kStages;
+          if (!mbar_wait(&empty[st], ((it / C::kStages) & 1) ^ 1, kErrTimeoutSmemEmpty, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = smem + st * C::kStage;
+          mbar_arrive_expect_tx(&full[st], kWTile + (uint32_t)pl.x_box * 128u);
+          tma_load_2d(dst, &wmap, &full[st], kb * 64, n0);
+          tma_load_2d(dst + kWTile, &xmap, &full[st], kb * 64, tt * BT);
+        }
+        const int* list = lists + (size_t)tt * pl.list_ld;
+        int s0, s1;
+        slice_range(list, s0, s1);
+        for (; ok && s0 < s1; s0 += 4, ++it) {
+          const int st = it % C::kStages, n = min(4, s1 - s0);
+          if (!mbar_wait(&empty[st], ((it / C::kStages) & 1) ^ 1, kErrTimeoutSmemEmpty, abort_flag)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive(&u_go[st]);
+          mbar_arrive_expect_tx(&full[st], (uint32_t)n * 4096u);
+          for (int i = 0; i < n; ++i)
+            tma_load_3d(smem + st * C::kStage + i * 4096, &bmap, &full[st], ((s0 + i) % pl.chunks) * kSliceRows, n0,
+                        list[2 + (s0 + i) / pl.chunks]);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_f16(kIsBf16, BT, 0);
+      int it = 0, n = 0;
+      uint32_t uses = 0;  // parity of each stage's uses for slices
+      bool ok = true;
+      for (int tile = tile0; ok && tile < total; tile += step, ++n) {
+        const int tt = tile / pl.n_tiles, buf = n & 1;
+        const uint32_t acc = tmem + (uint32_t)(buf * BT);
+        if (!mbar_wait(&acc_empty[buf], ((n >> 1) & 1) ^ 1, kErrTimeoutTmemEmpty, abort_flag)) break;
+        tc_fence_after();
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % C::kStages;
+          if (!mbar_wait(&full[st], (it / C::kStages) & 1, kErrTimeoutTmaFull, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t dw = sw128_desc(smem_u32(smem + st * C::kStage), 16, 1024);
+          const uint64_t dx = sw128_desc(smem_u32(smem + st * C::kStage + kWTile), 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) umma_f16_ss(acc, dw + 2 * kk, dx + 2 * kk, idesc, kb > kb0 || kk > 0);
+          umma_commit(&empty[st]);
+        }
+        int s0, s1;
+        slice_range(lists + (size_t)tt * pl.list_ld, s0, s1);
+        for (; ok && s0 < s1; s0 += 4, ++it) {
+          const int st = it % C::kStages, m = min(4, s1 - s0);
+          if (!mbar_wait(&u_full[st], uses >> st & 1, kErrTimeoutTmaFull, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uses ^= 1u << st;
+          tc_fence_after();
+          const uint64_t dw = sw32_desc(smem_u32(smem + st * C::kStage));
+          const uint64_t dx = sw32_desc(smem_u32(smem + st * C::kStage + kWTile));
+          for (int i = 0; i < m; ++i)
+            umma_f16_ss(acc, dw + (uint64_t)(i * (4096 >> 4)), dx + (uint64_t)(i * (BT * 32 >> 4)), idesc, 1u);
+          umma_commit(&empty[st]);
+        }
+        if (ok) umma_commit(&acc_full[buf]);
+      }
+    }
+  } else if (warp < 6) {
+    // ------------------------------------------------------------ U' of the slices
+    // These warps follow the ring by its slice stages alone: a stage is theirs once the
+    // producer says so, and is not used again before the MMA has had their U'.
+    const int i0 = threadIdx.x - 64;
+    int it = 0, n = 0;
+    uint32_t uses = 0;
+    bool ok = true;
+    const size_t part = (size_t)p.rows * p.rank;
+    for (int tile = tile0; ok && tile < total; tile += step, ++n) {
+      const int tt = tile / pl.n_tiles;
+      const int* list = lists + (size_t)tt * pl.list_ld;
+      int s0, s1;
+      slice_range(list, s0, s1);
+      it += kb1 - kb0;
+      for (; s0 < s1; s0 += 4, ++it) {
+        const int st = it % C::kStages, m = min(4, s1 - s0);
+        if (!mbar_wait(&u_go[st], uses >> st & 1, kErrTimeoutSmemEmpty, abort_flag)) {
+          ok = false;
+          break;
+        }
+        uses ^= 1u << st;
+        uint8_t* base = smem + st * C::kStage;
+        for (int x = i0; x < m * BT * 2; x += 128) {
+          const int i = x / (BT * 2), r = (x >> 1) % BT, half = x & 1;
+          const int s = s0 + i, a = list[2 + s / pl.chunks], c0 = (s % pl.chunks) * kSliceRows + half * 8;
+          const long long t = (long long)tt * BT + r;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = 0.f;
+          if (c0 < p.rank && row_id(p, t) == a) {
+            const float* u = static_cast<const float*>(p.ws) + t * p.rank + c0;
+            for (int k = 0; k < pl.down_split; ++k, u += part) {
+              const float4 lo = *reinterpret_cast<const float4*>(u), hi = *reinterpret_cast<const float4*>(u + 4);
+              v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+              v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+            }
+            const float sc = p.scales ? __ldg(p.scales + a) : 1.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= sc;
+          }
+          *reinterpret_cast<uint4*>(base + kWTile + i * (BT * 32) + r * 32 + ((half ^ (r >> 2 & 1)) << 4)) =
+              make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+        }
+        if (!mbar_wait(&full[st], (it / C::kStages) & 1, kErrTimeoutTmaFull, abort_flag)) {
+          ok = false;
+          break;
+        }
+        if (list[1]) {
+          for (int x = i0; x < m * 256; x += 128) {
+            uint4* at = reinterpret_cast<uint4*>(base + x * 16);
+            uint4 v = *at;
+            if (drop_nonfinite<T>(v)) {
+              *at = v;
+              s_dropped[n & 15] = n + 1;
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&u_full[st]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3, half = (warp - 6) >> 2;
+    int n = 0;
+    for (int tile = tile0; tile < total; tile += step, ++n) {
+      const int tt = tile / pl.n_tiles, buf = n & 1;
+      const int col = (tile - tt * pl.n_tiles) * 128 + q * 32 + lane;  // output column
+      const long long t0 = (long long)tt * BT;
+      const bool in = col < p.N;
+      const float bias = in && p.bias && rank == 0 ? __ldg(p.bias + col) : 0.f;
+      if (!mbar_wait(&acc_full[buf], (n >> 1) & 1, kErrTimeoutTmemFull, abort_flag)) break;
+      tc_fence_after();
+      const bool dropped = s_dropped[n & 15] == n + 1;
+      const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BT);
+      constexpr int kCols = BT >= 64 ? BT / 2 : BT;  // columns of this warp
+      if (BT >= 64 || half == 0) {
+        for (int c = half * kCols; c < (half + 1) * kCols; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(acc + (uint32_t)c, v);
+          tmem_ld_wait(v);
+          if (dropped && in) {
+            // the values left out of B_a, into the rows that have the adapter
+            const int* list = lists + (size_t)tt * pl.list_ld;
+            int s0, s1;
+            slice_range(list, s0, s1);
+            for (int s = s0; s < s1; ++s) {
+              const int a = list[2 + s / pl.chunks];
+              const int c0 = (s % pl.chunks) * kSliceRows, c1 = min(c0 + kSliceRows, p.rank);
+              const T* bw = static_cast<const T*>(p.lora_b) + ((size_t)a * p.N + col) * p.rank;
+              for (int r = c0; r < c1; ++r) {
+                const float bv = to_f32(bw[r]);
+                if (isfinite(bv)) continue;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (row_id(p, t0 + c + i) == a) {
+                    float u = 0.f;
+                    for (int k = 0; k < pl.down_split; ++k)
+                      u += static_cast<const float*>(p.ws)[((size_t)k * p.rows + t0 + c + i) * p.rank + r];
+                    u = to_f32(from_f32<T>(u * (p.scales ? __ldg(p.scales + a) : 1.f)));
+                    v[i] = __float_as_uint(__uint_as_float(v[i]) + u * bv);
+                  }
+              }
+            }
+          }
+          if (pl.split > 1) {
+            float* ex = reinterpret_cast<float*>(smem) + c * 128 + q * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ex[i * 128] = __uint_as_float(v[i]) + bias;
+          } else if (in) {
+            T* out = static_cast<T*>(p.out) + (t0 + c) * p.ldo + col;
+            const int left = (int)min(32LL, p.rows - (t0 + c));
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < left) out[i * p.ldo] = from_f32<T>(__uint_as_float(v[i]) + bias);
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&acc_empty[buf]);
+    }
+  }
+
+  if (pl.split > 1) {
+    // every CTA of the cluster adds up its share of the tile's rows, in rank order
+    __syncwarp();
+    cluster_sync_all();
+    const int tt = tile0 / pl.n_tiles, n0 = (tile0 - tt * pl.n_tiles) * 128;
+    const int r0 = BT * rank / pl.split, r1 = BT * (rank + 1) / pl.split;
+    const uint32_t base = smem_u32(smem);
+    for (int x = threadIdx.x; x < (r1 - r0) * 32; x += kThreadsA) {
+      const int r = r0 + (x >> 5), c = (x & 31) * 4;
+      const long long t = (long long)tt * BT + r;
+      if (t >= p.rows || n0 + c >= p.N) continue;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < pl.split; ++k) {
+        float4 v;
+        const uint32_t at = mapa_shared(base + (uint32_t)(r * 128 + c) * 4u, (uint32_t)k);
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                     : "r"(at)
+                     : "memory");
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.ldo + n0 + c) =
+          make_uint2(pack2<T>(sum.x, sum.y), pack2<T>(sum.z, sum.w));
+    }
+    __syncwarp();
+    cluster_sync_all();  // the parts stay until all have read them
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmem);
+  }
+}
+
+Plan make_plan(int rows, int K, int N, int rank, int num_sms) {
+  Plan pl{};
+  pl.bt = rows <= 32 ? 32 : (rows <= 64 ? 64 : (rows <= 128 ? 128 : 256));
+  pl.tiles = (rows + pl.bt - 1) / pl.bt;
+  pl.n_tiles = (N + 127) / 128;
+  pl.kblocks = (K + 63) / 64;
+  pl.chunks = (rank + kSliceRows - 1) / kSliceRows;
+  pl.down_split = std::max(1, std::min({num_sms / pl.tiles, kMaxDownSplit, pl.kblocks}));
+  pl.split = 1;
+  while (pl.split < 8 && (long long)pl.tiles * pl.n_tiles * pl.split * 2 <= num_sms && pl.split * 2 <= pl.kblocks)
+    pl.split *= 2;
+  pl.x_box = std::min(pl.bt, (rows + 7) / 8 * 8);
+  pl.list_ld = (pl.bt + 2 + 3) / 4 * 4;
+  return pl;
+}
+
+// 16-bit [count, rows, cols] in boxes of box_cols x box_rows
+CUtensorMap map_3d(const void* base, uint64_t cols, uint64_t rows, uint64_t count, uint32_t box_cols,
+                   uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  const uint64_t dims[3] = {cols, rows, count};
+  const uint64_t strides[2] = {cols * 2, cols * rows * 2};
+  const uint32_t box[3] = {box_cols, box_rows, 1};
+  return make_tensor_map(base, 3, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT16, swizzle);
+}
+
+template <typename T, int BT>
+cudaError_t launch_bt(const AdapterGemmParams& p, const Plan& pl, int num_sms, cudaStream_t s) {
+  static std::atomic<unsigned long long> configured[2];
+  cudaError_t e = ensure_smem_limit(adapter_down_kernel<T, BT>, (int)DownCfg<BT>::kSmem, configured[0]);
+  if (e == cudaSuccess) e = ensure_smem_limit(adapter_gemm_kernel<T, BT>, (int)GemmCfgA<BT>::kSmem, configured[1]);
+  if (e != cudaSuccess) return e;
   const double m = p.rows, k = p.K, n = p.N, r = p.rank;
+  const CUtensorMap mx = map_2d(p.x, (uint64_t)p.rows, (uint64_t)p.K, (uint64_t)p.ldx, (uint32_t)pl.x_box);
+  const CUtensorMap mw = map_2d(p.w, (uint64_t)p.N, (uint64_t)p.K, (uint64_t)p.K, 128);
+  // without adapters no row has one and neither map is read
+  const CUtensorMap ma = p.adapters ? map_3d(p.lora_a, (uint64_t)p.K, (uint64_t)p.rank, (uint64_t)p.adapters, 64,
+                                             kSliceRows, CU_TENSOR_MAP_SWIZZLE_128B)
+                                    : mx;
+  const CUtensorMap mb = p.adapters ? map_3d(p.lora_b, (uint64_t)p.rank, (uint64_t)p.N, (uint64_t)p.adapters,
+                                             kSliceRows, 128, CU_TENSOR_MAP_SWIZZLE_32B)
+                                    : mx;
   {
     LaunchScope scope("adapter_down", 2.0 * m * r * k, 2.0 * (m * k + p.adapters * r * k) + 4.0 * m * r, s);
-    adapter_down_simple_kernel<T><<<(unsigned)(((long long)p.rows * p.rank + 7) / 8), 256, 0, s>>>(p);
+    adapter_down_kernel<T, BT><<<pl.tiles * pl.down_split, 192, DownCfg<BT>::kSmem, s>>>(mx, ma, p, pl);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   LaunchScope scope("adapter_gemm", 2.0 * m * n * (k + r), 2.0 * (m * k + n * k + m * n + p.adapters * r * n), s);
-  adapter_gemm_simple_kernel<T>
-      <<<dim3((unsigned)((p.N + 15) / 16), (unsigned)((p.rows + 15) / 16)), 256, 0, s>>>(p);
-  return cudaGetLastError();
+  const long long tiles = (long long)pl.tiles * pl.n_tiles;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(pl.split > 1 ? tiles * pl.split : std::min<long long>(tiles, num_sms)));
+  cfg.blockDim = dim3(kThreadsA);
+  cfg.dynamicSmemBytes = GemmCfgA<BT>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)pl.split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, adapter_gemm_kernel<T, BT>, mx, mw, mb, p, pl);
+}
+
+template <typename T>
+cudaError_t launch_t(const AdapterGemmParams& p, int num_sms, cudaStream_t s) {
+  if (p.rows == 0) return cudaSuccess;
+  const Plan pl = make_plan(p.rows, p.K, p.N, p.rank, num_sms);
+  switch (pl.bt) {
+    case 32:
+      return launch_bt<T, 32>(p, pl, num_sms, s);
+    case 64:
+      return launch_bt<T, 64>(p, pl, num_sms, s);
+    case 128:
+      return launch_bt<T, 128>(p, pl, num_sms, s);
+    default:
+      return launch_bt<T, 256>(p, pl, num_sms, s);
+  }
 }
 
 }  // namespace
 
-cudaError_t launch_adapter_gemm(const AdapterGemmParams& p, int bf16, cudaStream_t stream) {
-  return bf16 ? launch_t<__nv_bfloat16>(p, stream) : launch_t<__half>(p, stream);
+long long adapter_gemm_workspace(int rows, int K, int N, int adapters, int rank, int num_sms) {
+  if (rows == 0) return 0;
+  const Plan pl = make_plan(rows, K, N, rank, num_sms);
+  return (long long)pl.down_split * rows * rank * 4 + (long long)pl.tiles * pl.list_ld * 4;
+}
+
+cudaError_t launch_adapter_gemm(const AdapterGemmParams& p, int bf16, int num_sms, cudaStream_t stream) {
+  return bf16 ? launch_t<__nv_bfloat16>(p, num_sms, stream) : launch_t<__half>(p, num_sms, stream);
 }
 
 MSST_DEFINE_ERROR_ACCESSOR(adapter_gemm_device_error)

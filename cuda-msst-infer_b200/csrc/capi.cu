@@ -521,7 +521,7 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
 int msst_adapter_gemm_workspace(long long rows, int K, int N, int adapters, int rank, long long* bytes) {
   return guarded([&] {
     MSST_REQUIRE(bytes && rows >= 0 && rows < (1LL << 31) && K > 0 && N > 0 && adapters >= 0 && rank > 0, "bad shape");
-    *bytes = rows * rank * 4;
+    *bytes = msst::adapter_gemm_workspace((int)rows, K, N, adapters, rank, sm_count());
   });
 }
 
@@ -545,7 +545,8 @@ int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const
     check_align(lora_a, "lora_a");
     check_align(lora_b, "lora_b");
     DeviceScope dev_scope(device_of(x));
-    check_workspace(workspace, workspace_bytes, rows * rank * 4);
+    check_workspace(workspace, workspace_bytes,
+                    msst::adapter_gemm_workspace((int)rows, K, N, adapters, rank, sm_count()));
     msst::AdapterGemmParams p{};
     p.x = x;
     p.w = w;
@@ -555,7 +556,7 @@ int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const
     p.scales = scales;
     p.row_adapter = row_adapter;
     p.out = out;
-    p.u = static_cast<float*>(workspace);
+    p.ws = workspace;
     p.ldx = ldx;
     p.ldo = ldo;
     p.rows = (int)rows;
@@ -563,7 +564,7 @@ int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const
     p.N = N;
     p.adapters = adapters;
     p.rank = rank;
-    MSST_CUDA(msst::launch_adapter_gemm(p, dtype, as_stream(stream)));
+    MSST_CUDA(msst::launch_adapter_gemm(p, dtype, sm_count(), as_stream(stream)));
   });
 }
 

@@ -53,10 +53,11 @@ struct AdapterGemmParams {
   const float* scales;       // [adapters] or nullptr (ones)
   const int* row_adapter;    // [rows], outside [0, adapters) = none
   void* out;                 // [rows, N], row stride ldo
-  float* u;                  // workspace [rows, rank]
+  void* ws;                  // adapter_gemm_workspace() bytes
   long long ldx, ldo;
   int rows, K, N, adapters, rank;
 };
-cudaError_t launch_adapter_gemm(const AdapterGemmParams& p, int bf16, cudaStream_t stream);
+long long adapter_gemm_workspace(int rows, int K, int N, int adapters, int rank, int num_sms);
+cudaError_t launch_adapter_gemm(const AdapterGemmParams& p, int bf16, int num_sms, cudaStream_t stream);
 
 }  // namespace msst
