@@ -33,6 +33,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "cross_attn.cuh"
 #include "operators.cuh"
 #include "runtime.h"
 
@@ -52,131 +53,6 @@ struct Cfg {
   static constexpr int kSlots = DP == 128 ? 5 : 8;             // ring of K and V tiles
   static constexpr size_t kSmem = 2 * kTile + kSlots * kTile + 2560;
   static constexpr uint32_t kColO = 256;
-};
-
-// Geometry of a launch.
-struct Geom {
-  int kv_heads, group;       // G query heads a key head
-  int gt, nt;                // heads and tokens of a tile
-  int g_tiles, n_tiles;      // tiles along heads and tokens
-  int full, lone;            // per key head: pairs, and 1 if a lone tile is left
-  int q_batched;             // 0: shared by the batch through stride 0
-  int k_batched, k_headed;
-  int v_batched, v_headed;
-  int ksteps;                // ceil(head_dim / 16)
-  int contribs;              // CTAs of the attention launch
-};
-
-__device__ __forceinline__ int key_count(const CrossAttnParams& p, int b) {
-  return p.key_lens ? min(max(__ldg(p.key_lens + b), 0), p.k_len) : p.k_len;
-}
-// K/V tiles of a batch entry (one masked tile where no key is left, so that every item
-// has a unit that writes its rows)
-__device__ __forceinline__ int key_tiles(const CrossAttnParams& p, int b) {
-  return max(1, (key_count(p, b) + 127) >> 7);
-}
-__device__ __forceinline__ long long batch_units(const Geom& g, int tiles) {
-  return (long long)g.kv_heads * ((long long)g.full * tiles + g.lone * ((tiles + 1) >> 1));
-}
-
-// A position in the list of units: batch entry, key head, item of the key head, unit.
-struct Spot {
-  int b, hk, t, j;
-};
-// Spot of unit u < batch_units(tiles of b), counted from batch entry b's first.
-__device__ __forceinline__ Spot spot_in_batch(const Geom& g, int b, int tiles, long long u) {
-  const long long per_head = batch_units(g, tiles) / g.kv_heads;
-  Spot s;
-  s.b = b;
-  s.hk = (int)(u / per_head);
-  const long long r = u - s.hk * per_head;
-  if (r < (long long)g.full * tiles) {
-    s.t = (int)(r / tiles);
-    s.j = (int)(r - (long long)s.t * tiles);
-  } else {
-    s.t = g.full;
-    s.j = (int)(r - (long long)g.full * tiles);
-  }
-  return s;
-}
-
-// One warp: total units of the launch, and for `want` < 2 unit indices their spots.
-// Ragged batches are summed 32 entries at a time.
-__device__ long long total_units(const CrossAttnParams& p, const Geom& g, int lane) {
-  if (!p.key_lens) return p.batch * batch_units(g, key_tiles(p, 0));
-  long long sum = 0;
-  for (int b = lane; b < p.batch; b += 32) sum += batch_units(g, key_tiles(p, b));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
-}
-// One warp: the spot of unit u and the units before its batch entry.
-__device__ Spot find_spot(const CrossAttnParams& p, const Geom& g, long long u, int lane) {
-  if (!p.key_lens) {
-    const int tiles = key_tiles(p, 0);
-    const long long per = batch_units(g, tiles);
-    const int b = (int)(u / per);
-    return spot_in_batch(g, b, tiles, u - b * per);
-  }
-  long long before = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const int tiles = b < p.batch ? key_tiles(p, b) : 0;
-    const long long mine = b < p.batch ? batch_units(g, tiles) : 0;
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const long long start = before + __shfl_sync(0xffffffffu, incl - mine, src);
-      return spot_in_batch(g, b0 + src, __shfl_sync(0xffffffffu, tiles, src), u - start);
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  return Spot{p.batch - 1, 0, 0, 0};  // u past the end: not reached
-}
-
-// Walks the segments (one item each) of a CTA's run.
-struct Walk {
-  Spot s;
-  long long left;
-  int seg;
-  // of the current segment: K/V tiles of the batch entry, its key count, units [j0, j1)
-  int tiles, keys, j0, j1, units;
-  bool lone;
-  __device__ Walk(const Spot& s0, long long n) : s(s0), left(n), seg(-1) {}
-  __device__ __forceinline__ bool next(const CrossAttnParams& p, const Geom& g) {
-    if (seg >= 0) {
-      s.j = 0;
-      if (++s.t == g.full + g.lone) {
-        s.t = 0;
-        if (++s.hk == g.kv_heads) {
-          s.hk = 0;
-          ++s.b;
-        }
-      }
-    }
-    if (left <= 0) return false;
-    ++seg;
-    keys = key_count(p, s.b);
-    tiles = max(1, (keys + 127) >> 7);
-    lone = s.t == g.full;
-    units = lone ? (tiles + 1) >> 1 : tiles;
-    j0 = s.j;
-    j1 = (int)min((long long)units, j0 + left);
-    left -= j1 - j0;
-    return true;
-  }
-  __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == units; }
-  // K/V tile of query tile w in unit j, and whether it has one
-  __device__ __forceinline__ int kv_tile(int w, int j) const { return lone ? 2 * j + w : j; }
-  __device__ __forceinline__ bool uses(int w, int j) const { return kv_tile(w, j) < tiles; }
-  // ring slots that unit j takes
-  __device__ __forceinline__ int slots(int j) const { return lone ? (uses(1, j) ? 4 : 2) : 2; }
 };
 
 // First token and head of row tile w of the current segment.
@@ -316,6 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   __syncthreads();
+  dependents_may_start();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Walk k(*s_spot, *s_count);
@@ -631,8 +508,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (warp_active) {
         T* out = static_cast<T*>(p.out.data) + (long long)k.s.b * p.out.batch_stride +
                  (long long)n * p.out.seq_stride + (long long)(k.s.hk * g.group + head) * p.out.head_stride;
-        const size_t part = (size_t)(2 * blockIdx.x + (k.seg > 0)) * 256 + (k.lone ? 0 : w * 128) + row;
-        float* po = p.ws + part * (size_t)(p.head_dim + 2);
+        const size_t part = (size_t)(2 * blockIdx.x + (k.seg > 0)) * g.slot_rows + (k.lone ? 0 : w * 128) + row;
+        float* po = p.ws + part * (size_t)part_ld(p.head_dim);
         for (int c0 = c_lo; c0 < c_hi; c0 += 16) {
           uint32_t r0[16], r1[16];
           tmem_ld16(src0 + c0, r0);
@@ -681,84 +558,169 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the partial results of the items that span CTAs.  Block (x, y): the item that
-// the boundary between CTAs x and x + 1 cuts, if it is that item's first cut; rows
-// [8 y, 8 y + 8) of its 256.  Up to 8 contributors: a warp per row; more: the warps
-// share the contributors out, row by row, and are joined in warp order.
-template <typename T>
+// Joins the partial results of the items that span CTAs, in CTA order.
+//
+// kByItem false (at least as many items as CTAs, so a cut item has two or three parts):
+// block (x, y) takes the item that the boundary between CTAs x and x + 1 cuts, if it is that
+// item's first cut, and rows [32 y, 32 y + 32) of it, LPR lanes a row, every load of a
+// warp's rows issued before the first use.
+// kByItem true (an item may span every CTA): block (x, y) takes item x and its row y, and the
+// 8 warps share the parts out.
+template <typename T, int LPR, bool kByItem>
 __global__ void __launch_bounds__(256)
     cross_combine_kernel(const __grid_constant__ CrossAttnParams p, const __grid_constant__ Geom g) {
-  __shared__ float s_o[8][128], s_m[8], s_l[8];
+  __shared__ long long s_start, s_units;
+  __shared__ Spot s_spot;
+  __shared__ __align__(16) float s_o[8][128];  // read and written 16 bytes at a time
+  __shared__ float s_m[8], s_l[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long G = g.contribs;
-  const long long U = total_units(p, g, lane);
-  const long long cut = U * (blockIdx.x + 1) / G;
-  if (cut >= U) return;
-  const Spot s = find_spot(p, g, cut, lane);
-  const long long start = cut - s.j;
-  if (s.j == 0 || U * blockIdx.x / G > start) return;  // no cut, or not its first
-  const int tiles = key_tiles(p, s.b);
+  wait_for_previous();
+  if (warp == 0) {
+    const long long U = total_units(p, g, lane);
+    long long start = -1;
+    Spot s{};
+    if constexpr (kByItem) {
+      // the item's first unit: units of the batch entries before, then inside its own
+      s.b = blockIdx.x / g.items_batch;
+      const int i = blockIdx.x - s.b * g.items_batch;
+      long long before = 0;
+      if (p.key_lens) {
+        for (int b = lane; b < s.b; b += 32) before += batch_units(g, key_tiles(p, g, b));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+      } else {
+        before = s.b * batch_units(g, key_tiles(p, g, 0));
+      }
+      const int tiles = key_tiles(p, g, s.b);
+      s.hk = i / (g.full + g.lone);
+      s.t = i - s.hk * (g.full + g.lone);
+      start = before + batch_units(g, tiles) / g.kv_heads * s.hk + (long long)s.t * tiles;
+    } else {
+      const long long cut = U * (blockIdx.x + 1) / G;
+      if (cut < U) {
+        s = find_spot(p, g, cut, lane);
+        start = cut - s.j;
+        if (s.j == 0 || U * blockIdx.x / G > start) start = -1;  // no cut, or not its first
+      }
+    }
+    if (lane == 0) {
+      s_start = start;
+      s_units = U;
+      s_spot = s;
+    }
+  }
+  __syncthreads();
+  const long long start = s_start, U = s_units;
+  if (start < 0) return;
+  const Spot s = s_spot;
+  const int tiles = key_tiles(p, g, s.b);
   const bool lone = s.t == g.full;
   const long long last = start + (lone ? (tiles + 1) >> 1 : tiles) - 1;
   const int c0 = (int)(((start + 1) * G - 1) / U), c1 = (int)(((last + 1) * G - 1) / U);
-  const int d = p.head_dim, ld = d + 2, count = c1 - c0 + 1;
-  auto part = [&](int c, int row) {
-    const int second = U * c / G < start;  // the item is the last of CTA c's run, not its first
-    return p.ws + ((size_t)(2 * c + second) * 256 + row) * (size_t)ld;
+  if (c0 == c1) return;  // one CTA had it whole
+  const int d = p.head_dim, ld = part_ld(d);
+  // the parts: CTA c's first item is in slot 2c, its last in 2c + 1; without units it has none
+  auto part = [&](int c) -> const float* {
+    const long long u0 = U * c / G;
+    if (u0 == U * (c + 1) / G) return nullptr;
+    return p.ws + (size_t)(2 * c + (u0 < start)) * g.slot_rows * (size_t)ld;
   };
-  for (int i = 0; i < 8; ++i) {
-    const bool shared_out = count > 8;
-    if (!shared_out && i > 0) break;
-    const int row = blockIdx.y * 8 + (shared_out ? i : warp);
+  auto place = [&](int row, int& n, int& head) {
     const int tile = lone ? 2 * g.full : 2 * s.t + (row >> 7), r = row & 127;
     const int gi = tile / g.n_tiles, rn = r / g.gt;
-    const int n = (tile - gi * g.n_tiles) * g.nt + rn, head = gi * g.gt + r - rn * g.gt;
-    const bool valid = rn < g.nt && n < p.q_len && head < g.group && !(lone && row >= 128);
-    if (!valid) {
-      if (shared_out) continue;
-      return;
-    }
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = c0 + (shared_out ? warp : 0); c <= c1; c += shared_out ? 8 : 1) {
-      const float* x = part(c, row);
-      if (U * c / G == U * (c + 1) / G) continue;  // a CTA without units
-      const float2 ml = *reinterpret_cast<const float2*>(x + d);
-      if (ml.y == 0.f) continue;
-      const float mn = fmaxf(m, ml.x), a = fast_exp2(m - mn), e = fast_exp2(ml.x - mn);
-      l = l * a + ml.y * e;
-      m = mn;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (lane + 32 * t < d) o[t] = o[t] * a + x[lane + 32 * t] * e;
-    }
-    if (shared_out) {
-      __syncthreads();  // the previous row's exchange has been read
-#pragma unroll
-      for (int t = 0; t < 4; ++t) s_o[warp][lane + 32 * t] = o[t];
-      if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-      }
-      __syncthreads();
-      if (warp != 0) continue;
-      m = -INFINITY;
-      for (int x = 0; x < 8; ++x) m = fmaxf(m, s_l[x] == 0.f ? -INFINITY : s_m[x]);
-      l = 0.f;
-      o[0] = o[1] = o[2] = o[3] = 0.f;
-      for (int x = 0; x < 8; ++x) {
-        if (s_l[x] == 0.f) continue;
-        const float e = fast_exp2(s_m[x] - m);
-        l += s_l[x] * e;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) o[t] += s_o[x][lane + 32 * t] * e;
-      }
-    }
+    n = (tile - gi * g.n_tiles) * g.nt + rn;
+    head = gi * g.gt + r - rn * g.gt;
+    return rn < g.nt && n < p.q_len && head < g.group && !(lone && row >= 128);
+  };
+  auto write = [&](int n, int head, int col, float4 o, float l) {
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     T* out = static_cast<T*>(p.out.data) + (long long)s.b * p.out.batch_stride + (long long)n * p.out.seq_stride +
-             (long long)(s.hk * g.group + head) * p.out.head_stride;
+             (long long)(s.hk * g.group + head) * p.out.head_stride + col;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+  };
+  if constexpr (!kByItem) {
+    constexpr int kRows = 32 / (8 * (32 / LPR));  // rows of a lane group
+    const int col = (lane % LPR) * 4;
+    float m[kRows], l[kRows];
+    float4 o[kRows];
+    int n[kRows], head[kRows];
+    bool ok[kRows];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      if (lane + 32 * t < d) out[lane + 32 * t] = from_f32<T>(o[t] * inv);
+    for (int i = 0; i < kRows; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+      o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      ok[i] = place(blockIdx.y * 32 + (i * 8 + warp) * (32 / LPR) + lane / LPR, n[i], head[i]) && col < d;
+    }
+    for (int c = c0; c <= c1; ++c) {
+      const float* base = part(c);
+      if (!base) continue;
+      float2 ml[kRows];
+      float4 x[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const float* r = base + (size_t)(blockIdx.y * 32 + (i * 8 + warp) * (32 / LPR) + lane / LPR) * ld;
+        ml[i] = ok[i] ? *reinterpret_cast<const float2*>(r + d) : make_float2(0.f, 0.f);
+        x[i] = ok[i] ? *reinterpret_cast<const float4*>(r + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        if (ml[i].y == 0.f) continue;
+        const float mn = fmaxf(m[i], ml[i].x), a = fast_exp2(m[i] - mn), e = fast_exp2(ml[i].x - mn);
+        l[i] = l[i] * a + ml[i].y * e;
+        m[i] = mn;
+        o[i] = make_float4(o[i].x * a + x[i].x * e, o[i].y * a + x[i].y * e, o[i].z * a + x[i].z * e,
+                           o[i].w * a + x[i].w * e);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (ok[i]) write(n[i], head[i], col, o[i], l[i]);
+  } else {
+    const int row = blockIdx.y, col = lane * 4;
+    int n, head;
+    if (!place(row, n, head)) return;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = c0 + warp; c <= c1; c += 8) {
+      const float* r = part(c);
+      float2 ml = make_float2(0.f, 0.f);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r) {
+        r += (size_t)row * ld;
+        ml = *reinterpret_cast<const float2*>(r + d);
+        if (col < d) x = *reinterpret_cast<const float4*>(r + col);
+      }
+      if (ml.y != 0.f) {
+        const float mn = fmaxf(m, ml.x), a = fast_exp2(m - mn), e = fast_exp2(ml.x - mn);
+        l = l * a + ml.y * e;
+        m = mn;
+        o = make_float4(o.x * a + x.x * e, o.y * a + x.y * e, o.z * a + x.z * e, o.w * a + x.w * e);
+      }
+    }
+    *reinterpret_cast<float4*>(&s_o[warp][col]) = o;
+    if (lane == 0) {
+      s_m[warp] = m;
+      s_l[warp] = l;
+    }
+    __syncthreads();
+    if (warp != 0 || col >= d) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) m = fmaxf(m, s_l[x] == 0.f ? -INFINITY : s_m[x]);
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      if (s_l[x] == 0.f) continue;
+      const float e = fast_exp2(s_m[x] - m);
+      const float4 v = *reinterpret_cast<const float4*>(&s_o[x][col]);
+      l += s_l[x] * e;
+      o = make_float4(o.x + v.x * e, o.y + v.y * e, o.z + v.z * e, o.w + v.w * e);
+    }
+    write(n, head, col, o, l);
   }
 }
 
@@ -785,35 +747,55 @@ Geom make_geom(int batch, int q_len, int k_len, int q_heads, int kv_heads, int h
   g.nt = 128 / g.gt;
   g.g_tiles = (g.group + g.gt - 1) / g.gt;
   g.n_tiles = (q_len + g.nt - 1) / g.nt;
-  const int tiles = g.g_tiles * g.n_tiles;
-  g.full = tiles / 2;
-  g.lone = tiles & 1;
   g.ksteps = (head_dim + 15) / 16;
-  const long long kt = (k_len + 127) / 128;
+  if ((long long)g.group * q_len <= kTokenRows) {
+    g.full = 1;  // one item a key head
+    g.tile_shift = 6;
+    g.slot_rows = kTokenRows;
+  } else {
+    const int tiles = g.g_tiles * g.n_tiles;
+    g.full = tiles / 2;
+    g.lone = tiles & 1;
+    g.tile_shift = 7;
+    g.slot_rows = 256;
+  }
+  g.items_batch = kv_heads * (g.full + g.lone);
+  const long long kt = (k_len + (1 << g.tile_shift) - 1) >> g.tile_shift;
   const long long units = (long long)batch * kv_heads * (g.full * kt + g.lone * ((kt + 1) / 2));
   g.contribs = (int)std::min<long long>(num_sms, std::max<long long>(units, 1));
   return g;
 }
 
-CUtensorMap seq_map(const HeadsView& v, int batch, int seq, int d, int rank5_group, int box_g, int box_n, int& batched,
-                    int& headed) {
-  // K / V: {d, seq, heads, batch}, boxes of 64 columns x 128 rows; Q: {d, group, seq, key
-  // heads, batch}, boxes of 64 x gt x nt.  A dimension walked with stride 0 is left out
-  // (extent 1, coordinate 0); a stride that is never walked only has to be a legal one.
-  batched = v.batch_stride != 0;
-  headed = v.head_stride != 0;
+// Whether the call's equal runs may cut an item (for ragged batches the device decides).
+bool may_cut(const Geom& g, int k_len, bool ragged) {
+  if (g.contribs <= 1) return false;
+  const long long kt = (k_len + (1 << g.tile_shift) - 1) >> g.tile_shift;
+  return ragged || kt > 1;
+}
+
+CUtensorMap query_map(const HeadsView& q, const CrossAttnParams& p, const Geom& g, int& batched) {
+  // {d, group, seq, key heads, batch} in boxes of 64 x gt x nt; see cross_kv_map on stride 0
+  batched = q.batch_stride != 0;
   auto st = [](long long s) { return (uint64_t)(s ? s * 2 : 16); };
-  if (rank5_group) {
-    const uint64_t dims[5] = {(uint64_t)d, (uint64_t)rank5_group, (uint64_t)seq, (uint64_t)(v.heads / rank5_group),
-                              batched ? (uint64_t)batch : 1};
-    const uint64_t str[4] = {st(v.head_stride), st(v.seq_stride), st(v.head_stride * rank5_group), st(v.batch_stride)};
-    const uint32_t box[5] = {64, (uint32_t)box_g, (uint32_t)box_n, 1, 1};
-    return make_tensor_map(v.data, 5, dims, str, box);
+  const uint64_t dims[5] = {(uint64_t)p.head_dim, (uint64_t)g.group, (uint64_t)p.q_len, (uint64_t)g.kv_heads,
+                            batched ? (uint64_t)p.batch : 1};
+  const uint64_t str[4] = {st(q.head_stride), st(q.seq_stride), st(q.head_stride * g.group), st(q.batch_stride)};
+  const uint32_t box[5] = {64, (uint32_t)g.gt, (uint32_t)g.nt, 1, 1};
+  return make_tensor_map(q.data, 5, dims, str, box);
+}
+
+template <typename T>
+cudaError_t launch_combine(const CrossAttnParams& p, const Geom& g, cudaStream_t s) {
+  const long long items = (long long)p.batch * g.items_batch;
+  const int rows = g.slot_rows == kTokenRows ? g.group * p.q_len : (g.full ? 256 : g.gt * std::min(g.nt, p.q_len));
+  LaunchScope scope("cross_combine", 0.0, 0.0, s);
+  if (items < g.contribs) {
+    DependentLaunch l(dim3((unsigned)items, rows), 256, 0, s);
+    return cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, 32, true>, p, g);
   }
-  const uint64_t dims[4] = {(uint64_t)d, (uint64_t)seq, headed ? (uint64_t)v.heads : 1, batched ? (uint64_t)batch : 1};
-  const uint64_t str[3] = {st(v.seq_stride), st(v.head_stride), st(v.batch_stride)};
-  const uint32_t box[4] = {64, 128, 1, 1};
-  return make_tensor_map(v.data, 4, dims, str, box);
+  DependentLaunch l(dim3(g.contribs - 1, (rows + 31) / 32), 256, 0, s);
+  return p.head_dim <= 64 ? cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, 16, false>, p, g)
+                          : cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, 32, false>, p, g);
 }
 
 template <typename T, int DP, bool kMask>
@@ -821,21 +803,12 @@ cudaError_t launch_k(const CrossAttnParams& p, Geom g, cudaStream_t s) {
   static std::atomic<unsigned long long> configured;
   cudaError_t e = ensure_smem_limit(cross_attention_kernel<T, DP, kMask>, (int)Cfg<DP>::kSmem, configured);
   if (e != cudaSuccess) return e;
-  int headed;
-  const CUtensorMap mq = seq_map(p.q, p.batch, p.q_len, p.head_dim, g.group, g.gt, g.nt, g.q_batched, headed);
-  const CUtensorMap mk = seq_map(p.k, p.batch, p.k_len, p.head_dim, 0, 0, 0, g.k_batched, g.k_headed);
-  const CUtensorMap mv = seq_map(p.v, p.batch, p.k_len, p.head_dim, 0, 0, 0, g.v_batched, g.v_headed);
+  const CUtensorMap mq = query_map(p.q, p, g, g.q_batched);
+  const CUtensorMap mk = cross_kv_map(p.k, p.batch, p.k_len, p.head_dim, 128, g.k_batched, g.k_headed);
+  const CUtensorMap mv = cross_kv_map(p.v, p.batch, p.k_len, p.head_dim, 128, g.v_batched, g.v_headed);
   const double rows = (double)p.batch * p.q_len * p.q.heads, keys = (double)p.batch * p.k_len * p.k.heads;
-  {
-    LaunchScope scope("cross_attention", 4.0 * rows * p.k_len * p.head_dim, 4.0 * (rows + keys) * p.head_dim, s);
-    cross_attention_kernel<T, DP, kMask><<<g.contribs, kThreads, Cfg<DP>::kSmem, s>>>(mq, mk, mv, p, g);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  }
-  if (g.contribs > 1) {
-    const int rows_max = g.full ? 256 : (int)std::min<long long>(128, (long long)g.gt * g.nt);
-    LaunchScope scope("cross_combine", 0.0, 0.0, s);
-    cross_combine_kernel<T><<<dim3(g.contribs - 1, (rows_max + 7) / 8), 256, 0, s>>>(p, g);
-  }
+  LaunchScope scope("cross_attention", 4.0 * rows * p.k_len * p.head_dim, 4.0 * (rows + keys) * p.head_dim, s);
+  cross_attention_kernel<T, DP, kMask><<<g.contribs, kThreads, Cfg<DP>::kSmem, s>>>(mq, mk, mv, p, g);
   return cudaGetLastError();
 }
 
@@ -848,8 +821,15 @@ cudaError_t launch_t(const CrossAttnParams& p, int num_sms, cudaStream_t s) {
     return cudaGetLastError();
   }
   const Geom g = make_geom(p.batch, p.q_len, p.k_len, p.q.heads, p.k.heads, p.head_dim, num_sms);
-  if (p.head_dim <= 64) return p.key_mask ? launch_k<T, 64, true>(p, g, s) : launch_k<T, 64, false>(p, g, s);
-  return p.key_mask ? launch_k<T, 128, true>(p, g, s) : launch_k<T, 128, false>(p, g, s);
+  cudaError_t e;
+  if (g.slot_rows == kTokenRows)
+    e = launch_cross_token<T>(p, g, s);
+  else if (p.head_dim <= 64)
+    e = p.key_mask ? launch_k<T, 64, true>(p, g, s) : launch_k<T, 64, false>(p, g, s);
+  else
+    e = p.key_mask ? launch_k<T, 128, true>(p, g, s) : launch_k<T, 128, false>(p, g, s);
+  if (e != cudaSuccess || !may_cut(g, p.k_len, p.key_lens != nullptr)) return e;
+  return launch_combine<T>(p, g, s);
 }
 
 }  // namespace
@@ -858,7 +838,19 @@ long long cross_attention_workspace(int batch, int q_len, int k_len, int q_heads
                                     int num_sms) {
   if (batch == 0 || q_len == 0 || k_len == 0) return 0;
   const Geom g = make_geom(batch, q_len, k_len, q_heads, kv_heads, head_dim, num_sms);
-  return g.contribs > 1 ? 2LL * g.contribs * 256 * (head_dim + 2) * 4 : 0;
+  return g.contribs > 1 ? 2LL * g.contribs * g.slot_rows * part_ld(head_dim) * 4 : 0;
+}
+
+// A dimension walked with stride 0 is left out (extent 1, coordinate 0); a stride that is
+// never walked only has to be a legal one.
+CUtensorMap cross_kv_map(const HeadsView& v, int batch, int seq, int d, int box_rows, int& batched, int& headed) {
+  batched = v.batch_stride != 0;
+  headed = v.head_stride != 0;
+  auto st = [](long long s) { return (uint64_t)(s ? s * 2 : 16); };
+  const uint64_t dims[4] = {(uint64_t)d, (uint64_t)seq, headed ? (uint64_t)v.heads : 1, batched ? (uint64_t)batch : 1};
+  const uint64_t str[3] = {st(v.seq_stride), st(v.head_stride), st(v.batch_stride)};
+  const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1};
+  return make_tensor_map(v.data, 4, dims, str, box);
 }
 
 cudaError_t launch_cross_attention(const CrossAttnParams& p, int bf16, int num_sms, cudaStream_t stream) {

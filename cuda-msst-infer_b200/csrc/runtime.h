@@ -170,11 +170,13 @@ unsigned kernels_device_error(bool clear);
 unsigned band_attention_device_error(bool clear);
 unsigned qk_norm_device_error(bool clear);
 unsigned cross_attn_device_error(bool clear);
+unsigned cross_token_device_error(bool clear);
 unsigned adapter_gemm_device_error(bool clear);
 
 inline unsigned device_error(bool clear) {
   return gemm_device_error(clear) | attention_device_error(clear) | kernels_device_error(clear) |
          band_attention_device_error(clear) | qk_norm_device_error(clear) | cross_attn_device_error(clear) |
+         cross_token_device_error(clear) |
          adapter_gemm_device_error(clear);
 }
 
