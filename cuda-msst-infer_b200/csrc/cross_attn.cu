@@ -340,16 +340,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               bool touched = false;
 #pragma unroll
               for (int ch = 0; ch < 4; ++ch) {
-                bool keep = ch * 32 + lane < khi;
-                if (kMask && keep) keep = p.key_mask[(size_t)k.s.b * p.k_len + key0 + ch * 32 + lane] != 0;
+                const int row = ch * 32 + lane;
+                bool keep = row < khi;
+                if (kMask && keep) keep = p.key_mask[(size_t)k.s.b * p.k_len + key0 + row] != 0;
                 const uint32_t word = __ballot_sync(0xffffffffu, keep);
                 if (kMask && lane == 0) s_words[slot * 4 + ch] = word;
-                for (uint32_t out = ~word; out; out &= out - 1) {
-                  const int row = ch * 32 + __ffs(out) - 1;
-                  if (lane < 8 * C::kHalves)
-                    *reinterpret_cast<uint4*>(sKV + slot * C::kTile + (lane >> 3) * kHalfBytes + row * 128 +
-                                              (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                  touched = true;
+                if (word == 0xffffffffu) continue;
+                touched = true;
+                if (!keep) {
+                  // a lane's row, its pieces in an order that keeps the lanes on different banks
+                  uint8_t* at = sKV + slot * C::kTile + row * 128;
+#pragma unroll
+                  for (int x = 0; x < 8 * C::kHalves; ++x)
+                    *reinterpret_cast<uint4*>(at + (x >> 3) * kHalfBytes + (((x + lane) & 7) << 4)) =
+                        make_uint4(0u, 0u, 0u, 0u);
                 }
               }
               if (touched) fence_proxy_async_smem();
@@ -508,8 +512,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (warp_active) {
         T* out = static_cast<T*>(p.out.data) + (long long)k.s.b * p.out.batch_stride +
                  (long long)n * p.out.seq_stride + (long long)(k.s.hk * g.group + head) * p.out.head_stride;
-        const size_t part = (size_t)(2 * blockIdx.x + (k.seg > 0)) * g.slot_rows + (k.lone ? 0 : w * 128) + row;
-        float* po = p.ws + part * (size_t)part_ld(p.head_dim);
+        // partial results go column by column, so that a warp's stores are contiguous
+        float* po = p.ws + (size_t)(2 * blockIdx.x + (k.seg > 0)) * g.slot_rows * part_ld(p.head_dim) +
+                    (k.lone ? 0 : w * 128) + row;
         for (int c0 = c_lo; c0 < c_hi; c0 += 16) {
           uint32_t r0[16], r1[16];
           tmem_ld16(src0 + c0, r0);
@@ -531,14 +536,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                                pack2<T>(v[8 * u + 4], v[8 * u + 5]), pack2<T>(v[8 * u + 6], v[8 * u + 7]));
               } else {
 #pragma unroll
-                for (int i = 0; i < 8; i += 2)
-                  *reinterpret_cast<float2*>(po + c0 + 8 * u + i) = make_float2(v[8 * u + i], v[8 * u + i + 1]);
+                for (int i = 0; i < 8; ++i) po[(c0 + 8 * u + i) * 256] = v[8 * u + i];
               }
             }
           }
         }
-        if (!whole && valid && (!k.lone || w == 0))
-          *reinterpret_cast<float2*>(po + p.head_dim) = make_float2(ref, l);
+        if (!whole && valid && (!k.lone || w == 0)) {
+          po[p.head_dim * 256] = ref;
+          po[(p.head_dim + 1) * 256] = l;
+        }
       }
       tc_fence_before();
       if (k.lone) {
@@ -560,19 +566,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Joins the partial results of the items that span CTAs, in CTA order.
 //
-// kByItem false (at least as many items as CTAs, so a cut item has two or three parts):
-// block (x, y) takes the item that the boundary between CTAs x and x + 1 cuts, if it is that
-// item's first cut, and rows [32 y, 32 y + 32) of it, LPR lanes a row, every load of a
-// warp's rows issued before the first use.
-// kByItem true (an item may span every CTA): block (x, y) takes item x and its row y, and the
-// 8 warps share the parts out.
-template <typename T, int LPR, bool kByItem>
-__global__ void __launch_bounds__(256)
+// kByItem false (at least as many items as CTAs, so a cut item has two or three parts): block
+// x takes the item that the boundary between CTAs x and x + 1 cuts, if it is that item's
+// first cut.  kByItem true (an item may span every CTA): block x takes item x.
+// Slots of 256 rows (column by column): block (x, y, z) joins columns [8 z, 8 z + 8), a lane a
+// row; with kByItem kShare warps share the parts of rows [32 y, 32 y + 32) out, else 8 warps
+// take 32 rows each.  Slots of 16 rows (row by row, cross_token.cu): block (x, y) joins row y,
+// 4 columns a lane, its kShare = 8 warps sharing the parts out.
+template <typename T, bool kByItem, bool kToken, int kShare>
+__global__ void __launch_bounds__(kShare > 1 ? 32 * kShare : 256)
     cross_combine_kernel(const __grid_constant__ CrossAttnParams p, const __grid_constant__ Geom g) {
   __shared__ long long s_start, s_units;
   __shared__ Spot s_spot;
-  __shared__ __align__(16) float s_o[8][128];  // read and written 16 bytes at a time
-  __shared__ float s_m[8], s_l[8];
+  __shared__ int s_c0, s_c1;
+  // sums, references and columns of the warps that share an item's parts out
+  __shared__ __align__(16) float s_o[kShare][kToken ? 128 : 8 * 32];
+  __shared__ float s_m[kShare][32], s_l[kShare][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long G = g.contribs;
   wait_for_previous();
@@ -608,17 +617,21 @@ __global__ void __launch_bounds__(256)
       s_start = start;
       s_units = U;
       s_spot = s;
+      s_c0 = s_c1 = 0;
+      if (start >= 0) {
+        const int tiles = key_tiles(p, g, s.b);
+        const long long last = start + (s.t == g.full ? (tiles + 1) >> 1 : tiles) - 1;
+        s_c0 = (int)(((start + 1) * G - 1) / U);
+        s_c1 = (int)(((last + 1) * G - 1) / U);
+      }
     }
   }
   __syncthreads();
   const long long start = s_start, U = s_units;
-  if (start < 0) return;
+  const int c0 = s_c0, c1 = s_c1;
+  if (c0 == c1) return;  // no cut, or one CTA had it whole
   const Spot s = s_spot;
-  const int tiles = key_tiles(p, g, s.b);
   const bool lone = s.t == g.full;
-  const long long last = start + (lone ? (tiles + 1) >> 1 : tiles) - 1;
-  const int c0 = (int)(((start + 1) * G - 1) / U), c1 = (int)(((last + 1) * G - 1) / U);
-  if (c0 == c1) return;  // one CTA had it whole
   const int d = p.head_dim, ld = part_ld(d);
   // the parts: CTA c's first item is in slot 2c, its last in 2c + 1; without units it has none
   auto part = [&](int c) -> const float* {
@@ -626,6 +639,7 @@ __global__ void __launch_bounds__(256)
     if (u0 == U * (c + 1) / G) return nullptr;
     return p.ws + (size_t)(2 * c + (u0 < start)) * g.slot_rows * (size_t)ld;
   };
+  // token and head of a row of the item, and whether it is one
   auto place = [&](int row, int& n, int& head) {
     const int tile = lone ? 2 * g.full : 2 * s.t + (row >> 7), r = row & 127;
     const int gi = tile / g.n_tiles, rn = r / g.gt;
@@ -633,95 +647,91 @@ __global__ void __launch_bounds__(256)
     head = gi * g.gt + r - rn * g.gt;
     return rn < g.nt && n < p.q_len && head < g.group && !(lone && row >= 128);
   };
-  auto write = [&](int n, int head, int col, float4 o, float l) {
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    T* out = static_cast<T*>(p.out.data) + (long long)s.b * p.out.batch_stride + (long long)n * p.out.seq_stride +
-             (long long)(s.hk * g.group + head) * p.out.head_stride + col;
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+  auto target = [&](int n, int head, int col) {
+    return static_cast<T*>(p.out.data) + (long long)s.b * p.out.batch_stride + (long long)n * p.out.seq_stride +
+           (long long)(s.hk * g.group + head) * p.out.head_stride + col;
   };
-  if constexpr (!kByItem) {
-    constexpr int kRows = 32 / (8 * (32 / LPR));  // rows of a lane group
-    const int col = (lane % LPR) * 4;
-    float m[kRows], l[kRows];
-    float4 o[kRows];
-    int n[kRows], head[kRows];
-    bool ok[kRows];
+  constexpr int kCols = kToken ? 4 : 8;
+  const int row = kToken ? blockIdx.y : blockIdx.y * (kByItem ? 32 : 256) + (kByItem ? 0 : warp * 32) + lane;
+  const int col = kToken ? lane * 4 : blockIdx.z * 8;
+  int n, head;
+  const bool valid = place(row, n, head) && col < d;
+  float m = -INFINITY, l = 0.f, o[kCols];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      m[i] = -INFINITY;
-      l[i] = 0.f;
-      o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      ok[i] = place(blockIdx.y * 32 + (i * 8 + warp) * (32 / LPR) + lane / LPR, n[i], head[i]) && col < d;
-    }
-    for (int c = c0; c <= c1; ++c) {
-      const float* base = part(c);
-      if (!base) continue;
-      float2 ml[kRows];
-      float4 x[kRows];
+  for (int i = 0; i < kCols; ++i) o[i] = 0.f;
+#pragma unroll 2
+  for (int c = c0 + (kShare > 1 ? warp : 0); c <= c1; c += kShare) {
+    const float* r = part(c);
+    if (!r || !valid) continue;
+    float pm, pl, x[kCols];
+    if constexpr (kToken) {
+      r += (size_t)row * ld;
+      const float2 ml = *reinterpret_cast<const float2*>(r + d);
+      pm = ml.x, pl = ml.y;
+      *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(r + col);
+    } else {
+      pm = r[d * 256 + row];
+      pl = r[(d + 1) * 256 + row];
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        const float* r = base + (size_t)(blockIdx.y * 32 + (i * 8 + warp) * (32 / LPR) + lane / LPR) * ld;
-        ml[i] = ok[i] ? *reinterpret_cast<const float2*>(r + d) : make_float2(0.f, 0.f);
-        x[i] = ok[i] ? *reinterpret_cast<const float4*>(r + col) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+      for (int i = 0; i < kCols; ++i) x[i] = r[(col + i) * 256 + row];
+    }
+    if (pl == 0.f) continue;  // no kept key in that part
+    const float mn = fmaxf(m, pm), a = fast_exp2(m - mn), e = fast_exp2(pm - mn);
+    l = l * a + pl * e;
+    m = mn;
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        if (ml[i].y == 0.f) continue;
-        const float mn = fmaxf(m[i], ml[i].x), a = fast_exp2(m[i] - mn), e = fast_exp2(ml[i].x - mn);
-        l[i] = l[i] * a + ml[i].y * e;
-        m[i] = mn;
-        o[i] = make_float4(o[i].x * a + x[i].x * e, o[i].y * a + x[i].y * e, o[i].z * a + x[i].z * e,
-                           o[i].w * a + x[i].w * e);
-      }
+    for (int i = 0; i < kCols; ++i) o[i] = o[i] * a + x[i] * e;
+  }
+  if constexpr (kShare > 1) {
+    const int at = kToken ? 0 : lane;  // a warp's rows
+    if (!kToken || lane == 0) {
+      s_m[warp][at] = m;
+      s_l[warp][at] = l;
     }
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
-      if (ok[i]) write(n[i], head[i], col, o[i], l[i]);
-  } else {
-    const int row = blockIdx.y, col = lane * 4;
-    int n, head;
-    if (!place(row, n, head)) return;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0 + warp; c <= c1; c += 8) {
-      const float* r = part(c);
-      float2 ml = make_float2(0.f, 0.f);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r) {
-        r += (size_t)row * ld;
-        ml = *reinterpret_cast<const float2*>(r + d);
-        if (col < d) x = *reinterpret_cast<const float4*>(r + col);
-      }
-      if (ml.y != 0.f) {
-        const float mn = fmaxf(m, ml.x), a = fast_exp2(m - mn), e = fast_exp2(ml.x - mn);
-        l = l * a + ml.y * e;
-        m = mn;
-        o = make_float4(o.x * a + x.x * e, o.y * a + x.y * e, o.z * a + x.z * e, o.w * a + x.w * e);
-      }
-    }
-    *reinterpret_cast<float4*>(&s_o[warp][col]) = o;
-    if (lane == 0) {
-      s_m[warp] = m;
-      s_l[warp] = l;
-    }
+    for (int i = 0; i < kCols; ++i) s_o[warp][kToken ? col + i : i * 32 + lane] = o[i];
     __syncthreads();
-    if (warp != 0 || col >= d) return;
+    // the first kCols warps (row-by-row slots: the first one) add up
+    if (warp >= (kToken ? 1 : kCols)) return;
     m = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) m = fmaxf(m, s_l[x] == 0.f ? -INFINITY : s_m[x]);
+    for (int x = 0; x < kShare; ++x) m = fmaxf(m, s_l[x][at] == 0.f ? -INFINITY : s_m[x][at]);
     l = 0.f;
-    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum[kCols];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      if (s_l[x] == 0.f) continue;
-      const float e = fast_exp2(s_m[x] - m);
-      const float4 v = *reinterpret_cast<const float4*>(&s_o[x][col]);
-      l += s_l[x] * e;
-      o = make_float4(o.x + v.x * e, o.y + v.y * e, o.z + v.z * e, o.w + v.w * e);
+    for (int i = 0; i < kCols; ++i) sum[i] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kShare; ++x) {
+      if (s_l[x][at] == 0.f) continue;
+      const float e = fast_exp2(s_m[x][at] - m);
+      l += s_l[x][at] * e;
+      if constexpr (kToken) {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) sum[i] += s_o[x][col + i] * e;
+      } else {
+        sum[0] += s_o[x][warp * 32 + lane] * e;
+      }
     }
-    write(n, head, col, o, l);
+    if constexpr (kToken) {
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) o[i] = sum[i];
+    } else {
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the kCols warps have read the shares
+      s_o[0][warp * 32 + lane] = sum[0];
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (warp != 0) return;
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) o[i] = s_o[0][i * 32 + lane];
+    }
   }
+  if (!valid) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  T* out = target(n, head, col);
+  if constexpr (kToken)
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+  else
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv),
+                                                pack2<T>(o[4] * inv, o[5] * inv), pack2<T>(o[6] * inv, o[7] * inv));
 }
 
 // No key at all: every row is zero.
@@ -787,15 +797,21 @@ CUtensorMap query_map(const HeadsView& q, const CrossAttnParams& p, const Geom& 
 template <typename T>
 cudaError_t launch_combine(const CrossAttnParams& p, const Geom& g, cudaStream_t s) {
   const long long items = (long long)p.batch * g.items_batch;
-  const int rows = g.slot_rows == kTokenRows ? g.group * p.q_len : (g.full ? 256 : g.gt * std::min(g.nt, p.q_len));
+  const bool by_item = items < g.contribs;
+  const unsigned x = (unsigned)(by_item ? items : g.contribs - 1);
   LaunchScope scope("cross_combine", 0.0, 0.0, s);
-  if (items < g.contribs) {
-    DependentLaunch l(dim3((unsigned)items, rows), 256, 0, s);
-    return cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, 32, true>, p, g);
+  if (g.slot_rows == kTokenRows) {
+    DependentLaunch l(dim3(x, g.group * p.q_len), 256, 0, s);
+    return by_item ? cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, true, true, 8>, p, g)
+                   : cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, false, true, 8>, p, g);
   }
-  DependentLaunch l(dim3(g.contribs - 1, (rows + 31) / 32), 256, 0, s);
-  return p.head_dim <= 64 ? cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, 16, false>, p, g)
-                          : cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, 32, false>, p, g);
+  const int rows = g.full ? 256 : g.gt * std::min(g.nt, p.q_len);
+  // an item has about contribs / items parts: more warps to share them where there are many
+  const int share = !by_item ? 1 : (g.contribs / items < 16 ? 8 : 32);
+  DependentLaunch l(dim3(x, by_item ? (rows + 31) / 32 : 1, p.head_dim / 8), share > 1 ? 32 * share : 256, 0, s);
+  return share == 1 ? cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, false, false, 1>, p, g)
+         : share == 8 ? cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, true, false, 8>, p, g)
+                      : cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, true, false, 32>, p, g);
 }
 
 template <typename T, int DP, bool kMask>
@@ -850,7 +866,13 @@ CUtensorMap cross_kv_map(const HeadsView& v, int batch, int seq, int d, int box_
   const uint64_t dims[4] = {(uint64_t)d, (uint64_t)seq, headed ? (uint64_t)v.heads : 1, batched ? (uint64_t)batch : 1};
   const uint64_t str[3] = {st(v.seq_stride), st(v.head_stride), st(v.batch_stride)};
   const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1};
-  return make_tensor_map(v.data, 4, dims, str, box);
+  // What a DRAM read may bring into L2 beside the bytes asked for: no more than a key's row,
+  // where the next bytes are another head's, which another CTA reads at another time
+  const bool dense = v.seq_stride == d;
+  return make_tensor_map(v.data, 4, dims, str, box, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_128B,
+                         dense || d >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                                           : (d >= 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                                      : CU_TENSOR_MAP_L2_PROMOTION_L2_64B));
 }
 
 cudaError_t launch_cross_attention(const CrossAttnParams& p, int bf16, int num_sms, cudaStream_t stream) {

@@ -137,7 +137,7 @@ struct Walk {
 
 // Partial results of the items that span CTAs: CTA c's first item in slot 2c, its last in
 // slot 2c + 1, each slot_rows rows of head_dim values of O, the reference (log2) and the
-// sum; rows are head_dim + 4 floats apart (16-byte rows).
+// sum: row by row, head_dim + 4 floats apart, for 16 rows; column by column for 256.
 __host__ __device__ inline int part_ld(int head_dim) { return head_dim + 4; }
 
 // cross_token.cu: up to 16 query rows a key head.

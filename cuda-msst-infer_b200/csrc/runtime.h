@@ -95,7 +95,8 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 inline CUtensorMap make_tensor_map(const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
                                    const uint32_t* box,
                                    CUtensorMapDataType dtype = CU_TENSOR_MAP_DATA_TYPE_UINT16,
-                                   CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+                                   CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B,
+                                   CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
   CUtensorMap m;
   cuuint64_t d[5];
   cuuint64_t s[4];
@@ -107,7 +108,7 @@ inline CUtensorMap make_tensor_map(const void* base, int rank, const uint64_t* d
   }
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides_bytes[i];
   CUresult r = tensor_map_encoder()(&m, dtype, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, e,
-                                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) fail(MSST_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
   return m;
