@@ -102,6 +102,25 @@ inline cudaError_t ensure_smem_limit(K kern, int bytes, std::atomic<unsigned lon
   return e;
 }
 
+// Launch configuration whose kernel may start before the previous one on the stream has
+// ended; the kernel waits (griddepcontrol.wait) before it reads that one's results.
+struct DependentLaunch {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[1];
+  DependentLaunch(dim3 grid, dim3 block, size_t smem, cudaStream_t s) {
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+  }
+};
+__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------
 // mbarrier
 // ---------------------------------------------------------------------------

@@ -148,23 +148,4 @@ cudaError_t launch_cross_token(const CrossAttnParams& p, Geom g, cudaStream_t s)
 // cross_attn.cu: a tensor map over k or v in boxes of 64 columns x box_rows keys.
 CUtensorMap cross_kv_map(const HeadsView& v, int batch, int seq, int d, int box_rows, int& batched, int& headed);
 
-// Launch configuration whose kernel may start before the previous one on the stream has
-// ended; the kernel waits (griddepcontrol.wait) before it reads that one's results.
-struct DependentLaunch {
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute at[1];
-  DependentLaunch(dim3 grid, dim3 block, size_t smem, cudaStream_t s) {
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-  }
-};
-__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 }  // namespace msst
