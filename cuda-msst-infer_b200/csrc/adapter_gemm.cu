@@ -5,17 +5,19 @@
 // adapter; adapter_gemm_kernel computes W x and adds B_a (s_a u) as a few more K steps
 // of the same accumulators, so the low-rank term costs no pass over the output.
 //
-// Both work on tiles of BT rows (32 to 256) and on the list of the distinct adapters
+// The second works on row tiles (32 to 128 rows) and on the list of the distinct adapters
 // of a tile.  An adapter's part of the extra K steps is a slice of 16 rank values
 // (ceil(rank / 16) slices an adapter): B_a's columns on one side, on the other U', which
 // holds s_a u for the rows whose adapter is a and zeros for all others.  So requests
 // may be mixed row by row: a tile costs as many slices as it has adapters.
 //
-// The weights are the MMA's M side (128 of their rows) and the rows of x its N side: with
-// few rows the instruction then still covers 4 KB of weights, where an M side of rows
-// would be padded to 128 and the one issuing thread, at about 60 cycles an MMA, would
-// bound the pass (K = N = 4096: 8 us of issue for 32 columns a CTA, against the 5.2 us
-// that reading W takes).  Few tiles are split along K over a cluster, whose CTAs add
+// Up to 128 rows the weights are the MMA's M side (128 of their rows) and the rows of x its N
+// side: the instruction then covers 4 KB of weights, where an M side of rows would be
+// padded to 128 and the one issuing thread, at about 60 cycles an MMA, would bound the pass
+// (K = N = 4096: 8 us of issue for 32 columns a CTA, against the 5.2 us that reading W
+// takes).  More rows are the M side and 256 weight rows the N side, so that a lane of the
+// epilogue holds consecutive output columns (with the rows on the N side its 2-byte stores
+// kept 48060 x 1536 outputs at 103 us).  Few tiles are split along K over a cluster, whose CTAs add
 // their parts through distributed shared memory in rank order.
 //
 // u is rounded to the operands' 16 bits once, as U' feeds the tensor cores; it is summed
@@ -30,17 +32,17 @@ namespace msst {
 
 namespace {
 
-constexpr uint32_t kWTile = 128 * 128;       // 128 weight rows x 64 columns of 16 bits
 constexpr int kSliceRows = 16;               // rank values of a slice
 
 // The plan of a call, the same for both launches.
 struct Plan {
+  int rows_on_m;    // second launch: rows of x on the MMA's M side
   int bt;           // rows of x a tile
   int tiles;        // ceil(rows / bt)
-  int n_tiles;      // ceil(N / 128)
+  int n_tiles;      // ceil(N / weight rows a tile)
   int kblocks;      // ceil(K / 64)
   int chunks;       // slices an adapter
-  // first launch: CTAs along the rows (of 32 * 8 / down_kw rows), along a tile's adapters and
+  // first launch: CTAs along the rows (of 32 * kDownWarps / down_kw rows), along a tile's adapters and
   // along K; warps of a CTA along K; 8-value rank pieces of a pass
   int down_x, down_y, down_split, down_kw, down_nt;
   int split;        // CTAs of a cluster along K in the second launch
@@ -61,11 +63,11 @@ __device__ __forceinline__ int row_id(const AdapterGemmParams& p, long long t) {
 
 // ---------------------------------------------------------------------------
 // First launch: u[t] = A_a x[t].  Bound: reading x once (and, for few rows, the adapters' A_a).
-// mma.sync m16n8k16 on fragments loaded straight from global memory: a lane takes 8
-// consecutive columns of a row (16 bytes; four lanes read 64 consecutive bytes), which serve
-// two K steps, x and A_a in the same order.  No barrier, no staging: a launch this short
-// is bound by latency, and many small CTAs hide it best.  (A tcgen05 form with 128-row A
-// slices took 35 us for 8192 rows of 4096 columns, mostly set-up and drain.)
+// mma.sync m16n8k16; each warp streams its rows through a ring of its own in shared memory
+// (cp.async, whole 128-byte lines, three stages of 64 columns in flight: up to 144 KB an SM) and
+// takes A_a, which stays in L2, straight from global memory one step ahead.  No barrier
+// until the end.  (Forms that held x in registers kept too little in flight: 37 us for
+// 8192 rows of 4096 columns; a tcgen05 form with 128-row slices of A_a took 35 us.)
 // A warp owns 32 rows; the warps of a CTA split K (down_kw of them) and rows.  For every
 // distinct adapter of its rows it computes all 32 x rank products from the rows that have
 // the adapter and keeps those.
@@ -88,7 +90,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 
 // The list of row tile `tile`: its adapters in order of first appearance.
 __device__ void write_list(const AdapterGemmParams& p, const Plan& pl, int tile) {
-  __shared__ int s_id[256], s_count[8], s_mixed;
+  __shared__ int s_id[128], s_count[4], s_mixed;
   const int r = threadIdx.x, warp = r >> 5, lane = r & 31;
   const long long t = (long long)tile * pl.bt + r;
   const bool in = r < pl.bt && t < p.rows;
@@ -104,7 +106,7 @@ __device__ void write_list(const AdapterGemmParams& p, const Plan& pl, int tile)
   if (lane == 0) s_count[warp] = __popc(firsts);
   __syncthreads();
   int at = __popc(firsts & ((1u << lane) - 1u)), count = 0;
-  for (int x = 0; x < 8; ++x) {
+  for (int x = 0; x < 4; ++x) {
     if (x < warp) at += s_count[x];
     count += s_count[x];
   }
@@ -116,62 +118,107 @@ __device__ void write_list(const AdapterGemmParams& p, const Plan& pl, int tile)
   }
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+
+constexpr int kDownWarps = 4;
+constexpr int kDownStages = 4;
+constexpr uint32_t kDownStage = 32 * 128;  // 32 rows x 64 columns
+constexpr int kDownSmem = kDownWarps * kDownStages * (int)kDownStage;  // three CTAs an SM
+
 template <typename T, int NT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(32 * kDownWarps)
     adapter_down_kernel(const __grid_constant__ AdapterGemmParams p, const __grid_constant__ Plan pl) {
-  extern __shared__ __align__(16) float s_part[];  // [8 warps][32 rows][NT * 8]
+  extern __shared__ __align__(128) uint8_t s_ring[];  // [warps][stages][32 rows][128 bytes]
   dependents_may_start();
   if (blockIdx.x >= pl.down_x) {
     if (blockIdx.y == 0 && blockIdx.z == 0) write_list(p, pl, blockIdx.x - pl.down_x);
     return;
   }
   constexpr int kR = NT * 8;
+  static_assert(32 * kR * 4 <= kDownStages * kDownStage, "the results reuse the ring");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kw = pl.down_kw, kwarp = warp % kw, group = warp / kw;
-  const long long t0 = ((long long)blockIdx.x * (8 / kw) + group) * 32;
+  const long long t0 = ((long long)blockIdx.x * (kDownWarps / kw) + group) * 32;
   if (t0 >= p.rows) return;
   const int id = row_id(p, t0 + lane);
   const unsigned same = __match_any_sync(0xffffffffu, id);
   unsigned firsts = __ballot_sync(0xffffffffu, id >= 0 && __ffs(same) - 1 == lane);
-  const int steps = (p.K + 31) / 32, parts = pl.down_split * kw, me = blockIdx.z * kw + kwarp;
+  const int steps = (p.K + 63) / 64, parts = pl.down_split * kw, me = blockIdx.z * kw + kwarp;
   const int s0 = (int)((long long)steps * me / parts), s1 = (int)((long long)steps * (me + 1) / parts);
   const int row = lane >> 2, quad = lane & 3;
-  const T* x = static_cast<const T*>(p.x) + t0 * p.ldx + quad * 8;
+  uint8_t* ring = s_ring + (size_t)warp * kDownStages * kDownStage;
+  const uint32_t ring_u = smem_u32(ring);
+  // copies: 8 lanes a row's 128 bytes; pieces of odd rows swap halves, so that the reads
+  // below (8 rows x 4 pieces at a time) meet no bank twice
+  const int crow = lane >> 3, cpiece = lane & 7;
   for (int li = 0; firsts; ++li, firsts &= firsts - 1) {
     if (li % pl.down_y != blockIdx.y) continue;
     const int src = __ffs(firsts) - 1;
     const int a = __shfl_sync(0xffffffffu, id, src);
     const unsigned mine = __shfl_sync(0xffffffffu, same, src);  // the rows that have adapter a
     for (int r0 = 0; r0 < p.rank; r0 += kR) {
-      const T* la = static_cast<const T*>(p.lora_a) + ((size_t)a * p.rank + r0) * p.K + quad * 8;
+      auto fetch = [&](int s) {
+        if (s < s1) {
+          const uint32_t dst = ring_u + (uint32_t)(s % kDownStages) * kDownStage;
+          const T* x = static_cast<const T*>(p.x) + t0 * p.ldx + s * 64 + cpiece * 8;
+          const bool in = s * 64 + cpiece * 8 < p.K;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + crow;
+            const bool take = in && (mine >> r & 1);
+            cp_async16(dst + (uint32_t)(r * 128 + ((cpiece ^ (r & 1) << 2) << 4)), take ? x + r * p.ldx : p.x, take);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      const T* la = static_cast<const T*>(p.lora_a) + ((size_t)a * p.rank + r0 + row) * p.K + quad * 8;
+      // this lane's 8 columns of each 32 of step s, rank values j * 8 + row
+      auto load_a = [&](int s, uint4 (&v)[2][NT]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            v[h][j] = make_uint4(0u, 0u, 0u, 0u);
+            if (s < s1 && s * 64 + h * 32 + quad * 8 < p.K && r0 + j * 8 < p.rank)
+              v[h][j] = __ldg(reinterpret_cast<const uint4*>(la + (size_t)j * 8 * p.K + s * 64 + h * 32));
+          }
+      };
       float acc[2][NT][4];
 #pragma unroll
       for (int i = 0; i < 2 * NT * 4; ++i) (&acc[0][0][0])[i] = 0.f;
-#pragma unroll 2
+#pragma unroll
+      for (int i = 0; i < kDownStages - 1; ++i) fetch(s0 + i);
+      uint4 next[2][NT];
+      load_a(s0, next);
       for (int s = s0; s < s1; ++s) {
-        const bool in = s * 32 + quad * 8 < p.K;
-        uint4 xv[4], av[NT];
+        uint4 av[2][NT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          xv[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (in && (mine >> (row + 8 * i) & 1))
-            xv[i] = *reinterpret_cast<const uint4*>(x + (row + 8 * i) * p.ldx + s * 32);
+        for (int i = 0; i < 2 * NT; ++i) (&av[0][0])[i] = (&next[0][0])[i];
+        load_a(s + 1, next);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDownStages - 2) : "memory");
+        __syncwarp();
+        const uint8_t* st = ring + (s % kDownStages) * kDownStage;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint4 xv[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            xv[i] = *reinterpret_cast<const uint4*>(st + (row + 8 * i) * 128 + (((h * 4 + quad) ^ (row & 1) << 2) << 4));
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint4 &x0 = xv[2 * i], &x1 = xv[2 * i + 1], &w = av[h][j];
+              mma16816<T>(acc[i][j], x0.x, x1.x, x0.y, x1.y, w.x, w.y);
+              mma16816<T>(acc[i][j], x0.z, x1.z, x0.w, x1.w, w.z, w.w);
+            }
         }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          av[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (in && r0 + j * 8 < p.rank)
-            av[j] = __ldg(reinterpret_cast<const uint4*>(la + (size_t)(j * 8 + row) * p.K + s * 32));
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma16816<T>(acc[i][j], xv[2 * i].x, xv[2 * i + 1].x, xv[2 * i].y, xv[2 * i + 1].y, av[j].x, av[j].y);
-            mma16816<T>(acc[i][j], xv[2 * i].z, xv[2 * i + 1].z, xv[2 * i].w, xv[2 * i + 1].w, av[j].z, av[j].w);
-          }
+        __syncwarp();
+        fetch(s + kDownStages - 1);  // into the stage read in the last step
       }
-      float* part = s_part + (size_t)warp * 32 * kR;
+      float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -182,14 +229,14 @@ __global__ void __launch_bounds__(256)
         }
       // the warps that share these rows meet; their parts are added in K order
       asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(kw * 32) : "memory");
-      const float* parts0 = s_part + (size_t)group * kw * 32 * kR;
       const int r_left = min(kR, p.rank - r0);
       float* u = static_cast<float*>(p.ws) + ((size_t)blockIdx.z * p.rows + t0) * p.rank + r0;
       for (int e = kwarp * 32 + lane; e < 32 * kR; e += kw * 32) {
         const int t = e / kR, r = e % kR;
         if (!(mine >> t & 1) || r >= r_left) continue;
         float sum = 0.f;
-        for (int k = 0; k < kw; ++k) sum += parts0[(size_t)k * 32 * kR + e];
+        for (int k = 0; k < kw; ++k)
+          sum += reinterpret_cast<const float*>(s_ring + (size_t)(group * kw + k) * kDownStages * kDownStage)[e];
         u[(size_t)t * p.rank + r] = sum;
       }
       asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(kw * 32) : "memory");
@@ -198,18 +245,24 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------------------
-// Second launch: tiles of 128 weight rows x BT rows of x.  448 threads: warp 0 TMA, warp 1
-// MMA, warps 2-5 U' of the slices, warps 6-13 epilogue (lane = weight row, so that 32 lanes
-// write 64 consecutive bytes of an output row).  Up to one tile a CTA the accumulators
-// are single, else double: the epilogue of a tile overlaps the next one's main loop.
-// A ring stage holds 64 columns of W and x, or 4 slices of B_a and U'.
+// Second launch: tiles of 128 on the M side by BT on the N side.  kRowsOnM: rows of x by
+// weight rows, else weight rows by rows of x.  448 threads: warp 0 TMA, warp 1 MMA, warps 2-5
+// U' of the slices, warps 6-13 epilogue.  The accumulators are double: the epilogue of a
+// tile overlaps the next one's main loop.  A ring stage holds 64 columns of W and x, or 4
+// slices of B_a and U'.
 // ---------------------------------------------------------------------------
-template <int BT>
+constexpr uint32_t kMTile = 128 * 128;       // the M side: 128 rows x 64 columns of 16 bits
+
+template <int BT, bool kRowsOnM>
 struct GemmCfgA {
-  static constexpr uint32_t kX = BT * 128;
-  static constexpr uint32_t kStage = kWTile + kX;
+  static constexpr int kRows = kRowsOnM ? 128 : BT, kCols = kRowsOnM ? BT : 128;
+  static constexpr uint32_t kStage = kMTile + BT * 128;
   static constexpr int kStages = BT == 256 ? 4 : (BT == 128 ? 6 : (BT == 64 ? 8 : 9));
-  static constexpr size_t kSmem = kStages * kStage + 512;
+  // a slice (32 bytes a row) and where the slices of U' and B_a lie in a stage
+  static constexpr uint32_t kUSlice = kRows * 32, kBSlice = kCols * 32;
+  static constexpr uint32_t kUAt = kRowsOnM ? 0 : kMTile, kBAt = kRowsOnM ? kMTile : 0;
+  static constexpr uint32_t kStaging = kRowsOnM ? 8 * 2048 : 0;  // 32 x 32 outputs a warp
+  static constexpr size_t kSmem = kStages * kStage + kStaging + 512;
   static constexpr uint32_t kTmem = 2 * BT;
   static_assert(4 * kStages * 8 + 48 + 16 * 4 <= 512, "barriers");
   static_assert(kStages * kStage >= BT * 128 * 4, "the split-K exchange reuses the ring");
@@ -230,16 +283,39 @@ __device__ __forceinline__ bool drop_nonfinite(uint4& v) {
   }
   return found;
 }
+// What drop_nonfinite left out of y[t, col] in slices [s0, s1) of the tile's list.
+template <typename T>
+__device__ __noinline__ float dropped_part(const AdapterGemmParams& p, const Plan& pl, const int* list, int s0, int s1,
+                                           long long t, int col) {
+  const int a = row_id(p, t);
+  float sum = 0.f;
+  if (a < 0 || col >= p.N) return sum;
+  const T* bw = static_cast<const T*>(p.lora_b) + ((size_t)a * p.N + col) * p.rank;
+  for (int s = s0; s < s1; ++s) {
+    if (list[2 + s / pl.chunks] != a) continue;
+    const int c0 = (s % pl.chunks) * kSliceRows, c1 = min(c0 + kSliceRows, p.rank);
+    for (int r = c0; r < c1; ++r) {
+      const float bv = to_f32(bw[r]);
+      if (isfinite(bv)) continue;
+      float u = 0.f;
+      for (int k = 0; k < pl.down_split; ++k)
+        u += static_cast<const float*>(p.ws)[((size_t)k * p.rows + t) * p.rank + r];
+      sum += to_f32(from_f32<T>(u * (p.scales ? __ldg(p.scales + a) : 1.f))) * bv;
+    }
+  }
+  return sum;
+}
 
-template <typename T, int BT>
+template <typename T, int BT, bool kRowsOnM>
 __global__ void __launch_bounds__(kThreadsA, 1)
     adapter_gemm_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
-                        const __grid_constant__ CUtensorMap bmap, const __grid_constant__ AdapterGemmParams p,
-                        const __grid_constant__ Plan pl) {
-  using C = GemmCfgA<BT>;
+                        const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap omap,
+                        const __grid_constant__ AdapterGemmParams p, const __grid_constant__ Plan pl) {
+  using C = GemmCfgA<BT, kRowsOnM>;
   constexpr uint32_t kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStage);
+  uint8_t* staging = smem + C::kStages * C::kStage;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::kStaging);
   uint64_t* empty = full + C::kStages;
   uint64_t* u_go = empty + C::kStages;    // [stages] the stage is free for U' (producer)
   uint64_t* u_full = u_go + C::kStages;   // [stages] U' written, B_a's slices landed
@@ -253,9 +329,9 @@ __global__ void __launch_bounds__(kThreadsA, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = pl.split > 1 ? (int)cluster_ctarank() : 0;
-  const int tile0 = pl.split > 1 ? blockIdx.x / pl.split : blockIdx.x;
-  const int step = pl.split > 1 ? pl.tiles * pl.n_tiles : gridDim.x;
   const int total = pl.tiles * pl.n_tiles;
+  const int tile0 = pl.split > 1 ? blockIdx.x / pl.split : blockIdx.x;
+  const int step = pl.split > 1 ? total : gridDim.x;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -273,6 +349,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
     tma_prefetch_desc(&xmap);
     tma_prefetch_desc(&wmap);
     tma_prefetch_desc(&bmap);
+    tma_prefetch_desc(&omap);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::kTmem);
@@ -281,8 +358,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // The first launch may still run: what reads its results waits for it first.  Plain loads
-  // (not the read-only path, which may hold older values).
+  // The first launch may still run: what reads its results waits for it first.
   const int* lists = reinterpret_cast<const int*>(static_cast<const uint8_t*>(p.ws) + list_offset(p, pl));
   const int kb0 = pl.kblocks * rank / pl.split, kb1 = pl.kblocks * (rank + 1) / pl.split;
   // this CTA's slices of a tile whose list is `list`
@@ -296,8 +372,9 @@ __global__ void __launch_bounds__(kThreadsA, 1)
     if (lane == 0) {
       int it = 0;
       bool ok = true;
+      const uint32_t bytes = (uint32_t)(pl.x_box + C::kCols) * 128u;
       for (int tile = tile0; ok && tile < total; tile += step) {
-        const int tt = tile / pl.n_tiles, n0 = (tile - tt * pl.n_tiles) * 128;
+        const int tt = tile / pl.n_tiles, n0 = (tile - tt * pl.n_tiles) * C::kCols;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int st = it % C::kStages;
           if (!mbar_wait(&empty[st], ((it / C::kStages) & 1) ^ 1, kErrTimeoutSmemEmpty, abort_flag)) {
@@ -305,9 +382,9 @@ __global__ void __launch_bounds__(kThreadsA, 1)
             break;
           }
           uint8_t* dst = smem + st * C::kStage;
-          mbar_arrive_expect_tx(&full[st], kWTile + (uint32_t)pl.x_box * 128u);
-          tma_load_2d(dst, &wmap, &full[st], kb * 64, n0);
-          tma_load_2d(dst + kWTile, &xmap, &full[st], kb * 64, tt * BT);
+          mbar_arrive_expect_tx(&full[st], bytes);
+          tma_load_2d(dst + C::kBAt, &wmap, &full[st], kb * 64, n0);
+          tma_load_2d(dst + C::kUAt, &xmap, &full[st], kb * 64, tt * C::kRows);
         }
         // the lists are the first launch's: wait for it only now that W and x are on their way
         if (tile == tile0) wait_for_previous();
@@ -321,10 +398,10 @@ __global__ void __launch_bounds__(kThreadsA, 1)
             break;
           }
           mbar_arrive(&u_go[st]);
-          mbar_arrive_expect_tx(&full[st], (uint32_t)n * 4096u);
+          mbar_arrive_expect_tx(&full[st], (uint32_t)n * C::kBSlice);
           for (int i = 0; i < n; ++i)
-            tma_load_3d(smem + st * C::kStage + i * 4096, &bmap, &full[st], ((s0 + i) % pl.chunks) * kSliceRows, n0,
-                        list[2 + (s0 + i) / pl.chunks]);
+            tma_load_3d(smem + st * C::kStage + C::kBAt + i * C::kBSlice, &bmap, &full[st],
+                        ((s0 + i) % pl.chunks) * kSliceRows, n0, list[2 + (s0 + i) / pl.chunks]);
         }
       }
     }
@@ -339,7 +416,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
         const uint32_t acc = tmem + (uint32_t)(buf * BT);
         if (!mbar_wait(&acc_empty[buf], ((n >> 1) & 1) ^ 1, kErrTimeoutTmemEmpty, abort_flag)) break;
         tc_fence_after();
-        int s0, s1;
+        int s0 = 0, s1 = 0;
         if (n > 0) slice_range(lists + (size_t)tt * pl.list_ld, s0, s1);  // fetched ahead of its use
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int st = it % C::kStages;
@@ -348,10 +425,10 @@ __global__ void __launch_bounds__(kThreadsA, 1)
             break;
           }
           tc_fence_after();
-          const uint64_t dw = sw128_desc(smem_u32(smem + st * C::kStage), 16, 1024);
-          const uint64_t dx = sw128_desc(smem_u32(smem + st * C::kStage + kWTile), 16, 1024);
+          const uint64_t dm = sw128_desc(smem_u32(smem + st * C::kStage), 16, 1024);
+          const uint64_t dn = sw128_desc(smem_u32(smem + st * C::kStage + kMTile), 16, 1024);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) umma_f16_ss(acc, dw + 2 * kk, dx + 2 * kk, idesc, kb > kb0 || kk > 0);
+          for (int kk = 0; kk < 4; ++kk) umma_f16_ss(acc, dm + 2 * kk, dn + 2 * kk, idesc, kb > kb0 || kk > 0);
           umma_commit(&empty[st]);
         }
         if (n == 0) {
@@ -366,10 +443,10 @@ __global__ void __launch_bounds__(kThreadsA, 1)
           }
           uses ^= 1u << st;
           tc_fence_after();
-          const uint64_t dw = sw32_desc(smem_u32(smem + st * C::kStage));
-          const uint64_t dx = sw32_desc(smem_u32(smem + st * C::kStage + kWTile));
+          const uint64_t dm = sw32_desc(smem_u32(smem + st * C::kStage));
+          const uint64_t dn = sw32_desc(smem_u32(smem + st * C::kStage + kMTile));
           for (int i = 0; i < m; ++i)
-            umma_f16_ss(acc, dw + (uint64_t)(i * (4096 >> 4)), dx + (uint64_t)(i * (BT * 32 >> 4)), idesc, 1u);
+            umma_f16_ss(acc, dm + (uint64_t)(i * (4096 >> 4)), dn + (uint64_t)(i * (BT * 32 >> 4)), idesc, 1u);
           umma_commit(&empty[st]);
         }
         if (ok) umma_commit(&acc_full[buf]);
@@ -379,9 +456,8 @@ __global__ void __launch_bounds__(kThreadsA, 1)
     // ------------------------------------------------------------ U' of the slices
     // These warps follow the ring by its slice stages alone: a stage is theirs once the
     // producer says so, and is not used again before the MMA has had their U'.
-    // A thread writes rows i0 and i0 + 128 of all slices.  Their values are fetched and
-    // rounded before the stage is waited for, so that the wait covers the loads.
-    constexpr int kPer = BT > 128 ? 2 : 1;
+    // A thread writes its row of all slices; the values are fetched and rounded before the
+    // stage is waited for, so that the wait covers the loads.
     const int i0 = threadIdx.x - 64;
     int it = 0, n = 0;
     uint32_t uses = 0;
@@ -394,33 +470,30 @@ __global__ void __launch_bounds__(kThreadsA, 1)
       int s0, s1;
       slice_range(list, s0, s1);
       it += kb1 - kb0;
-      int id[kPer];
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) id[e] = row_id(p, (long long)tt * BT + i0 + e * 128);
+      const long long t = (long long)tt * C::kRows + i0;
+      const int id = i0 < C::kRows ? row_id(p, t) : -1;
+      const float sc = id >= 0 && p.scales ? __ldg(p.scales + id) : 1.f;
       for (; s0 < s1; s0 += 4, ++it) {
         const int st = it % C::kStages, m = min(4, s1 - s0);
-        uint4 v[kPer][4][2];  // [row][slice][8 values]
+        uint4 v[4][2];  // [slice][8 values]
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int s = s0 + i, a = i < m ? list[2 + s / pl.chunks] : -2, c0 = (s % pl.chunks) * kSliceRows;
 #pragma unroll
-          for (int e = 0; e < kPer; ++e)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              v[e][i][half] = make_uint4(0u, 0u, 0u, 0u);
-              if (id[e] != a || c0 + half * 8 >= p.rank) continue;
-              const float* u = static_cast<const float*>(p.ws) + ((size_t)tt * BT + i0 + e * 128) * p.rank + c0 + half * 8;
-              float4 lo = *reinterpret_cast<const float4*>(u), hi = *reinterpret_cast<const float4*>(u + 4);
-              for (int k = 1; k < pl.down_split; ++k) {
-                u += part;
-                const float4 l2 = *reinterpret_cast<const float4*>(u), h2 = *reinterpret_cast<const float4*>(u + 4);
-                lo = make_float4(lo.x + l2.x, lo.y + l2.y, lo.z + l2.z, lo.w + l2.w);
-                hi = make_float4(hi.x + h2.x, hi.y + h2.y, hi.z + h2.z, hi.w + h2.w);
-              }
-              const float sc = p.scales ? __ldg(p.scales + a) : 1.f;
-              v[e][i][half] = make_uint4(pack2<T>(lo.x * sc, lo.y * sc), pack2<T>(lo.z * sc, lo.w * sc),
-                                         pack2<T>(hi.x * sc, hi.y * sc), pack2<T>(hi.z * sc, hi.w * sc));
+          for (int half = 0; half < 2; ++half) {
+            v[i][half] = make_uint4(0u, 0u, 0u, 0u);
+            if (id != a || c0 + half * 8 >= p.rank) continue;
+            const float* u = static_cast<const float*>(p.ws) + t * p.rank + c0 + half * 8;
+            float4 lo = *reinterpret_cast<const float4*>(u), hi = *reinterpret_cast<const float4*>(u + 4);
+            for (int k = 1; k < pl.down_split; ++k) {
+              u += part;
+              const float4 l2 = *reinterpret_cast<const float4*>(u), h2 = *reinterpret_cast<const float4*>(u + 4);
+              lo = make_float4(lo.x + l2.x, lo.y + l2.y, lo.z + l2.z, lo.w + l2.w);
+              hi = make_float4(hi.x + h2.x, hi.y + h2.y, hi.z + h2.z, hi.w + h2.w);
             }
+            v[i][half] = make_uint4(pack2<T>(lo.x * sc, lo.y * sc), pack2<T>(lo.z * sc, lo.w * sc),
+                                    pack2<T>(hi.x * sc, hi.y * sc), pack2<T>(hi.z * sc, hi.w * sc));
+          }
         }
         if (!mbar_wait(&u_go[st], uses >> st & 1, kErrTimeoutSmemEmpty, abort_flag)) {
           ok = false;
@@ -428,27 +501,25 @@ __global__ void __launch_bounds__(kThreadsA, 1)
         }
         uses ^= 1u << st;
         uint8_t* base = smem + st * C::kStage;
+        if (i0 < C::kRows) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < kPer; ++e)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int r = i0 + e * 128;
-              if (i < m && r < BT)
-                *reinterpret_cast<uint4*>(base + kWTile + i * (BT * 32) + r * 32 + ((half ^ (r >> 2 & 1)) << 4)) =
-                    v[e][i][half];
-            }
+            for (int half = 0; half < 2; ++half)
+              if (i < m)
+                *reinterpret_cast<uint4*>(base + C::kUAt + i * C::kUSlice + i0 * 32 + ((half ^ (i0 >> 2 & 1)) << 4)) =
+                    v[i][half];
+        }
         if (!mbar_wait(&full[st], (it / C::kStages) & 1, kErrTimeoutTmaFull, abort_flag)) {
           ok = false;
           break;
         }
         if (list[1]) {
-          for (int x = i0; x < m * 256; x += 128) {
-            uint4* at = reinterpret_cast<uint4*>(base + x * 16);
-            uint4 v = *at;
-            if (drop_nonfinite<T>(v)) {
-              *at = v;
+          for (int x = i0; x < m * C::kCols * 2; x += 128) {
+            uint4* at = reinterpret_cast<uint4*>(base + C::kBAt + x * 16);
+            uint4 b = *at;
+            if (drop_nonfinite<T>(b)) {
+              *at = b;
               s_dropped[n & 15] = n + 1;
             }
           }
@@ -459,90 +530,144 @@ __global__ void __launch_bounds__(kThreadsA, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue
+    // A warp has lane quarter q of the M side and half of the N side's columns (all of 32).
     const int q = warp & 3, half = (warp - 6) >> 2;
+    constexpr int kMine = BT >= 64 ? BT / 2 : BT;
+    uint8_t* stg = staging + (warp - 6) * 2048;
     int n = 0;
     wait_for_previous();
     for (int tile = tile0; tile < total; tile += step, ++n) {
       const int tt = tile / pl.n_tiles, buf = n & 1;
-      const int col = (tile - tt * pl.n_tiles) * 128 + q * 32 + lane;  // output column
-      const long long t0 = (long long)tt * BT;
-      const bool in = col < p.N;
-      const float bias = in && p.bias && rank == 0 ? __ldg(p.bias + col) : 0.f;
+      const int n0 = (tile - tt * pl.n_tiles) * C::kCols;
+      const long long t0 = (long long)tt * C::kRows;
+      const int col = n0 + q * 32 + lane;  // weights on the M side: this lane's output column
+      const float bias = !kRowsOnM && p.bias && rank == 0 && col < p.N ? __ldg(p.bias + col) : 0.f;
       if (!mbar_wait(&acc_full[buf], (n >> 1) & 1, kErrTimeoutTmemFull, abort_flag)) break;
       tc_fence_after();
       const bool dropped = s_dropped[n & 15] == n + 1;
+      const int* list = lists + (size_t)tt * pl.list_ld;
+      int s0 = 0, s1 = 0;
+      if (dropped) slice_range(list, s0, s1);
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BT);
-      constexpr int kCols = BT >= 64 ? BT / 2 : BT;  // columns of this warp
       if (BT >= 64 || half == 0) {
-        for (int c = half * kCols; c < (half + 1) * kCols; c += 32) {
+        for (int c = half * kMine; c < (half + 1) * kMine; c += 32) {
+          if (kRowsOnM && n0 + c >= p.N) break;
           uint32_t v[32];
           tmem_ld32(acc + (uint32_t)c, v);
           tmem_ld_wait(v);
-          if (dropped && in) {
-            // the values left out of B_a, into the rows that have the adapter
-            const int* list = lists + (size_t)tt * pl.list_ld;
-            int s0, s1;
-            slice_range(list, s0, s1);
-            for (int s = s0; s < s1; ++s) {
-              const int a = list[2 + s / pl.chunks];
-              const int c0 = (s % pl.chunks) * kSliceRows, c1 = min(c0 + kSliceRows, p.rank);
-              const T* bw = static_cast<const T*>(p.lora_b) + ((size_t)a * p.N + col) * p.rank;
-              for (int r = c0; r < c1; ++r) {
-                const float bv = to_f32(bw[r]);
-                if (isfinite(bv)) continue;
+          if (kRowsOnM && p.bias && rank == 0) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (row_id(p, t0 + c + i) == a) {
-                    float u = 0.f;
-                    for (int k = 0; k < pl.down_split; ++k)
-                      u += static_cast<const float*>(p.ws)[((size_t)k * p.rows + t0 + c + i) * p.rank + r];
-                    u = to_f32(from_f32<T>(u * (p.scales ? __ldg(p.scales + a) : 1.f)));
-                    v[i] = __float_as_uint(__uint_as_float(v[i]) + u * bv);
-                  }
+            for (int i = 0; i < 32; i += 4) {
+              if (n0 + c + i < p.N) {  // N is a multiple of 8
+                const float4 b = make_float4(__ldg(p.bias + n0 + c + i), __ldg(p.bias + n0 + c + i + 1),
+                                             __ldg(p.bias + n0 + c + i + 2), __ldg(p.bias + n0 + c + i + 3));
+                v[i] = __float_as_uint(__uint_as_float(v[i]) + b.x);
+                v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) + b.y);
+                v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) + b.z);
+                v[i + 3] = __float_as_uint(__uint_as_float(v[i + 3]) + b.w);
               }
             }
           }
           if (pl.split > 1) {
+            // [N side][M side], a lane's values 512 bytes apart
             float* ex = reinterpret_cast<float*>(smem) + c * 128 + q * 32 + lane;
 #pragma unroll
             for (int i = 0; i < 32; ++i) ex[i * 128] = __uint_as_float(v[i]) + bias;
-          } else if (in) {
+            if (dropped) {
+              for (int i = 0; i < 32; ++i)
+                ex[i * 128] += kRowsOnM ? dropped_part<T>(p, pl, list, s0, s1, t0 + q * 32 + lane, n0 + c + i)
+                                        : dropped_part<T>(p, pl, list, s0, s1, t0 + c + i, col);
+            }
+          } else if constexpr (kRowsOnM) {
+            // 32 rows x 32 columns through swizzled shared memory, out by TMA (which clips)
+            if (lane == 0) bulk_wait_read0();
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              uint4 o;
+              o.x = pack2<T>(__uint_as_float(v[8 * u]), __uint_as_float(v[8 * u + 1]));
+              o.y = pack2<T>(__uint_as_float(v[8 * u + 2]), __uint_as_float(v[8 * u + 3]));
+              o.z = pack2<T>(__uint_as_float(v[8 * u + 4]), __uint_as_float(v[8 * u + 5]));
+              o.w = pack2<T>(__uint_as_float(v[8 * u + 6]), __uint_as_float(v[8 * u + 7]));
+              *reinterpret_cast<uint4*>(stg + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) = o;
+            }
+            if (dropped) {
+              for (int i = 0; i < 32; ++i) {
+                const float x = dropped_part<T>(p, pl, list, s0, s1, t0 + q * 32 + lane, n0 + c + i);
+                T* at = reinterpret_cast<T*>(stg + lane * 64 + ((i >> 3 ^ (lane >> 1 & 3)) << 4)) + (i & 7);
+                if (x != 0.f) *at = from_f32<T>(to_f32(*at) + x);
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&omap, stg, n0 + c, (int)t0 + q * 32, 0);
+              bulk_commit();
+            }
+          } else if (col < p.N) {
             T* out = static_cast<T*>(p.out) + (t0 + c) * p.ldo + col;
             const int left = (int)min(32LL, p.rows - (t0 + c));
+            if (left == 32) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < left) out[i * p.ldo] = from_f32<T>(__uint_as_float(v[i]) + bias);
+              for (int i = 0; i < 32; ++i, out += p.ldo) *out = from_f32<T>(__uint_as_float(v[i]) + bias);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i, out += p.ldo)
+                if (i < left) *out = from_f32<T>(__uint_as_float(v[i]) + bias);
+            }
+            if (dropped) {
+              out = static_cast<T*>(p.out) + (t0 + c) * p.ldo + col;
+              for (int i = 0; i < left; ++i, out += p.ldo) {
+                const float x = dropped_part<T>(p, pl, list, s0, s1, t0 + c + i, col);
+                if (x != 0.f) *out = from_f32<T>(to_f32(*out) + x);
+              }
+            }
           }
         }
       }
       tc_fence_before();
       mbar_arrive(&acc_empty[buf]);
     }
+    if (kRowsOnM && lane == 0) bulk_wait0();
   }
 
   if (pl.split > 1) {
-    // every CTA of the cluster adds up its share of the tile's rows, in rank order
+    // every CTA of the cluster adds up its share of the N side, in rank order
     __syncwarp();
     cluster_sync_all();
-    const int tt = tile0 / pl.n_tiles, n0 = (tile0 - tt * pl.n_tiles) * 128;
-    const int r0 = BT * rank / pl.split, r1 = BT * (rank + 1) / pl.split;
+    const int tt = tile0 / pl.n_tiles, n0 = (tile0 - tt * pl.n_tiles) * C::kCols;
+    const long long t0 = (long long)tt * C::kRows;
     const uint32_t base = smem_u32(smem);
-    for (int x = threadIdx.x; x < (r1 - r0) * 32; x += kThreadsA) {
-      const int r = r0 + (x >> 5), c = (x & 31) * 4;
-      const long long t = (long long)tt * BT + r;
-      if (t >= p.rows || n0 + c >= p.N) continue;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    // 8 consecutive output columns of a row a thread
+    const int c0 = BT / 8 * rank / pl.split * 8, c1 = BT / 8 * (rank + 1) / pl.split * 8;
+    for (int x = threadIdx.x; x < (c1 - c0) * 16; x += kThreadsA) {
+      // rows on M: lanes along the rows; weights on M: 16 groups of 8 columns a row
+      const int m = kRowsOnM ? x & 127 : (x & 15) * 8, c = c0 + (kRowsOnM ? (x >> 7) * 8 : x >> 4);
+      const long long t = t0 + (kRowsOnM ? m : c);
+      const int col = n0 + (kRowsOnM ? c : m);
+      if (t >= p.rows || col >= p.N) continue;
+      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       for (int k = 0; k < pl.split; ++k) {
-        float4 v;
-        const uint32_t at = mapa_shared(base + (uint32_t)(r * 128 + c) * 4u, (uint32_t)k);
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                     : "r"(at)
-                     : "memory");
-        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        const uint32_t at = mapa_shared(base + (uint32_t)(c * 128 + m) * 4u, (uint32_t)k);
+        float v[8];
+        if constexpr (kRowsOnM) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i]) : "r"(at + (uint32_t)i * 512u) : "memory");
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i += 4)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3])
+                         : "r"(at + (uint32_t)i * 4u)
+                         : "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += v[i];
       }
-      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.ldo + n0 + c) =
-          make_uint2(pack2<T>(sum.x, sum.y), pack2<T>(sum.z, sum.w));
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.ldo + col) =
+          make_uint4(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]),
+                     pack2<T>(sum[6], sum[7]));
     }
     __syncwarp();
     cluster_sync_all();  // the parts stay until all have read them
@@ -556,19 +681,20 @@ __global__ void __launch_bounds__(kThreadsA, 1)
 
 Plan make_plan(int rows, int K, int N, int adapters, int rank, int num_sms) {
   Plan pl{};
-  pl.bt = rows <= 32 ? 32 : (rows <= 64 ? 64 : (rows <= 128 ? 128 : 256));
+  pl.rows_on_m = rows > 128;
+  pl.bt = rows <= 32 ? 32 : (rows <= 64 ? 64 : 128);
   pl.tiles = (rows + pl.bt - 1) / pl.bt;
-  pl.n_tiles = (N + 127) / 128;
+  pl.n_tiles = pl.rows_on_m ? (N + 255) / 256 : (N + 127) / 128;
   pl.kblocks = (K + 63) / 64;
   pl.chunks = (rank + kSliceRows - 1) / kSliceRows;
-  // first launch: at least 4 K steps of 32 a warp, about two CTAs an SM
-  const int steps = (K + 31) / 32;
+  // first launch: at least 3 K steps of 64 a warp, up to three CTAs for each SM
+  const int steps = (K + 63) / 64;
   pl.down_kw = 1;
-  while (pl.down_kw < 8 && pl.down_kw * 2 * 4 <= steps) pl.down_kw *= 2;
-  const int rows_cta = 32 * (8 / pl.down_kw);
+  while (pl.down_kw < kDownWarps && pl.down_kw * 2 * 3 <= steps) pl.down_kw *= 2;
+  const int rows_cta = 32 * (kDownWarps / pl.down_kw);
   pl.down_x = adapters ? (rows + rows_cta - 1) / rows_cta : 0;
-  const int want = 2 * num_sms;
-  pl.down_split = std::max(1, std::min({want / std::max(pl.down_x, 1), 8, steps / (pl.down_kw * 4)}));
+  const int want = 3 * num_sms;
+  pl.down_split = std::max(1, std::min({want / std::max(pl.down_x, 1), 8, steps / (pl.down_kw * 3)}));
   pl.down_y = std::max(1, std::min({want / std::max(pl.down_x * pl.down_split, 1), 32, adapters}));
   pl.down_nt = rank <= 8 ? 1 : (rank <= 16 ? 2 : (rank <= 32 ? 4 : 8));
   pl.split = 1;
@@ -591,27 +717,28 @@ CUtensorMap map_3d(const void* base, uint64_t cols, uint64_t rows, uint64_t coun
 template <typename T, int NT>
 cudaError_t launch_down(const AdapterGemmParams& p, const Plan& pl, cudaStream_t s) {
   static std::atomic<unsigned long long> configured;
-  constexpr int smem = 8 * 32 * NT * 8 * (int)sizeof(float);
-  cudaError_t e = ensure_smem_limit(adapter_down_kernel<T, NT>, smem, configured);
+  cudaError_t e = ensure_smem_limit(adapter_down_kernel<T, NT>, kDownSmem, configured);
   if (e != cudaSuccess) return e;
   const double m = p.rows, k = p.K, r = p.rank;
   LaunchScope scope("adapter_down", 2.0 * m * r * k, 2.0 * (m * k + p.adapters * r * k) + 4.0 * m * r, s);
-  adapter_down_kernel<T, NT><<<dim3(pl.down_x + pl.tiles, pl.down_y, pl.down_split), 256, smem, s>>>(p, pl);
+  adapter_down_kernel<T, NT><<<dim3(pl.down_x + pl.tiles, pl.down_y, pl.down_split), 32 * kDownWarps, kDownSmem, s>>>(p, pl);
   return cudaGetLastError();
 }
 
-template <typename T, int BT>
+template <typename T, int BT, bool kRowsOnM>
 cudaError_t launch_bt(const AdapterGemmParams& p, const Plan& pl, int num_sms, cudaStream_t s) {
+  using C = GemmCfgA<BT, kRowsOnM>;
   static std::atomic<unsigned long long> configured;
-  cudaError_t e = ensure_smem_limit(adapter_gemm_kernel<T, BT>, (int)GemmCfgA<BT>::kSmem, configured);
+  cudaError_t e = ensure_smem_limit(adapter_gemm_kernel<T, BT, kRowsOnM>, (int)C::kSmem, configured);
   if (e != cudaSuccess) return e;
   const double m = p.rows, k = p.K, n = p.N, r = p.rank;
   const CUtensorMap mx = map_2d(p.x, (uint64_t)p.rows, (uint64_t)p.K, (uint64_t)p.ldx, (uint32_t)pl.x_box);
-  const CUtensorMap mw = map_2d(p.w, (uint64_t)p.N, (uint64_t)p.K, (uint64_t)p.K, 128);
+  const CUtensorMap mw = map_2d(p.w, (uint64_t)p.N, (uint64_t)p.K, (uint64_t)p.K, (uint32_t)C::kCols);
   // without adapters no row has one and the map is not read
   const CUtensorMap mb = p.adapters ? map_3d(p.lora_b, (uint64_t)p.rank, (uint64_t)p.N, (uint64_t)p.adapters,
-                                             kSliceRows, 128, CU_TENSOR_MAP_SWIZZLE_32B)
+                                             kSliceRows, (uint32_t)C::kCols, CU_TENSOR_MAP_SWIZZLE_32B)
                                     : mx;
+  const CUtensorMap mo = kRowsOnM ? map_out_2d(p.out, false, (uint64_t)p.rows, (uint64_t)p.N, (uint64_t)p.ldo) : mx;
   e = pl.down_nt == 1   ? launch_down<T, 1>(p, pl, s)
       : pl.down_nt == 2 ? launch_down<T, 2>(p, pl, s)
       : pl.down_nt == 4 ? launch_down<T, 4>(p, pl, s)
@@ -622,7 +749,7 @@ cudaError_t launch_bt(const AdapterGemmParams& p, const Plan& pl, int num_sms, c
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(pl.split > 1 ? tiles * pl.split : std::min<long long>(tiles, num_sms)));
   cfg.blockDim = dim3(kThreadsA);
-  cfg.dynamicSmemBytes = GemmCfgA<BT>::kSmem;
+  cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -632,23 +759,17 @@ cudaError_t launch_bt(const AdapterGemmParams& p, const Plan& pl, int num_sms, c
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = pl.split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, adapter_gemm_kernel<T, BT>, mx, mw, mb, p, pl);
+  return cudaLaunchKernelEx(&cfg, adapter_gemm_kernel<T, BT, kRowsOnM>, mx, mw, mb, mo, p, pl);
 }
 
 template <typename T>
 cudaError_t launch_t(const AdapterGemmParams& p, int num_sms, cudaStream_t s) {
   if (p.rows == 0) return cudaSuccess;
   const Plan pl = make_plan(p.rows, p.K, p.N, p.adapters, p.rank, num_sms);
-  switch (pl.bt) {
-    case 32:
-      return launch_bt<T, 32>(p, pl, num_sms, s);
-    case 64:
-      return launch_bt<T, 64>(p, pl, num_sms, s);
-    case 128:
-      return launch_bt<T, 128>(p, pl, num_sms, s);
-    default:
-      return launch_bt<T, 256>(p, pl, num_sms, s);
-  }
+  if (pl.rows_on_m) return launch_bt<T, 256, true>(p, pl, num_sms, s);
+  return pl.bt == 32   ? launch_bt<T, 32, false>(p, pl, num_sms, s)
+         : pl.bt == 64 ? launch_bt<T, 64, false>(p, pl, num_sms, s)
+                       : launch_bt<T, 128, false>(p, pl, num_sms, s);
 }
 
 }  // namespace
