@@ -108,8 +108,8 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], uint32_t word
 }
 
 // P and the row sum of a whole 128-column row; the next chunk's load is in flight
-// while one is processed.
-template <typename T>
+// while one is processed.  kAll: every key of the tile is kept.
+template <typename T, bool kAll>
 __device__ __forceinline__ float row_exp(uint32_t sAddr, const uint32_t (&words)[4], float c, float ref,
                                          uint32_t (&pk)[64]) {
   const float2 c2 = make_float2(c, c), nref2 = make_float2(-ref, -ref);
@@ -118,15 +118,15 @@ __device__ __forceinline__ float row_exp(uint32_t sAddr, const uint32_t (&words)
   tmem_ld32(sAddr, ra);
   tmem_ld_wait(ra);
   tmem_ld32(sAddr + 32, rb);
-  chunk_exp<T>(ra, words[0], c2, nref2, sum2, pk);
+  chunk_exp<T>(ra, kAll ? 0xffffffffu : words[0], c2, nref2, sum2, pk);
   tmem_ld_wait(rb);
   tmem_ld32(sAddr + 64, ra);
-  chunk_exp<T>(rb, words[1], c2, nref2, sum2, pk + 16);
+  chunk_exp<T>(rb, kAll ? 0xffffffffu : words[1], c2, nref2, sum2, pk + 16);
   tmem_ld_wait(ra);
   tmem_ld32(sAddr + 96, rb);
-  chunk_exp<T>(ra, words[2], c2, nref2, sum2, pk + 32);
+  chunk_exp<T>(ra, kAll ? 0xffffffffu : words[2], c2, nref2, sum2, pk + 32);
   tmem_ld_wait(rb);
-  chunk_exp<T>(rb, words[3], c2, nref2, sum2, pk + 48);
+  chunk_exp<T>(rb, kAll ? 0xffffffffu : words[3], c2, nref2, sum2, pk + 48);
   return sum2.x + sum2.y;
 }
 
@@ -237,89 +237,136 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      const uint32_t idesc_s = umma_idesc_f16(kIsBf16, 128, 0);
-      const uint32_t idesc_o = umma_idesc_f16(kIsBf16, (uint32_t)g.ksteps * 16, 1);
-      const uint64_t dq0 = sw128_desc(smem_u32(sQ), 16, 1024);
-      const uint64_t dk0 = sw128_desc(smem_u32(sKV), 16, 1024);
-      const uint64_t dv0 = sw128_desc(smem_u32(sKV), kHalfBytes, 1024);
-      uint32_t slot = 0, phase = 0;
-      uint32_t pcnt[2] = {0, 0};
-      bool ok = true;
-      auto issue_s = [&](int w, int tile, uint32_t st) {
-        const uint64_t dq = dq0 + (uint64_t)((tile * C::kTile) >> 4);
-        const uint64_t dk = dk0 + (uint64_t)((st * C::kTile) >> 4);
-        const uint32_t dS = tmem + (uint32_t)(w * 128);
+    // The whole warp walks, lane 0 issues.  The issue loop is the critical path of short
+    // tiles, so it carries no arrays and no divisions.
+    const uint32_t lead = lane == 0;
+    const uint32_t idesc_s = umma_idesc_f16(kIsBf16, 128, 0);
+    const uint32_t idesc_o = umma_idesc_f16(kIsBf16, (uint32_t)g.ksteps * 16, 1);
+    const uint64_t dq0 = sw128_desc(smem_u32(sQ), 16, 1024);
+    const uint64_t dk0 = sw128_desc(smem_u32(sKV), 16, 1024);
+    const uint64_t dv0 = sw128_desc(smem_u32(sKV), kHalfBytes, 1024);
+    constexpr uint32_t kSlotDesc = C::kTile >> 4;
+    const int ksteps = g.ksteps;
+    struct Pos {
+      uint32_t slot, phase;
+      __device__ __forceinline__ Pos plus(uint32_t n) const {
+        return slot + n >= C::kSlots ? Pos{slot + n - C::kSlots, phase ^ 1} : Pos{slot + n, phase};
+      }
+    };
+    Pos pos{0, 0};              // ring position of the current unit's first slot
+    uint32_t pp0 = 0, pp1 = 0;  // phases of p_full
+    auto issue_s = [&](int w, int tile, Pos ks) {
+      const uint64_t dq = dq0 + (uint64_t)(tile * kSlotDesc), dk = dk0 + (uint64_t)(ks.slot * kSlotDesc);
+      const uint32_t dS = tmem + (uint32_t)(w * 128);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          if (kk >= g.ksteps) break;
-          const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
-          umma_f16_ss(dS, dq + off, dk + off, idesc_s, kk != 0);
-        }
-        umma_commit(&s_full[w]);
-      };
-      auto issue_pv = [&](int w, uint32_t st, bool first) -> bool {
-        if (!mbar_wait<false>(&p_full[w], pcnt[w] & 1, kErrTimeoutAttnP, abort_flag)) return false;
-        ++pcnt[w];
-        tc_fence_after();
-        const uint64_t dv = dv0 + (uint64_t)((st * C::kTile) >> 4);
-        const uint32_t pa = tmem + (uint32_t)(w * 128), dO = tmem + C::kColO + (uint32_t)(w * DP);
-        umma_f16_ts(dO, pa, dv, idesc_o, first ? 0u : 1u);
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        if (kk >= ksteps) break;
+        const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
+        umma_f16_ss_lead(lead, dS, dq + off, dk + off, idesc_s, kk != 0);
+      }
+      umma_commit_lead(lead, &s_full[w]);
+    };
+    auto issue_pv = [&](int w, Pos vs, uint32_t acc) {
+      const uint64_t dv = dv0 + (uint64_t)(vs.slot * kSlotDesc);
+      const uint32_t pa = tmem + (uint32_t)(w * 128), dO = tmem + C::kColO + (uint32_t)(w * DP);
+      umma_f16_ts_lead(lead, dO, pa, dv, idesc_o, acc);
 #pragma unroll
-        for (int kk = 1; kk < 8; ++kk) umma_f16_ts(dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
-        return true;
-      };
-      while (ok && k.next(p, g)) {
-        if (!mbar_wait<false>(q_full, k.seg & 1, kErrTimeoutAttnQ, abort_flag)) break;
-        tc_fence_after();
-        uint32_t vslot[2] = {0, 0};      // V slot of each tile's last unit
-        int count[2] = {0, 0};           // units of each tile so far
-        for (int j = k.j0; ok && j < k.j1; ++j) {
-          uint32_t kslot = 0, vs = 0;
-          for (int w = 0; w < 2; ++w) {
-            if (!k.uses(w, j)) continue;
-            if (w == 0 || k.lone) {
-              kslot = slot;
-              if (!mbar_wait<false>(&ready[slot], phase, kErrTimeoutAttnKV, abort_flag)) {
-                ok = false;
-                break;
-              }
-              if (++slot == C::kSlots) slot = 0, phase ^= 1;
-            }
-            tc_fence_after();
-            if (count[w] > 0) {
-              if (!issue_pv(w, vslot[w], count[w] == 1)) {
-                ok = false;
-                break;
-              }
-              if (w == 1 || k.lone) umma_commit(&empty[vslot[w]]);
-            }
-            issue_s(w, k.lone ? 0 : w, kslot);
-            if (w == 1 || k.lone) umma_commit(&empty[kslot]);
-            if (w == 0 || k.lone) {
-              vs = slot;
-              if (!mbar_wait<false>(&ready[slot], phase, kErrTimeoutAttnKV, abort_flag)) {
-                ok = false;
-                break;
-              }
-              if (++slot == C::kSlots) slot = 0, phase ^= 1;
-            }
-            vslot[w] = vs;
-            ++count[w];
-          }
+      for (int kk = 1; kk < 8; ++kk) umma_f16_ts_lead(lead, dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
+    };
+    auto landed = [&](Pos s) -> bool {
+      const bool r = mbar_wait<false>(&ready[s.slot], s.phase, kErrTimeoutAttnKV, abort_flag);
+      tc_fence_after();
+      return r;
+    };
+    auto wait_p = [&](int w, uint32_t& par) -> bool {
+      const bool r = mbar_wait<false>(&p_full[w], par, kErrTimeoutAttnP, abort_flag);
+      par ^= 1;
+      tc_fence_after();
+      return r;
+    };
+    auto release = [&](Pos s) { umma_commit_lead(lead, &empty[s.slot]); };
+    bool ok = true;
+    while (ok && k.next(p, g)) {
+      if (!mbar_wait<false>(q_full, k.seg & 1, kErrTimeoutAttnQ, abort_flag)) break;
+      tc_fence_after();
+      const int n = k.j1 - k.j0;
+      if (!k.lone) {
+        // ring: K, V per unit, both tiles' users of each
+        if (!(ok = landed(pos))) break;
+        issue_s(0, 0, pos);
+        issue_s(1, 1, pos);
+        release(pos);
+        for (int j = 1; j < n; ++j) {
+          const Pos v = pos.plus(1), kn = pos.plus(2);
+          if (!(ok = landed(v) && wait_p(0, pp0))) break;
+          issue_pv(0, v, j > 1);
+          if (!(ok = landed(kn))) break;
+          issue_s(0, 0, kn);
+          if (!(ok = wait_p(1, pp1))) break;
+          issue_pv(1, v, j > 1);
+          release(v);
+          issue_s(1, 1, kn);
+          release(kn);
+          pos = kn;
         }
         if (!ok) break;
-        umma_commit(q_empty);
-        for (int w = 0; w < 2; ++w) {
-          if (count[w] > 0) {
-            if (!issue_pv(w, vslot[w], count[w] == 1)) {
-              ok = false;
-              break;
-            }
-            if (w == 1 || k.lone) umma_commit(&empty[vslot[w]]);
-          }
-          umma_commit(&o_done[w]);
+        umma_commit_lead(lead, q_empty);
+        const Pos v = pos.plus(1);
+        if (!(ok = landed(v) && wait_p(0, pp0))) break;
+        issue_pv(0, v, n > 1);
+        umma_commit_lead(lead, &o_done[0]);
+        if (!(ok = wait_p(1, pp1))) break;
+        issue_pv(1, v, n > 1);
+        release(v);
+        umma_commit_lead(lead, &o_done[1]);
+        pos = pos.plus(2);
+      } else {
+        // ring: K, V of the first half's tile, then of the second's, which only the item's
+        // last unit may lack
+        bool second = k.uses(1, k.j0);
+        if (!(ok = landed(pos))) break;
+        issue_s(0, 0, pos);
+        release(pos);
+        if (second) {
+          const Pos kb = pos.plus(2);
+          if (!(ok = landed(kb))) break;
+          issue_s(1, 0, kb);
+          release(kb);
         }
+        for (int j = 1; j < n; ++j) {
+          const Pos va = pos.plus(1), vb = pos.plus(3), ka = pos.plus(4), kb = ka.plus(2);
+          second = k.uses(1, k.j0 + j);
+          if (!(ok = landed(va) && wait_p(0, pp0))) break;
+          issue_pv(0, va, j > 1);
+          release(va);
+          if (!(ok = landed(ka))) break;
+          issue_s(0, 0, ka);
+          release(ka);
+          if (!(ok = landed(vb) && wait_p(1, pp1))) break;
+          issue_pv(1, vb, j > 1);
+          release(vb);
+          if (second) {
+            if (!(ok = landed(kb))) break;
+            issue_s(1, 0, kb);
+            release(kb);
+          }
+          pos = ka;
+        }
+        if (!ok) break;
+        umma_commit_lead(lead, q_empty);
+        const Pos va = pos.plus(1);
+        if (!(ok = landed(va) && wait_p(0, pp0))) break;
+        issue_pv(0, va, n > 1);
+        release(va);
+        umma_commit_lead(lead, &o_done[0]);
+        if (second) {
+          const Pos vb = pos.plus(3);
+          if (!(ok = landed(vb) && wait_p(1, pp1))) break;
+          issue_pv(1, vb, n > 1);
+          release(vb);
+        }
+        umma_commit_lead(lead, &o_done[1]);
+        pos = pos.plus(second ? 4 : 2);
       }
     }
   } else if (warp == 2) {
@@ -386,12 +433,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool have = false;  // the reference is set
       int used = 0;
       for (int j = k.j0; j < k.j1; ++j) {
-        // the V slot of this tile's unit
-        const int ns = k.slots(j);
-        uint32_t vs = slot + (k.lone ? 2 * w : 0) + 1, vphase = phase;
-        if (vs >= C::kSlots) vs -= C::kSlots, vphase ^= 1;
-        slot += ns;
-        if (slot >= C::kSlots) slot -= C::kSlots, phase ^= 1;
+        // the V slot of this tile's unit, where its mask words are
+        uint32_t vs = 0, vphase = 0;
+        if constexpr (kMask) {
+          vs = slot + (k.lone ? 2 * w : 0) + 1;
+          vphase = phase;
+          if (vs >= C::kSlots) vs -= C::kSlots, vphase ^= 1;
+          slot += k.slots(j);
+          if (slot >= C::kSlots) slot -= C::kSlots, phase ^= 1;
+        }
         if (!k.uses(w, j)) continue;
         if (!mbar_wait<false>(&s_full[w], scnt & 1, kErrTimeoutAttnS, abort_flag)) {
           ok = false;
@@ -415,6 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp_active) {
           uint32_t pk[64];
           const bool any = (words[0] | words[1] | words[2] | words[3]) != 0u;
+          const bool all = (words[0] & words[1] & words[2] & words[3]) == 0xffffffffu;
           float sum = 0.f;
           if (!have && any) {
             const int ch = words[0] ? 0 : (words[1] ? 1 : (words[2] ? 2 : 3));
@@ -426,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             have = true;
           }
           if (any) {
-            sum = row_exp<T>(sAddr, words, c, ref, pk);
+            sum = all ? row_exp<T, true>(sAddr, words, c, ref, pk) : row_exp<T, false>(sAddr, words, c, ref, pk);
             if (__any_sync(0xffffffffu, valid && !(sum <= kSumLimit))) {
               // exact passes: the reference moves to the row's maximum, O and l with it
               float m = -INFINITY;
@@ -453,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               l *= alpha;
               ref = moved;
-              sum = row_exp<T>(sAddr, words, c, ref, pk);
+              sum = row_exp<T, false>(sAddr, words, c, ref, pk);
             }
           } else {
 #pragma unroll
