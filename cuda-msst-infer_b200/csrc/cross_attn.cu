@@ -237,9 +237,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    // The whole warp walks, lane 0 issues.  The issue loop is the critical path of short
-    // tiles, so it carries no arrays and no divisions.
-    const uint32_t lead = lane == 0;
+    // The whole warp walks, one lane issues.
+    const bool lead = elect_one();
     const uint32_t idesc_s = umma_idesc_f16(kIsBf16, 128, 0);
     const uint32_t idesc_o = umma_idesc_f16(kIsBf16, (uint32_t)g.ksteps * 16, 1);
     const uint64_t dq0 = sw128_desc(smem_u32(sQ), 16, 1024);
@@ -258,20 +257,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto issue_s = [&](int w, int tile, Pos ks) {
       const uint64_t dq = dq0 + (uint64_t)(tile * kSlotDesc), dk = dk0 + (uint64_t)(ks.slot * kSlotDesc);
       const uint32_t dS = tmem + (uint32_t)(w * 128);
+      if (lead) {
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        if (kk >= ksteps) break;
-        const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
-        umma_f16_ss_lead(lead, dS, dq + off, dk + off, idesc_s, kk != 0);
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          if (kk >= ksteps) break;
+          const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
+          umma_f16_ss(dS, dq + off, dk + off, idesc_s, kk != 0);
+        }
+        umma_commit(&s_full[w]);
       }
-      umma_commit_lead(lead, &s_full[w]);
     };
     auto issue_pv = [&](int w, Pos vs, uint32_t acc) {
       const uint64_t dv = dv0 + (uint64_t)(vs.slot * kSlotDesc);
       const uint32_t pa = tmem + (uint32_t)(w * 128), dO = tmem + C::kColO + (uint32_t)(w * DP);
-      umma_f16_ts_lead(lead, dO, pa, dv, idesc_o, acc);
+      if (lead) {
+        umma_f16_ts(dO, pa, dv, idesc_o, acc);
 #pragma unroll
-      for (int kk = 1; kk < 8; ++kk) umma_f16_ts_lead(lead, dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
+        for (int kk = 1; kk < 8; ++kk) umma_f16_ts(dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
+      }
     };
     auto landed = [&](Pos s) -> bool {
       const bool r = mbar_wait<false>(&ready[s.slot], s.phase, kErrTimeoutAttnKV, abort_flag);
@@ -284,7 +287,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       return r;
     };
-    auto release = [&](Pos s) { umma_commit_lead(lead, &empty[s.slot]); };
+    auto commit = [&](uint64_t* bar) {
+      if (lead) umma_commit(bar);
+    };
+    auto release = [&](Pos s) { commit(&empty[s.slot]); };
     bool ok = true;
     while (ok && k.next(p, g)) {
       if (!mbar_wait<false>(q_full, k.seg & 1, kErrTimeoutAttnQ, abort_flag)) break;
@@ -310,15 +316,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           pos = kn;
         }
         if (!ok) break;
-        umma_commit_lead(lead, q_empty);
+        commit(q_empty);
         const Pos v = pos.plus(1);
         if (!(ok = landed(v) && wait_p(0, pp0))) break;
         issue_pv(0, v, n > 1);
-        umma_commit_lead(lead, &o_done[0]);
+        commit(&o_done[0]);
         if (!(ok = wait_p(1, pp1))) break;
         issue_pv(1, v, n > 1);
         release(v);
-        umma_commit_lead(lead, &o_done[1]);
+        commit(&o_done[1]);
         pos = pos.plus(2);
       } else {
         // ring: K, V of the first half's tile, then of the second's, which only the item's
@@ -353,19 +359,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           pos = ka;
         }
         if (!ok) break;
-        umma_commit_lead(lead, q_empty);
+        commit(q_empty);
         const Pos va = pos.plus(1);
         if (!(ok = landed(va) && wait_p(0, pp0))) break;
         issue_pv(0, va, n > 1);
         release(va);
-        umma_commit_lead(lead, &o_done[0]);
+        commit(&o_done[0]);
         if (second) {
           const Pos vb = pos.plus(3);
           if (!(ok = landed(vb) && wait_p(1, pp1))) break;
           issue_pv(1, vb, n > 1);
           release(vb);
         }
-        umma_commit_lead(lead, &o_done[1]);
+        commit(&o_done[1]);
         pos = pos.plus(second ? 4 : 2);
       }
     }
