@@ -15,15 +15,19 @@
 // order.  So few rows against a long encoder and ragged batches fill the GPU alike.
 //
 // CTA = 384 threads:
-//   warp 0      TMA producer: Q tiles, K and V tiles through one ring of slots
-//   warp 1      MMA issuer: S_w = Q_w K^T (SS) and O_w += P_w V (P from TMEM), per
-//               tile PV_w(j - 1) then S_w(j); owns TMEM
+//   warp 0      TMA producer: Q tiles, K and V tiles through a ring each
+//   warp 1      MMA issuer: S_w = Q_w K^T (SS) and O_w += P_w V (P from TMEM); owns TMEM
 //   warp 2      once a V tile has landed: rows of keys that are not kept are zeroed
 //               (0 * NaN would reach the sum otherwise), the tile's mask words published
 //   warps 4-11  softmax, tile (warp - 4) / 4, one query row per thread
-// TMEM: S_0 [0,128) S_1 [128,256) (P_w over S_w's first 64 columns), O_0 at 256, O_1 at
-// 256 + DP.  S_w(j) overwrites P_w(j-1) only after PV_w(j-1), issued before it by the
-// same thread, has read it.
+// The two tiles' steps (one K/V tile each) form one sequence s = 0, 1, 2, ..., tile s % 2.  S(s)
+// goes to one of NB buffers of 128 columns in TMEM and P(s) over its first half; S(s + NB) is
+// issued right after PV(s) and overwrites P(s) only once PV(s), issued before it by the same
+// thread, has read it.  head_dim <= 64 leaves room for NB = 3 next to O_0 and O_1 (2 x 64
+// columns): a tile's next scores are there before its softmax asks for them (two buffers:
+// 116 us for 4 x 8 heads of 1895 x 3792, three: 99).  Above, NB = 2, one a tile (four of 64 keys:
+// 980 us for the long prompts against 752; the 64-column MMAs read as much of Q for half the
+// products).
 //
 // Softmax: the reference a row is exponentiated against starts at the maximum of its
 // first 32 kept scores and moves lazily: a tile is taken in one pass without a
@@ -43,6 +47,7 @@ namespace {
 
 constexpr int kThreads = 384;
 constexpr int kSoftmaxWarp0 = 4;
+// A step's row sum bounds each of its weights; 4096 stays far inside fp16's range.
 constexpr float kSumLimit = 4096.0f;
 constexpr uint32_t kHalfBytes = 128 * 64 * 2;  // 128 rows x 64 columns
 
@@ -50,9 +55,40 @@ template <int DP>
 struct Cfg {
   static constexpr int kHalves = DP / 64;
   static constexpr uint32_t kTile = kHalves * kHalfBytes;      // one Q, K or V tile
-  static constexpr int kSlots = DP == 128 ? 5 : 8;             // ring of K and V tiles
-  static constexpr size_t kSmem = 2 * kTile + kSlots * kTile + 2560;
-  static constexpr uint32_t kColO = 256;
+  static constexpr int kKSlots = DP == 128 ? 3 : 5, kVSlots = DP == 128 ? 2 : 5;
+  static constexpr size_t kSmem = (2 + kKSlots + kVSlots) * kTile + 2560;
+  static_assert((18 + 2 * kKSlots + 3 * kVSlots) * 8 + 40 + kVSlots * 16 + 2048 <= 2560, "barriers and exchange");
+  static constexpr int kBufs = DP == 128 ? 2 : 3;              // NB
+  static constexpr uint32_t kColO = kBufs * 128;
+};
+
+// A position in a ring of N slots: the slot and the parity of its current use.
+template <int N>
+struct RingPos {
+  uint32_t slot = 0, phase = 0;
+  __device__ __forceinline__ RingPos plus(uint32_t n) const {  // n <= N
+    RingPos r;
+    r.slot = slot + n >= N ? slot + n - N : slot + n;
+    r.phase = slot + n >= N ? phase ^ 1 : phase;
+    return r;
+  }
+};
+
+// The S buffer of a step and the parity of that use.  Two buffers: one a tile, by the
+// tile's own count of steps; three: in turn over the sequence of both tiles.
+template <int NB>
+struct StepBuf {
+  uint32_t buf, parity;
+  __device__ __forceinline__ StepBuf(int w, uint32_t mine, uint32_t seq) {
+    if constexpr (NB == 2) {
+      buf = (uint32_t)w;
+      parity = mine & 1;
+    } else {
+      const uint32_t q = seq / 3;
+      buf = seq - 3 * q;
+      parity = q & 1;
+    }
+  }
 };
 
 // First token and head of row tile w of the current segment.
@@ -107,8 +143,8 @@ __device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], uint32_t word
   }
 }
 
-// P and the row sum of a whole 128-column row; the next chunk's load is in flight
-// while one is processed.  kAll: every key of the tile is kept.
+// P and the row sum of a step's 128 columns; the next chunk's load is in flight while
+// one is processed.  kAll: every key is kept.
 template <typename T, bool kAll>
 __device__ __forceinline__ float row_exp(uint32_t sAddr, const uint32_t (&words)[4], float c, float ref,
                                          uint32_t (&pk)[64]) {
@@ -138,39 +174,53 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<DP>;
   constexpr uint32_t kIsBf16 = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   extern __shared__ __align__(1024) uint8_t smem[];  // the swizzled tiles start on 1024 bytes
+  constexpr int NB = C::kBufs;
+  using KPos = RingPos<C::kKSlots>;
+  using VPos = RingPos<C::kVSlots>;
   uint8_t* sQ = smem;
-  uint8_t* sKV = sQ + 2 * C::kTile;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::kSlots * C::kTile);
+  uint8_t* sK = sQ + 2 * C::kTile;
+  uint8_t* sV = sK + C::kKSlots * C::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + C::kVSlots * C::kTile);
   uint64_t* q_full = bars;
   uint64_t* q_empty = bars + 1;
-  uint64_t* s_full = bars + 2;   // [2]
-  uint64_t* p_full = bars + 4;   // [2]
-  uint64_t* o_done = bars + 6;   // [2]
-  uint64_t* meet = bars + 8;     // [4 lane quarters]: the two halves of a lone tile
-  uint64_t* full = bars + 12;    // [slots] landed
-  uint64_t* ready = full + C::kSlots;   // [slots] fit for the MMA
-  uint64_t* empty = ready + C::kSlots;  // [slots]
-  Spot* s_spot = reinterpret_cast<Spot*>(empty + C::kSlots);
+  uint64_t* s_full = bars + 2;   // [NB buffers]
+  uint64_t* p_full = bars + 6;   // [NB buffers]
+  uint64_t* pv_done = bars + 10; // [2 tiles], every step
+  uint64_t* o_done = bars + 12;  // [2 tiles], every item
+  uint64_t* meet = bars + 14;    // [4 lane quarters]: the two halves of a lone tile
+  uint64_t* k_full = bars + 18;
+  uint64_t* k_empty = k_full + C::kKSlots;
+  uint64_t* v_full = k_empty + C::kKSlots;   // landed
+  uint64_t* v_ready = v_full + C::kVSlots;   // fit for the MMA
+  uint64_t* v_empty = v_ready + C::kVSlots;
+  Spot* s_spot = reinterpret_cast<Spot*>(v_empty + C::kVSlots);
   long long* s_count = reinterpret_cast<long long*>(s_spot + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_count + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* s_words = tmem_slot + 4;                                 // [slots][4] kept keys of a V slot
-  float* s_ml = reinterpret_cast<float*>(s_words + C::kSlots * 4);   // [2 halves][ref, l][128]
+  uint32_t* s_words = tmem_slot + 4;                                  // [V slots][4] kept keys
+  float* s_ml = reinterpret_cast<float*>(s_words + C::kVSlots * 4);   // [2 halves][ref, l][128]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
+    for (int i = 0; i < NB; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+    }
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&s_full[w], 1);
-      mbar_init(&p_full[w], 128);
+      mbar_init(&pv_done[w], 1);
       mbar_init(&o_done[w], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
-    for (int i = 0; i < C::kSlots; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&ready[i], 1);
-      mbar_init(&empty[i], 1);
+    for (int i = 0; i < C::kKSlots; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < C::kVSlots; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_ready[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -200,7 +250,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      uint32_t slot = 0, phase = 0;  // ring position
+      KPos kp;
+      VPos vp;
       bool ok = true;
       while (ok && k.next(p, g)) {
         if (!mbar_wait<false>(q_empty, (k.seg & 1) ^ 1, kErrTimeoutAttnQ, abort_flag)) break;
@@ -214,23 +265,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int kh = k.s.hk * g.k_headed, kb = k.s.b * g.k_batched;
         const int vh = k.s.hk * g.v_headed, vb = k.s.b * g.v_batched;
-        for (int j = k.j0; ok && j < k.j1; ++j) {
-          const int n = k.slots(j);
-          for (int i = 0; i < n; ++i) {
-            if (!mbar_wait<false>(&empty[slot], phase ^ 1, kErrTimeoutAttnKV, abort_flag)) {
-              ok = false;
-              break;
-            }
-            mbar_arrive_expect_tx(&full[slot], C::kTile);
-            const int row = k.kv_tile(i >> 1, j) * 128;
-            for (int h = 0; h < C::kHalves; ++h) {
-              uint8_t* dst = sKV + slot * C::kTile + h * kHalfBytes;
-              if (i & 1)
-                tma_load_4d(dst, &vmap, &full[slot], h * 64, row, vh, vb);
-              else
-                tma_load_4d(dst, &kmap, &full[slot], h * 64, row, kh, kb);
-            }
-            if (++slot == C::kSlots) slot = 0, phase ^= 1;
+        const int streams = k.lone ? 2 : 1;  // K/V tiles of a unit
+        // with three buffers S runs ahead of PV by up to two units, so K goes first
+        constexpr int kLead = NB == 3 ? 1 : 0;
+        for (int i = k.j0; ok && i < k.j1 + kLead; ++i) {
+          for (int w = 0; w < streams && i < k.j1 && k.uses(w, i); ++w) {
+            if (!(ok = mbar_wait<false>(&k_empty[kp.slot], kp.phase ^ 1, kErrTimeoutAttnKV, abort_flag))) break;
+            mbar_arrive_expect_tx(&k_full[kp.slot], C::kTile);
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_load_4d(sK + kp.slot * C::kTile + h * kHalfBytes, &kmap, &k_full[kp.slot], h * 64,
+                          k.kv_tile(w, i) * 128, kh, kb);
+            kp = kp.plus(1);
+          }
+          const int v = i - kLead;
+          for (int w = 0; ok && w < streams && v >= k.j0 && k.uses(w, v); ++w) {
+            if (!(ok = mbar_wait<false>(&v_empty[vp.slot], vp.phase ^ 1, kErrTimeoutAttnKV, abort_flag))) break;
+            mbar_arrive_expect_tx(&v_full[vp.slot], C::kTile);
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_load_4d(sV + vp.slot * C::kTile + h * kHalfBytes, &vmap, &v_full[vp.slot], h * 64,
+                          k.kv_tile(w, v) * 128, vh, vb);
+            vp = vp.plus(1);
           }
         }
       }
@@ -242,179 +296,120 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t idesc_s = umma_idesc_f16(kIsBf16, 128, 0);
     const uint32_t idesc_o = umma_idesc_f16(kIsBf16, (uint32_t)g.ksteps * 16, 1);
     const uint64_t dq0 = sw128_desc(smem_u32(sQ), 16, 1024);
-    const uint64_t dk0 = sw128_desc(smem_u32(sKV), 16, 1024);
-    const uint64_t dv0 = sw128_desc(smem_u32(sKV), kHalfBytes, 1024);
-    constexpr uint32_t kSlotDesc = C::kTile >> 4;
+    const uint64_t dk0 = sw128_desc(smem_u32(sK), 16, 1024);
+    const uint64_t dv0 = sw128_desc(smem_u32(sV), kHalfBytes, 1024);
+    constexpr uint32_t kTileDesc = C::kTile >> 4;
     const int ksteps = g.ksteps;
-    struct Pos {
-      uint32_t slot, phase;
-      __device__ __forceinline__ Pos plus(uint32_t n) const {
-        return slot + n >= C::kSlots ? Pos{slot + n - C::kSlots, phase ^ 1} : Pos{slot + n, phase};
-      }
-    };
-    Pos pos{0, 0};              // ring position of the current unit's first slot
-    uint32_t pp0 = 0, pp1 = 0;  // phases of p_full
-    auto issue_s = [&](int w, int tile, Pos ks) {
-      const uint64_t dq = dq0 + (uint64_t)(tile * kSlotDesc), dk = dk0 + (uint64_t)(ks.slot * kSlotDesc);
-      const uint32_t dS = tmem + (uint32_t)(w * 128);
-      if (lead) {
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          if (kk >= ksteps) break;
-          const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
-          umma_f16_ss(dS, dq + off, dk + off, idesc_s, kk != 0);
-        }
-        umma_commit(&s_full[w]);
-      }
-    };
-    auto issue_pv = [&](int w, Pos vs, uint32_t acc) {
-      const uint64_t dv = dv0 + (uint64_t)(vs.slot * kSlotDesc);
-      const uint32_t pa = tmem + (uint32_t)(w * 128), dO = tmem + C::kColO + (uint32_t)(w * DP);
-      if (lead) {
-        umma_f16_ts(dO, pa, dv, idesc_o, acc);
-#pragma unroll
-        for (int kk = 1; kk < 8; ++kk) umma_f16_ts(dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
-      }
-    };
-    auto landed = [&](Pos s) -> bool {
-      const bool r = mbar_wait<false>(&ready[s.slot], s.phase, kErrTimeoutAttnKV, abort_flag);
-      tc_fence_after();
-      return r;
-    };
-    auto wait_p = [&](int w, uint32_t& par) -> bool {
-      const bool r = mbar_wait<false>(&p_full[w], par, kErrTimeoutAttnP, abort_flag);
-      par ^= 1;
-      tc_fence_after();
-      return r;
-    };
-    auto commit = [&](uint64_t* bar) {
-      if (lead) umma_commit(bar);
-    };
-    auto release = [&](Pos s) { commit(&empty[s.slot]); };
+    KPos kp;                    // next K slot to wait for
+    VPos vp;
+    uint32_t kc[2] = {0, 0};    // slots in use
+    uint32_t vc[2] = {0, 0};
+    uint32_t mine[2] = {0, 0}, pmine[2] = {0, 0};  // S and PV issued so far, per tile
+    uint32_t seq = 0;           // position in the sequence of the segment's first step
     bool ok = true;
     while (ok && k.next(p, g)) {
       if (!mbar_wait<false>(q_full, k.seg & 1, kErrTimeoutAttnQ, abort_flag)) break;
       tc_fence_after();
-      const int n = k.j1 - k.j0;
-      if (!k.lone) {
-        // ring: K, V per unit, both tiles' users of each
-        if (!(ok = landed(pos))) break;
-        issue_s(0, 0, pos);
-        issue_s(1, 1, pos);
-        release(pos);
-        for (int j = 1; j < n; ++j) {
-          const Pos v = pos.plus(1), kn = pos.plus(2);
-          if (!(ok = landed(v) && wait_p(0, pp0))) break;
-          issue_pv(0, v, j > 1);
-          if (!(ok = landed(kn))) break;
-          issue_s(0, 0, kn);
-          if (!(ok = wait_p(1, pp1))) break;
-          issue_pv(1, v, j > 1);
-          release(v);
-          issue_s(1, 1, kn);
-          release(kn);
-          pos = kn;
+      const int steps = k.j1 - k.j0;
+      // steps of the second tile: all, but for a lone tile's last unit without a K/V tile for it
+      const int steps1 = k.uses(1, k.j1 - 1) ? steps : steps - 1;
+      const bool lone = k.lone;
+      // S of step t of tile w
+      auto do_s = [&](const int w, const int t) -> bool {
+        if (t >= (w ? steps1 : steps)) return true;
+        if (w == 0 || lone) {
+          if (!mbar_wait<false>(&k_full[kp.slot], kp.phase, kErrTimeoutAttnKV, abort_flag)) return false;
+          kc[w] = kp.slot;
+          kp = kp.plus(1);
+          tc_fence_after();
         }
-        if (!ok) break;
-        commit(q_empty);
-        const Pos v = pos.plus(1);
-        if (!(ok = landed(v) && wait_p(0, pp0))) break;
-        issue_pv(0, v, n > 1);
-        commit(&o_done[0]);
-        if (!(ok = wait_p(1, pp1))) break;
-        issue_pv(1, v, n > 1);
-        release(v);
-        commit(&o_done[1]);
-        pos = pos.plus(2);
-      } else {
-        // ring: K, V of the first half's tile, then of the second's, which only the item's
-        // last unit may lack
-        bool second = k.uses(1, k.j0);
-        if (!(ok = landed(pos))) break;
-        issue_s(0, 0, pos);
-        release(pos);
-        if (second) {
-          const Pos kb = pos.plus(2);
-          if (!(ok = landed(kb))) break;
-          issue_s(1, 0, kb);
-          release(kb);
-        }
-        for (int j = 1; j < n; ++j) {
-          const Pos va = pos.plus(1), vb = pos.plus(3), ka = pos.plus(4), kb = ka.plus(2);
-          second = k.uses(1, k.j0 + j);
-          if (!(ok = landed(va) && wait_p(0, pp0))) break;
-          issue_pv(0, va, j > 1);
-          release(va);
-          if (!(ok = landed(ka))) break;
-          issue_s(0, 0, ka);
-          release(ka);
-          if (!(ok = landed(vb) && wait_p(1, pp1))) break;
-          issue_pv(1, vb, j > 1);
-          release(vb);
-          if (second) {
-            if (!(ok = landed(kb))) break;
-            issue_s(1, 0, kb);
-            release(kb);
+        const uint32_t slot = lone ? kc[w] : kc[0];
+        const StepBuf<NB> b(w, mine[w]++, seq + 2 * t + w);
+        if (lead) {
+          const uint64_t dq = dq0 + (uint64_t)((lone ? 0 : w) * kTileDesc);
+          const uint64_t dk = dk0 + (uint64_t)(slot * kTileDesc);
+          const uint32_t dS = tmem + b.buf * 128;
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            if (kk >= ksteps) break;
+            const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
+            umma_f16_ss(dS, dq + off, dk + off, idesc_s, kk != 0);
           }
-          pos = ka;
+          umma_commit(&s_full[b.buf]);
+          if (w == 1 || lone) umma_commit(&k_empty[slot]);
         }
-        if (!ok) break;
-        commit(q_empty);
-        const Pos va = pos.plus(1);
-        if (!(ok = landed(va) && wait_p(0, pp0))) break;
-        issue_pv(0, va, n > 1);
-        release(va);
-        commit(&o_done[0]);
-        if (second) {
-          const Pos vb = pos.plus(3);
-          if (!(ok = landed(vb) && wait_p(1, pp1))) break;
-          issue_pv(1, vb, n > 1);
-          release(vb);
+        return true;
+      };
+      // PV of step t of tile w
+      auto do_pv = [&](const int w, const int t) -> bool {
+        if (t >= (w ? steps1 : steps)) return true;
+        if (w == 0 || lone) {
+          if (!mbar_wait<false>(&v_ready[vp.slot], vp.phase, kErrTimeoutAttnKV, abort_flag)) return false;
+          vc[w] = vp.slot;
+          vp = vp.plus(1);
         }
-        commit(&o_done[1]);
-        pos = pos.plus(second ? 4 : 2);
+        const uint32_t slot = lone ? vc[w] : vc[0];
+        const StepBuf<NB> b(w, pmine[w]++, seq + 2 * t + w);
+        if (!mbar_wait<false>(&p_full[b.buf], b.parity, kErrTimeoutAttnP, abort_flag)) return false;
+        tc_fence_after();
+        if (lead) {
+          const uint64_t dv = dv0 + (uint64_t)(slot * kTileDesc);
+          const uint32_t pa = tmem + b.buf * 128, dO = tmem + C::kColO + (uint32_t)(w * DP);
+          umma_f16_ts(dO, pa, dv, idesc_o, t > 0);
+#pragma unroll
+          for (int kk = 1; kk < 8; ++kk) umma_f16_ts(dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
+          umma_commit(&pv_done[w]);
+          if (w == 1 || lone) umma_commit(&v_empty[slot]);
+        }
+        return true;
+      };
+      // S(s + NB) behind PV(s)
+      if (!(ok = do_s(0, 0) && do_s(1, 0) && (NB == 2 || do_s(0, 1)))) break;
+      for (int t = 0; t < steps; ++t) {
+        if (!(ok = do_pv(0, t))) break;
+        if (lead && t == steps - 1) umma_commit(&o_done[0]);
+        if (!(ok = NB == 3 ? do_s(1, t + 1) : do_s(0, t + 1))) break;
+        if (!(ok = do_pv(1, t) && (NB == 3 ? do_s(0, t + 2) : do_s(1, t + 1)))) break;
+        if (lead && t == (steps > 1 ? steps - 2 : 0)) umma_commit(q_empty);  // every S has been issued
       }
+      if (ok && lead) umma_commit(&o_done[1]);
+      seq += (uint32_t)(steps + steps1);
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ rows that are not kept
-    uint32_t slot = 0, phase = 0;
+    VPos vp;
     bool ok = true;
     while (ok && k.next(p, g)) {
+      const int streams = k.lone ? 2 : 1;
       for (int j = k.j0; ok && j < k.j1; ++j) {
-        const int n = k.slots(j);
-        for (int i = 0; i < n; ++i) {
-          if (!mbar_wait<false>(&full[slot], phase, kErrTimeoutAttnKV, abort_flag)) {
-            ok = false;
-            break;
-          }
-          if (i & 1) {
-            const int key0 = k.kv_tile(i >> 1, j) * 128, khi = k.keys - key0;
-            if (kMask || khi < 128) {
-              bool touched = false;
+        for (int w = 0; w < streams && k.uses(w, j); ++w) {
+          if (!(ok = mbar_wait<false>(&v_full[vp.slot], vp.phase, kErrTimeoutAttnKV, abort_flag))) break;
+          const int key0 = k.kv_tile(w, j) * 128, khi = k.keys - key0;
+          if (kMask || khi < 128) {
+            bool touched = false;
 #pragma unroll
-              for (int ch = 0; ch < 4; ++ch) {
-                const int row = ch * 32 + lane;
-                bool keep = row < khi;
-                if (kMask && keep) keep = p.key_mask[(size_t)k.s.b * p.k_len + key0 + row] != 0;
-                const uint32_t word = __ballot_sync(0xffffffffu, keep);
-                if (kMask && lane == 0) s_words[slot * 4 + ch] = word;
-                if (word == 0xffffffffu) continue;
-                touched = true;
-                if (!keep) {
-                  // a lane's row, its pieces in an order that keeps the lanes on different banks
-                  uint8_t* at = sKV + slot * C::kTile + row * 128;
+            for (int ch = 0; ch < 4; ++ch) {
+              const int row = ch * 32 + lane;
+              bool keep = row < khi;
+              if (kMask && keep) keep = p.key_mask[(size_t)k.s.b * p.k_len + key0 + row] != 0;
+              const uint32_t word = __ballot_sync(0xffffffffu, keep);
+              if (kMask && lane == 0) s_words[vp.slot * 4 + ch] = word;
+              if (word == 0xffffffffu) continue;
+              touched = true;
+              if (!keep) {
+                // a lane's row, its pieces in an order that keeps the lanes on different banks
+                uint8_t* at = sV + vp.slot * C::kTile + row * 128;
 #pragma unroll
-                  for (int x = 0; x < 8 * C::kHalves; ++x)
-                    *reinterpret_cast<uint4*>(at + (x >> 3) * kHalfBytes + (((x + lane) & 7) << 4)) =
-                        make_uint4(0u, 0u, 0u, 0u);
-                }
+                for (int x = 0; x < 8 * C::kHalves; ++x)
+                  *reinterpret_cast<uint4*>(at + (x >> 3) * kHalfBytes + (((x + lane) & 7) << 4)) =
+                      make_uint4(0u, 0u, 0u, 0u);
               }
-              if (touched) fence_proxy_async_smem();
-              __syncwarp();
             }
+            if (touched) fence_proxy_async_smem();
+            __syncwarp();
           }
-          if (lane == 0) mbar_arrive(&ready[slot]);
-          if (++slot == C::kSlots) slot = 0, phase ^= 1;
+          if (lane == 0) mbar_arrive(&v_ready[vp.slot]);
+          vp = vp.plus(1);
         }
       }
     }
@@ -423,11 +418,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int w = (warp - kSoftmaxWarp0) >> 2, q = warp & 3;
     const int row = q * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-    const uint32_t sAddr = tmem + lane_off + (uint32_t)(w * 128);
     const uint32_t oAddr = tmem + lane_off + C::kColO + (uint32_t)(w * DP);
     const float c = p.scale_log2;
-    uint32_t slot = 0, phase = 0;       // ring position (masks are read at V slots)
-    uint32_t scnt = 0, meets = 0;
+    VPos vp;                            // V slot of the current unit (its mask words)
+    uint32_t mine = 0, seq = 0;         // this tile's steps so far; sequence position of the segment
+    uint32_t meets = 0;
     bool ok = true;
     while (ok && k.next(p, g)) {
       int n0, g0;
@@ -437,66 +432,78 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool warp_active = __any_sync(0xffffffffu, valid);
       float ref = 0.f, l = 0.f;
       bool have = false;  // the reference is set
-      int used = 0;
-      for (int j = k.j0; j < k.j1; ++j) {
-        // the V slot of this tile's unit, where its mask words are
-        uint32_t vs = 0, vphase = 0;
-        if constexpr (kMask) {
-          vs = slot + (k.lone ? 2 * w : 0) + 1;
-          vphase = phase;
-          if (vs >= C::kSlots) vs -= C::kSlots, vphase ^= 1;
-          slot += k.slots(j);
-          if (slot >= C::kSlots) slot -= C::kSlots, phase ^= 1;
-        }
-        if (!k.uses(w, j)) continue;
-        if (!mbar_wait<false>(&s_full[w], scnt & 1, kErrTimeoutAttnS, abort_flag)) {
-          ok = false;
-          break;
-        }
-        ++scnt;
+      const int all_steps = k.j1 - k.j0, steps1 = k.uses(1, k.j1 - 1) ? all_steps : all_steps - 1;
+      const int steps = w ? steps1 : all_steps;
+      VPos vs = k.lone ? vp.plus(w) : vp;
+      for (int t = 0; t < steps; ++t, ++mine) {
+        const StepBuf<NB> b(w, mine, seq + 2 * t + w);
+        const uint32_t sAddr = tmem + lane_off + b.buf * 128;
         uint32_t words[4];
         if constexpr (kMask) {
-          if (!mbar_wait<false>(&ready[vs], vphase, kErrTimeoutAttnKV, abort_flag)) {
+          if (!mbar_wait<false>(&v_ready[vs.slot], vs.phase, kErrTimeoutAttnKV, abort_flag)) {
             ok = false;
             break;
           }
 #pragma unroll
-          for (int ch = 0; ch < 4; ++ch) words[ch] = s_words[vs * 4 + ch];
+          for (int ch = 0; ch < 4; ++ch) words[ch] = s_words[vs.slot * 4 + ch];
+          vs = vs.plus(k.lone ? 2 : 1);
         } else {
-          const int khi = k.keys - k.kv_tile(w, j) * 128;
+          const int khi = k.keys - k.kv_tile(w, k.j0 + t) * 128;
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch) words[ch] = len_word(khi, ch);
+        }
+        uint32_t all = 0xffffffffu, any = 0u;
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) all &= words[ch], any |= words[ch];
+        if (!mbar_wait<false>(&s_full[b.buf], b.parity, kErrTimeoutAttnS, abort_flag)) {
+          ok = false;
+          break;
         }
         tc_fence_after();
         if (warp_active) {
           uint32_t pk[64];
-          const bool any = (words[0] | words[1] | words[2] | words[3]) != 0u;
-          const bool all = (words[0] & words[1] & words[2] & words[3]) == 0xffffffffu;
-          float sum = 0.f;
-          if (!have && any) {
-            const int ch = words[0] ? 0 : (words[1] ? 1 : (words[2] ? 2 : 3));
-            uint32_t r[32];
-            tmem_ld32(sAddr + ch * 32, r);
-            tmem_ld_wait(r);
-            const float m = chunk_max(r, words[ch], c);
-            ref = m == -INFINITY ? 0.f : m;
-            have = true;
-          }
           if (any) {
-            sum = all ? row_exp<T, true>(sAddr, words, c, ref, pk) : row_exp<T, false>(sAddr, words, c, ref, pk);
+            if (!have) {
+              int ch = 0;
+#pragma unroll
+              for (int i = 3; i > 0; --i)
+                if (!words[0] && words[i]) ch = i;
+              uint32_t first = words[0];
+#pragma unroll
+              for (int i = 1; i < 4; ++i)
+                if (i == ch) first = words[i];
+              uint32_t r[32];
+              tmem_ld32(sAddr + ch * 32, r);
+              tmem_ld_wait(r);
+              const float m = chunk_max(r, first, c);
+              ref = m == -INFINITY ? 0.f : m;
+              have = true;
+            }
+            float sum = all == 0xffffffffu ? row_exp<T, true>(sAddr, words, c, ref, pk)
+                                           : row_exp<T, false>(sAddr, words, c, ref, pk);
             if (__any_sync(0xffffffffu, valid && !(sum <= kSumLimit))) {
               // exact passes: the reference moves to the row's maximum, O and l with it
               float m = -INFINITY;
 #pragma unroll 1
               for (int ch = 0; ch < 4; ++ch) {
-                uint32_t r[32];
+                uint32_t r[32], word = words[0];
+#pragma unroll
+                for (int i = 1; i < 4; ++i)
+                  if (i == ch) word = words[i];
                 tmem_ld32(sAddr + ch * 32, r);
                 tmem_ld_wait(r);
-                m = fmaxf(m, chunk_max(r, words[ch], c));
+                m = fmaxf(m, chunk_max(r, word, c));
               }
               const float moved = fmaxf(ref, m);
               const float alpha = fast_exp2(ref - moved);
-              if (used > 0) {
+              if (t > 0) {
+                // O holds the previous steps once the last PV is through (the one before it was
+                // when this step's S was issued, so the parity is the right phase's)
+                if (!mbar_wait<false>(&pv_done[w], (mine - 1) & 1, kErrTimeoutAttnO, abort_flag)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
 #pragma unroll 1
                 for (int h = 0; h < DP / 32; ++h) {
                   uint32_t r[32];
@@ -512,20 +519,29 @@ __global__ void __launch_bounds__(kThreads, 1)
               ref = moved;
               sum = row_exp<T, false>(sAddr, words, c, ref, pk);
             }
+            l += sum;
           } else {
 #pragma unroll
             for (int i = 0; i < 64; ++i) pk[i] = 0u;
           }
-          l += sum;
           tmem_st32(sAddr, *reinterpret_cast<const uint32_t(*)[32]>(pk));
           tmem_st32(sAddr + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
           tmem_st_wait();
         }
-        ++used;
+        // (a barrier a buffer: the tile's other warps may be a step ahead)
         tc_fence_before();
-        mbar_arrive(&p_full[w]);
+        mbar_arrive(&p_full[b.buf]);
       }
       if (!ok) break;
+      seq += (uint32_t)(all_steps + steps1);
+      if constexpr (kMask) {
+        // past the V slots of the segment
+        for (int i = k.lone ? all_steps + steps1 : all_steps; i > 0;) {
+          const int m = min(i, C::kVSlots);
+          vp = vp.plus(m);
+          i -= m;
+        }
+      }
       if (!mbar_wait<false>(&o_done[w], k.seg & 1, kErrTimeoutAttnO, abort_flag)) break;
       tc_fence_after();
       // a lone tile: the two halves meet, weigh each other in and write half the columns each
@@ -535,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (k.lone) {
         float* ml = s_ml;
         ml[w * 256 + row] = ref;
-        ml[w * 256 + 128 + row] = used > 0 ? l : -1.f;  // -1: no O
+        ml[w * 256 + 128 + row] = steps > 0 ? l : -1.f;  // -1: no O
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&meet[q]);

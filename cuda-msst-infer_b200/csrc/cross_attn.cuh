@@ -130,8 +130,6 @@ struct Walk {
   // K/V tile of query tile w in unit j, and whether it has one
   __device__ __forceinline__ int kv_tile(int w, int j) const { return lone ? 2 * j + w : j; }
   __device__ __forceinline__ bool uses(int w, int j) const { return kv_tile(w, j) < tiles; }
-  // ring slots that unit j takes
-  __device__ __forceinline__ int slots(int j) const { return lone ? (uses(1, j) ? 4 : 2) : 2; }
 };
 
 
