@@ -406,55 +406,51 @@ __global__ void __launch_bounds__(kThreadsA, 1)
       }
     }
   } else if (warp == 1) {
-    // the whole warp walks, one lane issues
-    const bool lead = elect_one();
-    const uint32_t idesc = umma_idesc_f16(kIsBf16, BT, 0);
-    int it = 0, n = 0;
-    uint32_t uses = 0;  // parity of each stage's uses for slices
-    bool ok = true;
-    for (int tile = tile0; ok && tile < total; tile += step, ++n) {
-      const int tt = tile / pl.n_tiles, buf = n & 1;
-      const uint32_t acc = tmem + (uint32_t)(buf * BT);
-      if (!mbar_wait(&acc_empty[buf], ((n >> 1) & 1) ^ 1, kErrTimeoutTmemEmpty, abort_flag)) break;
-      tc_fence_after();
-      int s0 = 0, s1 = 0;
-      if (n > 0) slice_range(lists + (size_t)tt * pl.list_ld, s0, s1);  // fetched ahead of its use
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int st = it % C::kStages;
-        if (!mbar_wait(&full[st], (it / C::kStages) & 1, kErrTimeoutTmaFull, abort_flag)) {
-          ok = false;
-          break;
-        }
+    if (elect_one()) {
+      const uint32_t idesc = umma_idesc_f16(kIsBf16, BT, 0);
+      int it = 0, n = 0;
+      uint32_t uses = 0;  // parity of each stage's uses for slices
+      bool ok = true;
+      for (int tile = tile0; ok && tile < total; tile += step, ++n) {
+        const int tt = tile / pl.n_tiles, buf = n & 1;
+        const uint32_t acc = tmem + (uint32_t)(buf * BT);
+        if (!mbar_wait(&acc_empty[buf], ((n >> 1) & 1) ^ 1, kErrTimeoutTmemEmpty, abort_flag)) break;
         tc_fence_after();
-        const uint64_t dm = sw128_desc(smem_u32(smem + st * C::kStage), 16, 1024);
-        const uint64_t dn = sw128_desc(smem_u32(smem + st * C::kStage + kMTile), 16, 1024);
-        if (lead) {
+        int s0 = 0, s1 = 0;
+        if (n > 0) slice_range(lists + (size_t)tt * pl.list_ld, s0, s1);  // fetched ahead of its use
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int st = it % C::kStages;
+          if (!mbar_wait(&full[st], (it / C::kStages) & 1, kErrTimeoutTmaFull, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t dm = sw128_desc(smem_u32(smem + st * C::kStage), 16, 1024);
+          const uint64_t dn = sw128_desc(smem_u32(smem + st * C::kStage + kMTile), 16, 1024);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) umma_f16_ss(acc, dm + 2 * kk, dn + 2 * kk, idesc, kb > kb0 || kk > 0);
           umma_commit(&empty[st]);
         }
-      }
-      if (n == 0) {
-        wait_for_previous();
-        slice_range(lists + (size_t)tt * pl.list_ld, s0, s1);
-      }
-      for (; ok && s0 < s1; s0 += 4, ++it) {
-        const int st = it % C::kStages, m = min(4, s1 - s0);
-        if (!mbar_wait(&u_full[st], uses >> st & 1, kErrTimeoutTmaFull, abort_flag)) {
-          ok = false;
-          break;
+        if (n == 0) {
+          wait_for_previous();
+          slice_range(lists + (size_t)tt * pl.list_ld, s0, s1);
         }
-        uses ^= 1u << st;
-        tc_fence_after();
-        const uint64_t dm = sw32_desc(smem_u32(smem + st * C::kStage));
-        const uint64_t dn = sw32_desc(smem_u32(smem + st * C::kStage + kMTile));
-        if (lead) {
+        for (; ok && s0 < s1; s0 += 4, ++it) {
+          const int st = it % C::kStages, m = min(4, s1 - s0);
+          if (!mbar_wait(&u_full[st], uses >> st & 1, kErrTimeoutTmaFull, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uses ^= 1u << st;
+          tc_fence_after();
+          const uint64_t dm = sw32_desc(smem_u32(smem + st * C::kStage));
+          const uint64_t dn = sw32_desc(smem_u32(smem + st * C::kStage + kMTile));
           for (int i = 0; i < m; ++i)
             umma_f16_ss(acc, dm + (uint64_t)(i * (4096 >> 4)), dn + (uint64_t)(i * (BT * 32 >> 4)), idesc, 1u);
           umma_commit(&empty[st]);
         }
+        if (ok) umma_commit(&acc_full[buf]);
       }
-      if (ok && lead) umma_commit(&acc_full[buf]);
     }
   } else if (warp < 6) {
     // ------------------------------------------------------------ U' of the slices

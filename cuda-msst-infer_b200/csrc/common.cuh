@@ -193,6 +193,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
   }
 }
 
+// The same for a warp that walks a role together, with a uniform result.  Every lane is held
+// until all have seen the phase: a lane left behind in the spin while the issuing lane went
+// on could find the barrier two phases further, which looks like the phase not completed.
+template <bool kSuspend = true>
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, unsigned code, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait<kSuspend>(bar, parity, code, abort));
+}
+
 // ---------------------------------------------------------------------------
 // TMA (cp.async.bulk.tensor), tiled mode, completion through an mbarrier.  No
 // cluster multicast anywhere in this library.
@@ -317,10 +325,10 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
 // ---------------------------------------------------------------------------
 // tcgen05 / UMMA
 // ---------------------------------------------------------------------------
-// One lane of a converged warp.  Issue blocks under this predicate compile to the plain
-// instructions; under lane == 0 the compiler cannot tell that one lane is left and wraps every
-// tcgen05.mma and commit (measured in cross_attention_kernel: 77 cycles an MMA and 70 a
-// commit against 26-61 and 12).
+// One lane of a converged warp.  A role under this predicate compiles its tcgen05.mma and
+// commits to the plain instructions; under lane == 0 the compiler cannot tell that one
+// lane is left and wraps each of them (measured in cross_attention_kernel: 77 cycles an
+// MMA and 70 a commit against 26-61 and 12).
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile(

@@ -47,6 +47,9 @@ namespace {
 
 constexpr int kThreads = 384;
 constexpr int kSoftmaxWarp0 = 4;
+// Registers a thread after the split: 128 x 88 + 256 x 208 = 384 x 168, the block's launch share
+// (softmax warps without spills: 2 % faster at both head sizes).
+constexpr int kFewRegs = 88, kSoftmaxRegs = 208;
 // A step's row sum bounds each of its weights; 4096 stays far inside fp16's range.
 constexpr float kSumLimit = 4096.0f;
 constexpr uint32_t kHalfBytes = 128 * 64 * 2;  // 128 rows x 64 columns
@@ -247,173 +250,173 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   Walk k(*s_spot, *s_count);
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      KPos kp;
+  if (warp < kSoftmaxWarp0) {
+    warpgroup_reg_dec<kFewRegs>();
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA producer
+      if (lane == 0) {
+        KPos kp;
+        VPos vp;
+        bool ok = true;
+        while (ok && k.next(p, g)) {
+          if (!mbar_wait<false>(q_empty, (k.seg & 1) ^ 1, kErrTimeoutAttnQ, abort_flag)) break;
+          const int nq = k.lone ? 1 : 2;
+          mbar_arrive_expect_tx(q_full, nq * C::kHalves * (uint32_t)(g.gt * g.nt) * 128u);
+          for (int w = 0; w < nq; ++w) {
+            int n0, g0;
+            tile_origin(k, g, w, n0, g0);
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_load_5d(sQ + w * C::kTile + h * kHalfBytes, &qmap, q_full, h * 64, g0, n0, k.s.hk, k.s.b * g.q_batched);
+          }
+          const int kh = k.s.hk * g.k_headed, kb = k.s.b * g.k_batched;
+          const int vh = k.s.hk * g.v_headed, vb = k.s.b * g.v_batched;
+          const int streams = k.lone ? 2 : 1;  // K/V tiles of a unit
+          // with three buffers S runs ahead of PV by up to two units, so K goes first
+          constexpr int kLead = NB == 3 ? 1 : 0;
+          for (int i = k.j0; ok && i < k.j1 + kLead; ++i) {
+            for (int w = 0; w < streams && i < k.j1 && k.uses(w, i); ++w) {
+              if (!(ok = mbar_wait<false>(&k_empty[kp.slot], kp.phase ^ 1, kErrTimeoutAttnKV, abort_flag))) break;
+              mbar_arrive_expect_tx(&k_full[kp.slot], C::kTile);
+              for (int h = 0; h < C::kHalves; ++h)
+                tma_load_4d(sK + kp.slot * C::kTile + h * kHalfBytes, &kmap, &k_full[kp.slot], h * 64,
+                            k.kv_tile(w, i) * 128, kh, kb);
+              kp = kp.plus(1);
+            }
+            const int v = i - kLead;
+            for (int w = 0; ok && w < streams && v >= k.j0 && k.uses(w, v); ++w) {
+              if (!(ok = mbar_wait<false>(&v_empty[vp.slot], vp.phase ^ 1, kErrTimeoutAttnKV, abort_flag))) break;
+              mbar_arrive_expect_tx(&v_full[vp.slot], C::kTile);
+              for (int h = 0; h < C::kHalves; ++h)
+                tma_load_4d(sV + vp.slot * C::kTile + h * kHalfBytes, &vmap, &v_full[vp.slot], h * 64,
+                            k.kv_tile(w, v) * 128, vh, vb);
+              vp = vp.plus(1);
+            }
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      if (elect_one()) {
+        const uint32_t idesc_s = umma_idesc_f16(kIsBf16, 128, 0);
+        const uint32_t idesc_o = umma_idesc_f16(kIsBf16, (uint32_t)g.ksteps * 16, 1);
+        const uint64_t dq0 = sw128_desc(smem_u32(sQ), 16, 1024);
+        const uint64_t dk0 = sw128_desc(smem_u32(sK), 16, 1024);
+        const uint64_t dv0 = sw128_desc(smem_u32(sV), kHalfBytes, 1024);
+        constexpr uint32_t kTileDesc = C::kTile >> 4;
+        const int ksteps = g.ksteps;
+        KPos kp;                    // next K slot to wait for
+        VPos vp;
+        uint32_t kc[2] = {0, 0};    // slots in use
+        uint32_t vc[2] = {0, 0};
+        uint32_t mine[2] = {0, 0}, pmine[2] = {0, 0};  // S and PV issued so far, per tile
+        uint32_t seq = 0;           // position in the sequence of the segment's first step
+        bool ok = true;
+        while (ok && k.next(p, g)) {
+          if (!mbar_wait<false>(q_full, k.seg & 1, kErrTimeoutAttnQ, abort_flag)) break;
+          tc_fence_after();
+          const int steps = k.j1 - k.j0;
+          // steps of the second tile: all, but for a lone tile's last unit without a K/V tile for it
+          const int steps1 = k.uses(1, k.j1 - 1) ? steps : steps - 1;
+          const bool lone = k.lone;
+          // S of step t of tile w
+          auto do_s = [&](const int w, const int t) -> bool {
+            if (t >= (w ? steps1 : steps)) return true;
+            if (w == 0 || lone) {
+              if (!mbar_wait<false>(&k_full[kp.slot], kp.phase, kErrTimeoutAttnKV, abort_flag)) return false;
+              kc[w] = kp.slot;
+              kp = kp.plus(1);
+              tc_fence_after();
+            }
+            const uint32_t slot = lone ? kc[w] : kc[0];
+            const StepBuf<NB> b(w, mine[w]++, seq + 2 * t + w);
+            const uint64_t dq = dq0 + (uint64_t)((lone ? 0 : w) * kTileDesc);
+            const uint64_t dk = dk0 + (uint64_t)(slot * kTileDesc);
+            const uint32_t dS = tmem + b.buf * 128;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+              if (kk >= ksteps) break;
+              const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
+              umma_f16_ss(dS, dq + off, dk + off, idesc_s, kk != 0);
+            }
+            umma_commit(&s_full[b.buf]);
+            if (w == 1 || lone) umma_commit(&k_empty[slot]);
+            return true;
+          };
+          // PV of step t of tile w
+          auto do_pv = [&](const int w, const int t) -> bool {
+            if (t >= (w ? steps1 : steps)) return true;
+            if (w == 0 || lone) {
+              if (!mbar_wait<false>(&v_ready[vp.slot], vp.phase, kErrTimeoutAttnKV, abort_flag)) return false;
+              vc[w] = vp.slot;
+              vp = vp.plus(1);
+            }
+            const uint32_t slot = lone ? vc[w] : vc[0];
+            const StepBuf<NB> b(w, pmine[w]++, seq + 2 * t + w);
+            if (!mbar_wait<false>(&p_full[b.buf], b.parity, kErrTimeoutAttnP, abort_flag)) return false;
+            tc_fence_after();
+            const uint64_t dv = dv0 + (uint64_t)(slot * kTileDesc);
+            const uint32_t pa = tmem + b.buf * 128, dO = tmem + C::kColO + (uint32_t)(w * DP);
+            umma_f16_ts(dO, pa, dv, idesc_o, t > 0);
+#pragma unroll
+            for (int kk = 1; kk < 8; ++kk) umma_f16_ts(dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
+            umma_commit(&pv_done[w]);
+            if (w == 1 || lone) umma_commit(&v_empty[slot]);
+            return true;
+          };
+          // S(s + NB) behind PV(s)
+          if (!(ok = do_s(0, 0) && do_s(1, 0) && (NB == 2 || do_s(0, 1)))) break;
+          for (int t = 0; t < steps; ++t) {
+            if (!(ok = do_pv(0, t))) break;
+            if (t == steps - 1) umma_commit(&o_done[0]);
+            if (!(ok = NB == 3 ? do_s(1, t + 1) : do_s(0, t + 1))) break;
+            if (!(ok = do_pv(1, t) && (NB == 3 ? do_s(0, t + 2) : do_s(1, t + 1)))) break;
+            if (t == (steps > 1 ? steps - 2 : 0)) umma_commit(q_empty);  // every S has been issued
+          }
+          if (ok) umma_commit(&o_done[1]);
+          seq += (uint32_t)(steps + steps1);
+        }
+      }
+    } else if (warp == 2) {
+      // ------------------------------------------------------------ rows that are not kept
       VPos vp;
       bool ok = true;
       while (ok && k.next(p, g)) {
-        if (!mbar_wait<false>(q_empty, (k.seg & 1) ^ 1, kErrTimeoutAttnQ, abort_flag)) break;
-        const int nq = k.lone ? 1 : 2;
-        mbar_arrive_expect_tx(q_full, nq * C::kHalves * (uint32_t)(g.gt * g.nt) * 128u);
-        for (int w = 0; w < nq; ++w) {
-          int n0, g0;
-          tile_origin(k, g, w, n0, g0);
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_5d(sQ + w * C::kTile + h * kHalfBytes, &qmap, q_full, h * 64, g0, n0, k.s.hk, k.s.b * g.q_batched);
-        }
-        const int kh = k.s.hk * g.k_headed, kb = k.s.b * g.k_batched;
-        const int vh = k.s.hk * g.v_headed, vb = k.s.b * g.v_batched;
-        const int streams = k.lone ? 2 : 1;  // K/V tiles of a unit
-        // with three buffers S runs ahead of PV by up to two units, so K goes first
-        constexpr int kLead = NB == 3 ? 1 : 0;
-        for (int i = k.j0; ok && i < k.j1 + kLead; ++i) {
-          for (int w = 0; w < streams && i < k.j1 && k.uses(w, i); ++w) {
-            if (!(ok = mbar_wait<false>(&k_empty[kp.slot], kp.phase ^ 1, kErrTimeoutAttnKV, abort_flag))) break;
-            mbar_arrive_expect_tx(&k_full[kp.slot], C::kTile);
-            for (int h = 0; h < C::kHalves; ++h)
-              tma_load_4d(sK + kp.slot * C::kTile + h * kHalfBytes, &kmap, &k_full[kp.slot], h * 64,
-                          k.kv_tile(w, i) * 128, kh, kb);
-            kp = kp.plus(1);
-          }
-          const int v = i - kLead;
-          for (int w = 0; ok && w < streams && v >= k.j0 && k.uses(w, v); ++w) {
-            if (!(ok = mbar_wait<false>(&v_empty[vp.slot], vp.phase ^ 1, kErrTimeoutAttnKV, abort_flag))) break;
-            mbar_arrive_expect_tx(&v_full[vp.slot], C::kTile);
-            for (int h = 0; h < C::kHalves; ++h)
-              tma_load_4d(sV + vp.slot * C::kTile + h * kHalfBytes, &vmap, &v_full[vp.slot], h * 64,
-                          k.kv_tile(w, v) * 128, vh, vb);
+        const int streams = k.lone ? 2 : 1;
+        for (int j = k.j0; ok && j < k.j1; ++j) {
+          for (int w = 0; w < streams && k.uses(w, j); ++w) {
+            if (!(ok = mbar_wait_warp<false>(&v_full[vp.slot], vp.phase, kErrTimeoutAttnKV, abort_flag))) break;
+            const int key0 = k.kv_tile(w, j) * 128, khi = k.keys - key0;
+            if (kMask || khi < 128) {
+              bool touched = false;
+#pragma unroll
+              for (int ch = 0; ch < 4; ++ch) {
+                const int row = ch * 32 + lane;
+                bool keep = row < khi;
+                if (kMask && keep) keep = p.key_mask[(size_t)k.s.b * p.k_len + key0 + row] != 0;
+                const uint32_t word = __ballot_sync(0xffffffffu, keep);
+                if (kMask && lane == 0) s_words[vp.slot * 4 + ch] = word;
+                if (word == 0xffffffffu) continue;
+                touched = true;
+                if (!keep) {
+                  // a lane's row, its pieces in an order that keeps the lanes on different banks
+                  uint8_t* at = sV + vp.slot * C::kTile + row * 128;
+#pragma unroll
+                  for (int x = 0; x < 8 * C::kHalves; ++x)
+                    *reinterpret_cast<uint4*>(at + (x >> 3) * kHalfBytes + (((x + lane) & 7) << 4)) =
+                        make_uint4(0u, 0u, 0u, 0u);
+                }
+              }
+              if (touched) fence_proxy_async_smem();
+              __syncwarp();
+            }
+            if (lane == 0) mbar_arrive(&v_ready[vp.slot]);
             vp = vp.plus(1);
           }
         }
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    // The whole warp walks, one lane issues.
-    const bool lead = elect_one();
-    const uint32_t idesc_s = umma_idesc_f16(kIsBf16, 128, 0);
-    const uint32_t idesc_o = umma_idesc_f16(kIsBf16, (uint32_t)g.ksteps * 16, 1);
-    const uint64_t dq0 = sw128_desc(smem_u32(sQ), 16, 1024);
-    const uint64_t dk0 = sw128_desc(smem_u32(sK), 16, 1024);
-    const uint64_t dv0 = sw128_desc(smem_u32(sV), kHalfBytes, 1024);
-    constexpr uint32_t kTileDesc = C::kTile >> 4;
-    const int ksteps = g.ksteps;
-    KPos kp;                    // next K slot to wait for
-    VPos vp;
-    uint32_t kc[2] = {0, 0};    // slots in use
-    uint32_t vc[2] = {0, 0};
-    uint32_t mine[2] = {0, 0}, pmine[2] = {0, 0};  // S and PV issued so far, per tile
-    uint32_t seq = 0;           // position in the sequence of the segment's first step
-    bool ok = true;
-    while (ok && k.next(p, g)) {
-      if (!mbar_wait<false>(q_full, k.seg & 1, kErrTimeoutAttnQ, abort_flag)) break;
-      tc_fence_after();
-      const int steps = k.j1 - k.j0;
-      // steps of the second tile: all, but for a lone tile's last unit without a K/V tile for it
-      const int steps1 = k.uses(1, k.j1 - 1) ? steps : steps - 1;
-      const bool lone = k.lone;
-      // S of step t of tile w
-      auto do_s = [&](const int w, const int t) -> bool {
-        if (t >= (w ? steps1 : steps)) return true;
-        if (w == 0 || lone) {
-          if (!mbar_wait<false>(&k_full[kp.slot], kp.phase, kErrTimeoutAttnKV, abort_flag)) return false;
-          kc[w] = kp.slot;
-          kp = kp.plus(1);
-          tc_fence_after();
-        }
-        const uint32_t slot = lone ? kc[w] : kc[0];
-        const StepBuf<NB> b(w, mine[w]++, seq + 2 * t + w);
-        if (lead) {
-          const uint64_t dq = dq0 + (uint64_t)((lone ? 0 : w) * kTileDesc);
-          const uint64_t dk = dk0 + (uint64_t)(slot * kTileDesc);
-          const uint32_t dS = tmem + b.buf * 128;
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk) {
-            if (kk >= ksteps) break;
-            const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
-            umma_f16_ss(dS, dq + off, dk + off, idesc_s, kk != 0);
-          }
-          umma_commit(&s_full[b.buf]);
-          if (w == 1 || lone) umma_commit(&k_empty[slot]);
-        }
-        return true;
-      };
-      // PV of step t of tile w
-      auto do_pv = [&](const int w, const int t) -> bool {
-        if (t >= (w ? steps1 : steps)) return true;
-        if (w == 0 || lone) {
-          if (!mbar_wait<false>(&v_ready[vp.slot], vp.phase, kErrTimeoutAttnKV, abort_flag)) return false;
-          vc[w] = vp.slot;
-          vp = vp.plus(1);
-        }
-        const uint32_t slot = lone ? vc[w] : vc[0];
-        const StepBuf<NB> b(w, pmine[w]++, seq + 2 * t + w);
-        if (!mbar_wait<false>(&p_full[b.buf], b.parity, kErrTimeoutAttnP, abort_flag)) return false;
-        tc_fence_after();
-        if (lead) {
-          const uint64_t dv = dv0 + (uint64_t)(slot * kTileDesc);
-          const uint32_t pa = tmem + b.buf * 128, dO = tmem + C::kColO + (uint32_t)(w * DP);
-          umma_f16_ts(dO, pa, dv, idesc_o, t > 0);
-#pragma unroll
-          for (int kk = 1; kk < 8; ++kk) umma_f16_ts(dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
-          umma_commit(&pv_done[w]);
-          if (w == 1 || lone) umma_commit(&v_empty[slot]);
-        }
-        return true;
-      };
-      // S(s + NB) behind PV(s)
-      if (!(ok = do_s(0, 0) && do_s(1, 0) && (NB == 2 || do_s(0, 1)))) break;
-      for (int t = 0; t < steps; ++t) {
-        if (!(ok = do_pv(0, t))) break;
-        if (lead && t == steps - 1) umma_commit(&o_done[0]);
-        if (!(ok = NB == 3 ? do_s(1, t + 1) : do_s(0, t + 1))) break;
-        if (!(ok = do_pv(1, t) && (NB == 3 ? do_s(0, t + 2) : do_s(1, t + 1)))) break;
-        if (lead && t == (steps > 1 ? steps - 2 : 0)) umma_commit(q_empty);  // every S has been issued
-      }
-      if (ok && lead) umma_commit(&o_done[1]);
-      seq += (uint32_t)(steps + steps1);
-    }
-  } else if (warp == 2) {
-    // ------------------------------------------------------------ rows that are not kept
-    VPos vp;
-    bool ok = true;
-    while (ok && k.next(p, g)) {
-      const int streams = k.lone ? 2 : 1;
-      for (int j = k.j0; ok && j < k.j1; ++j) {
-        for (int w = 0; w < streams && k.uses(w, j); ++w) {
-          if (!(ok = mbar_wait<false>(&v_full[vp.slot], vp.phase, kErrTimeoutAttnKV, abort_flag))) break;
-          const int key0 = k.kv_tile(w, j) * 128, khi = k.keys - key0;
-          if (kMask || khi < 128) {
-            bool touched = false;
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-              const int row = ch * 32 + lane;
-              bool keep = row < khi;
-              if (kMask && keep) keep = p.key_mask[(size_t)k.s.b * p.k_len + key0 + row] != 0;
-              const uint32_t word = __ballot_sync(0xffffffffu, keep);
-              if (kMask && lane == 0) s_words[vp.slot * 4 + ch] = word;
-              if (word == 0xffffffffu) continue;
-              touched = true;
-              if (!keep) {
-                // a lane's row, its pieces in an order that keeps the lanes on different banks
-                uint8_t* at = sV + vp.slot * C::kTile + row * 128;
-#pragma unroll
-                for (int x = 0; x < 8 * C::kHalves; ++x)
-                  *reinterpret_cast<uint4*>(at + (x >> 3) * kHalfBytes + (((x + lane) & 7) << 4)) =
-                      make_uint4(0u, 0u, 0u, 0u);
-              }
-            }
-            if (touched) fence_proxy_async_smem();
-            __syncwarp();
-          }
-          if (lane == 0) mbar_arrive(&v_ready[vp.slot]);
-          vp = vp.plus(1);
-        }
-      }
-    }
-  } else if (warp >= kSoftmaxWarp0) {
+  } else {
+    warpgroup_reg_inc<kSoftmaxRegs>();
     // ------------------------------------------------------------ softmax + epilogue
     const int w = (warp - kSoftmaxWarp0) >> 2, q = warp & 3;
     const int row = q * 32 + lane;
@@ -459,6 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
+        __syncwarp();
         tc_fence_after();
         if (warp_active) {
           uint32_t pk[64];
@@ -503,6 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   ok = false;
                   break;
                 }
+                __syncwarp();
                 tc_fence_after();
 #pragma unroll 1
                 for (int h = 0; h < DP / 32; ++h) {
@@ -543,6 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!mbar_wait<false>(&o_done[w], k.seg & 1, kErrTimeoutAttnO, abort_flag)) break;
+      __syncwarp();
       tc_fence_after();
       // a lone tile: the two halves meet, weigh each other in and write half the columns each
       float a0 = 1.f, a1 = 0.f;
@@ -557,6 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&meet[q]);
         if (!mbar_wait<false>(&meet[q], meets & 1, kErrTimeoutAttnO, abort_flag)) break;
         ++meets;
+        __syncwarp();
         tc_fence_after();
         const float r0 = ml[row], r1 = ml[256 + row], l0 = ml[128 + row], l1 = ml[256 + 128 + row];
         const bool has1 = l1 != -1.f;
@@ -629,6 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   }
+
 
   __syncthreads();
   if (warp == 1) {
