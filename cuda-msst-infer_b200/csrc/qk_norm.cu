@@ -14,6 +14,18 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+template <bool kStream, typename V>
+__device__ __forceinline__ V load(const V* p) {
+  return kStream ? __ldcs(p) : *p;
+}
+template <bool kStream, typename V>
+__device__ __forceinline__ void store(V* p, const V& v) {
+  if constexpr (kStream)
+    __stcs(p, v);
+  else
+    *p = v;
+}
+
 // The table row of a token, or -1 (and a recorded error) outside the tables: such
 // a token is normed but not rotated.
 __device__ __forceinline__ int table_row(const QkNormParams& p, long long token, int n) {
@@ -32,9 +44,13 @@ __device__ __forceinline__ int table_row(const QkNormParams& p, long long token,
 // [4l, 4l + 4) and [rot/2 + 4l, rot/2 + 4l + 4), two 8-byte loads instead of one of
 // 16 bytes, which costs issue slots that this kernel has to spare (shuffling the
 // partner's 8 values would cost more of them).
+// Bound: HBM.  kStream marks loads and stores as read and written once: 63.8 -> 59.5 us for
+// 338 MB (5.7 TB/s), no difference below L2's size, where the results should stay for the
+// attention that reads them.  Two heads a group took 75 us, eight 77, 256 threads a
+// block 67.
 constexpr int kHeads = 4;
 
-template <typename T, int LPV, bool kHalves>
+template <typename T, int LPV, bool kHalves, bool kStream>
 __global__ void __launch_bounds__(128) qk_norm_kernel(const __grid_constant__ QkNormParams p, unsigned items,
                                                       int chunks_q, int chunks) {
   const unsigned item = (blockIdx.x * 128u + threadIdx.x) / LPV;
@@ -62,10 +78,10 @@ __global__ void __launch_bounds__(128) qk_norm_kernel(const __grid_constant__ Qk
     if (active && u < left) {
       const T* s = src + u * in.head_stride;
       if constexpr (kHalves) {
-        raw[u][0] = *reinterpret_cast<const uint2*>(s + c0);
-        raw[u][1] = *reinterpret_cast<const uint2*>(s + c1);
+        raw[u][0] = load<kStream>(reinterpret_cast<const uint2*>(s + c0));
+        raw[u][1] = load<kStream>(reinterpret_cast<const uint2*>(s + c1));
       } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(s + c0);
+        const uint4 v = load<kStream>(reinterpret_cast<const uint4*>(s + c0));
         raw[u][0] = make_uint2(v.x, v.y);
         raw[u][1] = make_uint2(v.z, v.w);
       }
@@ -122,10 +138,10 @@ __global__ void __launch_bounds__(128) qk_norm_kernel(const __grid_constant__ Qk
     if (active) {
       T* t = dst + u * to.head_stride;
       if constexpr (kHalves) {
-        *reinterpret_cast<uint2*>(t + c0) = y0;
-        *reinterpret_cast<uint2*>(t + c1) = y1;
+        store<kStream>(reinterpret_cast<uint2*>(t + c0), y0);
+        store<kStream>(reinterpret_cast<uint2*>(t + c1), y1);
       } else {
-        *reinterpret_cast<uint4*>(t + c0) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+        store<kStream>(reinterpret_cast<uint4*>(t + c0), make_uint4(y0.x, y0.y, y1.x, y1.y));
       }
     }
   }
@@ -209,10 +225,13 @@ void launch_wide(const QkNormParams& p, cudaStream_t s) {
   const int cq = (p.x[0].heads + kHeads - 1) / kHeads, ck = (p.x[1].heads + kHeads - 1) / kHeads;
   const unsigned items = (unsigned)((long long)p.batch * p.seq * (cq + ck));
   const unsigned grid = (unsigned)(((long long)items * LPV + 127) / 128);
+  // more than L2 (126 MB) holds is streamed
+  const bool stream = 4.0 * p.batch * p.seq * (p.x[0].heads + p.x[1].heads) * p.head_dim > 126e6;
+  auto go = [&](auto kernel) { kernel<<<grid, 128, 0, s>>>(p, items, cq, cq + ck); };
   if (p.halves)
-    qk_norm_kernel<T, LPV, true><<<grid, 128, 0, s>>>(p, items, cq, cq + ck);
+    stream ? go(qk_norm_kernel<T, LPV, true, true>) : go(qk_norm_kernel<T, LPV, true, false>);
   else
-    qk_norm_kernel<T, LPV, false><<<grid, 128, 0, s>>>(p, items, cq, cq + ck);
+    stream ? go(qk_norm_kernel<T, LPV, false, true>) : go(qk_norm_kernel<T, LPV, false, false>);
 }
 
 template <typename T>
