@@ -476,3 +476,98 @@ def test_operators_on_a_side_stream(cuda):
         gotn, _ = ops.qk_norm_rope(late_q)
     s.synchronize()
     assert torch.equal(got, want) and torch.equal(got2, want2) and torch.equal(gotn, qn)
+
+
+@pytest.mark.parametrize("op", ["masked", "pairs", "token", "adapters"])
+def test_calls_back_to_back(cuda, op):
+    """Many calls queued without a host wait between them give the first call's bits, and no kernel
+    wait gives up (a wait that runs out takes two seconds and is recorded)."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    if op == "adapters":
+        x, w, la, lb, ids, scales, bias = _adapter_inputs(torch, 300, 640, 520, 9, 24, "bf16", 51)
+        call = lambda: ops.adapter_gemm(x, w, la, lb, ids, scales=scales, bias=bias)  # noqa: E731
+    else:
+        B, Nq, Nk, Hq, Hk, d = dict(masked=(5, 77, 1501, 12, 4, 80), pairs=(2, 600, 1000, 4, 4, 64),
+                                    token=(6, 1, 900, 8, 2, 128))[op]
+        q, k, v = _cross_inputs(torch, B, Nq, Nk, Hq, Hk, d, "fp16", 52)
+        _, lens, km = _keep(torch, B, Nk, "keys" if op == "masked" else "lens", 53)
+        call = lambda: ops.cross_attention(q, k, v, key_lens=lens, key_mask=km)  # noqa: E731
+    want = call()
+    for _ in range(8):
+        got = [call() for _ in range(40)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for y in got)
+    assert device_error(True) == 0
+
+
+def test_cross_attention_far_reference(cuda):
+    """The first kept scores far below the later ones and far above them, in turns along the keys:
+    the exponentials' reference has to move in the middle of a sequence, more than once."""
+    torch = cuda
+    from msst_b200 import ops
+
+    for d, prec in ((64, "fp16"), (128, "bf16"), (96, "fp16")):
+        q, k, v = _cross_inputs(torch, 1, 300, 1100, 2, 2, d, prec, 61)
+        q = q.abs()
+        level = torch.zeros(1100, device="cuda")
+        level[100:130] = 3.0
+        level[400:430] = 6.0
+        level[900:910] = 9.0
+        k = (k.float() * 0.2 + level[None, :, None, None]).to(k.dtype)
+        keep = torch.ones(1, 1100, dtype=torch.bool, device="cuda")
+        _cross_check(torch, ops.cross_attention(q, k, v), q, k, v, keep, d ** -0.5, prec)
+        _cross_check(torch, ops.cross_attention(q[:, :1], k, v), q[:, :1], k, v, keep, d ** -0.5, prec)
+
+
+# ------------------------------------------------------------------ the block they form
+@pytest.mark.parametrize("prec", ["fp16", "bf16"])
+def test_conditioned_block(cuda, prec):
+    """ConditionedBlock against the same block in 64 bits.  Each of its four 16-bit intermediate
+    results (q, k, attention, projection) is rounded once, u relative each, and a rounding of
+    q or k moves a score by up to 2 u |q||k| scale <= 2 u sqrt(d) for normed vectors (gammas
+    about 1); with the weights' rounding of the attention that is below
+    u (4 + 2 * 2 * sqrt(64)) = 36 u of the attention's and the projections' size in the 2-norm."""
+    torch = cuda
+    from msst_b200 import device_error
+    from msst_b200.conditioned import random_block
+
+    blk = random_block(dtype=_dt(torch, prec), seed=3)
+    g = _gen(torch, 8)
+    B, Nq, Nk, d = 3, 70, 333, 64
+    x = torch.randn(B, Nq, 512, generator=g, device="cuda").to(_dt(torch, prec))
+    enc = torch.randn(B, Nk, 384, generator=g, device="cuda").to(_dt(torch, prec))
+    lens = torch.tensor([333, 100, 0], dtype=torch.int32, device="cuda")
+    who = torch.tensor([1, -1, 2], dtype=torch.int32, device="cuda")
+    k, v = blk.encode(enc, who)
+    y = blk(x, k, v, who, key_lens=lens)
+    pos = torch.full((B, 1), Nq - 1, dtype=torch.int32, device="cuda")
+    tok = blk(x[:, -1:], k, v, who, positions=pos, key_lens=lens)
+    assert device_error(True) == 0
+
+    def project(name, t):
+        a, b, s = blk.adapters[name]
+        out = t @ blk.w[name].double().T
+        for i in range(B):
+            if who[i] >= 0:
+                out[i] += float(s[who[i]]) * (t[i] @ a[who[i]].double().T) @ b[who[i]].double().T
+        return out
+
+    q64 = project("q", x.double()).view(B, Nq, 8, d)
+    kv = project("kv", enc.double()).view(B, Nk, 2, 2, d)
+    q64, _ = _qk_ref(torch, q64, blk.q_gamma, blk.cos, blk.sin, torch.arange(Nq, device="cuda").expand(B, Nq), 1e-6, "halves")
+    k64, _ = _qk_ref(torch, kv[:, :, 0], blk.k_gamma, blk.cos, blk.sin, torch.arange(Nk, device="cuda").expand(B, Nk), 1e-6, "halves")
+    att = torch.zeros(B, Nq, 8, d, dtype=torch.float64, device="cuda")
+    for i in range(B):
+        n = int(lens[i])
+        for h in range(8):
+            if n:
+                p = torch.softmax(q64[i, :, h] @ k64[i, :n, h // 4].T / math.sqrt(d), -1)
+                att[i, :, h] = p @ kv[i, :n, 1, h // 4]
+    delta = project("o", att.reshape(B, Nq, -1))
+    ref = x.double() + delta
+    bar = 36 * U[prec] * float(delta.norm()) + U[prec] * float(ref.norm())
+    assert float((y.double() - ref).norm()) <= bar
+    assert float((tok.double() - ref[:, -1:]).norm()) <= 36 * U[prec] * float(delta[:, -1:].norm()) + \
+        U[prec] * float(ref[:, -1:].norm())
