@@ -651,8 +651,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // x takes the item that the boundary between CTAs x and x + 1 cuts, if it is that item's
 // first cut.  kByItem true (an item may span every CTA): block x takes item x.
 // Slots of 256 rows (column by column): block (x, y, z) joins columns [8 z, 8 z + 8), a lane a
-// row; with kByItem kShare warps share the parts of rows [32 y, 32 y + 32) out, else 8 warps
-// take 32 rows each.  Slots of 16 rows (row by row, cross_token.cu): block (x, y) joins row y,
+// row; kShare = 1: 8 warps take 32 rows each, kShare > 1 (items of many parts): the warps share
+// the parts of rows [32 y, 32 y + 32) out.  Slots of 16 rows (row by row, cross_token.cu): block (x, y) joins row y,
 // 4 columns a lane, its kShare = 8 warps sharing the parts out.
 template <typename T, bool kByItem, bool kToken, int kShare>
 __global__ void __launch_bounds__(kShare > 1 ? 32 * kShare : 256)
@@ -733,14 +733,14 @@ __global__ void __launch_bounds__(kShare > 1 ? 32 * kShare : 256)
            (long long)(s.hk * g.group + head) * p.out.head_stride + col;
   };
   constexpr int kCols = kToken ? 4 : 8;
-  const int row = kToken ? blockIdx.y : blockIdx.y * (kByItem ? 32 : 256) + (kByItem ? 0 : warp * 32) + lane;
+  const int row = kToken ? blockIdx.y : (kShare > 1 ? blockIdx.y : warp) * 32 + lane;
   const int col = kToken ? lane * 4 : blockIdx.z * 8;
   int n, head;
   const bool valid = place(row, n, head) && col < d;
   float m = -INFINITY, l = 0.f, o[kCols];
 #pragma unroll
   for (int i = 0; i < kCols; ++i) o[i] = 0.f;
-#pragma unroll 2
+#pragma unroll 4
   for (int c = c0 + (kShare > 1 ? warp : 0); c <= c1; c += kShare) {
     const float* r = part(c);
     if (!r || !valid) continue;
@@ -887,12 +887,12 @@ cudaError_t launch_combine(const CrossAttnParams& p, const Geom& g, cudaStream_t
                    : cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, false, true, 8>, p, g);
   }
   const int rows = g.full ? 256 : g.gt * std::min(g.nt, p.q_len);
-  // an item has about contribs / items parts: more warps to share them where there are many
-  const int share = !by_item ? 1 : (g.contribs / items < 16 ? 8 : 32);
-  DependentLaunch l(dim3(x, by_item ? (rows + 31) / 32 : 1, p.head_dim / 8), share > 1 ? 32 * share : 256, 0, s);
-  return share == 1 ? cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, false, false, 1>, p, g)
-         : share == 8 ? cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, true, false, 8>, p, g)
-                      : cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, true, false, 32>, p, g);
+  // an item has about contribs / items parts: 32 warps share them where there are many
+  const bool share = by_item && g.contribs / items >= 16;
+  DependentLaunch l(dim3(x, share ? (rows + 31) / 32 : 1, p.head_dim / 8), share ? 1024 : 256, 0, s);
+  return share     ? cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, true, false, 32>, p, g)
+         : by_item ? cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, true, false, 1>, p, g)
+                   : cudaLaunchKernelEx(&l.cfg, cross_combine_kernel<T, false, false, 1>, p, g);
 }
 
 template <typename T, int DP, bool kMask>

@@ -217,6 +217,22 @@ def _current_stream(device: int) -> int:
     return _torch()._C._cuda_getCurrentRawStream(device)
 
 
+_space = {}  # bytes of workspace by (operator, device, sizes): a function of the sizes alone
+
+
+def _workspace(name, device, *sizes):
+    """Workspace bytes of operator `name` for a call's sizes (asked for once per sizes)."""
+    key = (name, device, sizes)
+    n = _space.get(key)
+    if n is None:
+        need = ctypes.c_longlong()
+        check(getattr(lib(), f"msst_{name}_workspace")(*sizes, ctypes.byref(need)))
+        if len(_space) > 4096:
+            _space.clear()
+        n = _space[key] = need.value
+    return n
+
+
 def _need(ok, msg):
     if not ok:
         raise ValueError(msg)
@@ -433,13 +449,11 @@ class ops:
                   "key_mask must be bool [B, Nk] on q's device")
             key_mask = key_mask.contiguous()
             mask = key_mask.data_ptr()
-        L, need = lib(), ctypes.c_longlong()
-        check(L.msst_cross_attention_workspace(B, Nq, Nk, Hq, Hk, d, ctypes.byref(need)))
-        need = need.value
+        need = _workspace("cross_attention", dev, B, Nq, Nk, Hq, Hk, d)
         if need:
             space = torch.empty(need, dtype=torch.uint8, device=q.device)
             ws = space.data_ptr()
-        check(L.msst_cross_attention(_heads(q, Hq, sq), _heads(k, Hk, sk), _heads(v, Hk, sv), B, Nq, Nk, d, scale, lens,
+        check(lib().msst_cross_attention(_heads(q, Hq, sq), _heads(k, Hk, sk), _heads(v, Hk, sv), B, Nq, Nk, d, scale, lens,
                                      mask, code, _heads(out, Hq, so), ws, need, _current_stream(dev)))
         return out
 
@@ -486,15 +500,14 @@ class ops:
                 keep.append(t)
             return t.data_ptr()
 
-        L, need, ws = lib(), ctypes.c_longlong(), None
-        check(L.msst_adapter_gemm_workspace(rows, K, N, count, rank, ctypes.byref(need)))
-        need = need.value
+        bias, scales = _f32_ptr(bias, N, dev, keep, "bias"), _f32_ptr(scales, count, dev, keep, "scales")
+        need, ws = _workspace("adapter_gemm", dev, rows, K, N, count, rank), None
         if need:
             space = torch.empty(need, dtype=torch.uint8, device=x.device)
             ws = space.data_ptr()
-        check(L.msst_adapter_gemm(x.data_ptr(), rows, K, ldx, ptr(w), N, _f32_ptr(bias, N, dev, keep, "bias"),
-                                  ptr(lora_a), ptr(lora_b), _f32_ptr(scales, count, dev, keep, "scales"), count, rank,
-                                  ptr(row_adapter), code, out.data_ptr(), ldo, ws, need, _current_stream(dev)))
+        check(lib().msst_adapter_gemm(
+            x.data_ptr(), rows, K, ldx, ptr(w), N, bias, ptr(lora_a), ptr(lora_b), scales, count, rank, ptr(row_adapter),
+            code, out.data_ptr(), ldo, ws, need, _current_stream(dev)))
         return out
 
     @staticmethod
