@@ -214,7 +214,7 @@ def _heads(t, heads, strides):
 
 def _current_stream(device: int) -> int:
     """The current stream's handle on GPU `device`."""
-    return _torch()._C._cuda_getCurrentRawStream(device)
+    return _torch_module._C._cuda_getCurrentRawStream(device)
 
 
 _space = {}  # bytes of workspace by (operator, device, sizes): a function of the sizes alone
@@ -254,12 +254,32 @@ def _f32_ptr(t, n, device, keep, what):
     """Address of an optional float32 tensor of n values (a contiguous copy is kept alive in `keep`)."""
     if t is None:
         return None
-    _need(t.dtype is _torch().float32 and t.get_device() == device and t.numel() == n,
-          f"{what} must be float32 on the operands' device, {n} values")
+    if t.dtype is not _torch_module.float32 or t.get_device() != device or t.numel() != n:
+        raise ValueError(f"{what} must be float32 on the operands' device, {n} values")
     if not t.is_contiguous():
         t = t.contiguous()
         keep.append(t)
     return t.data_ptr()
+
+
+def _side(x, shape, out, what, keep):
+    """One tensor of qk_norm_rope: (output, msst_heads of x, msst_heads of the output)."""
+    st = x.stride()
+    if st[3] != 1 and shape[3] > 1:
+        x = x.contiguous()
+        keep.append(x)
+        st = x.stride()
+    if out is None:
+        out = _torch_module.empty_like(x, memory_format=_torch_module.contiguous_format)
+        ost = out.stride()
+    else:
+        ost = out.stride()
+        if (out.shape != shape or out.dtype is not x.dtype or out.get_device() != x.get_device()
+                or (ost[3] != 1 and shape[3] > 1)):
+            raise ValueError(f"out_{what} must have {what}'s shape, type and device, and unit last stride")
+    heads = shape[2]
+    return (out, _HEADS(x.data_ptr(), heads, st[0], st[1], st[2]),
+            _HEADS(out.data_ptr(), heads, ost[0], ost[1], ost[2]))
 
 
 class ops:
@@ -371,28 +391,13 @@ class ops:
         _need(len(shape) == 4, "q must be [B, N, heads, head_dim]")
         B, N, Hq, d = shape
 
-        def side(x, xshape, out, what):
-            st = x.stride()
-            if st[3] != 1 and d > 1:
-                x = x.contiguous()
-                keep.append(x)
-                st = x.stride()
-            if out is None:
-                out = torch.empty_like(x, memory_format=torch.contiguous_format)
-                ost = out.stride()
-            else:
-                ost = out.stride()
-                _need(out.shape == xshape and out.dtype is dt and out.get_device() == dev and (ost[3] == 1 or d == 1),
-                      f"out_{what} must have {what}'s shape, type and device, and unit last stride")
-            return out, _heads(x, xshape[2], st), _heads(out, xshape[2], ost)
-
-        out_q, hq, ho = side(q, shape, out_q, "q")
+        out_q, hq, ho = _side(q, shape, out_q, "q", keep)
         hk = hko = None
         if k is not None:
             ks = k.shape
             _need(len(ks) == 4 and ks[0] == B and ks[1] == N and ks[3] == d and k.dtype is dt and k.get_device() == dev,
                   "k must be [B, N, heads, head_dim] with q's B, N, head_dim, type and device")
-            out_k, hk, hko = side(k, ks, out_k, "k")
+            out_k, hk, hko = _side(k, ks, out_k, "k", keep)
         else:
             out_k = None
         num_pos, half = (0, 0) if cos is None else cos.shape
@@ -451,7 +456,7 @@ class ops:
             mask = key_mask.data_ptr()
         need = _workspace("cross_attention", dev, B, Nq, Nk, Hq, Hk, d)
         if need:
-            space = torch.empty(need, dtype=torch.uint8, device=q.device)
+            space = q.new_empty(need // 2)  # 16-bit values; sizes are whole floats
             ws = space.data_ptr()
         check(lib().msst_cross_attention(_heads(q, Hq, sq), _heads(k, Hk, sk), _heads(v, Hk, sv), B, Nq, Nk, d, scale, lens,
                                      mask, code, _heads(out, Hq, so), ws, need, _current_stream(dev)))
@@ -486,7 +491,7 @@ class ops:
               "row_adapter must be int32 with one entry per row")
         ldo = N
         if out is None:
-            out = torch.empty(shape[:-1] + (N,), dtype=dt, device=x.device)
+            out = x.new_empty(shape[:-1] + (N,))
         else:
             _need(out.shape == shape[:-1] + (N,) and out.dtype is dt and out.get_device() == dev and
                   (out.is_contiguous() or (out.dim() == 2 and out.stride(1) == 1)),
@@ -503,7 +508,7 @@ class ops:
         bias, scales = _f32_ptr(bias, N, dev, keep, "bias"), _f32_ptr(scales, count, dev, keep, "scales")
         need, ws = _workspace("adapter_gemm", dev, rows, K, N, count, rank), None
         if need:
-            space = torch.empty(need, dtype=torch.uint8, device=x.device)
+            space = x.new_empty(need // 2)  # 16-bit values; sizes are whole floats
             ws = space.data_ptr()
         check(lib().msst_adapter_gemm(
             x.data_ptr(), rows, K, ldx, ptr(w), N, bias, ptr(lora_a), ptr(lora_b), scales, count, rank, ptr(row_adapter),
