@@ -559,8 +559,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               if (n0 + c + i < p.N) {  // N is a multiple of 8
-                const float4 b = make_float4(__ldg(p.bias + n0 + c + i), __ldg(p.bias + n0 + c + i + 1),
-                                             __ldg(p.bias + n0 + c + i + 2), __ldg(p.bias + n0 + c + i + 3));
+                const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + n0 + c + i));
                 v[i] = __float_as_uint(__uint_as_float(v[i]) + b.x);
                 v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) + b.y);
                 v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) + b.z);

@@ -542,6 +542,7 @@ int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const
     check_align(x, "x");
     check_align(w, "w");
     check_align(out, "out");
+    check_align(bias, "bias");
     check_align(lora_a, "lora_a");
     check_align(lora_b, "lora_b");
     DeviceScope dev_scope(device_of(x));

@@ -251,13 +251,14 @@ def _aligned_heads(t, shape, shared=False):
 
 
 def _f32_ptr(t, n, device, keep, what):
-    """Address of an optional float32 tensor of n values (a contiguous copy is kept alive in `keep`)."""
+    """Address of an optional float32 tensor of n values, contiguous and on 16 bytes (a copy is
+    kept alive in `keep`)."""
     if t is None:
         return None
     if t.dtype is not _torch_module.float32 or t.get_device() != device or t.numel() != n:
         raise ValueError(f"{what} must be float32 on the operands' device, {n} values")
-    if not t.is_contiguous():
-        t = t.contiguous()
+    if not t.is_contiguous() or t.data_ptr() & 15:
+        t = t.clone(memory_format=_torch_module.contiguous_format)
         keep.append(t)
     return t.data_ptr()
 
@@ -500,8 +501,8 @@ class ops:
                 ldo = out.stride(0)
 
         def ptr(t):
-            if not t.is_contiguous():
-                t = t.contiguous()
+            if not t.is_contiguous() or t.data_ptr() & 15:
+                t = t.clone(memory_format=torch.contiguous_format)
                 keep.append(t)
             return t.data_ptr()
 

@@ -209,7 +209,8 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
  * [N, K], bias fp32 [N] or NULL, lora_a 16-bit [adapters, rank, K] (the A_a), lora_b
  * 16-bit [adapters, N, rank] (the B_a), scales fp32 [adapters] or NULL (ones),
  * row_adapter int32 [rows], out row stride ldo.  K, N, rank, ldx and ldo are
- * multiples of 8, rank <= 256; rows of one request need not be adjacent.  An index
+ * multiples of 8, rank <= 256, and all pointers but scales and row_adapter 16-byte
+ * aligned; rows of one request need not be adjacent.  An index
  * outside [-1, adapters) counts as -1, and msst_device_error reports it.  A row's
  * result does not depend on the other rows of the call beyond the order of sums.
  * `workspace` as in msst_cross_attention. */
