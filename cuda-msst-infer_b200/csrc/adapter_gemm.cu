@@ -5,20 +5,13 @@
 // adapter; adapter_gemm_kernel computes W x and adds B_a (s_a u) as a few more K steps
 // of the same accumulators, so the low-rank term costs no pass over the output.
 //
-// The second works on row tiles (32 to 128 rows) and on the list of the distinct adapters
+// The second works on row tiles (32, 64 or 128 rows) and on the list of the distinct adapters
 // of a tile.  An adapter's part of the extra K steps is a slice of 16 rank values
 // (ceil(rank / 16) slices an adapter): B_a's columns on one side, on the other U', which
 // holds s_a u for the rows whose adapter is a and zeros for all others.  So requests
 // may be mixed row by row: a tile costs as many slices as it has adapters.
 //
-// Up to 128 rows the weights are the MMA's M side (128 of their rows) and the rows of x its N
-// side: the instruction then covers 4 KB of weights, where an M side of rows would be
-// padded to 128 and the one issuing thread, at about 60 cycles an MMA, would bound the pass
-// (K = N = 4096: 8 us of issue for 32 columns a CTA, against the 5.2 us that reading W
-// takes).  More rows are the M side and 256 weight rows the N side, so that a lane of the
-// epilogue holds consecutive output columns (with the rows on the N side its 2-byte stores
-// kept 48060 x 1536 outputs at 103 us).  Few tiles are split along K over a cluster, whose CTAs add
-// their parts through distributed shared memory in rank order.
+// Which side of the MMA the rows take, and the split along K: make_plan.
 //
 // u is rounded to the operands' 16 bits once, as U' feeds the tensor cores; it is summed
 // in fp32 before that (split-K parts of the first launch in order).
@@ -265,7 +258,7 @@ struct GemmCfgA {
   static constexpr size_t kSmem = kStages * kStage + kStaging + 512;
   static constexpr uint32_t kTmem = 2 * BT;
   static_assert(4 * kStages * 8 + 48 + 16 * 4 <= 512, "barriers");
-  static_assert(kStages * kStage >= BT * 128 * 4, "the split-K exchange reuses the ring");
+  static_assert(kRowsOnM || kStages * kStage >= BT * 128 * 4, "the split-K exchange reuses the ring");
 };
 constexpr int kThreadsA = 448;
 
@@ -283,6 +276,35 @@ __device__ __forceinline__ bool drop_nonfinite(uint4& v) {
   }
   return found;
 }
+// 16-bit maxima of the magnitudes of a piece's 8 values: at or above kExp where one is not finite.
+__device__ __forceinline__ uint32_t magnitudes(const uint4& v) {
+  constexpr uint32_t kAbs = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(v.x & kAbs, v.y & kAbs), __vmaxu2(v.z & kAbs, v.w & kAbs));
+}
+
+// The next four slices of a tile's list: adapter (-2 past the end) and slice of that adapter.
+// Read a stage ahead by counting: with two divisions and a wait for the list at every slice, in the
+// one producing thread, a slice took about 0.5 us instead of 0.2 (32 rows, K = N = 4096).
+struct Slices {
+  const int* at;
+  int c, chunks, left;
+  int id[4], part[4];
+  __device__ __forceinline__ Slices(const int* list, int s0, int s1, int n) : chunks(n), left(s1 - s0) {
+    at = list + 2 + s0 / n;
+    c = s0 % n;
+    next();
+  }
+  __device__ __forceinline__ void next() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      id[i] = left > 0 ? *at : -2;
+      part[i] = c;
+      --left;
+      if (++c == chunks) c = 0, ++at;
+    }
+  }
+};
+
 // What drop_nonfinite left out of y[t, col] in slices [s0, s1) of the tile's list.
 template <typename T>
 __device__ __noinline__ float dropped_part(const AdapterGemmParams& p, const Plan& pl, const int* list, int s0, int s1,
@@ -328,10 +350,11 @@ __global__ void __launch_bounds__(kThreadsA, 1)
   volatile int* s_dropped = reinterpret_cast<volatile int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = pl.split > 1 ? (int)cluster_ctarank() : 0;
+  const int split = kRowsOnM ? 1 : pl.split;
+  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
   const int total = pl.tiles * pl.n_tiles;
-  const int tile0 = pl.split > 1 ? blockIdx.x / pl.split : blockIdx.x;
-  const int step = pl.split > 1 ? total : gridDim.x;
+  const int tile0 = split > 1 ? blockIdx.x / split : blockIdx.x;
+  const int step = split > 1 ? total : gridDim.x;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -360,12 +383,12 @@ __global__ void __launch_bounds__(kThreadsA, 1)
   const uint32_t tmem = *tmem_slot;
   // The first launch may still run: what reads its results waits for it first.
   const int* lists = reinterpret_cast<const int*>(static_cast<const uint8_t*>(p.ws) + list_offset(p, pl));
-  const int kb0 = pl.kblocks * rank / pl.split, kb1 = pl.kblocks * (rank + 1) / pl.split;
+  const int kb0 = pl.kblocks * rank / split, kb1 = pl.kblocks * (rank + 1) / split;
   // this CTA's slices of a tile whose list is `list`
   auto slice_range = [&](const int* list, int& s0, int& s1) {
     const int n = list[0] * pl.chunks;
-    s0 = n * rank / pl.split;
-    s1 = n * (rank + 1) / pl.split;
+    s0 = n * rank / split;
+    s1 = n * (rank + 1) / split;
   };
 
   if (warp == 0) {
@@ -391,7 +414,8 @@ __global__ void __launch_bounds__(kThreadsA, 1)
         const int* list = lists + (size_t)tt * pl.list_ld;
         int s0, s1;
         slice_range(list, s0, s1);
-        for (; ok && s0 < s1; s0 += 4, ++it) {
+        Slices sl(list, s0, s1, pl.chunks);
+        for (; ok && s0 < s1; s0 += 4, ++it, sl.next()) {
           const int st = it % C::kStages, n = min(4, s1 - s0);
           if (!mbar_wait(&empty[st], ((it / C::kStages) & 1) ^ 1, kErrTimeoutSmemEmpty, abort_flag)) {
             ok = false;
@@ -399,9 +423,11 @@ __global__ void __launch_bounds__(kThreadsA, 1)
           }
           mbar_arrive(&u_go[st]);
           mbar_arrive_expect_tx(&full[st], (uint32_t)n * C::kBSlice);
-          for (int i = 0; i < n; ++i)
-            tma_load_3d(smem + st * C::kStage + C::kBAt + i * C::kBSlice, &bmap, &full[st],
-                        ((s0 + i) % pl.chunks) * kSliceRows, n0, list[2 + (s0 + i) / pl.chunks]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < n)
+              tma_load_3d(smem + st * C::kStage + C::kBAt + i * C::kBSlice, &bmap, &full[st], sl.part[i] * kSliceRows,
+                          n0, sl.id[i]);
         }
       }
     }
@@ -456,8 +482,9 @@ __global__ void __launch_bounds__(kThreadsA, 1)
     // ------------------------------------------------------------ U' of the slices
     // These warps follow the ring by its slice stages alone: a stage is theirs once the
     // producer says so, and is not used again before the MMA has had their U'.
-    // A thread writes its row of all slices; the values are fetched and rounded before the
-    // stage is waited for, so that the wait covers the loads.
+    // A thread writes its row of all slices.  It fetches its row's s_a u once a tile, 32 rank
+    // values at a time, and holds them rounded: fetched as their slice came up, every slice of a
+    // mixed tile paid the latency of another thread's loads (0.9 us a slice instead of 0.5).
     const int i0 = threadIdx.x - 64;
     int it = 0, n = 0;
     uint32_t uses = 0;
@@ -473,28 +500,45 @@ __global__ void __launch_bounds__(kThreadsA, 1)
       const long long t = (long long)tt * C::kRows + i0;
       const int id = i0 < C::kRows ? row_id(p, t) : -1;
       const float sc = id >= 0 && p.scales ? __ldg(p.scales + id) : 1.f;
+      uint4 held[4];  // slices held0 and held0 + 1 of this row, 8 values each
+      int held0;
+      auto fetch = [&](int c) {
+        float4 f[8] = {};
+        const float* u = static_cast<const float*>(p.ws) + t * p.rank + c * kSliceRows;
+        const int left = p.rank - c * kSliceRows;
+        for (int k = 0; k < pl.down_split; ++k, u += part) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (i * 4 >= left) continue;
+            const float4 x = *reinterpret_cast<const float4*>(u + 4 * i);
+            f[i] = make_float4(f[i].x + x.x, f[i].y + x.y, f[i].z + x.z, f[i].w + x.w);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 lo = f[2 * i], hi = f[2 * i + 1];
+          held[i] = make_uint4(pack2<T>(lo.x * sc, lo.y * sc), pack2<T>(lo.z * sc, lo.w * sc),
+                               pack2<T>(hi.x * sc, hi.y * sc), pack2<T>(hi.z * sc, hi.w * sc));
+        }
+        held0 = c;
+      };
+      held0 = -2;
+      if (id >= 0 && s0 < s1) fetch(0);
+      const bool mixed = list[1] != 0;
+      Slices sl(list, s0, s1, pl.chunks);
       for (; s0 < s1; s0 += 4, ++it) {
         const int st = it % C::kStages, m = min(4, s1 - s0);
         uint4 v[4][2];  // [slice][8 values]
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int s = s0 + i, a = i < m ? list[2 + s / pl.chunks] : -2, c0 = (s % pl.chunks) * kSliceRows;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            v[i][half] = make_uint4(0u, 0u, 0u, 0u);
-            if (id != a || c0 + half * 8 >= p.rank) continue;
-            const float* u = static_cast<const float*>(p.ws) + t * p.rank + c0 + half * 8;
-            float4 lo = *reinterpret_cast<const float4*>(u), hi = *reinterpret_cast<const float4*>(u + 4);
-            for (int k = 1; k < pl.down_split; ++k) {
-              u += part;
-              const float4 l2 = *reinterpret_cast<const float4*>(u), h2 = *reinterpret_cast<const float4*>(u + 4);
-              lo = make_float4(lo.x + l2.x, lo.y + l2.y, lo.z + l2.z, lo.w + l2.w);
-              hi = make_float4(hi.x + h2.x, hi.y + h2.y, hi.z + h2.z, hi.w + h2.w);
-            }
-            v[i][half] = make_uint4(pack2<T>(lo.x * sc, lo.y * sc), pack2<T>(lo.z * sc, lo.w * sc),
-                                    pack2<T>(hi.x * sc, hi.y * sc), pack2<T>(hi.z * sc, hi.w * sc));
-          }
+          const int c = sl.part[i];
+          v[i][0] = v[i][1] = make_uint4(0u, 0u, 0u, 0u);
+          if (id != sl.id[i]) continue;
+          if ((c & ~1) != held0) fetch(c & ~1);
+          v[i][0] = c & 1 ? held[2] : held[0];
+          v[i][1] = c & 1 ? held[3] : held[1];
         }
+        sl.next();
         if (!mbar_wait(&u_go[st], uses >> st & 1, kErrTimeoutSmemEmpty, abort_flag)) {
           ok = false;
           break;
@@ -514,14 +558,21 @@ __global__ void __launch_bounds__(kThreadsA, 1)
           ok = false;
           break;
         }
-        if (list[1]) {
-          for (int x = i0; x < m * C::kCols * 2; x += 128) {
-            uint4* at = reinterpret_cast<uint4*>(base + C::kBAt + x * 16);
-            uint4 b = *at;
-            if (drop_nonfinite<T>(b)) {
-              *at = b;
-              s_dropped[n & 15] = n + 1;
+        if (mixed) {
+          // all of a thread's pieces are looked at before the rare rewrite
+          constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+          uint4* at = reinterpret_cast<uint4*>(base + C::kBAt) + i0;
+          uint32_t top = 0;
+          for (int i = 0; i < m; ++i) {
+#pragma unroll
+            for (int x = 0; x < C::kCols / 64; ++x) top = __vmaxu2(top, magnitudes(at[(i * (C::kCols / 64) + x) * 128]));
+          }
+          if ((top & 0xffffu) >= kExp || top >> 16 >= kExp) {
+            for (int x = 0; x < m * (C::kCols / 64); ++x) {
+              uint4 b = at[x * 128];
+              if (drop_nonfinite<T>(b)) at[x * 128] = b;
             }
+            s_dropped[n & 15] = n + 1;
           }
         }
         fence_proxy_async_smem();
@@ -555,7 +606,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
           uint32_t v[32];
           tmem_ld32(acc + (uint32_t)c, v);
           tmem_ld_wait(v);
-          if (kRowsOnM && p.bias && rank == 0) {
+          if (kRowsOnM && p.bias) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               if (n0 + c + i < p.N) {  // N is a multiple of 8
@@ -567,17 +618,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
               }
             }
           }
-          if (pl.split > 1) {
-            // [N side][M side], a lane's values 512 bytes apart
-            float* ex = reinterpret_cast<float*>(smem) + c * 128 + q * 32 + lane;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) ex[i * 128] = __uint_as_float(v[i]) + bias;
-            if (dropped) {
-              for (int i = 0; i < 32; ++i)
-                ex[i * 128] += kRowsOnM ? dropped_part<T>(p, pl, list, s0, s1, t0 + q * 32 + lane, n0 + c + i)
-                                        : dropped_part<T>(p, pl, list, s0, s1, t0 + c + i, col);
-            }
-          } else if constexpr (kRowsOnM) {
+          if constexpr (kRowsOnM) {
             // 32 rows x 32 columns through swizzled shared memory, out by TMA (which clips)
             if (lane == 0) bulk_wait_read0();
             __syncwarp();
@@ -602,6 +643,14 @@ __global__ void __launch_bounds__(kThreadsA, 1)
             if (lane == 0) {
               tma_store_3d(&omap, stg, n0 + c, (int)t0 + q * 32, 0);
               bulk_commit();
+            }
+          } else if (split > 1) {
+            // [N side][M side], a lane's values 512 bytes apart
+            float* ex = reinterpret_cast<float*>(smem) + c * 128 + q * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ex[i * 128] = __uint_as_float(v[i]) + bias;
+            if (dropped) {
+              for (int i = 0; i < 32; ++i) ex[i * 128] += dropped_part<T>(p, pl, list, s0, s1, t0 + c + i, col);
             }
           } else if (col < p.N) {
             T* out = static_cast<T*>(p.out) + (t0 + c) * p.ldo + col;
@@ -630,37 +679,30 @@ __global__ void __launch_bounds__(kThreadsA, 1)
     if (kRowsOnM && lane == 0) bulk_wait0();
   }
 
-  if (pl.split > 1) {
-    // every CTA of the cluster adds up its share of the N side, in rank order
+  if (split > 1) {
+    // every CTA of the cluster adds up its share of the rows, in rank order
     __syncwarp();
     cluster_sync_all();
     const int tt = tile0 / pl.n_tiles, n0 = (tile0 - tt * pl.n_tiles) * C::kCols;
     const long long t0 = (long long)tt * C::kRows;
     const uint32_t base = smem_u32(smem);
-    // 8 consecutive output columns of a row a thread
-    const int c0 = BT / 8 * rank / pl.split * 8, c1 = BT / 8 * (rank + 1) / pl.split * 8;
+    // 8 consecutive output columns of a row a thread, 16 such groups a row
+    const int c0 = BT / 8 * rank / split * 8, c1 = BT / 8 * (rank + 1) / split * 8;
     for (int x = threadIdx.x; x < (c1 - c0) * 16; x += kThreadsA) {
-      // rows on M: lanes along the rows; weights on M: 16 groups of 8 columns a row
-      const int m = kRowsOnM ? x & 127 : (x & 15) * 8, c = c0 + (kRowsOnM ? (x >> 7) * 8 : x >> 4);
-      const long long t = t0 + (kRowsOnM ? m : c);
-      const int col = n0 + (kRowsOnM ? c : m);
+      const int m = (x & 15) * 8, c = c0 + (x >> 4);
+      const long long t = t0 + c;
+      const int col = n0 + m;
       if (t >= p.rows || col >= p.N) continue;
       float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < pl.split; ++k) {
+      for (int k = 0; k < split; ++k) {
         const uint32_t at = mapa_shared(base + (uint32_t)(c * 128 + m) * 4u, (uint32_t)k);
         float v[8];
-        if constexpr (kRowsOnM) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i]) : "r"(at + (uint32_t)i * 512u) : "memory");
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; i += 4)
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3])
-                         : "r"(at + (uint32_t)i * 4u)
-                         : "memory");
-        }
+        for (int i = 0; i < 8; i += 4)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3])
+                       : "r"(at + (uint32_t)i * 4u)
+                       : "memory");
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[i] += v[i];
       }
@@ -680,7 +722,15 @@ __global__ void __launch_bounds__(kThreadsA, 1)
 
 Plan make_plan(int rows, int K, int N, int adapters, int rank, int num_sms) {
   Plan pl{};
-  pl.rows_on_m = rows > 128;
+  // The weights are the MMA's M side (128 of their rows) and up to 128 rows of x its N side
+  // while such tiles fit the SMs in one wave, or one tile takes all rows.  More rows are the M side
+  // and 256 weight rows the N side: half as many tiles, and a lane of the epilogue holds consecutive
+  // output columns, which leave by TMA (weights on the M side: 2-byte stores).  Both sides, weights
+  // on M / rows on M, K = N = 4096, rank 16: 512 rows (128 tiles) 22.7 / 26.3 us, 576 (160)
+  // 31.9 / 30.6, 1536 53-55 / 56-58, 8192 282 / 243; K = 384, N = 1536: 1536 rows (144 tiles) 9.7 / 14.2,
+  // 1600 (156) 11.1 / 10.6, 8192 22.7 / 19.9.
+  const long long narrow = (long long)((rows + 127) / 128) * ((N + 127) / 128);
+  pl.rows_on_m = rows > 128 && narrow > num_sms;
   pl.bt = rows <= 32 ? 32 : (rows <= 64 ? 64 : 128);
   pl.tiles = (rows + pl.bt - 1) / pl.bt;
   pl.n_tiles = pl.rows_on_m ? (N + 255) / 256 : (N + 127) / 128;
@@ -697,8 +747,18 @@ Plan make_plan(int rows, int K, int N, int adapters, int rank, int num_sms) {
   pl.down_y = std::max(1, std::min({want / std::max(pl.down_x * pl.down_split, 1), 32, adapters}));
   pl.down_nt = rank <= 8 ? 1 : (rank <= 16 ? 2 : (rank <= 32 ? 4 : 8));
   pl.split = 1;
-  while (pl.split < 8 && (long long)pl.tiles * pl.n_tiles * pl.split * 2 <= num_sms && pl.split * 2 <= pl.kblocks)
-    pl.split *= 2;
+  // Few tiles are split along K over a cluster, whose CTAs add their parts through distributed
+  // shared memory, so that a CTA keeps at least 16 steps: K steps of 64 and slices, as many as the tile
+  // may have.  Below that the exchange (1 to 4 us) costs more than it saves: 32 rows of K = N = 1024,
+  // rank 16, one adapter 7.8 us whole, 9.1 in two, 9.9 in eight; 128 rows with 64 adapters 25.7, 23.8,
+  // 21.4.  K = 4096, N = 1536, 32 rows with one adapter 15.0, 12.4, 14.0; with 32 21.9, 22.9, 19.4.
+  // Clusters of 4 or 8 take up to half the SMs only, since not all of those can hold one: 33 clusters
+  // of 4 and 15 of 8 fit at a time (36 of 4 took 27.5 us where 36 of 2 took 16.1; K = 4096, N = 1536).
+  // Rows on the M side are never split: their tiles are more than half the SMs.
+  const long long tiles = (long long)pl.tiles * pl.n_tiles;
+  const int most = pl.kblocks + std::min(pl.bt, adapters) * pl.chunks;
+  for (int s = 2; !pl.rows_on_m && s <= 8 && s <= pl.kblocks && most >= 16 * s; s *= 2)
+    if (tiles * s <= (s == 2 ? num_sms : num_sms / 2)) pl.split = s;
   pl.x_box = std::min(pl.bt, (rows + 7) / 8 * 8);
   pl.list_ld = (pl.bt + 2 + 3) / 4 * 4;
   return pl;

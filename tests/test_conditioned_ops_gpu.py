@@ -571,3 +571,24 @@ def test_conditioned_block(cuda, prec):
     assert float((y.double() - ref).norm()) <= bar
     assert float((tok.double() - ref[:, -1:]).norm()) <= 36 * U[prec] * float(delta[:, -1:].norm()) + \
         U[prec] * float(ref[:, -1:].norm())
+
+
+# many tiles (rows on the MMA's M side: more 128 x 128 tiles than SMs), several tiles of rows beside
+# the weights, and each width of the split along K (2, 4 and 8 CTAs)
+ADAPTER_PLANS = [
+    (2501, 264, 1032, 6, 24, "mixed"),
+    (3333, 72, 776, 9, 8, "sorted"),
+    (1290, 136, 2056, 3, 128, "mixed"),
+    (130, 2048, 1032, 4, 16, "mixed"),
+    (385, 2056, 1544, 2, 40, "sorted"),
+    (40, 4096, 648, 40, 16, "each"),
+    (257, 4104, 520, 5, 16, "mixed"),
+    (5, 8200, 264, 5, 16, "mixed"),
+    (150, 8192, 136, 3, 72, "mixed"),
+]
+
+
+@pytest.mark.parametrize("prec", ["fp16", "bf16"])
+@pytest.mark.parametrize("case", ADAPTER_PLANS, ids=lambda c: "-".join(map(str, c)))
+def test_adapter_gemm_plans(cuda, case, prec):
+    test_adapter_gemm(cuda, case, prec)
