@@ -59,7 +59,8 @@ __device__ __forceinline__ int row_id(const AdapterGemmParams& p, long long t) {
 // mma.sync m16n8k16; each warp streams its rows through a ring of its own in shared memory
 // (cp.async, whole 128-byte lines, three stages of 64 columns in flight: up to 144 KB an SM) and
 // takes A_a, which stays in L2, straight from global memory one step ahead.  No barrier
-// until the end.  (Forms that held x in registers kept too little in flight: 37 us for
+// until the end.  8192 rows of 4096 columns, rank 32: 40 us alone, about half of it under the
+// second launch (187 alone, 209 for both); 32 rows, 16 adapters: 10 us.  (Forms that held x in registers kept too little in flight: 37 us for
 // 8192 rows of 4096 columns; a tcgen05 form with 128-row slices of A_a took 35 us.)
 // A warp owns 32 rows; the warps of a CTA split K (down_kw of them) and rows.  For every
 // distinct adapter of its rows it computes all 32 x rank products from the rows that have
@@ -243,6 +244,9 @@ __global__ void __launch_bounds__(32 * kDownWarps)
 // U' of the slices, warps 6-13 epilogue.  The accumulators are double: the epilogue of a
 // tile overlaps the next one's main loop.  A ring stage holds 64 columns of W and x, or 4
 // slices of B_a and U'.
+// Bound: the tensor cores for large K (8192 rows, K = N = 4096: 209 us with the first launch, 1335
+// TFLOP/s); 48060 rows, K = 384, N = 1536: 73 us (2.55 TB/s), 65 of them this one's, tensor pipe
+// 49 % busy; latency for few rows (32 rows, 16 adapters, K = N = 4096: 20 us).
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMTile = 128 * 128;       // the M side: 128 rows x 64 columns of 16 bits
 

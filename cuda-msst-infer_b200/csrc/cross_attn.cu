@@ -29,6 +29,10 @@
 // 980 us for the long prompts against 752; the 64-column MMAs read as much of Q for half the
 // products).
 //
+// Bound: the chain scores, softmax, product.  4 x 8 heads of 1895 x 3792 x 64: 101 us (583 TFLOP/s), XU
+// pipe 62 %, tensor pipe 31 % busy.  4 x 32/8 heads of 4096 x 4096 x 128, ragged: 778 us
+// (1148 TFLOP/s).
+//
 // Softmax: the reference a row is exponentiated against starts at the maximum of its
 // first 32 kept scores and moves lazily: a tile is taken in one pass without a
 // maximum, and only a row sum above kSumLimit (or not finite) sends the warp through
@@ -654,6 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // row; kShare = 1: 8 warps take 32 rows each, kShare > 1 (items of many parts): the warps share
 // the parts of rows [32 y, 32 y + 32) out.  Slots of 16 rows (row by row, cross_token.cu): block (x, y) joins row y,
 // 4 columns a lane, its kShare = 8 warps sharing the parts out.
+// Bound: latency.  7 to 22 us alone; its start overlaps the end of the first launch.
 template <typename T, bool kByItem, bool kToken, int kShare>
 __global__ void __launch_bounds__(kShare > 1 ? 32 * kShare : 256)
     cross_combine_kernel(const __grid_constant__ CrossAttnParams p, const __grid_constant__ Geom g) {

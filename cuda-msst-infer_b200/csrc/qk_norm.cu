@@ -44,8 +44,9 @@ __device__ __forceinline__ int table_row(const QkNormParams& p, long long token,
 // [4l, 4l + 4) and [rot/2 + 4l, rot/2 + 4l + 4), two 8-byte loads instead of one of
 // 16 bytes, which costs issue slots that this kernel has to spare (shuffling the
 // partner's 8 values would cost more of them).
-// Bound: HBM.  kStream marks loads and stores as read and written once: 63.8 -> 59.5 us for
-// 338 MB (5.7 TB/s), no difference below L2's size, where the results should stay for the
+// Bound: HBM.  338 MB (4 x 4096 tokens, 32 + 8 heads of 128) take 64 us (5.3 TB/s), 197 MB of packed
+// rows 36 us (5.5 TB/s).  kStream marks loads and stores as read and written once: 63.9 -> 59.5 us
+// for one set of buffers of the first, no difference below L2's size, where the results should stay for the
 // attention that reads them.  Two heads a group took 75 us, eight 77, 256 threads a
 // block 67.
 constexpr int kHeads = 4;
