@@ -9,7 +9,7 @@
 // its two halves in turn, which are merged at the end.
 //
 // Work is cut into units (one K/V tile for a pair, two for a lone tile) and every CTA
-// takes an equal contiguous run of all units, over items of any length; the two
+// takes an equal contiguous run of all units, over items of any length (align_runs); the two
 // items a run may share with its neighbours leave partial results (O, running
 // reference and sum, fp32) in the workspace, which cross_combine_kernel joins in CTA
 // order.  So few rows against a long encoder and ragged batches fill the GPU alike.
@@ -862,11 +862,31 @@ Geom make_geom(int batch, int q_len, int k_len, int q_heads, int kv_heads, int h
   return g;
 }
 
-// Whether the call's equal runs may cut an item (for ragged batches the device decides).
-bool may_cut(const Geom& g, int k_len, bool ragged) {
+// Takes fewer CTAs where runs of a few units more than an equal share end with the items, or cut
+// them into equal parts; returns whether an item may be cut (for ragged batches, whose units the
+// device counts, the runs stay equal).
+// An item that is cut in odd places costs both CTAs another start and end, and the joining
+// launch: 8 x 8 heads of 100 x 600 x 64, items of 3 units: 148 runs of 1.3 units 19.6 us, 64 of 3 units, whole
+// items without a joining launch, 11.6; 5 x 12/4 heads of 77 x 1501 x 80, items of 12: 148 runs of 1.6
+// 29.6, 120 of 2 23.5; one token, 32/8 heads of 128, 4096 keys: 148 runs of 3.5 14.5, 128 of 4 11.2.
+// At most two units more than an equal share, as a unit of 128-row tiles takes 1.5 to 3 us and a cut
+// and its joining 3 to 8.  Such tiles' runs have two units at least for the same reason (items of
+// 12, 48 units in all: one 23.3 us, two 20.4; the other way: items of 16, 128 in all, 17.2 and 18.0 to 18.5).
+bool align_runs(Geom& g, const CrossAttnParams& p, int num_sms) {
   if (g.contribs <= 1) return false;
-  const long long kt = (k_len + (1 << g.tile_shift) - 1) >> g.tile_shift;
-  return ragged || kt > 1;
+  if (p.key_lens) return true;
+  const long long kt = (p.k_len + (1 << g.tile_shift) - 1) >> g.tile_shift, kl = (kt + 1) / 2;
+  const long long head = g.full * kt + g.lone * kl, units = (long long)p.batch * g.kv_heads * head;
+  if ((g.full ? kt : kl) == 1) return false;  // items of one unit
+  const long long least = (units + num_sms - 1) / num_sms;
+  for (long long r = std::max<long long>(least, g.tile_shift == 7 ? 2 : 1); r * num_sms <= units + 2 * num_sms; ++r) {
+    const bool whole = r % head == 0 || (!g.lone && r % kt == 0) || (!g.full && r % kl == 0);
+    const bool even = (!g.full || kt % r == 0) && (!g.lone || kl % r == 0);
+    if (units % r != 0 || !(whole || even)) continue;
+    g.contribs = (int)(units / r);
+    return !whole;
+  }
+  return true;
 }
 
 CUtensorMap query_map(const HeadsView& q, const CrossAttnParams& p, const Geom& g, int& batched) {
@@ -922,7 +942,8 @@ cudaError_t launch_t(const CrossAttnParams& p, int num_sms, cudaStream_t s) {
     cross_zero_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p);
     return cudaGetLastError();
   }
-  const Geom g = make_geom(p.batch, p.q_len, p.k_len, p.q.heads, p.k.heads, p.head_dim, num_sms);
+  Geom g = make_geom(p.batch, p.q_len, p.k_len, p.q.heads, p.k.heads, p.head_dim, num_sms);
+  const bool cut = align_runs(g, p, num_sms);
   cudaError_t e;
   if (g.slot_rows == kTokenRows)
     e = launch_cross_token<T>(p, g, s);
@@ -930,7 +951,7 @@ cudaError_t launch_t(const CrossAttnParams& p, int num_sms, cudaStream_t s) {
     e = p.key_mask ? launch_k<T, 64, true>(p, g, s) : launch_k<T, 64, false>(p, g, s);
   else
     e = p.key_mask ? launch_k<T, 128, true>(p, g, s) : launch_k<T, 128, false>(p, g, s);
-  if (e != cudaSuccess || !may_cut(g, p.k_len, p.key_lens != nullptr)) return e;
+  if (e != cudaSuccess || !cut) return e;
   return launch_combine<T>(p, g, s);
 }
 

@@ -592,3 +592,25 @@ ADAPTER_PLANS = [
 @pytest.mark.parametrize("case", ADAPTER_PLANS, ids=lambda c: "-".join(map(str, c)))
 def test_adapter_gemm_plans(cuda, case, prec):
     test_adapter_gemm(cuda, case, prec)
+
+
+# runs that end with the items (one item, several, a key head's pairs and lone tile) or cut them evenly
+CROSS_RUNS = [
+    (8, 100, 600, 8, 8, 64, "none", "kv"),
+    (16, 32, 300, 8, 8, 64, "keys", "kv"),
+    (30, 16, 300, 32, 16, 64, "none", "kv"),
+    (4, 257, 256, 16, 16, 64, "keys", "bhnd"),
+    (2, 77, 1501, 12, 12, 64, "none", "kv"),
+    (1, 300, 2000, 16, 4, 128, "keys", "kv"),
+    (4, 257, 1024, 16, 16, 64, "none", "kv"),
+    (2, 300, 77, 8, 8, 128, "keys", "kv"),      # items of one unit
+    (1, 1, 4096, 32, 8, 128, "none", "kv"),
+    (4, 1, 1500, 8, 8, 64, "keys", "kv"),
+    (64, 1, 200, 8, 8, 64, "none", "bhnd"),
+]
+
+
+@pytest.mark.parametrize("prec", ["fp16", "bf16"])
+@pytest.mark.parametrize("case", CROSS_RUNS, ids=lambda c: "-".join(map(str, c)))
+def test_cross_attention_runs(cuda, case, prec):
+    test_cross_attention(cuda, case, prec)
