@@ -29,9 +29,9 @@
 // 980 us for the long prompts against 752; the 64-column MMAs read as much of Q for half the
 // products).
 //
-// Bound: the chain scores, softmax, product.  4 x 8 heads of 1895 x 3792 x 64: 101 us (583 TFLOP/s), XU
-// pipe 62 %, tensor pipe 31 % busy.  4 x 32/8 heads of 4096 x 4096 x 128, ragged: 778 us
-// (1148 TFLOP/s).
+// Bound: the chain scores, softmax, product.  4 x 8 heads of 1895 x 3792 x 64: 101 us (582 TFLOP/s), XU
+// pipe 62 %, tensor pipe 31 % busy.  4 x 32/8 heads of 4096 x 4096 x 128, ragged: 772 to 778 us
+// (1150 TFLOP/s).
 //
 // Softmax: the reference a row is exponentiated against starts at the maximum of its
 // first 32 kept scores and moves lazily: a tile is taken in one pass without a
