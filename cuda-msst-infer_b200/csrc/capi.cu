@@ -175,6 +175,13 @@ msst::HeadsView heads_view(const msst_heads* t, int batch, int seq, int align, c
   return v;
 }
 
+// The heads of a cross attention (its sizes are computed from their quotient).
+void check_cross_heads(int q_heads, int kv_heads, int head_dim) {
+  MSST_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "head_dim must be a multiple of 8, <= 128");
+  MSST_REQUIRE(q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0,
+               "k and v need the same number of heads, and q a multiple of it");
+}
+
 void check_workspace(const void* p, long long have, long long need) {
   MSST_REQUIRE(need == 0 || (p && have >= need), "the workspace holds " + std::to_string(have) + " bytes, " +
                                                      std::to_string(need) + " are needed");
@@ -475,8 +482,8 @@ int msst_qk_norm_rope(const msst_heads* q, const msst_heads* k, int batch, int s
 int msst_cross_attention_workspace(int batch, int q_len, int k_len, int q_heads, int kv_heads, int head_dim,
                                    long long* bytes) {
   return guarded([&] {
-    MSST_REQUIRE(bytes && batch >= 0 && q_len >= 0 && k_len >= 0 && q_heads > 0 && kv_heads > 0 && head_dim > 0,
-                 "bad shape");
+    MSST_REQUIRE(bytes && batch >= 0 && q_len >= 0 && k_len >= 0, "bad shape");
+    check_cross_heads(q_heads, kv_heads, head_dim);
     *bytes = msst::cross_attention_workspace(batch, q_len, k_len, q_heads, kv_heads, head_dim, sm_count());
   });
 }
@@ -487,7 +494,6 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
   return guarded([&] {
     check_dtype(dtype);
     MSST_REQUIRE(batch >= 0 && q_len >= 0 && k_len >= 0, "bad shape");
-    MSST_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "head_dim must be a multiple of 8, <= 128");
     MSST_REQUIRE(std::isfinite(scale), "scale must be finite");
     msst::CrossAttnParams p{};
     p.q = heads_view(q, batch, q_len, 8, "q");
@@ -495,8 +501,8 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
     p.v = heads_view(v, batch, k_len, 8, "v");
     p.out = heads_view(out, batch, q_len, 8, "out");
     MSST_REQUIRE(p.out.heads == p.q.heads, "out must have q's heads");
-    MSST_REQUIRE(p.k.heads == p.v.heads && p.q.heads % p.k.heads == 0,
-                 "k and v need the same number of heads, and q a multiple of it");
+    MSST_REQUIRE(p.k.heads == p.v.heads, "k and v need the same number of heads, and q a multiple of it");
+    check_cross_heads(p.q.heads, p.k.heads, head_dim);
     MSST_REQUIRE((long long)batch * q_len <= (1LL << 31) / p.q.heads, "too many query rows");
     if (batch == 0 || q_len == 0) return;
     MSST_REQUIRE((q_len == 1 || p.q.seq_stride > 0) && (p.q.heads == 1 || p.q.head_stride > 0) &&

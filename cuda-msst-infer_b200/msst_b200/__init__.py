@@ -434,6 +434,7 @@ class ops:
         _, Nk, Hk, _ = ks
         _need(ks[0] == B and ks[3] == d and v.shape == ks,
               "k and v must be [B, Nk, heads, head_dim] with q's B and head_dim")
+        _need(Hk > 0 and Hq > 0 and Hq % Hk == 0, "q must have a multiple of k's and v's heads")
         _need(k.dtype is dt and v.dtype is dt and k.get_device() == dev and v.get_device() == dev,
               "q, k and v must share one 16-bit dtype and one device")
         (q, sq), (k, sk), (v, sv) = _aligned_heads(q, shape), _aligned_heads(k, ks, True), _aligned_heads(v, ks, True)
