@@ -31,6 +31,12 @@ struct QkNormParams {
   const int* positions;     // [batch, seq] or nullptr (the index in the sequence)
 };
 cudaError_t launch_qk_norm(const QkNormParams& p, int bf16, cudaStream_t stream);
+// The group of heads that a thread of the 8-column kernel works on: blocks of 128 threads, lpv (a
+// divisor of 128) threads a group.  Dividing first keeps the index in 32 bits for as many groups as
+// 32 bits count; the number of threads before a block may pass 2^32.
+__host__ __device__ __forceinline__ unsigned qk_norm_item(unsigned block, unsigned thread, unsigned lpv) {
+  return block * (128u / lpv) + thread / lpv;
+}
 
 struct CrossAttnParams {
   HeadsView q, k, v, out;

@@ -54,7 +54,7 @@ constexpr int kHeads = 4;
 template <typename T, int LPV, bool kHalves, bool kStream>
 __global__ void __launch_bounds__(128) qk_norm_kernel(const __grid_constant__ QkNormParams p, unsigned items,
                                                       int chunks_q, int chunks) {
-  const unsigned item = (blockIdx.x * 128u + threadIdx.x) / LPV;
+  const unsigned item = qk_norm_item(blockIdx.x, threadIdx.x, LPV);
   const int l = threadIdx.x % LPV;
   if (item >= items) return;  // whole groups: the shuffles below stay inside a group
   const unsigned token = item / (unsigned)chunks;

@@ -2,8 +2,27 @@
 from __future__ import annotations
 
 import ctypes
+import os
+import shutil
+import subprocess
 
 import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "cuda-msst-infer_b200", "csrc")
+
+
+def _run_on_host(tmp_path, program):
+    """Compiles `program` against the kernels' headers and runs its host code."""
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("nvcc not available")
+    src, exe = tmp_path / "check.cu", tmp_path / "check"
+    src.write_text(program)
+    subprocess.run([nvcc, "-std=c++17", "-O1", "-gencode", "arch=compute_100a,code=sm_100a", "-I", CSRC, "-I",
+                    os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True, capture_output=True, timeout=300)
+    out = subprocess.run([str(exe)], check=False, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stdout + out.stderr
 
 
 @pytest.mark.parametrize("q_heads, kv_heads, head_dim", [(2, 4, 64), (3, 2, 64), (1, 1 << 30, 8), (4, 4, 136), (4, 4, 12)])
@@ -26,3 +45,23 @@ def test_cross_attention_refuses_heads_in_python(Hq, Hk):
     k = torch.zeros(1, 5, Hk, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="heads"):
         ops.cross_attention(q, k, k)
+
+
+def test_qk_norm_items_past_32_bits_of_threads(tmp_path):
+    """The item of every thread against the same division in 64 bits, up to 2^31 items (the most head
+    vectors that a call may have), where the threads' own numbers reach 2^36."""
+    _run_on_host(tmp_path, r"""
+#include <cstdio>
+#include "operators.cuh"
+int main() {
+  for (unsigned lpv = 1; lpv <= 32; lpv *= 2) {
+    const unsigned long long last = ((1ull << 31) * lpv + 127) / 128;  // blocks of the largest call
+    for (unsigned long long b = 0; b < last; b = b < 1000 || b + 5 > last ? b + 1 : (b * 3 / 2 < last - 4 ? b * 3 / 2 : last - 4))
+      for (unsigned t = 0; t < 128; ++t)
+        if (msst::qk_norm_item((unsigned)b, t, lpv) != (b * 128 + t) / lpv) {
+          std::printf("lpv %u block %llu thread %u\n", lpv, b, t);
+          return 1;
+        }
+  }
+}
+""")

@@ -1,0 +1,33 @@
+"""GPU tests of the conditioned-block operators at the edges of their ranges: values that do not
+fit 16 bits, infinities, many keys of tiny weight, codes of several errors, graphs and threads.
+Reference forms and tolerances as in test_conditioned_ops_gpu.py, unless a test derives its own."""
+from __future__ import annotations
+
+import pytest
+
+from test_conditioned_ops_gpu import U, _gen, _qk_ref, _within
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ norms: very many tokens
+@pytest.mark.parametrize("d, tokens", [(136, 2 ** 27 + 5), (72, 2 ** 28 + 5)])
+def test_qk_norm_rope_past_32_bits_of_threads(cuda, d, tokens):
+    """In place over 36 to 39 GB of one-head tokens, more than 2^32 threads: the first and the last
+    tokens are normed, once."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    if torch.cuda.mem_get_info()[0] < 45e9:
+        pytest.skip("needs 45 GB of device memory")
+    x = torch.empty(1, tokens, 1, d, dtype=torch.bfloat16, device="cuda")
+    some = torch.tensor([0, 1, 2, 3, 4, 5, tokens // 2, tokens - 6, tokens - 5, tokens - 4, tokens - 1], device="cuda")
+    before = (3 * torch.randn(1, some.numel(), 1, d, generator=_gen(torch, 2), device="cuda")).bfloat16()
+    x[:, some] = before
+    ops.qk_norm_rope(x, out_q=x)
+    got = x[:, some]
+    del x
+    torch.cuda.empty_cache()
+    ref, arith = _qk_ref(torch, before, None, None, None, None, 1e-6, "halves")
+    _within(got, ref, U["bf16"] * ref.abs() + arith * 2 + 1e-30, "qk_norm_rope")
+    assert device_error(True) == 0
