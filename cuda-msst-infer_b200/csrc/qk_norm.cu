@@ -98,54 +98,65 @@ __global__ void __launch_bounds__(128) qk_norm_kernel(const __grid_constant__ Qk
     *reinterpret_cast<float4*>(g) = __ldg(reinterpret_cast<const float4*>(gamma + c0));
     *reinterpret_cast<float4*>(g + 4) = __ldg(reinterpret_cast<const float4*>(gamma + c1));
   }
-  if (turned) {
-    const int row = table_row(p, token, n);
-    if (row >= 0) {
-      const size_t at = (size_t)row * half + 4 * l;  // pairs 4l .. 4l + 3 with either pairing
-      *reinterpret_cast<float4*>(co) = __ldg(reinterpret_cast<const float4*>(p.cos_tab + at));
-      *reinterpret_cast<float4*>(si) = __ldg(reinterpret_cast<const float4*>(p.sin_tab + at));
-    }
+  const int row = half > 0 ? table_row(p, token, n) : -1;
+  const bool rotate = turned && row >= 0;
+  if (rotate) {
+    const size_t at = (size_t)row * half + 4 * l;  // pairs 4l .. 4l + 3 with either pairing
+    *reinterpret_cast<float4*>(co) = __ldg(reinterpret_cast<const float4*>(p.cos_tab + at));
+    *reinterpret_cast<float4*>(si) = __ldg(reinterpret_cast<const float4*>(p.sin_tab + at));
   }
   const unsigned group = LPV == 32 ? 0xffffffffu : ((1u << LPV) - 1u) << ((threadIdx.x & 31) / LPV * LPV);
   const float inv_d = 1.f / (float)p.head_dim;
+  // kAsk: pairs that are not rotated (a tail, a position outside the tables) keep their values, which
+  // (1, 0) as a rotation would not do for an infinity's neighbour (0 * inf).  Interleaved groups whose
+  // pairs all turn do not ask: 35.8 us for 60 x 801 tokens, 8 + 8 heads of 64, asking 36.1, a branch
+  // in each head 36.9.  With halves the second form costs more than the question: 65.9 us for
+  // 4 x 4096 tokens, 32 + 8 heads of 128, 64.4 always asking.
+  auto heads = [&](auto ask) {
+    constexpr bool kAsk = decltype(ask)::value;
 #pragma unroll
-  for (int u = 0; u < kHeads; ++u) {
-    if (u >= left) break;
-    float x[8];
-    unpack2<T>(raw[u][0].x, x[0], x[1]);
-    unpack2<T>(raw[u][0].y, x[2], x[3]);
-    unpack2<T>(raw[u][1].x, x[4], x[5]);
-    unpack2<T>(raw[u][1].y, x[6], x[7]);
-    float ss = 0.f;
+    for (int u = 0; u < kHeads; ++u) {
+      if (u >= left) break;
+      float x[8];
+      unpack2<T>(raw[u][0].x, x[0], x[1]);
+      unpack2<T>(raw[u][0].y, x[2], x[3]);
+      unpack2<T>(raw[u][1].x, x[4], x[5]);
+      unpack2<T>(raw[u][1].y, x[6], x[7]);
+      float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
 #pragma unroll
-    for (int o = LPV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-    const float r = rsqrtf(ss * inv_d + p.eps);
+      for (int o = LPV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+      const float r = rsqrtf(ss * inv_d + p.eps);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= r * g[i];
+      for (int i = 0; i < 8; ++i) x[i] *= r * g[i];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // kHalves: (x[i], x[4 + i]); interleaved: (x[2i], x[2i + 1])
-      float& a = kHalves ? x[i] : x[2 * i];
-      float& c = kHalves ? x[4 + i] : x[2 * i + 1];
-      if (kHalves && !turned) break;  // the unrotated tail of a vector
-      const float t = a * co[i] - c * si[i];
-      c = c * co[i] + a * si[i];
-      a = t;
-    }
-    const uint2 y0 = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
-    const uint2 y1 = make_uint2(pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
-    if (active) {
-      T* t = dst + u * to.head_stride;
-      if constexpr (kHalves) {
-        store<kStream>(reinterpret_cast<uint2*>(t + c0), y0);
-        store<kStream>(reinterpret_cast<uint2*>(t + c1), y1);
-      } else {
-        store<kStream>(reinterpret_cast<uint4*>(t + c0), make_uint4(y0.x, y0.y, y1.x, y1.y));
+      for (int i = 0; i < 4; ++i) {
+        // kHalves: (x[i], x[4 + i]); interleaved: (x[2i], x[2i + 1])
+        float& a = kHalves ? x[i] : x[2 * i];
+        float& c = kHalves ? x[4 + i] : x[2 * i + 1];
+        if (kHalves && !turned) break;  // the unrotated tail of a vector
+        const float t = a * co[i] - c * si[i], w = c * co[i] + a * si[i];
+        a = !kAsk || rotate ? t : a;
+        c = !kAsk || rotate ? w : c;
+      }
+      const uint2 y0 = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+      const uint2 y1 = make_uint2(pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+      if (active) {
+        T* t = dst + u * to.head_stride;
+        if constexpr (kHalves) {
+          store<kStream>(reinterpret_cast<uint2*>(t + c0), y0);
+          store<kStream>(reinterpret_cast<uint2*>(t + c1), y1);
+        } else {
+          store<kStream>(reinterpret_cast<uint4*>(t + c0), make_uint4(y0.x, y0.y, y1.x, y1.y));
+        }
       }
     }
-  }
+  };
+  if (!kHalves && row >= 0 && p.rot_dim == p.head_dim)
+    heads(std::false_type{});
+  else
+    heads(std::true_type{});
 }
 
 // Any even head_dim, stride and alignment: one warp per head vector, a pair of

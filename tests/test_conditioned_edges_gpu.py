@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import pytest
 
-from test_conditioned_ops_gpu import U, _gen, _qk_ref, _within
+from test_conditioned_ops_gpu import U, _dt, _gen, _qk_ref, _tables, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +31,29 @@ def test_qk_norm_rope_past_32_bits_of_threads(cuda, d, tokens):
     ref, arith = _qk_ref(torch, before, None, None, None, None, 1e-6, "halves")
     _within(got, ref, U["bf16"] * ref.abs() + arith * 2 + 1e-30, "qk_norm_rope")
     assert device_error(True) == 0
+
+
+# ------------------------------------------------------------------ norms: infinities
+@pytest.mark.parametrize("prec", ["fp16", "bf16"])
+@pytest.mark.parametrize("pairing", ["interleaved", "halves"])
+@pytest.mark.parametrize("d, rot", [(64, 32), (48, 0), (10, 6)])
+def test_qk_norm_rope_infinity_beside_the_rotation(cuda, d, rot, pairing, prec):
+    """An infinite column that is not rotated, in the tail or for a position outside the tables, is NaN
+    after its norm (inf / inf); its neighbour is x / inf = 0, since nothing turns it."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    q = torch.randn(1, 4, 3, d, generator=_gen(torch, 9), device="cuda").to(_dt(torch, prec))
+    col = d - 2
+    q[0, 1, 1, col] = float("inf")
+    q[0, 2, 2, col + 1] = -float("inf")
+    q[0, 3, 0, 0] = float("inf")
+    cos, sin = _tables(torch, 4, rot // 2) if rot else (None, None)
+    pos = torch.tensor([[0, 1, 2, 4]], dtype=torch.int32, device="cuda")
+    y, _ = ops.qk_norm_rope(q, None, None, None, cos, sin, positions=pos, pairing=pairing)
+    assert device_error(True) == (14 if rot else 0)
+    want = torch.zeros(1, 4, 3, d, dtype=torch.bool, device="cuda")
+    want[0, 1, 1, col] = want[0, 2, 2, col + 1] = want[0, 3, 0, 0] = True
+    assert torch.equal(y.isnan(), want)
+    hurt = want.any(-1, keepdim=True)
+    assert bool((y[hurt.expand_as(y) & ~want] == 0).all()) and bool(y[~hurt.expand_as(y)].isfinite().all())
