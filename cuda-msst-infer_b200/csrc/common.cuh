@@ -12,46 +12,23 @@
 #include <atomic>
 #include <type_traits>
 
+#include "device_errors.h"
+
 namespace msst {
 
 // ---------------------------------------------------------------------------
 // Device-side error reporting.  Every spin-wait in the library is bounded; a wait
-// that gives up records a code here (first one wins) and the kernel unwinds.
-// The host reads it with msst_device_error().
+// that gives up records a code here (first one wins) and the kernel unwinds.  Data of a
+// call outside its documented range is kept beside it, a bit for each kind, so that
+// neither hides the other.  The host reads them with msst_device_error().
 // ---------------------------------------------------------------------------
-enum DeviceError : unsigned {
-  kErrNone = 0,
-  kErrTimeoutTmaFull = 1,
-  kErrTimeoutSmemEmpty = 2,
-  kErrTimeoutTmemFull = 3,
-  kErrTimeoutTmemEmpty = 4,
-  kErrTimeoutAttnS = 5,
-  kErrTimeoutAttnP = 6,
-  kErrTimeoutAttnO = 7,
-  kErrTimeoutAttnQ = 8,
-  kErrTimeoutAttnKV = 9,
-  kErrTimeoutFfnS = 10,
-  kErrTimeoutFfnP = 11,
-  kErrTimeoutFfnO = 12,
-  kErrTimeoutFfnFlag = 13,
-  // not a wait: data of the call outside its documented range (see the operator)
-  kErrPosition = 14,
-  kErrAdapter = 15,
-};
+static __device__ DeviceErrors g_device_errors = {0, 0};
 
-// One flag per translation unit; each .cu exposes a host accessor (see
-// MSST_DEFINE_ERROR_ACCESSOR) and the C ABI ORs them together.
-static __device__ unsigned g_device_error = 0;
-
-#define MSST_DEFINE_ERROR_ACCESSOR(fn)                                              \
-  unsigned fn(bool clear) {                                                         \
-    unsigned v = 0;                                                                 \
-    if (cudaMemcpyFromSymbol(&v, g_device_error, sizeof(v)) != cudaSuccess) return ~0u; \
-    if (clear && v) {                                                               \
-      unsigned z = 0;                                                               \
-      cudaMemcpyToSymbol(g_device_error, &z, sizeof(z));                            \
-    }                                                                               \
-    return v;                                                                       \
+// Each .cu exposes its record to the C ABI: fn(e, store) reads or writes it.
+#define MSST_DEFINE_ERROR_ACCESSOR(fn)                                         \
+  bool fn(DeviceErrors& e, bool store) {                                       \
+    return (store ? cudaMemcpyToSymbol(g_device_errors, &e, sizeof(e))         \
+                  : cudaMemcpyFromSymbol(&e, g_device_errors, sizeof(e))) == cudaSuccess; \
   }
 
 // Wall-clock limit for one mbarrier wait (ns).  Real waits in these kernels last
@@ -68,7 +45,12 @@ __device__ __forceinline__ unsigned long long global_timer_ns() {
   return t;
 }
 
-__device__ __forceinline__ void record_error(unsigned code) { atomicCAS(&g_device_error, 0u, code); }
+__device__ __forceinline__ void record_error(unsigned code) {
+  if (code >= kFirstDataError)
+    atomicOr(&g_device_errors.data, 1u << (code - kFirstDataError));
+  else
+    atomicCAS(&g_device_errors.wait, 0u, code);
+}
 
 // Host: accounting of this library's kernel launches.  Each launcher opens a
 // LaunchScope right before its <<<>>>: the scope counts the launch

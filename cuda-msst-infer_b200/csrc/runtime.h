@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/msst_b200.h"
+#include "device_errors.h"
 
 namespace msst {
 
@@ -164,21 +165,31 @@ inline int device_sm_count() {
   return n;
 }
 
-// Per-translation-unit device error flags, ORed by msst_device_error().
-unsigned gemm_device_error(bool clear);
-unsigned attention_device_error(bool clear);
-unsigned kernels_device_error(bool clear);
-unsigned band_attention_device_error(bool clear);
-unsigned qk_norm_device_error(bool clear);
-unsigned cross_attn_device_error(bool clear);
-unsigned cross_token_device_error(bool clear);
-unsigned adapter_gemm_device_error(bool clear);
+// The translation units' device error records (MSST_DEFINE_ERROR_ACCESSOR).
+bool gemm_device_error(DeviceErrors& e, bool store);
+bool attention_device_error(DeviceErrors& e, bool store);
+bool kernels_device_error(DeviceErrors& e, bool store);
+bool band_attention_device_error(DeviceErrors& e, bool store);
+bool qk_norm_device_error(DeviceErrors& e, bool store);
+bool cross_attn_device_error(DeviceErrors& e, bool store);
+bool cross_token_device_error(DeviceErrors& e, bool store);
+bool adapter_gemm_device_error(DeviceErrors& e, bool store);
 
+// The code that msst_device_error reports; `clear` takes that one out.
 inline unsigned device_error(bool clear) {
-  return gemm_device_error(clear) | attention_device_error(clear) | kernels_device_error(clear) |
-         band_attention_device_error(clear) | qk_norm_device_error(clear) | cross_attn_device_error(clear) |
-         cross_token_device_error(clear) |
-         adapter_gemm_device_error(clear);
+  constexpr int n = 8;
+  bool (*const unit[n])(DeviceErrors&, bool) = {
+      gemm_device_error,    attention_device_error,  kernels_device_error,     band_attention_device_error,
+      qk_norm_device_error, cross_attn_device_error, cross_token_device_error, adapter_gemm_device_error};
+  DeviceErrors was[n], now[n];
+  for (int i = 0; i < n; ++i) {
+    if (!unit[i](was[i], false)) return ~0u;
+    now[i] = was[i];
+  }
+  const unsigned code = take_error(now, n);
+  for (int i = 0; clear && i < n; ++i)
+    if ((now[i].wait != was[i].wait || now[i].data != was[i].data) && !unit[i](now[i], true)) return ~0u;
+  return code;
 }
 
 // Launch accounting (launch_stats.cu; see LaunchScope in common.cuh).

@@ -76,8 +76,10 @@ typedef struct msst_model_info {
 } msst_model_info;
 
 const char* msst_last_error(void);
-/* Code recorded by a kernel whose bounded wait gave up, or that met a position or an
- * adapter index outside the range its operator documents (0 = none); clear != 0 resets it. */
+/* Code recorded by kernels since the last reset, 0 = none: 1 to 13 where a bounded wait gave up
+ * (results since then are garbage), 14 where a position and 15 where an adapter index lay outside
+ * the range that its operator documents.  A wait comes before the others; where several are
+ * recorded, clear != 0 resets the returned one (of the waits, all) and the next call gives the next. */
 unsigned msst_device_error(int clear);
 int msst_version(void);
 /* Number of kernels this library has launched (process-wide); reset != 0 returns and zeroes it. */

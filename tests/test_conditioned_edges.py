@@ -65,3 +65,39 @@ int main() {
   }
 }
 """)
+
+
+def test_device_errors_do_not_hide_one_another(tmp_path):
+    """Every pair of codes, recorded in one translation unit or in two: a wait that gave up is reported
+    as itself and before data errors, each data error as itself, and none is lost."""
+    _run_on_host(tmp_path, r"""
+#include <cstdio>
+#include "device_errors.h"
+using namespace msst;
+static void record(DeviceErrors& e, unsigned code) {  // as the kernels' record_error
+  if (code >= kFirstDataError) e.data |= 1u << (code - kFirstDataError);
+  else if (!e.wait) e.wait = code;
+}
+int main() {
+  static_assert(kErrPosition == 14 && kErrAdapter == 15 && kErrTimeoutFfnFlag == 13, "documented codes");
+  for (unsigned a = 0; a <= 15; ++a)
+    for (unsigned b = 0; b <= 15; ++b)
+      for (int second = 0; second < 2; ++second) {
+        DeviceErrors e[3] = {};
+        if (a) record(e[0], a);
+        if (b) record(e[second], b);
+        unsigned want[3], n = 0;
+        const bool wa = a && a < 14, wb = b && b < 14;
+        if (wa || wb) want[n++] = wa ? a : b;
+        for (unsigned k = 14; k <= 15; ++k)
+          if (a == k || b == k) want[n++] = k;
+        for (unsigned i = 0; i <= n; ++i) {
+          const unsigned got = take_error(e, 3);
+          if (got != (i < n ? want[i] : 0)) {
+            std::printf("%u %u %d: %u\n", a, b, second, got);
+            return 1;
+          }
+        }
+      }
+}
+""")

@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import pytest
 
-from test_conditioned_ops_gpu import U, _dt, _gen, _qk_ref, _tables, _within
+from test_conditioned_ops_gpu import U, _adapter_inputs, _dt, _gen, _qk_ref, _tables, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,20 @@ def test_qk_norm_rope_infinity_beside_the_rotation(cuda, d, rot, pairing, prec):
     assert torch.equal(y.isnan(), want)
     hurt = want.any(-1, keepdim=True)
     assert bool((y[hurt.expand_as(y) & ~want] == 0).all()) and bool(y[~hurt.expand_as(y)].isfinite().all())
+
+
+# ------------------------------------------------------------------ codes of several errors
+def test_device_error_of_two_operators(cuda):
+    """A position and an adapter index outside their ranges before the host asks: both are reported."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    device_error(True)
+    q = torch.randn(1, 3, 2, 64, generator=_gen(torch, 6), device="cuda").half()
+    cos, sin = _tables(torch, 4, 32)
+    x, w, la, lb, ids, _, _ = _adapter_inputs(torch, 10, 64, 64, 2, 8, "fp16", 7)
+    ids[3] = 2
+    ops.adapter_gemm(x, w, la, lb, ids)
+    ops.qk_norm_rope(q, None, None, None, cos, sin, positions=torch.full((1, 3), 4, dtype=torch.int32, device="cuda"))
+    assert device_error(False) == 14 and device_error(False) == 14
+    assert device_error(True) == 14 and device_error(True) == 15 and device_error(True) == 0
