@@ -261,7 +261,7 @@ struct GemmCfgA {
   static constexpr uint32_t kStaging = kRowsOnM ? 8 * 2048 : 0;  // 32 x 32 outputs a warp
   static constexpr size_t kSmem = kStages * kStage + kStaging + 512;
   static constexpr uint32_t kTmem = 2 * BT;
-  static_assert(4 * kStages * 8 + 48 + 16 * 4 <= 512, "barriers");
+  static_assert(4 * kStages * 8 + 56 + 16 * 4 <= 512, "barriers");
   static_assert(kRowsOnM || kStages * kStage >= BT * 128 * 4, "the split-K exchange reuses the ring");
 };
 constexpr int kThreadsA = 448;
@@ -347,7 +347,8 @@ __global__ void __launch_bounds__(kThreadsA, 1)
   uint64_t* u_full = u_go + C::kStages;   // [stages] U' written, B_a's slices landed
   uint64_t* acc_full = u_full + C::kStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;     // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* mma_end = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_end + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // [tile count % 16] = tile count + 1 where values of B_a were left out (U' runs ahead of
   // the epilogue by fewer tiles than the ring has stages, plus the two accumulators)
@@ -371,6 +372,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 256);
     }
+    mbar_init(mma_end, 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&xmap);
@@ -434,6 +436,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
                           n0, sl.id[i]);
         }
       }
+      mbar_drain_ring(full, C::kStages, it % C::kStages, it / C::kStages & 1);
     }
   } else if (warp == 1) {
     if (elect_one()) {
@@ -481,6 +484,8 @@ __global__ void __launch_bounds__(kThreadsA, 1)
         }
         if (ok) umma_commit(&acc_full[buf]);
       }
+      umma_commit(mma_end);  // TMEM and the ring are not given up under an MMA
+      mbar_drain(mma_end, 0);
     }
   } else if (warp < 6) {
     // ------------------------------------------------------------ U' of the slices
@@ -597,7 +602,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
       const long long t0 = (long long)tt * C::kRows;
       const int col = n0 + q * 32 + lane;  // weights on the M side: this lane's output column
       const float bias = !kRowsOnM && p.bias && rank == 0 && col < p.N ? __ldg(p.bias + col) : 0.f;
-      if (!mbar_wait(&acc_full[buf], (n >> 1) & 1, kErrTimeoutTmemFull, abort_flag)) break;
+      if (!mbar_wait_warp(&acc_full[buf], (n >> 1) & 1, kErrTimeoutTmemFull, abort_flag)) break;
       tc_fence_after();
       const bool dropped = s_dropped[n & 15] == n + 1;
       const int* list = lists + (size_t)tt * pl.list_ld;

@@ -177,10 +177,27 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
 
 // The same for a warp that walks a role together, with a uniform result.  Every lane is held
 // until all have seen the phase: a lane left behind in the spin while the issuing lane went
-// on could find the barrier two phases further, which looks like the phase not completed.
+// on could find the barrier two phases further, which looks like the phase not completed; and
+// where the wait gives up, no lane may go on to a full-mask or .aligned instruction that
+// another, gone from the loop, does not reach.
 template <bool kSuspend = true>
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, unsigned code, volatile int* abort) {
   return __all_sync(0xffffffffu, mbar_wait<kSuspend>(bar, parity, code, abort));
+}
+
+// Waits for a role's own copies or MMAs in flight at its end, so that no memory is given up under them
+// where their reader gave up: bounded, without looking at the abort flag and without a record.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = smem_u32(bar);
+  if (mbar_try_wait(a, parity)) return;
+  const unsigned long long t0 = global_timer_ns();
+  while (!mbar_try_wait(a, parity) && global_timer_ns() - t0 < kWaitLimitNs) {
+  }
+}
+// The same for the copies of a ring of n slots whose next use is that of `slot` in `phase` (a barrier
+// that was never used has the phase before its first completed).
+__device__ inline void mbar_drain_ring(uint64_t* full, int n, int slot, uint32_t phase) {
+  for (int i = 0; i < n; ++i) mbar_drain(&full[i], i < slot ? phase : phase ^ 1);
 }
 
 // ---------------------------------------------------------------------------

@@ -64,7 +64,7 @@ struct Cfg {
   static constexpr uint32_t kTile = kHalves * kHalfBytes;      // one Q, K or V tile
   static constexpr int kKSlots = DP == 128 ? 3 : 5, kVSlots = DP == 128 ? 2 : 5;
   static constexpr size_t kSmem = (2 + kKSlots + kVSlots) * kTile + 2560;
-  static_assert((18 + 2 * kKSlots + 3 * kVSlots) * 8 + 40 + kVSlots * 16 + 2048 <= 2560, "barriers and exchange");
+  static_assert((19 + 2 * kKSlots + 3 * kVSlots) * 8 + 40 + kVSlots * 16 + 2048 <= 2560, "barriers and exchange");
   static constexpr int kBufs = DP == 128 ? 2 : 3;              // NB
   static constexpr uint32_t kColO = kBufs * 128;
 };
@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* pv_done = bars + 10; // [2 tiles], every step
   uint64_t* o_done = bars + 12;  // [2 tiles], every item
   uint64_t* meet = bars + 14;    // [4 lane quarters]: the two halves of a lone tile
-  uint64_t* k_full = bars + 18;
+  uint64_t* mma_end = bars + 18;
+  uint64_t* k_full = bars + 19;
   uint64_t* k_empty = k_full + C::kKSlots;
   uint64_t* v_full = k_empty + C::kKSlots;   // landed
   uint64_t* v_ready = v_full + C::kVSlots;   // fit for the MMA
@@ -220,6 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&o_done[w], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
+    mbar_init(mma_end, 1);
     for (int i = 0; i < C::kKSlots; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -261,9 +263,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         KPos kp;
         VPos vp;
+        uint32_t q_phase = 0;
         bool ok = true;
         while (ok && k.next(p, g)) {
-          if (!mbar_wait<false>(q_empty, (k.seg & 1) ^ 1, kErrTimeoutAttnQ, abort_flag)) break;
+          if (!(ok = mbar_wait<false>(q_empty, q_phase ^ 1, kErrTimeoutAttnQ, abort_flag))) break;
+          q_phase ^= 1;
           const int nq = k.lone ? 1 : 2;
           mbar_arrive_expect_tx(q_full, nq * C::kHalves * (uint32_t)(g.gt * g.nt) * 128u);
           for (int w = 0; w < nq; ++w) {
@@ -297,6 +301,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        mbar_drain(q_full, q_phase ^ 1);
+        mbar_drain_ring(k_full, C::kKSlots, kp.slot, kp.phase);
+        mbar_drain_ring(v_full, C::kVSlots, vp.slot, vp.phase);
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer
@@ -379,6 +386,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ok) umma_commit(&o_done[1]);
           seq += (uint32_t)(steps + steps1);
         }
+        umma_commit(mma_end);  // TMEM and the tiles are not given up under an MMA
+        mbar_drain(mma_end, 0);
       }
     } else if (warp == 2) {
       // ------------------------------------------------------------ rows that are not kept
@@ -447,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t sAddr = tmem + lane_off + b.buf * 128;
         uint32_t words[4];
         if constexpr (kMask) {
-          if (!mbar_wait<false>(&v_ready[vs.slot], vs.phase, kErrTimeoutAttnKV, abort_flag)) {
+          if (!mbar_wait_warp<false>(&v_ready[vs.slot], vs.phase, kErrTimeoutAttnKV, abort_flag)) {
             ok = false;
             break;
           }
@@ -462,11 +471,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t all = 0xffffffffu, any = 0u;
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) all &= words[ch], any |= words[ch];
-        if (!mbar_wait<false>(&s_full[b.buf], b.parity, kErrTimeoutAttnS, abort_flag)) {
+        if (!mbar_wait_warp<false>(&s_full[b.buf], b.parity, kErrTimeoutAttnS, abort_flag)) {
           ok = false;
           break;
         }
-        __syncwarp();
         tc_fence_after();
         if (warp_active) {
           uint32_t pk[64];
@@ -507,11 +515,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (t > 0) {
                 // O holds the previous steps once the last PV is through (the one before it was
                 // when this step's S was issued, so the parity is the right phase's)
-                if (!mbar_wait<false>(&pv_done[w], (mine - 1) & 1, kErrTimeoutAttnO, abort_flag)) {
+                if (!mbar_wait_warp<false>(&pv_done[w], (mine - 1) & 1, kErrTimeoutAttnO, abort_flag)) {
                   ok = false;
                   break;
                 }
-                __syncwarp();
                 tc_fence_after();
 #pragma unroll 1
                 for (int h = 0; h < DP / 32; ++h) {
@@ -551,8 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           i -= m;
         }
       }
-      if (!mbar_wait<false>(&o_done[w], k.seg & 1, kErrTimeoutAttnO, abort_flag)) break;
-      __syncwarp();
+      if (!mbar_wait_warp<false>(&o_done[w], k.seg & 1, kErrTimeoutAttnO, abort_flag)) break;
       tc_fence_after();
       // a lone tile: the two halves meet, weigh each other in and write half the columns each
       float a0 = 1.f, a1 = 0.f;
@@ -565,9 +571,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&meet[q]);
-        if (!mbar_wait<false>(&meet[q], meets & 1, kErrTimeoutAttnO, abort_flag)) break;
+        if (!mbar_wait_warp<false>(&meet[q], meets & 1, kErrTimeoutAttnO, abort_flag)) break;
         ++meets;
-        __syncwarp();
         tc_fence_after();
         const float r0 = ml[row], r1 = ml[256 + row], l0 = ml[128 + row], l1 = ml[256 + 128 + row];
         const bool has1 = l1 != -1.f;
@@ -635,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // neither half may go on (and overwrite O or the exchange) before both have read
         __syncwarp();
         if (lane == 0) mbar_arrive(&meet[q]);
-        if (!mbar_wait<false>(&meet[q], meets & 1, kErrTimeoutAttnO, abort_flag)) break;
+        if (!mbar_wait_warp<false>(&meet[q], meets & 1, kErrTimeoutAttnO, abort_flag)) break;
         ++meets;
       }
     }

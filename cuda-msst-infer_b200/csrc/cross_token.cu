@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages];
   __shared__ Spot s_spot;
   __shared__ long long s_count;
-  __shared__ int s_abort;
+  __shared__ int s_abort, s_stop;
   __shared__ float s_m[kWarps][16], s_l[kWarps][16];
   volatile int* abort_flag = &s_abort;
   float* s_o = reinterpret_cast<float*>(smem + (size_t)stages * kStage);  // [warps][rows][DP]
@@ -124,8 +124,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++st == stages) st = 0, phase ^= 1;
         }
       }
+      mbar_drain_ring(full, stages, st, phase);
     }
-    return;  // the producer's copies are all waited for by the consumers
+    return;
   }
 
   const int set = warp >> 2, wk = warp & 3;  // tiles of this parity; 16 keys of each
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t par = phase;
       if (++st == stages) st = 0, phase ^= 1;
       if ((stage & 1) != set) continue;
-      if (!mbar_wait<false>(&full[stage], par, kErrTimeoutAttnKV, abort_flag)) {
+      if (!mbar_wait_warp<false>(&full[stage], par, kErrTimeoutAttnKV, abort_flag)) {
         ok = false;
         break;
       }
@@ -283,6 +284,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
+    // one reading for all: the producer may set the flag while they read it
+    if (threadIdx.x == 0) s_stop = *abort_flag;
     const bool whole = k.whole();
     for (int x = threadIdx.x; x < rows * (p.head_dim / 4); x += 256) {
       const int r = x / (p.head_dim / 4), col = (x - r * (p.head_dim / 4)) * 4;
@@ -313,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    ok = *abort_flag == 0;
+    ok = s_stop == 0;  // not written again before all have been at the next item's first barrier
   }
 }
 

@@ -101,3 +101,54 @@ int main() {
       }
 }
 """)
+
+
+def _source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return f.read()
+
+
+@pytest.mark.parametrize("name, begin, end", [
+    ("cross_attn.cu", "softmax + epilogue", "// Joins the partial results"),
+    ("cross_attn.cu", "rows that are not kept", "softmax + epilogue"),
+    ("cross_token.cu", "const int set = warp >> 2", "cudaError_t launch_k"),
+    ("adapter_gemm.cu", "// ------------------------------------------------------------ epilogue", "if (split > 1) {"),
+])
+def test_whole_warp_roles_wait_together(name, begin, end):
+    """Where a wait gives up, lanes must not part: one that left its loop never reaches the others'
+    full-mask instructions, and a kernel that should return with its code hangs.  Such a wait cannot be
+    made to run out from outside, so the sources are read: these roles wait by the warp."""
+    text = _source(name)
+    assert text.count(begin) == 1
+    role = text[text.index(begin):]
+    role = role[:role.index(end)]
+    assert "mbar_wait_warp" in role and "mbar_wait<" not in role and "mbar_wait(" not in role
+
+
+def test_roles_end_after_their_own_copies():
+    """Every producer waits for its ring, every MMA issuer for its last commit, and the token kernel's
+    warps leave their common barrier by one reading of the flag."""
+    for name, rings in (("cross_attn.cu", 2), ("cross_token.cu", 1), ("adapter_gemm.cu", 1)):
+        text = _source(name)
+        assert text.count("mbar_drain_ring(") == rings
+        if "umma_commit" in text:
+            assert text.count("umma_commit(mma_end)") == text.count("mbar_drain(mma_end, 0)") == 1
+    token = _source("cross_token.cu")
+    assert token.count("= *abort_flag") == 1 and "ok = s_stop == 0" in token
+
+
+def test_drain_of_a_ring():
+    """mbar_drain_ring's parities against a ring walked use by use (a barrier's phase parity flips with
+    each completed use; a wait for parity p returns where the current phase has the other one)."""
+    for n in (1, 2, 3, 5, 9):
+        uses, slot, phase = [0] * n, 0, 0
+        for _ in range(4 * n + 3):
+            for i in range(n):
+                p = phase if i < slot else phase ^ 1
+                # the last use counts as in flight: its phase is current and incomplete
+                current = (uses[i] - 1) % 2 if uses[i] else 0
+                assert (current == p) == (uses[i] > 0), (n, i, uses)
+            uses[slot] += 1
+            slot += 1
+            if slot == n:
+                slot, phase = 0, phase ^ 1
