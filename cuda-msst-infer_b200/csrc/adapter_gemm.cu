@@ -14,7 +14,10 @@
 // Which side of the MMA the rows take, and the split along K: make_plan.
 //
 // u is rounded to the operands' 16 bits once, as U' feeds the tensor cores; it is summed
-// in fp32 before that (split-K parts of the first launch in order).
+// in fp32 before that (split-K parts of the first launch in order).  What U' cannot hold in fp16,
+// the part of s_a u beyond +-65504, is multiplied by B_a in fp32 and added to the accumulators by
+// the epilogue, before the one rounding of y; so are products of B_a's infinities and NaN, which
+// would reach other rows of a tile as 0 * Inf.  Both are rare and slow: left_out.
 #include <algorithm>
 
 #include "common.cuh"
@@ -266,11 +269,14 @@ struct GemmCfgA {
 };
 constexpr int kThreadsA = 448;
 
+// The exponent of a 16-bit type's infinities and NaN; its largest magnitude is one below.
+template <typename T>
+constexpr uint32_t kExpBits = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
 // Non-finite values of a 16-byte piece of B_a, which would reach every row of the tile as
 // 0 * Inf: replaced by zeros here; the epilogue adds them to their own rows.
 template <typename T>
 __device__ __forceinline__ bool drop_nonfinite(uint4& v) {
-  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  constexpr uint32_t kExp = kExpBits<T>;
   uint32_t* w = reinterpret_cast<uint32_t*>(&v);
   bool found = false;
 #pragma unroll
@@ -309,27 +315,62 @@ struct Slices {
   }
 };
 
-// What drop_nonfinite left out of y[t, col] in slices [s0, s1) of the tile's list.
+// s_a u as U' holds it: rounded, the largest finite value where that gives an infinity.
 template <typename T>
-__device__ __noinline__ float dropped_part(const AdapterGemmParams& p, const Plan& pl, const int* list, int s0, int s1,
-                                           long long t, int col) {
+__device__ __forceinline__ bool clamp_infinities(uint4& v) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & 0x7fffu) == kExpBits<T>) w[i] -= 1u, found = true;
+    if ((w[i] >> 16 & 0x7fffu) == kExpBits<T>) w[i] -= 0x10000u, found = true;
+  }
+  return found;
+}
+
+// What the operands of slices [s0, s1) of the tile's list leave out of y[t, col]: the products of the
+// part of s_a u beyond what U' holds, and, where the tile's rows differ (`mixed`), those of the values
+// that drop_nonfinite took out of B_a.
+template <typename T>
+__device__ __forceinline__ float left_out(const AdapterGemmParams& p, const Plan& pl, const int* list, int s0, int s1,
+                                          bool mixed, long long t, int col) {
   const int a = row_id(p, t);
   float sum = 0.f;
   if (a < 0 || col >= p.N) return sum;
+  const float sc = p.scales ? __ldg(p.scales + a) : 1.f;
   const T* bw = static_cast<const T*>(p.lora_b) + ((size_t)a * p.N + col) * p.rank;
+  const float* u0 = static_cast<const float*>(p.ws) + t * p.rank;
   for (int s = s0; s < s1; ++s) {
     if (list[2 + s / pl.chunks] != a) continue;
     const int c0 = (s % pl.chunks) * kSliceRows, c1 = min(c0 + kSliceRows, p.rank);
     for (int r = c0; r < c1; ++r) {
-      const float bv = to_f32(bw[r]);
-      if (isfinite(bv)) continue;
       float u = 0.f;
-      for (int k = 0; k < pl.down_split; ++k)
-        u += static_cast<const float*>(p.ws)[((size_t)k * p.rows + t) * p.rank + r];
-      sum += to_f32(from_f32<T>(u * (p.scales ? __ldg(p.scales + a) : 1.f))) * bv;
+      for (int k = 0; k < pl.down_split; ++k) u += u0[(size_t)k * p.rows * p.rank + r];
+      u *= sc;
+      const float bv = to_f32(bw[r]);
+      if (mixed && !isfinite(bv)) {
+        sum += u * bv;
+      } else if (isinf(to_f32(from_f32<T>(u)))) {
+        const float most = std::is_same<T, __half>::value ? 65504.f : 3.38953139e38f;
+        sum += (u - copysignf(most, u)) * bv;
+      }
     }
   }
   return sum;
+}
+
+// Adds it to the accumulators of columns [c, c_end) of this warp's lanes, at `acc` + c: lane the row t
+// and column the output column col + c (kRowsOnM), or lane the output column and column the row t + c.
+template <typename T, bool kRowsOnM>
+__device__ __noinline__ void add_left_out(const AdapterGemmParams& p, const Plan& pl, const int* list, int s0, int s1,
+                                          long long t, int col, uint32_t acc, int c, int c_end) {
+  for (; c < c_end; ++c) {
+    const float x = left_out<T>(p, pl, list, s0, s1, list[1] != 0, kRowsOnM ? t : t + c, kRowsOnM ? col + c : col);
+    if (__any_sync(0xffffffffu, x != 0.f)) {
+      const float y = __uint_as_float(tmem_ld1(acc + (uint32_t)c));
+      tmem_st1(acc + (uint32_t)c, __float_as_uint(x != 0.f ? y + x : y));
+    }
+  }
 }
 
 template <typename T, int BT, bool kRowsOnM>
@@ -350,9 +391,9 @@ __global__ void __launch_bounds__(kThreadsA, 1)
   uint64_t* mma_end = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_end + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  // [tile count % 16] = tile count + 1 where values of B_a were left out (U' runs ahead of
-  // the epilogue by fewer tiles than the ring has stages, plus the two accumulators)
-  volatile int* s_dropped = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  // [tile count % 16] = tile count + 1 where the operands leave products out (written behind the ring,
+  // so ahead of the epilogue by fewer tiles than the ring has stages, plus the two accumulators)
+  volatile int* s_left_out = reinterpret_cast<volatile int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = kRowsOnM ? 1 : pl.split;
@@ -367,7 +408,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
       mbar_init(&u_go[i], 1);
       mbar_init(&u_full[i], 128);
     }
-    for (int i = 0; i < 16; ++i) s_dropped[i] = 0;
+    for (int i = 0; i < 16; ++i) s_left_out[i] = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 256);
@@ -511,6 +552,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
       const float sc = id >= 0 && p.scales ? __ldg(p.scales + id) : 1.f;
       uint4 held[4];  // slices held0 and held0 + 1 of this row, 8 values each
       int held0;
+      bool beyond = false;  // a value of this row is more than U' holds
       auto fetch = [&](int c) {
         float4 f[8] = {};
         const float* u = static_cast<const float*>(p.ws) + t * p.rank + c * kSliceRows;
@@ -528,6 +570,12 @@ __global__ void __launch_bounds__(kThreadsA, 1)
           const float4 lo = f[2 * i], hi = f[2 * i + 1];
           held[i] = make_uint4(pack2<T>(lo.x * sc, lo.y * sc), pack2<T>(lo.z * sc, lo.w * sc),
                                pack2<T>(hi.x * sc, hi.y * sc), pack2<T>(hi.z * sc, hi.w * sc));
+        }
+        const uint32_t top = __vmaxu2(__vmaxu2(magnitudes(held[0]), magnitudes(held[1])),
+                                      __vmaxu2(magnitudes(held[2]), magnitudes(held[3])));
+        if ((top & 0xffffu) >= kExpBits<T> || top >> 16 >= kExpBits<T>) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) beyond |= clamp_infinities<T>(held[i]);
         }
         held0 = c;
       };
@@ -569,7 +617,7 @@ __global__ void __launch_bounds__(kThreadsA, 1)
         }
         if (mixed) {
           // all of a thread's pieces are looked at before the rare rewrite
-          constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+          constexpr uint32_t kExp = kExpBits<T>;
           uint4* at = reinterpret_cast<uint4*>(base + C::kBAt) + i0;
           uint32_t top = 0;
           for (int i = 0; i < m; ++i) {
@@ -581,9 +629,10 @@ __global__ void __launch_bounds__(kThreadsA, 1)
               uint4 b = at[x * 128];
               if (drop_nonfinite<T>(b)) at[x * 128] = b;
             }
-            s_dropped[n & 15] = n + 1;
+            s_left_out[n & 15] = n + 1;
           }
         }
+        if (beyond) s_left_out[n & 15] = n + 1;
         fence_proxy_async_smem();
         mbar_arrive(&u_full[st]);
       }
@@ -604,11 +653,14 @@ __global__ void __launch_bounds__(kThreadsA, 1)
       const float bias = !kRowsOnM && p.bias && rank == 0 && col < p.N ? __ldg(p.bias + col) : 0.f;
       if (!mbar_wait_warp(&acc_full[buf], (n >> 1) & 1, kErrTimeoutTmemFull, abort_flag)) break;
       tc_fence_after();
-      const bool dropped = s_dropped[n & 15] == n + 1;
-      const int* list = lists + (size_t)tt * pl.list_ld;
-      int s0 = 0, s1 = 0;
-      if (dropped) slice_range(list, s0, s1);
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BT);
+      if (s_left_out[n & 15] == n + 1 && (BT >= 64 || half == 0)) {
+        const int* list = lists + (size_t)tt * pl.list_ld;
+        int s0, s1;
+        slice_range(list, s0, s1);
+        add_left_out<T, kRowsOnM>(p, pl, list, s0, s1, kRowsOnM ? t0 + q * 32 + lane : t0, kRowsOnM ? n0 : col, acc,
+                                  half * kMine, (half + 1) * kMine);
+      }
       if (BT >= 64 || half == 0) {
         for (int c = half * kMine; c < (half + 1) * kMine; c += 32) {
           if (kRowsOnM && n0 + c >= p.N) break;
@@ -640,13 +692,6 @@ __global__ void __launch_bounds__(kThreadsA, 1)
               o.w = pack2<T>(__uint_as_float(v[8 * u + 6]), __uint_as_float(v[8 * u + 7]));
               *reinterpret_cast<uint4*>(stg + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) = o;
             }
-            if (dropped) {
-              for (int i = 0; i < 32; ++i) {
-                const float x = dropped_part<T>(p, pl, list, s0, s1, t0 + q * 32 + lane, n0 + c + i);
-                T* at = reinterpret_cast<T*>(stg + lane * 64 + ((i >> 3 ^ (lane >> 1 & 3)) << 4)) + (i & 7);
-                if (x != 0.f) *at = from_f32<T>(to_f32(*at) + x);
-              }
-            }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -658,9 +703,6 @@ __global__ void __launch_bounds__(kThreadsA, 1)
             float* ex = reinterpret_cast<float*>(smem) + c * 128 + q * 32 + lane;
 #pragma unroll
             for (int i = 0; i < 32; ++i) ex[i * 128] = __uint_as_float(v[i]) + bias;
-            if (dropped) {
-              for (int i = 0; i < 32; ++i) ex[i * 128] += dropped_part<T>(p, pl, list, s0, s1, t0 + c + i, col);
-            }
           } else if (col < p.N) {
             T* out = static_cast<T*>(p.out) + (t0 + c) * p.ldo + col;
             const int left = (int)min(32LL, p.rows - (t0 + c));
@@ -671,13 +713,6 @@ __global__ void __launch_bounds__(kThreadsA, 1)
 #pragma unroll
               for (int i = 0; i < 32; ++i, out += p.ldo)
                 if (i < left) *out = from_f32<T>(__uint_as_float(v[i]) + bias);
-            }
-            if (dropped) {
-              out = static_cast<T*>(p.out) + (t0 + c) * p.ldo + col;
-              for (int i = 0; i < left; ++i, out += p.ldo) {
-                const float x = dropped_part<T>(p, pl, list, s0, s1, t0 + c + i, col);
-                if (x != 0.f) *out = from_f32<T>(to_f32(*out) + x);
-              }
             }
           }
         }

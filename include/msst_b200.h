@@ -215,6 +215,9 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
  * aligned; rows of one request need not be adjacent.  An index
  * outside [-1, adapters) counts as -1, and msst_device_error reports it.  A row's
  * result does not depend on the other rows of the call beyond the order of sums.
+ * Sums are fp32; scales[a] A_a x is rounded once to the operands' type (fp16: to within
+ * 2^-25 where it is subnormal; what lies beyond +-65504 is kept in fp32, at a lower
+ * speed), the result once.
  * `workspace` as in msst_cross_attention. */
 int msst_adapter_gemm_workspace(long long rows, int K, int N, int adapters, int rank, long long* bytes);
 int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const void* w, int N, const float* bias,

@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import pytest
 
-from test_conditioned_ops_gpu import U, _adapter_inputs, _dt, _gen, _qk_ref, _tables, _within
+from test_conditioned_ops_gpu import U, _adapter_check, _adapter_inputs, _dt, _gen, _qk_ref, _tables, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +74,89 @@ def test_device_error_of_two_operators(cuda):
     ops.qk_norm_rope(q, None, None, None, cos, sin, positions=torch.full((1, 3), 4, dtype=torch.int32, device="cuda"))
     assert device_error(False) == 14 and device_error(False) == 14
     assert device_error(True) == 14 and device_error(True) == 15 and device_error(True) == 0
+
+
+# ------------------------------------------------------------------ adapters: values off fp16's range
+# rows, K, N, adapters, rank: weights on the MMA's M side whole and split along K, rows on it
+ADAPTER_SIDES = [(40, 264, 136, 3, 16), (5, 8200, 264, 5, 24), (2501, 264, 1032, 6, 24)]
+
+
+@pytest.mark.parametrize("prec", ["fp16", "bf16"])
+@pytest.mark.parametrize("order", ["mixed", "sorted"])
+@pytest.mark.parametrize("case", ADAPTER_SIDES, ids=lambda c: "-".join(map(str, c)))
+def test_adapter_gemm_large_low_rank_values(cuda, case, order, prec):
+    """A_a x about 1e5 (above fp16's 65504 for about half the values) against a B_a about 1e-4."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    x, w, la, lb, ids, scales, bias = _adapter_inputs(torch, *case, prec, 5 + case[0])
+    ids[0], ids[1], ids[2] = 0, -1, 1
+    if order == "sorted":
+        ids = ids.sort().values
+    la[0] *= 2.0 ** 17
+    lb[0] *= 2.0 ** -14
+    u = x[ids == 0].double() @ la[0].double().T
+    assert bool((u.abs() > 65504).any()) and bool((u.abs() < 65504).any())
+    y = ops.adapter_gemm(x, w, la, lb, ids, scales=scales, bias=bias)
+    assert device_error(True) == 0
+    _adapter_check(torch, y, x, w, la, lb, ids, scales, bias, prec)
+    assert torch.equal(y, ops.adapter_gemm(x, w, la, lb, ids, scales=scales, bias=bias))
+    # rows of the other adapters are as they are without those values
+    la[0] *= 2.0 ** -17
+    z = ops.adapter_gemm(x, w, la, lb, ids, scales=scales, bias=bias)
+    assert torch.equal(z[ids != 0], y[ids != 0])
+
+
+@pytest.mark.parametrize("rows", [3, 2501])
+def test_adapter_gemm_large_values_cancel(cuda, rows):
+    """-2.2 * 64992 + 1 * 150000: neither the first product nor the sum without the part above 65504
+    fits fp16, the result does."""
+    torch = cuda
+    from msst_b200 import ops
+
+    N = 1032
+    x = torch.zeros(rows, 64, dtype=torch.float16, device="cuda")
+    x[:, 0], x[:, 1] = 1, 2.5
+    la = torch.zeros(2, 8, 64, dtype=torch.float16, device="cuda")
+    la[1, 0, 0], la[1, 1, 1] = 64992, 60000
+    lb = torch.zeros(2, N, 8, dtype=torch.float16, device="cuda")
+    lb[1, :, 0], lb[1, :, 1] = -2.2, 1
+    w = torch.zeros(N, 64, dtype=torch.float16, device="cuda")
+    ids = torch.ones(rows, dtype=torch.int32, device="cuda")
+    ids[1::2] = -1
+    y = ops.adapter_gemm(x, w, la, lb, ids)
+    _adapter_check(torch, y, x, w, la, lb, ids, None, None, "fp16")
+    assert bool((y[::2] > 6000).all()) and bool((y[1::2] == 0).all())
+
+
+# ------------------------------------------------------------------ adapters: infinities in a B_a
+@pytest.mark.parametrize("prec", ["fp16", "bf16"])
+@pytest.mark.parametrize("order", ["mixed", "sorted"])
+@pytest.mark.parametrize("case", ADAPTER_SIDES, ids=lambda c: "-".join(map(str, c)))
+def test_adapter_gemm_nonfinite_b(cuda, case, order, prec):
+    """Single Inf, -Inf and NaN entries of one adapter's B_a reach that adapter's rows in their own
+    columns, with the right sign, and nothing else."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    x, w, la, lb, ids, scales, bias = _adapter_inputs(torch, *case, prec, 15 + case[0])
+    ids[0], ids[1], ids[2] = 0, -1, 1
+    if order == "sorted":
+        ids = ids.sort().values
+    y = ops.adapter_gemm(x, w, la, lb, ids, scales=scales, bias=bias)
+    N, rank = lb.shape[1:]
+    plus, minus, nan = (3, 2), (N // 2 + 1, rank - 1), (N - 1, 5)
+    bad = lb.clone()
+    bad[1][plus], bad[1][minus], bad[1][nan] = float("inf"), -float("inf"), float("nan")
+    z = ops.adapter_gemm(x, w, la, bad, ids, scales=scales, bias=bias)
+    assert device_error(True) == 0
+    hit = torch.zeros_like(y, dtype=torch.bool)
+    rows = ids == 1
+    for col, _ in (plus, minus, nan):
+        hit[rows, col] = True
+    assert torch.equal(z[~hit], y[~hit])
+    u = scales[1].double() * (x[rows].double() @ la[1].double().T)
+    for (col, r), sign in ((plus, 1), (minus, -1)):
+        sure = u[:, r].abs() > 1e-2  # far from where a sum in fp32 could turn the sign
+        assert torch.equal(z[rows, col].double()[sure], sign * u[sure, r].sign() * float("inf"))
+    assert bool(z[rows, nan[0]].isnan().all())
