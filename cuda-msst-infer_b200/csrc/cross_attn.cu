@@ -34,7 +34,7 @@
 // (1150 TFLOP/s).
 //
 // Softmax: the reference a row is exponentiated against starts at the maximum of its
-// first 32 kept scores and moves lazily: a tile is taken in one pass without a
+// first 32 kept scores (less kRefShift) and moves lazily: a tile is taken in one pass without a
 // maximum, and only a row sum above kSumLimit (or not finite) sends the warp through
 // the exact two passes, which move the reference and rescale O.  Statistics are fp32;
 // P is rounded to the operands' 16 bits for the tensor cores.
@@ -54,8 +54,13 @@ constexpr int kSoftmaxWarp0 = 4;
 // Registers a thread after the split: 128 x 88 + 256 x 208 = 384 x 168, the block's launch share
 // (softmax warps without spills: 2 % faster at both head sizes).
 constexpr int kFewRegs = 88, kSoftmaxRegs = 208;
-// A step's row sum bounds each of its weights; 4096 stays far inside fp16's range.
-constexpr float kSumLimit = 4096.0f;
+// fp16 weights are taken 2^4 larger (the reference 4 lower, in powers of two): they are dropped below
+// 2^-25, and many of those count together, in the row sum at least.  A step's row sum bounds each of
+// its weights, and 61440 is inside fp16's 65504, so it may grow by as much as without the shift.
+template <typename T>
+constexpr float kRefShift = std::is_same<T, __half>::value ? 4.f : 0.f;
+template <typename T>
+constexpr float kSumLimit = std::is_same<T, __half>::value ? 61440.f : 4096.f;
 constexpr uint32_t kHalfBytes = 128 * 64 * 2;  // 128 rows x 64 columns
 
 template <int DP>
@@ -492,12 +497,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_ld32(sAddr + ch * 32, r);
               tmem_ld_wait(r);
               const float m = chunk_max(r, first, c);
-              ref = m == -INFINITY ? 0.f : m;
+              ref = m == -INFINITY ? 0.f : m - kRefShift<T>;
               have = true;
             }
             float sum = all == 0xffffffffu ? row_exp<T, true>(sAddr, words, c, ref, pk)
                                            : row_exp<T, false>(sAddr, words, c, ref, pk);
-            if (__any_sync(0xffffffffu, valid && !(sum <= kSumLimit))) {
+            if (__any_sync(0xffffffffu, valid && !(sum <= kSumLimit<T>))) {
               // exact passes: the reference moves to the row's maximum, O and l with it
               float m = -INFINITY;
 #pragma unroll 1
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_ld_wait(r);
                 m = fmaxf(m, chunk_max(r, word, c));
               }
-              const float moved = fmaxf(ref, m);
+              const float moved = fmaxf(ref, m - kRefShift<T>);
               const float alpha = fast_exp2(ref - moved);
               if (t > 0) {
                 // O holds the previous steps once the last PV is through (the one before it was

@@ -194,7 +194,9 @@ int msst_qk_norm_rope(const msst_heads* q, const msst_heads* k, int batch, int s
  * selects 1/sqrt(head_dim).  Kept are the first key_lens[b] keys (int32, taken into
  * [0, k_len]; NULL: all k_len) whose key_mask[b*k_len + j] is nonzero (NULL: all).
  * What the others hold, infinities and NaN included, has no influence.  A row
- * without a kept key gives zeros.  Data pointers are 16-byte aligned and strides
+ * without a kept key gives zeros.  Scores, sums and products are fp32; the softmax's
+ * weights are rounded to the operands' type before the product with v (fp16: to within
+ * 2^-29 of the largest where they are subnormal), the result once.  Data pointers are 16-byte aligned and strides
  * multiples of 8 elements; batch and head strides of k and v may be 0 (states shared
  * by the whole batch).  `workspace` holds at least the bytes that
  * msst_cross_attention_workspace gives for the call's sizes (16-byte aligned; may be

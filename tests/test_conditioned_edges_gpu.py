@@ -3,6 +3,8 @@ fit 16 bits, infinities, many keys of tiny weight, codes of several errors, grap
 Reference forms and tolerances as in test_conditioned_ops_gpu.py, unless a test derives its own."""
 from __future__ import annotations
 
+import math
+
 import pytest
 
 from test_conditioned_ops_gpu import U, _adapter_check, _adapter_inputs, _dt, _gen, _qk_ref, _tables, _within
@@ -160,3 +162,30 @@ def test_adapter_gemm_nonfinite_b(cuda, case, order, prec):
         sure = u[:, r].abs() > 1e-2  # far from where a sum in fp32 could turn the sign
         assert torch.equal(z[rows, col].double()[sure], sign * u[sure, r].sign() * float("inf"))
     assert bool(z[rows, nan[0]].isnan().all())
+
+
+# ------------------------------------------------------------------ cross attention: many tiny weights
+@pytest.mark.parametrize("form", ["token", "tiles"])
+def test_cross_attention_many_small_weights(cuda, form):
+    """fp16 weights just below 2^-25 of their reference, 2^18 of them for each large one: they are
+    0.8 % of the sum.  Every v is 1, so every output is 1.
+
+    Bound: the result's and the weights' roundings, 2^-11 each; the fp32 sums: 2^14 products of 16
+    keys added to about 1, truncated, 2^-23 each; 2^14 additions of the row sum, 2^-24 each; the
+    weights themselves on fp16's subnormal grid after their shift (2^4 at least), 2^18 2^-29."""
+    torch = cuda
+    from msst_b200 import ops
+
+    items = torch.cuda.get_device_properties(0).multi_processor_count  # one a CTA, whole
+    # a running maximum belongs to 16 keys of every second 64 (token form) or to every second 128
+    Nk, every, heads, Nq = (2 ** 21, 16, 8, 1) if form == "token" else (2 ** 19, 128, 2, 32)
+    q = torch.zeros(1, Nq, 1, 8, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1
+    k = torch.zeros(1, Nk, 1, 8, dtype=torch.float16, device="cuda")
+    k[..., 0] = -25.015625
+    k[:, 0:every * heads:every, :, 0] = 0
+    v = torch.ones_like(k)
+    wide = (items, -1, -1, -1)
+    y = ops.cross_attention(q.expand(wide), k.expand(wide), v.expand(wide), scale=math.log(2))
+    bound = 2 * 2.0 ** -11 + 2.0 ** 14 * 2.0 ** -23 + 2.0 ** 14 * 2.0 ** -24 + 2.0 ** 18 * 2.0 ** -29
+    assert float((y.double() - 1).abs().max()) <= bound
