@@ -496,8 +496,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               uint32_t r[32];
               tmem_ld32(sAddr + ch * 32, r);
               tmem_ld_wait(r);
-              const float m = chunk_max(r, first, c);
-              ref = m == -INFINITY ? 0.f : m - kRefShift<T>;
+              // -inf where these scores are: no reference yet, and sums against it are not finite,
+              // which sends every step through the exact passes until one finds a score
+              ref = chunk_max(r, first, c) - kRefShift<T>;
               have = true;
             }
             float sum = all == 0xffffffffu ? row_exp<T, true>(sAddr, words, c, ref, pk)
@@ -515,8 +516,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_ld_wait(r);
                 m = fmaxf(m, chunk_max(r, word, c));
               }
-              const float moved = fmaxf(ref, m - kRefShift<T>);
-              const float alpha = fast_exp2(ref - moved);
+              const float moved = fmaxf(ref, m - kRefShift<T>), base = moved == -INFINITY ? 0.f : moved;
+              const float alpha = fast_exp2(ref - base);
               if (t > 0) {
                 // O holds the previous steps once the last PV is through (the one before it was
                 // when this step's S was issued, so the parity is the right phase's)
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               l *= alpha;
               ref = moved;
-              sum = row_exp<T, false>(sAddr, words, c, ref, pk);
+              sum = row_exp<T, false>(sAddr, words, c, base, pk);
             }
             l += sum;
           } else {

@@ -7,7 +7,8 @@ import math
 
 import pytest
 
-from test_conditioned_ops_gpu import U, _adapter_check, _adapter_inputs, _dt, _gen, _qk_ref, _tables, _within
+from test_conditioned_ops_gpu import (U, _adapter_check, _adapter_inputs, _cross_check, _cross_inputs, _dt, _gen, _qk_ref,
+                                      _tables, _within)
 
 pytestmark = pytest.mark.gpu
 
@@ -189,3 +190,24 @@ def test_cross_attention_many_small_weights(cuda, form):
     y = ops.cross_attention(q.expand(wide), k.expand(wide), v.expand(wide), scale=math.log(2))
     bound = 2 * 2.0 ** -11 + 2.0 ** 14 * 2.0 ** -23 + 2.0 ** 14 * 2.0 ** -24 + 2.0 ** 18 * 2.0 ** -29
     assert float((y.double() - 1).abs().max()) <= bound
+
+
+# ------------------------------------------------------------------ cross attention: scores of -inf
+@pytest.mark.parametrize("Nq", [1, 40, 300])
+@pytest.mark.parametrize("prec", ["fp16", "bf16"])
+def test_cross_attention_infinitely_low_first(cuda, Nq, prec):
+    """Kept keys whose scores are -inf have weight zero, wherever they lie; the others' scores are
+    far below zero, so a reference of zero would leave nothing of them."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    for d, dead in ((64, 33), (64, 130), (128, 300), (40, 128)):
+        q, k, v = _cross_inputs(torch, 2, Nq, 500, 4, 2, d, prec, 91 + d)
+        q, k = q.abs() + 0.5, -(k.abs() + 20)
+        keep = torch.ones(2, 500, dtype=torch.bool, device="cuda")
+        keep[0, :dead] = False
+        keep[1, 1:dead:2] = False
+        low = torch.where(keep[:, :, None, None], k, torch.full_like(k, -float("inf")))
+        y = ops.cross_attention(q, low, v)
+        _cross_check(torch, y, q, k, v, keep, d ** -0.5, prec)
+    assert device_error(True) == 0
