@@ -159,14 +159,17 @@ int device_of(const void* p) {
 }
 
 // A tensor operand of the conditioned-block operators: `align` > 1 wants its base on
-// 16 bytes and every stride that is walked (extent > 1) a multiple of `align` elements.
-msst::HeadsView heads_view(const msst_heads* t, int batch, int seq, int align, const char* what) {
+// 16 bytes and every stride that is walked (extent > 1) a multiple of `align` elements; `written`
+// wants those above 0, so that no two values share a place.
+msst::HeadsView heads_view(const msst_heads* t, int batch, int seq, int align, const char* what, bool written = false) {
   const std::string name(what);
   MSST_REQUIRE(t && t->heads > 0, name + " needs at least one head");
   MSST_REQUIRE(t->data || batch == 0 || seq == 0, name + " is null");
   MSST_REQUIRE(t->batch_stride >= 0 && t->seq_stride >= 0 && t->head_stride >= 0, name + " has a negative stride");
   msst::HeadsView v{t->data, t->heads, batch > 1 ? t->batch_stride : 0, seq > 1 ? t->seq_stride : 0,
                     t->heads > 1 ? t->head_stride : 0};
+  MSST_REQUIRE(!written || ((batch < 2 || v.batch_stride) && (seq < 2 || v.seq_stride) && (v.heads < 2 || v.head_stride)),
+               name + " is written and needs strides above 0");
   if (align > 1) {
     check_align(t->data, what);
     MSST_REQUIRE(v.batch_stride % align == 0 && v.seq_stride % align == 0 && v.head_stride % align == 0,
@@ -453,11 +456,11 @@ int msst_qk_norm_rope(const msst_heads* q, const msst_heads* k, int batch, int s
     MSST_REQUIRE(eps >= 0.f, "eps must be >= 0");
     msst::QkNormParams p{};
     p.x[0] = heads_view(q, batch, seq, 1, "q");
-    p.out[0] = heads_view(q_out, batch, seq, 1, "q_out");
+    p.out[0] = heads_view(q_out, batch, seq, 1, "q_out", true);
     MSST_REQUIRE(p.x[0].heads == p.out[0].heads, "q_out must have q's heads");
     if (k) {
       p.x[1] = heads_view(k, batch, seq, 1, "k");
-      p.out[1] = heads_view(k_out, batch, seq, 1, "k_out");
+      p.out[1] = heads_view(k_out, batch, seq, 1, "k_out", true);
       MSST_REQUIRE(p.x[1].heads == p.out[1].heads, "k_out must have k's heads");
     }
     MSST_REQUIRE((long long)batch * seq <= (1LL << 31) / (p.x[0].heads + p.x[1].heads), "too many head vectors");
@@ -499,7 +502,7 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
     p.q = heads_view(q, batch, q_len, 8, "q");
     p.k = heads_view(k, batch, k_len, 8, "k");
     p.v = heads_view(v, batch, k_len, 8, "v");
-    p.out = heads_view(out, batch, q_len, 8, "out");
+    p.out = heads_view(out, batch, q_len, 8, "out", true);
     MSST_REQUIRE(p.out.heads == p.q.heads, "out must have q's heads");
     MSST_REQUIRE(p.k.heads == p.v.heads, "k and v need the same number of heads, and q a multiple of it");
     check_cross_heads(p.q.heads, p.k.heads, head_dim);

@@ -160,7 +160,8 @@ int msst_sdpa(const void* q, const void* k, const void* v, int B, int H, int Nq,
 
 /* A 16-bit tensor [batch, sequence, heads, head_dim] in any order of its first three
  * dimensions: element (b, n, h, i) at data + b*batch_stride + n*seq_stride +
- * h*head_stride + i, strides in elements and >= 0.  Batch, sequence and head_dim
+ * h*head_stride + i, strides in elements and >= 0 (of a tensor that is written, above 0
+ * wherever the extent is above 1).  Batch, sequence and head_dim
  * are arguments of the call. */
 typedef struct msst_heads {
   void* data;

@@ -152,3 +152,24 @@ def test_drain_of_a_ring():
             slot += 1
             if slot == n:
                 slot, phase = 0, phase ^ 1
+
+
+@pytest.mark.parametrize("out", [dict(sb=0), dict(sn=0), dict(sh=0)])
+@pytest.mark.parametrize("op", ["q_out", "k_out", "cross"])
+def test_outputs_that_share_places_are_refused(op, out):
+    """An expanded output (stride 0 along an extent above 1) would be written by several threads, and
+    normed several times where it is the input too."""
+    from msst_b200 import MSST_ERR_INVALID, lib
+    from test_conditioned_ops import _cross, _heads, _qk
+
+    shape = dict(batch=2)
+    if op == "cross":
+        rc = _cross(out=_heads(**out), **shape)
+    elif op == "q_out":
+        rc = _qk(qo=_heads(**out), **shape)
+    else:
+        rc = _qk(k=_heads(), ko=_heads(**out), **shape)
+    assert rc == MSST_ERR_INVALID and "strides above 0" in lib().msst_last_error().decode()
+    # strides that nothing walks may be 0
+    assert _qk(q=_heads(heads=1, sb=0, sn=0, sh=0), qo=_heads(heads=1, sb=0, sn=0, sh=0), batch=1, seq=1) != MSST_ERR_INVALID \
+        or "strides above 0" not in lib().msst_last_error().decode()
