@@ -178,6 +178,9 @@ msst::HeadsView heads_view(const msst_heads* t, int batch, int seq, int align, c
   return v;
 }
 
+// Rows, columns, queries or keys of a call: 32-bit numbers still when rounded up to a tile.
+constexpr long long kMostRows = (1LL << 31) - 512;
+
 // The heads of a cross attention (its sizes are computed from their quotient).
 void check_cross_heads(int q_heads, int kv_heads, int head_dim) {
   MSST_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "head_dim must be a multiple of 8, <= 128");
@@ -486,6 +489,7 @@ int msst_cross_attention_workspace(int batch, int q_len, int k_len, int q_heads,
                                    long long* bytes) {
   return guarded([&] {
     MSST_REQUIRE(bytes && batch >= 0 && q_len >= 0 && k_len >= 0, "bad shape");
+    MSST_REQUIRE(q_len <= kMostRows && k_len <= kMostRows, "too many queries or keys");
     check_cross_heads(q_heads, kv_heads, head_dim);
     *bytes = msst::cross_attention_workspace(batch, q_len, k_len, q_heads, kv_heads, head_dim, sm_count());
   });
@@ -497,6 +501,7 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
   return guarded([&] {
     check_dtype(dtype);
     MSST_REQUIRE(batch >= 0 && q_len >= 0 && k_len >= 0, "bad shape");
+    MSST_REQUIRE(q_len <= kMostRows && k_len <= kMostRows, "too many queries or keys");
     MSST_REQUIRE(std::isfinite(scale), "scale must be finite");
     msst::CrossAttnParams p{};
     p.q = heads_view(q, batch, q_len, 8, "q");
@@ -529,7 +534,7 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
 
 int msst_adapter_gemm_workspace(long long rows, int K, int N, int adapters, int rank, long long* bytes) {
   return guarded([&] {
-    MSST_REQUIRE(bytes && rows >= 0 && rows < (1LL << 31) && K > 0 && N > 0 && adapters >= 0 && rank > 0, "bad shape");
+    MSST_REQUIRE(bytes && rows >= 0 && rows <= kMostRows && K > 0 && K <= kMostRows && N > 0 && N <= kMostRows && adapters >= 0 && rank > 0, "bad shape");
     *bytes = msst::adapter_gemm_workspace((int)rows, K, N, adapters, rank, sm_count());
   });
 }
@@ -540,8 +545,9 @@ int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const
                       long long workspace_bytes, void* stream) {
   return guarded([&] {
     check_dtype(dtype);
-    MSST_REQUIRE(rows >= 0 && rows < (1LL << 31), "bad rows");
+    MSST_REQUIRE(rows >= 0 && rows <= kMostRows, "bad rows");
     MSST_REQUIRE(K > 0 && K % 8 == 0 && N > 0 && N % 8 == 0, "K and N must be positive multiples of 8");
+    MSST_REQUIRE(K <= kMostRows && N <= kMostRows, "K or N is too large");
     MSST_REQUIRE(rank > 0 && rank <= 256 && rank % 8 == 0, "rank must be a multiple of 8, <= 256");
     MSST_REQUIRE(adapters >= 0, "adapters must be >= 0");
     MSST_REQUIRE(ldx >= K && ldx % 8 == 0 && ldo >= N && ldo % 8 == 0,

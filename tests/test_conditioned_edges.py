@@ -173,3 +173,21 @@ def test_outputs_that_share_places_are_refused(op, out):
     # strides that nothing walks may be 0
     assert _qk(q=_heads(heads=1, sb=0, sn=0, sh=0), qo=_heads(heads=1, sb=0, sn=0, sh=0), batch=1, seq=1) != MSST_ERR_INVALID \
         or "strides above 0" not in lib().msst_last_error().decode()
+
+
+def test_lengths_within_a_tile_of_32_bits_are_refused():
+    """Rounded up to a tile they would pass 2^31 - 1 and come out negative: no tile, a result that is not
+    written or not finished."""
+    from msst_b200 import MSST_ERR_INVALID, lib
+    from test_conditioned_ops import _adapter, _cross, _heads
+
+    n, most = ctypes.c_longlong(-1), (1 << 31) - 1
+    one = dict(q=_heads(heads=1), k=_heads(heads=1), v=_heads(heads=1), out=_heads(heads=1))
+    for call, word in ((lambda: _cross(nq=most, **one), "too many"), (lambda: _cross(nk=most, **one), "too many"),
+                       (lambda: _adapter(rows=most), "rows"), (lambda: _adapter(N=most - 7, ldo=most - 7), "N is too large"),
+                       (lambda: _adapter(K=most - 7, ldx=most - 7), "N is too large")):
+        assert call() == MSST_ERR_INVALID and word in lib().msst_last_error().decode()
+    for nq, nk in ((most, 8), (8, most)):
+        assert lib().msst_cross_attention_workspace(1, nq, nk, 1, 1, 8, ctypes.byref(n)) == MSST_ERR_INVALID
+    for rows, K, N in ((most, 8, 8), (8, most - 7, 8), (8, 8, most - 7)):
+        assert lib().msst_adapter_gemm_workspace(rows, K, N, 1, 8, ctypes.byref(n)) == MSST_ERR_INVALID
