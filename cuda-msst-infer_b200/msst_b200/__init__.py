@@ -226,7 +226,8 @@ def _workspace(name, device, *sizes):
     n = _space.get(key)
     if n is None:
         need = ctypes.c_longlong()
-        check(getattr(lib(), f"msst_{name}_workspace")(*sizes, ctypes.byref(need)))
+        with _torch().cuda.device(device):  # the size goes by the SMs of the GPU that the call runs on
+            check(getattr(lib(), f"msst_{name}_workspace")(*sizes, ctypes.byref(need)))
         if len(_space) > 4096:
             _space.clear()
         n = _space[key] = need.value

@@ -200,8 +200,8 @@ int msst_qk_norm_rope(const msst_heads* q, const msst_heads* k, int batch, int s
  * 2^-29 of the largest where they are subnormal), the result once.  Data pointers are 16-byte aligned and strides
  * multiples of 8 elements; batch and head strides of k and v may be 0 (states shared
  * by the whole batch).  `workspace` holds at least the bytes that
- * msst_cross_attention_workspace gives for the call's sizes (16-byte aligned; may be
- * NULL when that is 0); calls that may overlap need workspaces of their own. */
+ * msst_cross_attention_workspace gives for the call's sizes with the operands' GPU
+ * current (16-byte aligned; may be NULL when that is 0); calls that may overlap need workspaces of their own. */
 int msst_cross_attention_workspace(int batch, int q_len, int k_len, int q_heads, int kv_heads, int head_dim,
                                    long long* bytes);
 int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_heads* v, int batch, int q_len, int k_len,

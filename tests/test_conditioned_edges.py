@@ -191,3 +191,33 @@ def test_lengths_within_a_tile_of_32_bits_are_refused():
         assert lib().msst_cross_attention_workspace(1, nq, nk, 1, 1, 8, ctypes.byref(n)) == MSST_ERR_INVALID
     for rows, K, N in ((most, 8, 8), (8, most - 7, 8), (8, 8, most - 7)):
         assert lib().msst_adapter_gemm_workspace(rows, K, N, 1, 8, ctypes.byref(n)) == MSST_ERR_INVALID
+
+
+def test_workspace_is_asked_for_on_the_operands_device(monkeypatch):
+    """With another GPU current, and once for each device and size."""
+    import contextlib
+
+    import msst_b200 as M
+    import torch
+
+    current, asked = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], d
+        yield
+        current[0] = before
+
+    class Lib:
+        @staticmethod
+        def msst_cross_attention_workspace(*args):
+            asked.append(current[0])
+            args[-1]._obj.value = 100 + 48 * current[0]
+            return M.MSST_OK
+
+    monkeypatch.setattr(M, "lib", lambda: Lib)
+    monkeypatch.setattr(M, "_space", {})
+    monkeypatch.setattr(torch.cuda, "device", device)
+    sizes = (1, 2, 3, 4, 4, 64)
+    assert [M._workspace("cross_attention", d, *sizes) for d in (1, 0, 1, 0)] == [148, 100, 148, 100]
+    assert asked == [1, 0] and current == [0]
