@@ -4,6 +4,7 @@ Reference forms and tolerances as in test_conditioned_ops_gpu.py, unless a test 
 from __future__ import annotations
 
 import math
+import threading
 
 import pytest
 
@@ -211,3 +212,121 @@ def test_cross_attention_infinitely_low_first(cuda, Nq, prec):
         y = ops.cross_attention(q, low, v)
         _cross_check(torch, y, q, k, v, keep, d ** -0.5, prec)
     assert device_error(True) == 0
+
+
+# ------------------------------------------------------------------ graphs and threads
+def _three_operators(torch, ops, seed):
+    """Calls of each operator, cross attention by tiles and by tokens, as functions of one input."""
+    g = _gen(torch, seed)
+    cos, sin = _tables(torch, 128, 32)
+    _, k, v = _cross_inputs(torch, 2, 1, 900, 4, 2, 64, "fp16", seed + 1)
+    lens = torch.tensor([900, 411], dtype=torch.int32, device="cuda")
+    keep = torch.rand(2, 900, generator=g, device="cuda") < 0.5
+    _, w, la, lb, ids, scales, bias = _adapter_inputs(torch, 200, 256, 264, 4, 16, "fp16", seed + 2)
+    calls = [
+        lambda x: ops.qk_norm_rope(x, None, None, None, cos, sin)[0],
+        lambda x: ops.cross_attention(x, k, v, key_lens=lens),
+        lambda x: ops.cross_attention(x[:, :1], k, v, key_mask=keep),
+        lambda x: ops.adapter_gemm(x.reshape(200, 256), w, la, lb, ids, scales=scales, bias=bias),
+    ]
+    make = lambda: torch.randn(2, 100, 4, 64, generator=g, device="cuda").half()  # noqa: E731
+    return calls, make
+
+
+def test_operators_in_a_graph(cuda):
+    """Captured once, replayed over new inputs: the same bits as the calls themselves."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    calls, make = _three_operators(torch, ops, 71)
+    x = make()
+    for call in calls:
+        call(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [call(x) for call in calls]
+    for _ in range(3):
+        x.copy_(make())
+        graph.replay()
+        torch.cuda.synchronize()
+        for call, y in zip(calls, outs):
+            assert torch.equal(call(x), y)
+    assert device_error(True) == 0
+
+
+def test_operators_from_two_threads(cuda):
+    """Two threads on streams of their own, calls interleaved as they come: each its own results."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    work = [_three_operators(torch, ops, seed) for seed in (81, 82)]
+    inputs = [[make() for _ in range(6)] for _, make in work]
+    wants = [[[call(x) for call in calls] for x in xs] for (calls, _), xs in zip(work, inputs)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def body(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = [[call(x) for call in work[i][0]] for x in inputs[i]]
+                    torch.cuda.current_stream().synchronize()
+                    for a, b in zip(got, wants[i]):
+                        if not all(torch.equal(y, z) for y, z in zip(a, b)):
+                            wrong.append(i)
+        except Exception as e:  # a thread's exception would be lost
+            wrong.append(e)
+
+    threads = [threading.Thread(target=body, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and device_error(True) == 0
+
+
+@pytest.mark.parametrize("Nq, Nk, dims", [(1, 1, dict(dim=64, enc_dim=72, q_heads=3, kv_heads=1, head_dim=24, rank=8)),
+                                          (33, 515, dict(dim=320, enc_dim=200, q_heads=4, kv_heads=4, head_dim=80, rank=40)),
+                                          (200, 130, dict(dim=1024, enc_dim=512, q_heads=8, kv_heads=2, head_dim=128))])
+def test_conditioned_block_sizes(cuda, Nq, Nk, dims):
+    """The block against its own operators' plain forms in 64 bits at other sizes: tolerance as in
+    test_conditioned_block, 4 + 4 sqrt(head_dim) roundings of the sizes in the 2-norm."""
+    torch = cuda
+    from msst_b200 import device_error
+    from msst_b200.conditioned import random_block
+
+    blk = random_block(dtype=torch.float16, seed=5, **dims)
+    g, d, hq, hk = _gen(torch, 4), dims["head_dim"], dims["q_heads"], dims["kv_heads"]
+    B = 3
+    x = torch.randn(B, Nq, dims["dim"], generator=g, device="cuda").half()
+    enc = torch.randn(B, Nk, dims["enc_dim"], generator=g, device="cuda").half()
+    keep = torch.rand(B, Nk, generator=g, device="cuda") < 0.7
+    keep[1], keep[2] = True, False
+    who = torch.tensor([1, -1, 2], dtype=torch.int32, device="cuda")
+    y = blk(x, *blk.encode(enc, who), who, key_mask=keep)
+    assert device_error(True) == 0
+
+    def project(name, t):
+        a, b, s = blk.adapters[name]
+        out = t @ blk.w[name].double().T
+        for i in range(B):
+            if who[i] >= 0:
+                out[i] += float(s[who[i]]) * (t[i] @ a[who[i]].double().T) @ b[who[i]].double().T
+        return out
+
+    at = lambda n: torch.arange(n, device="cuda").expand(B, n)  # noqa: E731
+    q64, _ = _qk_ref(torch, project("q", x.double()).view(B, Nq, hq, d), blk.q_gamma, blk.cos, blk.sin, at(Nq), 1e-6, "halves")
+    kv = project("kv", enc.double()).view(B, Nk, 2, hk, d)
+    k64, _ = _qk_ref(torch, kv[:, :, 0], blk.k_gamma, blk.cos, blk.sin, at(Nk), 1e-6, "halves")
+    att = torch.zeros(B, Nq, hq, d, dtype=torch.float64, device="cuda")
+    for i in range(2):
+        for h in range(hq):
+            j = h * hk // hq
+            p = torch.softmax(q64[i, :, h] @ k64[i, keep[i], j].T / math.sqrt(d), -1)
+            att[i, :, h] = p @ kv[i, keep[i], 1, j]
+    delta = project("o", att.reshape(B, Nq, -1))
+    ref = x.double() + delta
+    bar = (4 + 4 * math.sqrt(d)) * U["fp16"] * float(delta.norm()) + U["fp16"] * float(ref.norm())
+    assert float((y.double() - ref).norm()) <= bar
+    assert torch.equal(y[2], x[2])
