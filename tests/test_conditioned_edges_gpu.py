@@ -330,3 +330,19 @@ def test_conditioned_block_sizes(cuda, Nq, Nk, dims):
     bar = (4 + 4 * math.sqrt(d)) * U["fp16"] * float(delta.norm()) + U["fp16"] * float(ref.norm())
     assert float((y.double() - ref).norm()) <= bar
     assert torch.equal(y[2], x[2])
+
+
+@pytest.mark.parametrize("case", [(2501, 264, 1032, 6, 24), (40, 4104, 136, 3, 16)], ids=lambda c: "-".join(map(str, c)))
+def test_adapter_gemm_writes_its_columns_alone(cuda, case):
+    """x and out as columns of wider rows: the same bits, and nothing beside them."""
+    torch = cuda
+    from msst_b200 import ops
+
+    x, w, la, lb, ids, scales, bias = _adapter_inputs(torch, *case, "bf16", 3)
+    y = ops.adapter_gemm(x, w, la, lb, ids, scales=scales, bias=bias)
+    wide = torch.full((case[0], case[1] + 24), float("nan"), dtype=x.dtype, device="cuda")
+    wide[:, 8:8 + case[1]] = x
+    big = torch.full((case[0], case[2] + 16), 3.0, dtype=x.dtype, device="cuda")
+    ops.adapter_gemm(wide[:, 8:8 + case[1]], w, la, lb, ids, scales=scales, bias=bias, out=big[:, 8:8 + case[2]])
+    assert torch.equal(big[:, 8:8 + case[2]], y)
+    assert bool((big[:, :8] == 3).all()) and bool((big[:, 8 + case[2]:] == 3).all())
