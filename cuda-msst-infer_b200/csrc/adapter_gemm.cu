@@ -60,10 +60,11 @@ __device__ __forceinline__ int row_id(const AdapterGemmParams& p, long long t) {
 // ---------------------------------------------------------------------------
 // First launch: u[t] = A_a x[t].  Bound: reading x once (and, for few rows, the adapters' A_a).
 // mma.sync m16n8k16; each warp streams its rows through a ring of its own in shared memory
-// (cp.async, whole 128-byte lines, three stages of 64 columns in flight: up to 144 KB an SM) and
+// (cp.async, whole 128-byte lines, three stages of 64 columns in flight: 144 KB an SM with the three CTAs
+// that fit up to rank 16, 96 KB with two above, whose accumulators take 202 and 252 registers) and
 // takes A_a, which stays in L2, straight from global memory one step ahead.  No barrier
 // until the end.  8192 rows of 4096 columns, rank 32: 40 us alone, about half of it under the
-// second launch (187 alone, 209 for both); 32 rows, 16 adapters: 10 us.  (Forms that held x in registers kept too little in flight: 37 us for
+// second launch (188 alone, 210 to 214 for both); 32 rows, 16 adapters: 10 us.  (Forms that held x in registers kept too little in flight: 37 us for
 // 8192 rows of 4096 columns; a tcgen05 form with 128-row slices of A_a took 35 us.)
 // A warp owns 32 rows; the warps of a CTA split K (down_kw of them) and rows.  For every
 // distinct adapter of its rows it computes all 32 x rank products from the rows that have
@@ -122,7 +123,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool t
 constexpr int kDownWarps = 4;
 constexpr int kDownStages = 4;
 constexpr uint32_t kDownStage = 32 * 128;  // 32 rows x 64 columns
-constexpr int kDownSmem = kDownWarps * kDownStages * (int)kDownStage;  // three CTAs an SM
+constexpr int kDownSmem = kDownWarps * kDownStages * (int)kDownStage;  // 64 KB: up to three CTAs an SM
 
 template <typename T, int NT>
 __global__ void __launch_bounds__(32 * kDownWarps)
@@ -247,9 +248,9 @@ __global__ void __launch_bounds__(32 * kDownWarps)
 // U' of the slices, warps 6-13 epilogue.  The accumulators are double: the epilogue of a
 // tile overlaps the next one's main loop.  A ring stage holds 64 columns of W and x, or 4
 // slices of B_a and U'.
-// Bound: the tensor cores for large K (8192 rows, K = N = 4096: 209 us with the first launch, 1335
-// TFLOP/s); 48060 rows, K = 384, N = 1536: 73 us (2.55 TB/s), 65 of them this one's, tensor pipe
-// 49 % busy; latency for few rows (32 rows, 16 adapters, K = N = 4096: 20 us).
+// Bound: the tensor cores for large K (8192 rows, K = N = 4096: 210 to 214 us with the first
+// launch, 1320 TFLOP/s); 48060 rows, K = 384, N = 1536: 71 to 74 us (2.55 TB/s), 64 of them this one's, tensor pipe
+// 51 % busy; latency for few rows (32 rows, 16 adapters, K = N = 4096: 20 us).
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMTile = 128 * 128;       // the M side: 128 rows x 64 columns of 16 bits
 
@@ -780,7 +781,8 @@ Plan make_plan(int rows, int K, int N, int adapters, int rank, int num_sms) {
   pl.n_tiles = pl.rows_on_m ? (N + 255) / 256 : (N + 127) / 128;
   pl.kblocks = (K + 63) / 64;
   pl.chunks = (rank + kSliceRows - 1) / kSliceRows;
-  // first launch: at least 3 K steps of 64 a warp, up to three CTAs for each SM
+  // first launch: at least 3 K steps of 64 a warp, up to three CTAs for each SM (above rank 16 two are
+  // resident at a time)
   const int steps = (K + 63) / 64;
   pl.down_kw = 1;
   while (pl.down_kw < kDownWarps && pl.down_kw * 2 * 3 <= steps) pl.down_kw *= 2;
@@ -798,6 +800,9 @@ Plan make_plan(int rows, int K, int N, int adapters, int rank, int num_sms) {
   // 21.4.  K = 4096, N = 1536, 32 rows with one adapter 15.0, 12.4, 14.0; with 32 21.9, 22.9, 19.4.
   // Clusters of 4 or 8 take up to half the SMs only, since not all of those can hold one: 33 clusters
   // of 4 and 15 of 8 fit at a time (36 of 4 took 27.5 us where 36 of 2 took 16.1; K = 4096, N = 1536).
+  // 132 SMs would do for the clusters of 4, and the rule is not the best everywhere: it takes 2 for
+  // (whole / 2 / 4) K = N = 4096, 32 rows with 16 adapters 18.6 / 19.9 / 19.4, with 32 22.4 / 23.9 / 22.8, 128
+  // rows with 16 28.3 / 24.1 / 22.8, with 64 42.1 / 35.2 / 31.6; N = 1536, 256 rows with 16 28.1 / 26.0 / 24.9.
   // Rows on the M side are never split: their tiles are more than half the SMs.
   const long long tiles = (long long)pl.tiles * pl.n_tiles;
   const int most = pl.kblocks + std::min(pl.bt, adapters) * pl.chunks;

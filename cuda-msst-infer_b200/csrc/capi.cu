@@ -534,7 +534,9 @@ int msst_cross_attention(const msst_heads* q, const msst_heads* k, const msst_he
 
 int msst_adapter_gemm_workspace(long long rows, int K, int N, int adapters, int rank, long long* bytes) {
   return guarded([&] {
-    MSST_REQUIRE(bytes && rows >= 0 && rows <= kMostRows && K > 0 && K <= kMostRows && N > 0 && N <= kMostRows && adapters >= 0 && rank > 0, "bad shape");
+    MSST_REQUIRE(bytes && rows >= 0 && rows <= kMostRows && K > 0 && K <= kMostRows && N > 0 && N <= kMostRows &&
+                     adapters >= 0 && rank > 0,
+                 "bad shape");
     *bytes = msst::adapter_gemm_workspace((int)rows, K, N, adapters, rank, sm_count());
   });
 }

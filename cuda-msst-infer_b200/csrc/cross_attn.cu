@@ -29,9 +29,9 @@
 // 980 us for the long prompts against 752; the 64-column MMAs read as much of Q for half the
 // products).
 //
-// Bound: the chain scores, softmax, product.  4 x 8 heads of 1895 x 3792 x 64: 101 us (582 TFLOP/s), XU
-// pipe 62 %, tensor pipe 31 % busy.  4 x 32/8 heads of 4096 x 4096 x 128, ragged: 772 to 778 us
-// (1150 TFLOP/s).
+// Bound: the chain scores, softmax, product.  4 x 8 heads of 1895 x 3792 x 64: 101 us (584 TFLOP/s), XU
+// pipe 63 %, tensor pipe 32 % busy.  4 x 32/8 heads of 4096 x 4096 x 128, ragged: 754 to 759 us
+// (1180 TFLOP/s); XU and tensor pipe 59 % busy for one batch entry of it.
 //
 // Softmax: the reference a row is exponentiated against starts at the maximum of its
 // first 32 kept scores (less kRefShift) and moves lazily: a tile is taken in one pass without a
@@ -52,11 +52,12 @@ namespace {
 constexpr int kThreads = 384;
 constexpr int kSoftmaxWarp0 = 4;
 // Registers a thread after the split: 128 x 88 + 256 x 208 = 384 x 168, the block's launch share
-// (softmax warps without spills: 2 % faster at both head sizes).
+// (2 % faster at both head sizes).  The compiler allocates 168 for every role and spills 88 (head_dim
+// <= 64) to 128 bytes; none with the softmax role left out.
 constexpr int kFewRegs = 88, kSoftmaxRegs = 208;
-// fp16 weights are taken 2^4 larger (the reference 4 lower, in powers of two): they are dropped below
-// 2^-25, and many of those count together, in the row sum at least.  A step's row sum bounds each of
-// its weights, and 61440 is inside fp16's 65504, so it may grow by as much as without the shift.
+// fp16 weights are taken 2^4 larger (the reference 4 lower, in powers of two), since fp16 drops what is
+// below 2^-25 while the row sum counts it: 2^18 such keys were 0.8 % of a result.  A step's row sum bounds
+// each of its weights, and 61440 is inside fp16's 65504, so a row may grow as far as without the shift.
 template <typename T>
 constexpr float kRefShift = std::is_same<T, __half>::value ? 4.f : 0.f;
 template <typename T>

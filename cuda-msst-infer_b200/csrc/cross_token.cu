@@ -5,8 +5,8 @@
 // m16n8k16, whose fragments come straight from 128-byte swizzled TMA tiles by ldmatrix
 // (an M of 128 rows on the tcgen05 path holds each K/V tile in shared memory for the length
 // of a full tile's chain and leaves too little of it for loads in flight: 62.9 us against
-// 42.9 for 16 sequences of up to 4096 keys, 32/8 heads of 128).  That call is 43 us, 40 of them
-// this kernel's alone (206 MB, 5.2 TB/s); one sequence of 131072 keys, 8 heads of 64, 56 to 57.5 us.
+// 42.9 for 16 sequences of up to 4096 keys, 32/8 heads of 128).  That call is 43 us, 41 of them
+// this kernel's alone (206 MB, 5.1 TB/s); one sequence of 131072 keys, 8 heads of 64, 56 to 58 us.
 //
 // CTA = 288 threads: warp 8 brings tiles of 64 keys into a ring as deep as shared memory
 // allows; warps 0-3 take the even tiles of the CTA's run and warps 4-7 the odd ones (the
