@@ -11,6 +11,7 @@
 #include <utility>
 
 #include "attention.cuh"
+#include "cache_ops.cuh"
 #include "gemm.cuh"
 #include "kernels.cuh"
 #include "model.h"
@@ -186,6 +187,25 @@ void check_cross_heads(int q_heads, int kv_heads, int head_dim) {
   MSST_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "head_dim must be a multiple of 8, <= 128");
   MSST_REQUIRE(q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0,
                "k and v need the same number of heads, and q a multiple of it");
+}
+
+// The pages of a cache: a power of two of tokens each, all slots counted in 32 bits.  Returns log2(page_size).
+int check_pages(int pages, int page_size) {
+  MSST_REQUIRE(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
+               "page_size must be a power of two from 16 to 256");
+  MSST_REQUIRE(pages > 0 && (long long)pages * page_size < (1LL << 31), "bad number of pages");
+  int shift = 0;
+  while (1 << shift < page_size) ++shift;
+  return shift;
+}
+
+// A block table [requests, blocks] whose rows count their tokens in 32 bits.
+void check_table(const int* table, int requests, int blocks, long long stride, int page_size) {
+  MSST_REQUIRE(requests >= 0 && requests <= msst::kMostPlanRequests,
+               "at most " + std::to_string(msst::kMostPlanRequests) + " requests");
+  MSST_REQUIRE(blocks >= 0 && (long long)blocks * page_size < (1LL << 31), "bad number of blocks");
+  MSST_REQUIRE(requests < 2 || stride >= blocks, "the block table's rows overlap");
+  MSST_REQUIRE(table || blocks == 0 || requests == 0, "block_table is null");
 }
 
 void check_workspace(const void* p, long long have, long long need) {
@@ -583,6 +603,149 @@ int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const
     p.adapters = adapters;
     p.rank = rank;
     MSST_CUDA(msst::launch_adapter_gemm(p, dtype, sm_count(), as_stream(stream)));
+  });
+}
+
+int msst_cache_plan(const int* new_tokens, const int* lens, int requests, int* block_table, int blocks,
+                    long long table_stride, int* free_pages, int pages, const int* free_count, int page_size, int start,
+                    int tokens, int* out_lens, int* out_free_count, int* q_starts, int* slots, int* positions,
+                    void* stream) {
+  return guarded([&] {
+    msst::CachePlanParams p{};
+    p.page_shift = check_pages(pages, page_size);
+    check_table(block_table, requests, blocks, table_stride, page_size);
+    MSST_REQUIRE(tokens >= 0 && tokens <= kMostRows, "bad number of tokens");
+    MSST_REQUIRE(start >= 0 && start + (long long)blocks * page_size < (1LL << 31), "positions pass 32 bits");
+    MSST_REQUIRE(free_pages && free_count && out_free_count && q_starts && (tokens == 0 || (slots && positions)) &&
+                     (requests == 0 || (new_tokens && lens && out_lens)),
+                 "null argument");
+    p.new_tokens = new_tokens;
+    p.lens = lens;
+    p.table = block_table;
+    p.free_pages = free_pages;
+    p.free_count = free_count;
+    p.out_lens = out_lens;
+    p.out_count = out_free_count;
+    p.q_starts = q_starts;
+    p.slots = slots;
+    p.positions = positions;
+    p.table_stride = requests > 1 ? table_stride : 0;
+    p.requests = requests;
+    p.blocks = blocks;
+    p.pages = pages;
+    p.start = start;
+    p.tokens = tokens;
+    DeviceScope dev_scope(device_of(free_pages));
+    MSST_CUDA(msst::launch_cache_plan(p, as_stream(stream)));
+  });
+}
+
+int msst_rope_append(const msst_heads* q, const msst_heads* k, const msst_heads* v, int tokens, int head_dim,
+                     const int* positions, const int* slots, const double* inv_freq, int rot_dim, float amplitude,
+                     int pairing, const msst_heads* k_cache, const msst_heads* v_cache, int pages, int page_size,
+                     int dtype, const msst_heads* q_out, void* stream) {
+  return guarded([&] {
+    check_dtype(dtype);
+    msst::RopeAppendParams p{};
+    p.page_shift = check_pages(pages, page_size);
+    MSST_REQUIRE(tokens >= 0 && tokens <= kMostRows, "bad number of tokens");
+    MSST_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "head_dim must be a multiple of 8, <= 256");
+    MSST_REQUIRE(rot_dim >= 0 && rot_dim <= head_dim && rot_dim % 8 == 0,
+                 "rot_dim must be a multiple of 8, <= head_dim");
+    MSST_REQUIRE(pairing == MSST_PAIRS_INTERLEAVED || pairing == MSST_PAIRS_HALVES, "bad pairing");
+    MSST_REQUIRE(std::isfinite(amplitude), "amplitude must be finite");
+    p.q = heads_view(q, 1, tokens, 8, "q");
+    p.k = heads_view(k, 1, tokens, 8, "k");
+    p.v = heads_view(v, 1, tokens, 8, "v");
+    p.out_q = heads_view(q_out, 1, tokens, 8, "q_out", true);
+    p.k_cache = heads_view(k_cache, pages, page_size, 8, "k_cache", true);
+    p.v_cache = heads_view(v_cache, pages, page_size, 8, "v_cache", true);
+    MSST_REQUIRE(p.out_q.heads == p.q.heads, "q_out must have q's heads");
+    MSST_REQUIRE(p.v.heads == p.k.heads && p.k_cache.heads == p.k.heads && p.v_cache.heads == p.k.heads,
+                 "k, v and the caches need the same number of heads");
+    MSST_REQUIRE(tokens <= (1LL << 31) / ((long long)p.q.heads + 2 * p.k.heads), "too many head vectors");
+    if (tokens == 0) return;
+    MSST_REQUIRE(slots && (rot_dim == 0 || (positions && inv_freq)), "null argument");
+    p.positions = positions;
+    p.slots = slots;
+    p.freq = inv_freq;
+    p.amplitude = amplitude;
+    p.tokens = tokens;
+    p.head_dim = head_dim;
+    p.rot_dim = rot_dim;
+    p.halves = pairing == MSST_PAIRS_HALVES;
+    p.num_slots = (long long)pages * page_size;
+    DeviceScope dev_scope(device_of(q->data));
+    MSST_CUDA(msst::launch_rope_append(p, dtype, as_stream(stream)));
+  });
+}
+
+int msst_prefix_attention_workspace(int tokens, int requests, int prefix_len, int q_heads, int kv_heads, int head_dim,
+                                    long long* bytes) {
+  return guarded([&] {
+    MSST_REQUIRE(bytes && tokens >= 0 && requests >= 0 && prefix_len >= 0, "bad shape");
+    MSST_REQUIRE(tokens <= kMostRows && prefix_len <= kMostRows, "too many tokens");
+    check_cross_heads(q_heads, kv_heads, head_dim);
+    MSST_REQUIRE(tokens <= (1LL << 31) / q_heads, "too many query rows");
+    *bytes = msst::prefix_attention_workspace(tokens, requests, prefix_len, q_heads, kv_heads, head_dim, sm_count());
+  });
+}
+
+int msst_prefix_attention(const msst_heads* q, int tokens, const int* q_starts, int requests,
+                          const msst_heads* prefix_k, const msst_heads* prefix_v, int prefix_len,
+                          const msst_heads* k_cache, const msst_heads* v_cache, int pages, int page_size,
+                          const int* block_table, int blocks, long long table_stride, const int* lens, int head_dim,
+                          float scale, int dtype, const msst_heads* out, void* workspace, long long workspace_bytes,
+                          void* stream) {
+  return guarded([&] {
+    check_dtype(dtype);
+    msst::PrefixAttnParams p{};
+    p.page_shift = check_pages(pages, page_size);
+    check_table(block_table, requests, blocks, table_stride, page_size);
+    MSST_REQUIRE(tokens >= 0 && prefix_len >= 0, "bad shape");
+    MSST_REQUIRE(tokens <= kMostRows && prefix_len <= kMostRows, "too many tokens");
+    MSST_REQUIRE(q_starts || tokens == requests, "without q_starts each request has one token");
+    MSST_REQUIRE(std::isfinite(scale), "scale must be finite");
+    p.q = heads_view(q, 1, tokens, 8, "q");
+    p.out = heads_view(out, 1, tokens, 8, "out", true);
+    p.k_cache = heads_view(k_cache, pages, page_size, 8, "k_cache");
+    p.v_cache = heads_view(v_cache, pages, page_size, 8, "v_cache");
+    MSST_REQUIRE(p.out.heads == p.q.heads, "out must have q's heads");
+    MSST_REQUIRE(p.v_cache.heads == p.k_cache.heads, "the caches need the same number of heads");
+    check_cross_heads(p.q.heads, p.k_cache.heads, head_dim);
+    MSST_REQUIRE(tokens <= (1LL << 31) / p.q.heads, "too many query rows");
+    if (prefix_len > 0) {
+      p.prefix_k = heads_view(prefix_k, 1, prefix_len, 8, "prefix_k");
+      p.prefix_v = heads_view(prefix_v, 1, prefix_len, 8, "prefix_v");
+      MSST_REQUIRE(p.prefix_k.heads == p.k_cache.heads && p.prefix_v.heads == p.k_cache.heads,
+                   "the prefix needs the caches' heads");
+      MSST_REQUIRE(prefix_len == 1 || (p.prefix_k.seq_stride > 0 && p.prefix_v.seq_stride > 0),
+                   "the prefix's sequence strides must not be 0");
+    }
+    if (tokens == 0 || requests == 0) return;
+    MSST_REQUIRE(lens, "lens is null");
+    MSST_REQUIRE((tokens == 1 || p.q.seq_stride > 0) && (p.q.heads == 1 || p.q.head_stride > 0) &&
+                     p.k_cache.seq_stride > 0 && p.v_cache.seq_stride > 0 &&
+                     (pages == 1 || (p.k_cache.batch_stride > 0 && p.v_cache.batch_stride > 0)),
+                 "strides of q, and page and sequence strides of the caches must not be 0");
+    p.q_starts = q_starts;
+    p.lens = lens;
+    p.table = block_table;
+    p.table_stride = requests > 1 ? table_stride : 0;
+    p.tokens = tokens;
+    p.requests = requests;
+    p.prefix = prefix_len;
+    p.pages = pages;
+    p.blocks = blocks;
+    p.head_dim = head_dim;
+    const float s = scale == 0.f ? 1.0f / std::sqrt((float)head_dim) : scale;
+    p.scale_log2 = s * 1.4426950408889634f;
+    DeviceScope dev_scope(device_of(q->data));
+    check_workspace(workspace, workspace_bytes,
+                    msst::prefix_attention_workspace(tokens, requests, prefix_len, p.q.heads, p.k_cache.heads, head_dim,
+                                                     sm_count()));
+    p.ws = static_cast<float*>(workspace);
+    MSST_CUDA(msst::launch_prefix_attention(p, dtype, sm_count(), as_stream(stream)));
   });
 }
 

@@ -21,9 +21,12 @@ enum DeviceError : unsigned {
   // not a wait: data of the call outside its documented range (see the operator)
   kErrPosition = 14,
   kErrAdapter = 15,
+  kErrCacheFull = 16,
+  kErrSlot = 17,
+  kErrPage = 18,
 };
 
-constexpr unsigned kFirstDataError = kErrPosition, kDataErrors = 2;
+constexpr unsigned kFirstDataError = kErrPosition, kDataErrors = 5;
 
 // What a translation unit's kernels have recorded: the first wait that gave up, and the data
 // errors (bit i: kFirstDataError + i).

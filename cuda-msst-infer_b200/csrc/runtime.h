@@ -174,13 +174,17 @@ bool qk_norm_device_error(DeviceErrors& e, bool store);
 bool cross_attn_device_error(DeviceErrors& e, bool store);
 bool cross_token_device_error(DeviceErrors& e, bool store);
 bool adapter_gemm_device_error(DeviceErrors& e, bool store);
+bool cache_plan_device_error(DeviceErrors& e, bool store);
+bool rope_append_device_error(DeviceErrors& e, bool store);
+bool prefix_attn_device_error(DeviceErrors& e, bool store);
 
 // The code that msst_device_error reports; `clear` takes that one out.
 inline unsigned device_error(bool clear) {
-  constexpr int n = 8;
+  constexpr int n = 11;
   bool (*const unit[n])(DeviceErrors&, bool) = {
       gemm_device_error,    attention_device_error,  kernels_device_error,     band_attention_device_error,
-      qk_norm_device_error, cross_attn_device_error, cross_token_device_error, adapter_gemm_device_error};
+      qk_norm_device_error, cross_attn_device_error, cross_token_device_error, adapter_gemm_device_error,
+      cache_plan_device_error, rope_append_device_error, prefix_attn_device_error};
   DeviceErrors was[n], now[n];
   for (int i = 0; i < n; ++i) {
     if (!unit[i](was[i], false)) return ~0u;

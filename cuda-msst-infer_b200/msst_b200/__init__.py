@@ -10,6 +10,7 @@ CUDA library, and importing the bindings fails loudly when it is not built.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import struct
 import wave
@@ -31,7 +32,8 @@ EXPORTS = [
     "msst_last_error", "msst_device_error", "msst_version", "msst_kernel_launches", "msst_kernel_timing",
     "msst_kernel_timing_report", "msst_rmsnorm", "msst_gemm", "msst_gemm_qkv_rope",
     "msst_attention", "msst_layernorm", "msst_sdpa", "msst_qk_norm_rope", "msst_cross_attention_workspace",
-    "msst_cross_attention", "msst_adapter_gemm_workspace", "msst_adapter_gemm", "msst_grouped_gemm", "msst_band_gather", "msst_mask_apply", "msst_model_band_tables",
+    "msst_cross_attention", "msst_adapter_gemm_workspace", "msst_adapter_gemm", "msst_cache_plan", "msst_rope_append",
+    "msst_prefix_attention_workspace", "msst_prefix_attention", "msst_grouped_gemm", "msst_band_gather", "msst_mask_apply", "msst_model_band_tables",
     "msst_roformer_attn_block", "msst_roformer_ffn_block", "msst_model_load", "msst_model_free", "msst_model_get_info", "msst_model_forward",
     "msst_model_masks", "msst_model_transformer", "msst_model_transformer_noalloc", "msst_model_separate", "msst_model_separate_host",
     "msst_model_chunk_plan", "msst_model_forward_chunks", "msst_model_stitch",
@@ -104,6 +106,12 @@ def lib():
     L.msst_adapter_gemm_workspace.argtypes = [i64, c_int, c_int, c_int, c_int, pi64]
     L.msst_adapter_gemm.argtypes = [vp, i64, c_int, i64, vp, c_int, vp, vp, vp, vp, c_int, c_int, vp, c_int, vp, i64,
                                     vp, i64, vp]
+    L.msst_cache_plan.argtypes = [vp, vp, c_int, vp, c_int, i64, vp, c_int, vp, c_int, c_int, c_int, vp, vp, vp, vp, vp, vp]
+    L.msst_rope_append.argtypes = [vp, vp, vp, c_int, c_int, vp, vp, vp, c_int, c_float, c_int, vp, vp, c_int, c_int,
+                                   c_int, vp, vp]
+    L.msst_prefix_attention_workspace.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int, pi64]
+    L.msst_prefix_attention.argtypes = [vp, c_int, vp, c_int, vp, vp, c_int, vp, vp, c_int, c_int, vp, c_int, i64, vp,
+                                        c_int, c_float, c_int, vp, vp, i64, vp]
     L.msst_grouped_gemm.argtypes = [c_int, ctypes.POINTER(GemmGroupC), vp, i64, i64, vp, i64, i64, c_int, c_int,
                                     c_int, vp, i64, i64, vp]
     L.msst_band_gather.argtypes = [vp, c_int, c_int, ctypes.POINTER(BandTables), c_int, vp, i64, vp]
@@ -282,6 +290,66 @@ def _side(x, shape, out, what, keep):
     heads = shape[2]
     return (out, _HEADS(x.data_ptr(), heads, st[0], st[1], st[2]),
             _HEADS(out.data_ptr(), heads, ost[0], ost[1], ost[2]))
+
+
+def _int32(t, shape, device, what):
+    """Address of an int32 tensor of `shape`, contiguous (never a copy: some are written)."""
+    if (t is None or t.dtype is not _torch_module.int32 or t.get_device() != device or t.shape != shape
+            or not t.is_contiguous()):
+        raise ValueError(f"{what} must be int32 {list(shape)}, contiguous, on the operands' device")
+    return t.data_ptr()
+
+
+def _table(t, requests, device):
+    """(address, blocks, row stride) of a block table [requests, blocks]."""
+    if (t.dtype is not _torch_module.int32 or t.get_device() != device or t.dim() != 2 or t.shape[0] != requests
+            or (t.stride(1) != 1 and t.shape[1] > 1)):
+        raise ValueError("block_table must be int32 [requests, blocks] on the operands' device, unit last stride")
+    return t.data_ptr(), t.shape[1], t.stride(0)
+
+
+def _flat_heads(t, keep):
+    """The msst_heads of a [tokens, heads, head_dim] tensor; one that 16-byte loads cannot walk is
+    copied first (kept alive in `keep`)."""
+    n, h, d = t.shape
+    st = t.stride()
+    if ((st[2] != 1 and d > 1) or t.data_ptr() & 15 or ((st[0] & 7 or not st[0]) and n > 1)
+            or ((st[1] & 7 or not st[1]) and h > 1)):
+        t = t.clone(memory_format=_torch_module.contiguous_format)
+        keep.append(t)
+        st = t.stride()
+    return _HEADS(t.data_ptr(), h, 0, st[0], st[1])
+
+
+def _cache_heads(t, dt, dev, what):
+    """The msst_heads of a cache [pages, page_size, heads, head_dim] (never a copy)."""
+    if t.dim() != 4 or t.dtype is not dt or t.get_device() != dev or (t.stride(3) != 1 and t.shape[3] > 1):
+        raise ValueError(f"{what} must be [pages, page_size, heads, head_dim] with q's type and device, unit last stride")
+    st = t.stride()
+    return _HEADS(t.data_ptr(), t.shape[2], st[0], st[1], st[2])
+
+
+def rope_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, original=8192, slow=1.0, fast=32.0, device=None):
+    """(inv_freq float64 [rot_dim / 2], amplitude) for ops.rope_append: base ** (-2 i / rot_dim), stretched
+    to `factor` times as many positions by `scaling`: None, "linear" (all frequencies / factor), "base" (a
+    larger base, so that the slowest pair is stretched by factor and the fastest kept) or "parts"
+    (pairs that turn less than `slow` times over `original` positions / factor, those that turn more than
+    `fast` times kept, a ramp over the turns between; amplitude 1 + 0.1 ln factor)."""
+    torch = _torch()
+    _need(rot_dim > 0 and rot_dim % 2 == 0 and base > 0 and factor > 0, "rot_dim must be even, base and factor above 0")
+    _need(scaling in (None, "linear", "base", "parts"), "scaling must be None, 'linear', 'base' or 'parts'")
+    if scaling == "base" and rot_dim > 2:
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    freq = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    amplitude = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "parts":
+        _need(original > 0 and fast > slow, "original must be above 0 and fast above slow")
+        keep = ((freq * (original / (2 * math.pi)) - slow) / (fast - slow)).clamp(0, 1)
+        freq = freq * (keep + (1 - keep) / factor)
+        amplitude = 1.0 + 0.1 * math.log(factor) if factor > 1 else 1.0
+    return freq.to(device), amplitude
 
 
 class ops:
@@ -516,6 +584,131 @@ class ops:
         check(lib().msst_adapter_gemm(
             x.data_ptr(), rows, K, ldx, ptr(w), N, bias, ptr(lora_a), ptr(lora_b), scales, count, rank, ptr(row_adapter),
             code, out.data_ptr(), ldo, ws, need, _current_stream(dev)))
+        return out
+
+    @staticmethod
+    def cache_plan(new_tokens, lens, block_table, free_pages, free_count, page_size, tokens, start=0, out_lens=None,
+                   out_free_count=None):
+        """Block tables and slots of a paged cache from request lengths, on the GPU.
+
+        new_tokens, lens int32 [R]: requests with new_tokens < 0 have ended and give their pages
+        back, then the others take pages for that many more tokens.  block_table int32 [R, blocks]
+        and the stack free_pages int32 [pages] (free_count int32 [1] entries high) are updated in
+        place; page_size is a power of two from 16 to 256; `tokens` rows for new tokens, `start` the
+        position of a request's first token.  A request without room stays as it was, its rows get
+        slot -1, and device_error() returns 16.  Returns (q_starts [R + 1], slots [tokens],
+        positions [tokens], lens [R], free_count [1]), the last two in out_lens / out_free_count
+        where given (lens / free_count themselves allowed)."""
+        torch = _torch()
+        dev, shape = new_tokens.get_device(), new_tokens.shape
+        _need(len(shape) == 1 and free_pages.dim() == 1, "new_tokens and free_pages must have one dimension")
+        R = shape[0]
+        new, old = _int32(new_tokens, shape, dev, "new_tokens"), _int32(lens, shape, dev, "lens")
+        table, blocks, stride = _table(block_table, R, dev)
+        free, count = _int32(free_pages, free_pages.shape, dev, "free_pages"), _int32(free_count, (1,), dev, "free_count")
+        if out_lens is None:
+            out_lens = torch.empty_like(lens)
+        if out_free_count is None:
+            out_free_count = torch.empty_like(free_count)
+        _need(tokens >= 0, "tokens must be >= 0")
+        made = new_tokens.new_empty(R + 1 + 2 * tokens)
+        q_starts, slots, positions = made[:R + 1], made[R + 1:R + 1 + tokens], made[R + 1 + tokens:]
+        at = made.data_ptr()
+        check(lib().msst_cache_plan(
+            new, old, R, table, blocks, stride, free, free_pages.shape[0], count, page_size, start, tokens,
+            _int32(out_lens, shape, dev, "out_lens"), _int32(out_free_count, (1,), dev, "out_free_count"), at,
+            at + 4 * (R + 1), at + 4 * (R + 1 + tokens), _current_stream(dev)))
+        return q_starts, slots, positions, out_lens, out_free_count
+
+    @staticmethod
+    def rope_append(q, k, v, positions, slots, inv_freq, k_cache, v_cache, amplitude=1.0, pairing="interleaved",
+                    out_q=None):
+        """The position rotation of queries and keys, keys and values written to a paged cache.
+
+        q [T, Hq, d], k and v [T, Hk, d], 16-bit, any strides (what 16-byte loads cannot walk is
+        copied first); positions, slots int32 [T] (slot < 0: not written); inv_freq float64
+        [rot / 2] radians a position for the pairs of the first `rot` columns (see
+        rope_frequencies; None: no rotation), cos and sin multiplied by `amplitude`; pairing as in
+        qk_norm_rope.  Caches [pages, page_size, Hk, d], slot = page * page_size + place.  d and rot
+        are multiples of 8, d <= 256.  Returns the rotated q, or out_q (which may be q itself)."""
+        torch = _torch()
+        dt, dev, shape, ks, keep = q.dtype, q.get_device(), q.shape, k.shape, []
+        code = _dtype_code(dt)
+        _need(len(shape) == 3 and len(ks) == 3 and ks[0] == shape[0] and ks[2] == shape[2] and v.shape == ks,
+              "q must be [T, heads, head_dim], k and v [T, heads, head_dim] with q's T and head_dim")
+        _need(k.dtype is dt and v.dtype is dt and k.get_device() == dev and v.get_device() == dev,
+              "q, k and v must share one 16-bit dtype and one device")
+        T, Hq, d = shape
+        hk, hv = _cache_heads(k_cache, dt, dev, "k_cache"), _cache_heads(v_cache, dt, dev, "v_cache")
+        _need(k_cache.shape == v_cache.shape and k_cache.shape[2:] == ks[1:], "the caches must have k's heads and head_dim")
+        half, freq, pos = 0, None, None
+        if inv_freq is not None:
+            _need(inv_freq.dtype is torch.float64 and inv_freq.dim() == 1 and inv_freq.get_device() == dev,
+                  "inv_freq must be float64 [rot / 2] on q's device")
+            half, inv_freq = inv_freq.shape[0], inv_freq.contiguous()
+            freq, pos = inv_freq.data_ptr(), _int32(positions, (T,), dev, "positions")
+        if out_q is None:
+            out_q = torch.empty_like(q, memory_format=torch.contiguous_format)
+        else:
+            _need(out_q.shape == shape and out_q.dtype is dt and out_q.get_device() == dev and
+                  (out_q.stride(2) == 1 or d < 2), "out_q must have q's shape, type and device, and unit last stride")
+        ost = out_q.stride()
+        check(lib().msst_rope_append(
+            _flat_heads(q, keep), _flat_heads(k, keep), _flat_heads(v, keep), T, d, pos,
+            _int32(slots, (T,), dev, "slots"), freq, 2 * half, amplitude, PAIRING[pairing], hk, hv, k_cache.shape[0],
+            k_cache.shape[1], code, _HEADS(out_q.data_ptr(), Hq, 0, ost[0], ost[1]), _current_stream(dev)))
+        return out_q
+
+    @staticmethod
+    def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, block_table, lens, q_starts=None, scale=0.0, out=None):
+        """Attention of new tokens to a prefix that all requests share (read once for all of them) and
+        to each request's own tokens in a paged cache, causal among the new ones.
+
+        q [T, Hq, d]; prefix_k / prefix_v [P, Hk, d] (None: no prefix); caches [pages, page_size,
+        Hk, d]; one 16-bit type, Hq a multiple of Hk, d a multiple of 8 and <= 128.  block_table
+        int32 [R, blocks], lens int32 [R] own tokens with the new ones included; request r has the
+        rows q_starts[r] to q_starts[r + 1] (int32 [R + 1]; None: one row each, T = R).  Rows that
+        see no key give zeros; rows of no request are left as they were in `out`, zeros without
+        one.  Returns [T, Hq, d]."""
+        torch = _torch()
+        dt, dev, shape, cs, keep = q.dtype, q.get_device(), q.shape, k_cache.shape, []
+        code = _dtype_code(dt)
+        _need(len(shape) == 3 and len(cs) == 4 and cs[3] == shape[2] and v_cache.shape == cs,
+              "q must be [T, heads, head_dim], the caches [pages, page_size, heads, head_dim]")
+        T, Hq, d = shape
+        Hk = cs[2]
+        _need(Hk > 0 and Hq > 0 and Hq % Hk == 0, "q must have a multiple of the caches' heads")
+        hk, hv = _cache_heads(k_cache, dt, dev, "k_cache"), _cache_heads(v_cache, dt, dev, "v_cache")
+        _need((prefix_k is None) == (prefix_v is None), "prefix_k and prefix_v go together")
+        P, pk, pv = 0, None, None
+        if prefix_k is not None:
+            ps = prefix_k.shape
+            _need(len(ps) == 3 and ps[1] == Hk and ps[2] == d and prefix_v.shape == ps,
+                  "prefix_k and prefix_v must be [P, heads, head_dim] with the caches' heads and head_dim")
+            _need(prefix_k.dtype is dt and prefix_v.dtype is dt and prefix_k.get_device() == dev and
+                  prefix_v.get_device() == dev, "q and the prefix must share one 16-bit dtype and one device")
+            P = ps[0]
+            if P:
+                pk, pv = _flat_heads(prefix_k, keep), _flat_heads(prefix_v, keep)
+        _need(lens.dim() == 1, "lens must be int32 [requests]")
+        R = lens.shape[0]
+        table, blocks, stride = _table(block_table, R, dev)
+        own, starts = _int32(lens, (R,), dev, "lens"), None
+        if q_starts is not None:
+            starts = _int32(q_starts, (R + 1,), dev, "q_starts")
+        if out is None:
+            out = q.new_empty(shape) if q_starts is None else q.new_zeros(shape)
+        else:
+            _need(out.shape == shape and out.dtype is dt and out.get_device() == dev and (out.stride(2) == 1 or d < 2),
+                  "out must have q's shape, type and device, and unit last stride")
+        so = out.stride()
+        need, ws = _workspace("prefix_attention", dev, T, R, P, Hq, Hk, d), None
+        if need:
+            space = q.new_empty(need // 2)  # 16-bit values; sizes are whole floats
+            ws = space.data_ptr()
+        check(lib().msst_prefix_attention(
+            _flat_heads(q, keep), T, starts, R, pk, pv, P, hk, hv, cs[0], cs[1], table, blocks, stride, own, d, scale,
+            code, _HEADS(out.data_ptr(), Hq, 0, so[0], so[1]), ws, need, _current_stream(dev)))
         return out
 
     @staticmethod

@@ -77,8 +77,9 @@ typedef struct msst_model_info {
 
 const char* msst_last_error(void);
 /* Code recorded by kernels since the last reset, 0 = none: 1 to 13 where a bounded wait gave up
- * (results since then are garbage), 14 where a position and 15 where an adapter index lay outside
- * the range that its operator documents.  A wait comes before the others; where several are
+ * (results since then are garbage), 14 where a position, 15 where an adapter index, 17 where a
+ * slot and 18 where a page lay outside the range that its operator documents, 16 where a cache had
+ * no room for a request's tokens.  A wait comes before the others; where several are
  * recorded, clear != 0 resets the returned one (of the waits, all) and the next call gives the next. */
 unsigned msst_device_error(int clear);
 int msst_version(void);
@@ -227,6 +228,71 @@ int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const
                       const void* lora_a, const void* lora_b, const float* scales, int adapters, int rank,
                       const int* row_adapter, int dtype, void* out, long long ldo, void* workspace,
                       long long workspace_bytes, void* stream);
+
+/* ---- operators of a cache of generated tokens behind one shared prefix: what a block
+ * with single tokens needs beside its cross attention.  Requests have their own tokens in
+ * pages of page_size tokens (a power of two from 16 to 256; slot = page * page_size +
+ * place in the page), a block table [requests, blocks] int32 (row stride table_stride)
+ * names a request's pages in order.  At most 8192 requests a call. */
+
+/* Block tables and slots from request lengths.  free_pages [pages] is a stack of free
+ * pages, *free_count its height (the entries below it are distinct and in no row).
+ * First, in order of requests, each with new_tokens[r] < 0 has ended: its ceil(lens[r] /
+ * page_size) pages go on top of the stack and its length becomes 0.  Then, in the same
+ * order, the others take the pages that new_tokens[r] more tokens need off its top.  A
+ * request whose need, added to those before it, passes what is free, whose tokens pass
+ * its row of the table, or end past row `tokens`, is refused: it stays as it was, its rows have
+ * slots -1, and msst_device_error reports 16.
+ * Written: out_lens [requests] and *out_free_count (which may be lens and free_count
+ * themselves), block_table and free_pages in place; q_starts [requests + 1], the first
+ * row of each request among the call's new tokens, and for each of the `tokens` rows its
+ * slot and its position start + place in the request (rows behind the last request: -1
+ * and 0).  With outputs of their own a call may be repeated with the same result.
+ * Lengths are taken into [0, blocks * page_size], the count into [0, pages]. */
+int msst_cache_plan(const int* new_tokens, const int* lens, int requests, int* block_table, int blocks,
+                    long long table_stride, int* free_pages, int pages, const int* free_count, int page_size, int start,
+                    int tokens, int* out_lens, int* out_free_count, int* q_starts, int* slots, int* positions,
+                    void* stream);
+
+/* The position rotation of queries and keys, whose keys go to the pages with their
+ * values.  q, k, v and q_out are [tokens, heads, head_dim] (msst_heads with tokens as the
+ * sequence, batch_stride unused), the caches [pages, page_size, heads, head_dim] (pages as the
+ * batch).  Each pair (a, b) of the first rot_dim columns of q and k (`pairing` as in
+ * msst_qk_norm_rope) becomes amplitude * (a cos - b sin, b cos + a sin) of the angle
+ * positions[t] * inv_freq[i] (double, [rot_dim / 2], radians; the angle is reduced in 64
+ * bits, so far positions lose nothing), fp32 inside, one rounding.  The other columns and v
+ * are copied.  q goes to q_out (which may be q itself, same strides, and otherwise must not
+ * overlap it), k and v to slots[t] of the caches.  A token with a negative slot is not written to
+ * them, one with a slot past the last page neither, and msst_device_error reports 17; the
+ * slots of a call's tokens differ (of tokens that share one, either's columns may end up
+ * there).  head_dim is a multiple of 8, <= 256, rot_dim a multiple of 8, <= head_dim (0:
+ * no rotation); data pointers are 16-byte aligned, strides multiples of 8 elements. */
+int msst_rope_append(const msst_heads* q, const msst_heads* k, const msst_heads* v, int tokens, int head_dim,
+                     const int* positions, const int* slots, const double* inv_freq, int rot_dim, float amplitude,
+                     int pairing, const msst_heads* k_cache, const msst_heads* v_cache, int pages, int page_size,
+                     int dtype, const msst_heads* q_out, void* stream);
+
+/* Attention to a prefix that all requests share and to each request's own tokens:
+ * out = softmax(scale * q k^T) v over the prefix_len keys of prefix_k / prefix_v [prefix_len,
+ * heads, head_dim] (none: prefix_len 0, the views may be NULL) and the request's own keys in the
+ * caches.  q and out are [tokens, q.heads, head_dim], rows q_starts[r] to q_starts[r + 1]
+ * (ascending, [requests + 1]; NULL: one row a request) request r's new tokens, which are
+ * the last of its lens[r] own ones: the i-th of n sees the first lens[r] - n + i + 1 of them (not below 0).
+ * q.heads is a multiple of the caches' heads, head_dim a multiple of 8 and <= 128,
+ * scale 0 selects 1/sqrt(head_dim).  What a row does not see, the rest of a page
+ * included, has no influence on it, whatever it holds.  A row that sees no key gives zeros; rows of no request are left as
+ * they were.  A page outside the caches counts as not there, and
+ * msst_device_error reports 18.  lens is taken into [0, blocks * page_size].  out must
+ * not overlap the inputs.  Precision, alignment and workspace as in msst_cross_attention
+ * (head strides of the prefix and the caches may be 0). */
+int msst_prefix_attention_workspace(int tokens, int requests, int prefix_len, int q_heads, int kv_heads, int head_dim,
+                                    long long* bytes);
+int msst_prefix_attention(const msst_heads* q, int tokens, const int* q_starts, int requests,
+                          const msst_heads* prefix_k, const msst_heads* prefix_v, int prefix_len,
+                          const msst_heads* k_cache, const msst_heads* v_cache, int pages, int page_size,
+                          const int* block_table, int blocks, long long table_stride, const int* lens, int head_dim,
+                          float scale, int dtype, const msst_heads* out, void* workspace, long long workspace_bytes,
+                          void* stream);
 
 /* One problem of msst_grouped_gemm: rows [a_row0, a_row0 + m) and columns
  * [a_col0, a_col0 + k) of x times rows [b_row0, b_row0 + n) (same k columns from

@@ -1,0 +1,139 @@
+"""Refusals of the operators of a paged cache behind a shared prefix (no GPU: every check comes
+before a device is touched)."""
+from __future__ import annotations
+
+import ctypes
+import struct
+
+import pytest
+
+
+def _heads(ptr=16, heads=2, sb=2048, sn=128, sh=64):
+    return struct.pack("Pi4xqqq", ptr, heads, sb, sn, sh)
+
+
+def _plan(**kw):
+    from msst_b200 import lib
+
+    a = dict(new=16, lens=16, R=4, table=16, blocks=8, stride=8, free=16, pages=64, count=16, page=16, start=0, tokens=4,
+             out_lens=16, out_count=16, starts=16, slots=16, positions=16)
+    a.update(kw)
+    return lib().msst_cache_plan(*a.values(), None)
+
+
+@pytest.mark.parametrize("bad, word", [
+    (dict(page=8), "page_size"), (dict(page=512), "page_size"), (dict(page=48), "page_size"), (dict(pages=0), "pages"),
+    (dict(pages=1 << 27), "pages"), (dict(R=-1), "requests"), (dict(R=8193), "requests"), (dict(blocks=-1), "blocks"),
+    (dict(blocks=1 << 27, stride=1 << 27), "blocks"), (dict(stride=7), "overlap"), (dict(table=None), "block_table"),
+    (dict(tokens=-1), "tokens"), (dict(tokens=0x7fffffff), "tokens"), (dict(start=-1), "positions"),
+    (dict(start=0x7fffffff), "positions"), (dict(new=None), "null"), (dict(lens=None), "null"), (dict(free=None), "null"),
+    (dict(count=None), "null"), (dict(out_lens=None), "null"), (dict(out_count=None), "null"), (dict(starts=None), "null"),
+    (dict(slots=None), "null"), (dict(positions=None), "null"),
+])
+def test_cache_plan_refuses(bad, word):
+    from msst_b200 import MSST_ERR_INVALID, lib
+
+    assert _plan(**bad) == MSST_ERR_INVALID
+    assert word in lib().msst_last_error().decode()
+
+
+def _append(**kw):
+    from msst_b200 import lib
+
+    a = dict(q=_heads(), k=_heads(), v=_heads(), tokens=4, d=64, positions=16, slots=16, freq=16, rot=64, amplitude=1.0,
+             pairing=0, k_cache=_heads(), v_cache=_heads(), pages=4, page=16, dtype=0, out=_heads())
+    a.update(kw)
+    return lib().msst_rope_append(*a.values(), None)
+
+
+@pytest.mark.parametrize("bad, word", [
+    (dict(q=None), "q needs"), (dict(k=None), "k needs"), (dict(out=None), "q_out"), (dict(k_cache=None), "k_cache"),
+    (dict(d=0), "head_dim"), (dict(d=60), "head_dim"), (dict(d=264), "head_dim"), (dict(rot=4), "rot_dim"),
+    (dict(rot=72), "rot_dim"), (dict(rot=-8), "rot_dim"), (dict(pairing=2), "pairing"), (dict(dtype=2), "dtype"),
+    (dict(amplitude=float("nan")), "amplitude"), (dict(page=17), "page_size"), (dict(pages=-1), "pages"),
+    (dict(q=_heads(ptr=24)), "aligned"), (dict(k=_heads(sn=132)), "multiples of 8"), (dict(v=_heads(heads=1)), "same number"),
+    (dict(v_cache=_heads(heads=1)), "same number"), (dict(out=_heads(heads=3)), "q's heads"), (dict(tokens=-1), "tokens"),
+    (dict(k_cache=_heads(sb=0)), "strides above 0"), (dict(out=_heads(sn=0)), "strides above 0"),
+    (dict(q=_heads(sn=-8)), "negative"), (dict(slots=None), "null"), (dict(positions=None), "null"), (dict(freq=None), "null"),
+    (dict(tokens=1 << 29), "too many"),
+])
+def test_rope_append_refuses(bad, word):
+    from msst_b200 import MSST_ERR_INVALID, lib
+
+    assert _append(**bad) == MSST_ERR_INVALID
+    assert word in lib().msst_last_error().decode()
+
+
+def _attention(**kw):
+    from msst_b200 import lib
+
+    a = dict(q=_heads(), tokens=4, starts=16, requests=2, pk=_heads(), pv=_heads(), prefix=8, kc=_heads(), vc=_heads(),
+             pages=4, page=16, table=16, blocks=2, stride=2, lens=16, d=64, scale=0.0, dtype=0, out=_heads(), ws=None,
+             wsb=0)
+    a.update(kw)
+    return lib().msst_prefix_attention(*a.values(), None)
+
+
+@pytest.mark.parametrize("bad, word", [
+    (dict(q=None), "q needs"), (dict(out=None), "out"), (dict(kc=None), "k_cache"), (dict(vc=None), "v_cache"),
+    (dict(pk=None), "prefix_k"), (dict(pv=None), "prefix_v"), (dict(tokens=-1), "shape"), (dict(prefix=-1), "shape"),
+    (dict(prefix=0x7fffffff), "too many"), (dict(starts=None), "one token"), (dict(requests=-1), "requests"),
+    (dict(requests=9000), "requests"), (dict(d=136), "head_dim"), (dict(d=12), "head_dim"), (dict(scale=float("inf")), "scale"),
+    (dict(dtype=2), "dtype"), (dict(page=12), "page_size"), (dict(pages=0), "pages"), (dict(blocks=-1), "blocks"),
+    (dict(stride=1), "overlap"), (dict(table=None), "block_table"), (dict(lens=None), "lens"),
+    (dict(q=_heads(heads=3), out=_heads(heads=3)), "multiple of it"), (dict(out=_heads(heads=4)), "q's heads"), (dict(vc=_heads(heads=1)), "same number"),
+    (dict(pk=_heads(heads=1)), "caches' heads"), (dict(kc=_heads(sn=0)), "must not be 0"), (dict(q=_heads(sn=0)), "must not be 0"),
+    (dict(pv=_heads(sn=0)), "must not be 0"), (dict(kc=_heads(ptr=8)), "aligned"), (dict(pk=_heads(sh=60)), "multiples of 8"),
+    (dict(tokens=(1 << 30) + 1), "too many"),
+])
+def test_prefix_attention_refuses(bad, word):
+    from msst_b200 import MSST_ERR_INVALID, lib
+
+    assert _attention(**bad) == MSST_ERR_INVALID
+    assert word in lib().msst_last_error().decode()
+
+
+@pytest.mark.parametrize("q_heads, kv_heads, head_dim", [(2, 4, 64), (3, 2, 64), (4, 4, 136), (4, 4, 12), (0, 1, 64)])
+def test_workspace_refuses_heads(q_heads, kv_heads, head_dim):
+    from msst_b200 import MSST_ERR_INVALID, lib
+
+    n = ctypes.c_longlong(-1)
+    assert lib().msst_prefix_attention_workspace(8, 2, 64, q_heads, kv_heads, head_dim, ctypes.byref(n)) == MSST_ERR_INVALID
+    assert n.value == -1
+
+
+def test_empty_calls_need_no_device():
+    from msst_b200 import MSST_OK
+
+    assert _append(tokens=0) == MSST_OK and _attention(tokens=0) == MSST_OK and _attention(requests=0) == MSST_OK
+
+
+def test_python_argument_checks():
+    import torch
+    from msst_b200 import ops
+
+    def i32(*shape):
+        return torch.zeros(*shape, dtype=torch.int32)
+
+    plan = dict(new_tokens=i32(3), lens=i32(3), block_table=i32(3, 4), free_pages=i32(20), free_count=i32(1), page_size=16,
+                tokens=3)
+    t, h = torch.zeros(4, 2, 64, dtype=torch.float16), torch.zeros(5, 16, 2, 64, dtype=torch.float16)
+    append = dict(q=t, k=t, v=t, positions=i32(4), slots=i32(4), inv_freq=torch.zeros(32, dtype=torch.float64), k_cache=h,
+                  v_cache=h)
+    attend = dict(q=t, prefix_k=t, prefix_v=t, k_cache=h, v_cache=h, block_table=i32(4, 2), lens=i32(4))
+    for op, good, bads in (
+        (ops.cache_plan, plan, (dict(new_tokens=i32(3, 1)), dict(lens=i32(2)), dict(lens=i32(3).long()),
+                                dict(block_table=i32(2, 4)), dict(block_table=i32(4, 3).t()[:3]), dict(free_count=i32(2)),
+                                dict(free_pages=i32(40)[::2]), dict(out_lens=i32(6)[::2]), dict(tokens=-1))),
+        (ops.rope_append, append, (dict(q=t[0]), dict(k=t[:3]), dict(v=t[:, :1]), dict(k=t.bfloat16()), dict(q=t.float()),
+                                   dict(positions=i32(3)), dict(positions=None), dict(slots=i32(4).long()),
+                                   dict(inv_freq=torch.zeros(32)), dict(k_cache=h[..., :32]), dict(v_cache=h[:4]),
+                                   dict(k_cache=h.transpose(2, 3)), dict(out_q=t[:, :1]))),
+        (ops.prefix_attention, attend, (dict(q=t[0]), dict(prefix_k=None), dict(prefix_v=t[:3]), dict(prefix_k=t.bfloat16()),
+                                        dict(k_cache=h[..., :32]), dict(v_cache=h.bfloat16()), dict(block_table=i32(3, 2)),
+                                        dict(lens=i32(4).long()), dict(lens=i32(8)[::2]), dict(q_starts=i32(4)),
+                                        dict(out=t[:3]), dict(q=t[:, :1].expand(4, 3, 64)))),
+    ):
+        for bad in bads:
+            with pytest.raises(ValueError):
+                op(**{**good, **bad})
