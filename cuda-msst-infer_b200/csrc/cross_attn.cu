@@ -40,6 +40,7 @@
 // P is rounded to the operands' 16 bits for the tensor cores.
 #include <algorithm>
 
+#include "attn_steps.cuh"
 #include "common.cuh"
 #include "cross_attn.cuh"
 #include "operators.cuh"
@@ -55,13 +56,6 @@ constexpr int kSoftmaxWarp0 = 4;
 // (2 % faster at both head sizes).  The compiler allocates 168 for every role and spills 88 (head_dim
 // <= 64) to 128 bytes; none with the softmax role left out.
 constexpr int kFewRegs = 88, kSoftmaxRegs = 208;
-// fp16 weights are taken 2^4 larger (the reference 4 lower, in powers of two), since fp16 drops what is
-// below 2^-25 while the row sum counts it: 2^18 such keys were 0.8 % of a result.  A step's row sum bounds
-// each of its weights, and 61440 is inside fp16's 65504, so a row may grow as far as without the shift.
-template <typename T>
-constexpr float kRefShift = std::is_same<T, __half>::value ? 4.f : 0.f;
-template <typename T>
-constexpr float kSumLimit = std::is_same<T, __half>::value ? 61440.f : 4096.f;
 constexpr uint32_t kHalfBytes = 128 * 64 * 2;  // 128 rows x 64 columns
 
 template <int DP>
@@ -75,108 +69,12 @@ struct Cfg {
   static constexpr uint32_t kColO = kBufs * 128;
 };
 
-// A position in a ring of N slots: the slot and the parity of its current use.
-template <int N>
-struct RingPos {
-  uint32_t slot = 0, phase = 0;
-  __device__ __forceinline__ RingPos plus(uint32_t n) const {  // n <= N
-    RingPos r;
-    r.slot = slot + n >= N ? slot + n - N : slot + n;
-    r.phase = slot + n >= N ? phase ^ 1 : phase;
-    return r;
-  }
-};
-
-// The S buffer of a step and the parity of that use.  Two buffers: one a tile, by the
-// tile's own count of steps; three: in turn over the sequence of both tiles.
-template <int NB>
-struct StepBuf {
-  uint32_t buf, parity;
-  __device__ __forceinline__ StepBuf(int w, uint32_t mine, uint32_t seq) {
-    if constexpr (NB == 2) {
-      buf = (uint32_t)w;
-      parity = mine & 1;
-    } else {
-      const uint32_t q = seq / 3;
-      buf = seq - 3 * q;
-      parity = q & 1;
-    }
-  }
-};
-
 // First token and head of row tile w of the current segment.
 __device__ __forceinline__ void tile_origin(const Walk& k, const Geom& g, int w, int& n0, int& g0) {
   const int tile = k.lone ? 2 * g.full : 2 * k.s.t + w;
   const int gi = tile / g.n_tiles;
   n0 = (tile - gi * g.n_tiles) * g.nt;
   g0 = gi * g.gt;
-}
-
-// Kept keys among the 32 of chunk ch of a tile that has khi valid keys.
-__device__ __forceinline__ uint32_t len_word(int khi, int ch) {
-  const int n = khi - 32 * ch;
-  return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
-}
-
-// Maximum of s c over the kept scores of a chunk.
-__device__ __forceinline__ float chunk_max(const uint32_t (&r)[32], uint32_t word, float c) {
-  float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < 32; i += 2) {
-    if (word >> i & 1) m0 = fmaxf(m0, __uint_as_float(r[i]) * c);
-    if (word >> (i + 1) & 1) m1 = fmaxf(m1, __uint_as_float(r[i + 1]) * c);
-  }
-  return fmaxf(m0, m1);
-}
-
-// P of one 32-column chunk against the reference: 2^(s c - ref), packed into pk.
-template <typename T>
-__device__ __forceinline__ void chunk_exp(const uint32_t (&r)[32], uint32_t word, float2 c2, float2 nref2, float2& sum2,
-                                          uint32_t* pk) {
-  if (word == 0xffffffffu) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 a = __ffma2_rn(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), c2, nref2);
-      const float2 e = make_float2(fast_exp2(a.x), fast_exp2(a.y));
-      sum2 = __fadd2_rn(sum2, e);
-      pk[i] = pack2<T>(e.x, e.y);
-    }
-  } else if (word == 0u) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) pk[i] = 0u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 a = __ffma2_rn(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), c2, nref2);
-      const float e0 = word >> (2 * i) & 1 ? fast_exp2(a.x) : 0.f;
-      const float e1 = word >> (2 * i + 1) & 1 ? fast_exp2(a.y) : 0.f;
-      sum2 = __fadd2_rn(sum2, make_float2(e0, e1));
-      pk[i] = pack2<T>(e0, e1);
-    }
-  }
-}
-
-// P and the row sum of a step's 128 columns; the next chunk's load is in flight while
-// one is processed.  kAll: every key is kept.
-template <typename T, bool kAll>
-__device__ __forceinline__ float row_exp(uint32_t sAddr, const uint32_t (&words)[4], float c, float ref,
-                                         uint32_t (&pk)[64]) {
-  const float2 c2 = make_float2(c, c), nref2 = make_float2(-ref, -ref);
-  float2 sum2 = make_float2(0.f, 0.f);
-  uint32_t ra[32], rb[32];
-  tmem_ld32(sAddr, ra);
-  tmem_ld_wait(ra);
-  tmem_ld32(sAddr + 32, rb);
-  chunk_exp<T>(ra, kAll ? 0xffffffffu : words[0], c2, nref2, sum2, pk);
-  tmem_ld_wait(rb);
-  tmem_ld32(sAddr + 64, ra);
-  chunk_exp<T>(rb, kAll ? 0xffffffffu : words[1], c2, nref2, sum2, pk + 16);
-  tmem_ld_wait(ra);
-  tmem_ld32(sAddr + 96, rb);
-  chunk_exp<T>(ra, kAll ? 0xffffffffu : words[2], c2, nref2, sum2, pk + 32);
-  tmem_ld_wait(rb);
-  chunk_exp<T>(rb, kAll ? 0xffffffffu : words[3], c2, nref2, sum2, pk + 48);
-  return sum2.x + sum2.y;
 }
 
 template <typename T, int DP, bool kMask>

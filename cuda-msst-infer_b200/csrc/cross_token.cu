@@ -15,6 +15,7 @@
 // item.  Runs of units, partial results and the joining launch are cross_attn.cu's.
 #include <algorithm>
 
+#include "attn_steps.cuh"
 #include "common.cuh"
 #include "cross_attn.cuh"
 #include "operators.cuh"
@@ -29,38 +30,6 @@ constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kKeys = 64;
 constexpr int kMaxStages = 12;
 constexpr uint32_t kBox = kKeys * 128;  // 64 keys x 64 columns
-// fp16 weights reach up to 2^15 instead of 1 (the reference is the maximum), so that they are dropped
-// below 2^-40 of the largest and not below 2^-25: a long row can hold many of those.
-template <typename T>
-constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
-
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-
 // 16-byte piece `chunk` (8 columns) of key `row` in a 128B-swizzled tile of 64-column boxes
 __device__ __forceinline__ uint32_t piece(uint32_t tile, int row, int chunk) {
   return tile + (uint32_t)((chunk >> 3) * kBox + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));

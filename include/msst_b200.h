@@ -281,7 +281,7 @@ int msst_rope_append(const msst_heads* q, const msst_heads* k, const msst_heads*
  * q.heads is a multiple of the caches' heads, head_dim a multiple of 8 and <= 128,
  * scale 0 selects 1/sqrt(head_dim).  What a row does not see, the rest of a page
  * included, has no influence on it, whatever it holds.  A row that sees no key gives zeros; rows of no request are left as
- * they were.  A page outside the caches counts as not there, and
+ * they were.  A page outside the caches reads as zeros, and
  * msst_device_error reports 18.  lens is taken into [0, blocks * page_size].  out must
  * not overlap the inputs.  Precision, alignment and workspace as in msst_cross_attention
  * (head strides of the prefix and the caches may be 0). */
