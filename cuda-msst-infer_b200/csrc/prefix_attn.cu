@@ -40,9 +40,10 @@ constexpr int kThreads = 384;
 constexpr int kSoftmaxWarp0 = 4;
 constexpr int kFewRegs = 88, kSoftmaxRegs = 208;  // 128 x 88 + 256 x 208 = 384 x 168, as cross_attn.cu
 constexpr uint32_t kHalfBytes = 128 * 64 * 2;     // 128 rows x 64 columns
-constexpr int kTokenKeys = 64, kTokenWarps = 8;
-constexpr uint32_t kTokenBox = kTokenKeys * 128;  // 64 keys x 64 columns
-constexpr int kMaxStages = 12;
+constexpr int kTokenKeys = 32, kTokenShift = 5;   // a token item's K/V tile
+constexpr uint32_t kTokenBox = kTokenKeys * 128;  // 32 keys x 64 columns
+constexpr int kTokenWarps = 8;                    // that multiply; the other four bring tiles, one a team
+constexpr int kMostTeams = 4, kMostEntries = 12;
 constexpr int kRecompute = -1;
 
 template <int DP>
@@ -50,13 +51,13 @@ struct PCfg {
   static constexpr int kHalves = DP / 64;
   static constexpr uint32_t kTile = kHalves * kHalfBytes;  // one Q, K or V tile
   static constexpr int kKSlots = DP == 128 ? 3 : 5, kVSlots = DP == 128 ? 2 : 5;
-  static constexpr uint32_t kTail = 2560;  // barriers and exchange of either role
-  static constexpr size_t kSmem = (2 + kKSlots + kVSlots) * kTile + kTail;
-  static_assert((19 + 2 * kKSlots + 3 * kVSlots) * 8 + 16 + 2048 <= kTail, "tile role");
-  static_assert(2 * kMaxStages * 8 + 16 + 2 * kTokenWarps * 16 * 4 <= kTail, "token role");
+  static constexpr uint32_t kTiles = (2 + kKSlots + kVSlots) * kTile;
+  static constexpr uint32_t kTail = 3072;  // segments, barriers and exchange of either role
+  static constexpr size_t kSmem = kTiles + kTail;
+  static_assert(kSmem <= 227 * 1024, "");
+  static constexpr uint32_t kEntry = kHalves * kTokenBox;  // token role: K or V of one head and tile
   static constexpr int kBufs = DP == 128 ? 2 : 3;
   static constexpr uint32_t kColO = kBufs * 128;
-  static constexpr uint32_t kStage = 2 * kHalves * kTokenBox;  // token role: K, then V
 };
 
 // What the host knows of a launch.
@@ -65,15 +66,19 @@ struct PrefixGeom {
   int gt, nt, g_tiles;        // heads and tokens of a row tile, tiles along the group
   int ksteps;
   int concat;                 // an item's keys are the prefix's and then its own (no items for the prefix alone)
-  int prefix_tiles, prefix_tiles64;
+  int prefix_tiles, prefix_tiles32;
   int prefix_token;           // all rows of a key head are at most 16: the prefix's item is a token item
   int n_tiles, full, lone;    // the prefix's tile items
   int box;                    // rows of a cache's TMA box
-  int pk_headed, pv_headed, kc_headed, vc_headed;
-  int stages, slot_rows, ld;  // ring of the token role; rows and row length (floats) of a partial result
+  int pk_headed, pv_headed, kc_headed, vc_headed;  // 0: key heads share one (stride 0)
+  int heads, groups, teams;   // token items: key heads of an item, items of a request, teams of a CTA
+  int entries, q_rows, q_slots;  // of a team: K or V tiles of all its heads, query rows a head, segments of those
+  int tile_rows, token_rows, ld;  // rows of a partial result's slot (tile items, token items), floats of a row
   int tile_cost, token_cost;  // of a unit
+  int tile_item, token_item;  // of an item's start and end, in units
   int* where;                 // [phase][tokens * q_heads] which partial results a row has
-  float* slots;               // [CTA][begins, ends][slot_rows][ld]
+  float* tile_slots;          // [CTA][begins, ends][tile_rows][ld]
+  float* token_slots;         // [CTA * teams][begins, ends][heads][token_rows][ld]
   float* whole;               // [phase][tokens * q_heads][ld] results of items that one CTA had whole
 };
 
@@ -117,220 +122,302 @@ struct Items {
       const int a = 2 * t, b = t < full ? a + 1 : a;
       end = min((max(a % n_tiles, b % n_tiles) + 1) * g.nt, q.n);
     }
-    const int keys = q.own ? q.limit(end - 1) : 0, shift = token ? 6 : 7;
+    const int keys = q.own ? q.limit(end - 1) : 0, shift = token ? kTokenShift : 7;
     return max(1, ptiles + ((keys + (1 << shift) - 1) >> shift));
   }
   __device__ __forceinline__ int units(int t, int tiles) const { return t < full ? tiles : (tiles + 1) >> 1; }
-  __device__ __forceinline__ long long head_units(const PrefixGeom& g, const Request& q, bool token, int ptiles) const {
+  // What the item counts for in the sharing out: its units, and the start and end of an item in units
+  __device__ __forceinline__ int weight(int t, int tiles, const PrefixGeom& g, bool token) const {
+    return units(t, tiles) + (token ? g.token_item : g.tile_item);
+  }
+  __device__ __forceinline__ long long head_weight(const PrefixGeom& g, const Request& q, bool token, int ptiles) const {
     long long sum = 0;
-    for (int t = 0; t < full + lone; ++t) sum += units(t, tiles(g, q, token, t, ptiles));
+    for (int t = 0; t < full + lone; ++t) sum += weight(t, tiles(g, q, token, t, ptiles), g, token);
     return sum;
   }
 };
 
 __device__ __forceinline__ int prefix_part(const PrefixGeom& g, bool token) {
-  return token ? g.prefix_tiles64 : g.prefix_tiles;
+  return token ? g.prefix_tiles32 : g.prefix_tiles;
 }
-// Units of the prefix's own items in the sequence of token or tile items.
-__device__ __forceinline__ long long prefix_units(const PrefixGeom& g, bool token) {
+// Weight of the prefix's own items in the sequence of token or tile items.
+__device__ __forceinline__ long long prefix_weight(const PrefixGeom& g, bool token) {
   if (g.concat || (bool)g.prefix_token != token) return 0;
-  if (token) return (long long)g.kv_heads * g.prefix_tiles64;
-  return (long long)g.kv_heads * ((long long)g.full * g.prefix_tiles + g.lone * ((g.prefix_tiles + 1) >> 1));
+  if (token) return (long long)g.groups * (g.prefix_tiles32 + g.token_item);
+  return (long long)g.kv_heads * ((long long)g.full * (g.prefix_tiles + g.tile_item) +
+                                  g.lone * (((prefix_part(g, false) + 1) >> 1) + g.tile_item));
 }
 
-// A CTA's run: units [u0, u0 + count) of the U of its sequence, CTAs [base, base + ctas); where it starts.
+// The run of a CTA (tile items) or of a team of its warps (token items): weights [u0, u0 + count) of the U of its sequence,
+// worker `self` of `workers`; where it starts.
 struct Run {
   long long u0, count, U;
-  int token, base, ctas;
+  int token, self, workers;
   int phase, r, hk, t, j;
 };
 
-// Exclusive sum over the CTA's threads and the total (s: a slot a warp).
-__device__ __forceinline__ long long cta_scan(long long v, long long* s, long long& total) {
+// Exclusive sums over the CTA's threads of two values, and the totals (s: two slots a warp).
+struct Two {
+  long long a, b;
+};
+__device__ __forceinline__ Two cta_scan(Two v, Two* s, Two& total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  long long incl = v;
+  Two incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
+    const long long x = __shfl_up_sync(0xffffffffu, incl.a, o), y = __shfl_up_sync(0xffffffffu, incl.b, o);
+    if (lane >= o) incl.a += x, incl.b += y;
   }
   if (lane == 31) s[warp] = incl;
   __syncthreads();
-  long long before = 0;
-  total = 0;
+  Two before{0, 0};
+  total = before;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += s[w];
-    total += s[w];
+    const Two x = s[w];
+    if (w < warp) before.a += x.a, before.b += x.b;
+    total.a += x.a, total.b += x.b;
   }
   __syncthreads();
-  return before + incl - v;
+  return Two{before.a + incl.a - v.a, before.b + incl.b - v.b};
 }
 
-// All threads: this CTA's run, from the lengths of all requests.
-__device__ void find_run(const PrefixAttnParams& p, const PrefixGeom& g, Run* run, long long* scratch) {
+// a b / c; a 32-bit division (a fifth of the time) where the numbers allow one.
+__host__ __device__ __forceinline__ long long mul_div(long long a, long long b, long long c) {
+  const unsigned long long n = (unsigned long long)a * (unsigned long long)b;
+  return (n | (unsigned long long)c) >> 32 ? (long long)(n / (unsigned long long)c)
+                                           : (long long)((unsigned)n / (unsigned)c);
+}
+
+// All threads: the run of this CTA, or of each of its teams, from the lengths of all requests.
+__device__ void find_runs(const PrefixAttnParams& p, const PrefixGeom& g, Run* runs, Two* scratch) {
   const int R = p.requests, tid = threadIdx.x;
-  auto units_of = [&](int r, long long& a, long long& b) {
-    a = b = 0;
-    if (r >= R) return;
+  // weight of request r for a key head: .a as tile items, .b as a token item (for a group of heads)
+  auto weights = [&](int r) -> Two {
+    if (r >= R) return Two{0, 0};
     const Request q = load_request(p, r);
-    if (q.n == 0) return;
+    if (q.n == 0) return Two{0, 0};
     const bool token = is_token(g, q);
-    const long long u = Items(g, q, token).head_units(g, q, token, g.concat ? prefix_part(g, token) : 0) * g.kv_heads;
-    (token ? b : a) = u;
+    const long long u = Items(g, q, token).head_weight(g, q, token, g.concat ? prefix_part(g, token) : 0);
+    return token ? Two{0, u} : Two{u, 0};
   };
-  long long a = 0, b = 0, mine_a, mine_b;
+  Two mine{0, 0}, total;
   for (int r = tid; r < R; r += kThreads) {
-    units_of(r, mine_a, mine_b);
-    a += mine_a;
-    b += mine_b;
+    const Two x = weights(r);
+    mine.a += x.a, mine.b += x.b;
   }
-  long long total_a, total_b;
-  cta_scan(a, scratch, total_a);
-  cta_scan(b, scratch, total_b);
-  total_a += prefix_units(g, false);
-  total_b += prefix_units(g, true);
-  // CTAs of the tile items and of the token items
-  const long long G = gridDim.x, cost_a = total_a * g.tile_cost, cost_b = total_b * g.token_cost;
-  long long ca = cost_a + cost_b > 0 ? (G * cost_a + (cost_a + cost_b) / 2) / (cost_a + cost_b) : 0;
-  if (total_a > 0) ca = max(ca, 1LL);
+  Two before = cta_scan(mine, scratch, total);
+  const long long pre_a = prefix_weight(g, false), pre_b = prefix_weight(g, true);
+  const long long total_a = total.a * g.kv_heads + pre_a, total_b = total.b * g.groups + pre_b;
+  // CTAs of the tile items and of the token items, by what their units cost
+  const int G = (int)gridDim.x;
+  const float cost_a = (float)total_a * g.tile_cost, cost_b = (float)total_b * g.token_cost;
+  int ca = cost_a + cost_b > 0.f ? (int)(G * (cost_a / (cost_a + cost_b)) + 0.5f) : 0;
+  if (total_a > 0) ca = max(ca, 1);
   if (total_b > 0) ca = min(ca, G - 1);
-  const long long cb = min(G - ca, total_b);
-  const bool token = blockIdx.x >= ca;
-  ca = min(ca, total_a);
-  Run x;
+  const bool token = (int)blockIdx.x >= ca;
+  Run x{};
   x.token = token;
   x.U = token ? total_b : total_a;
-  // the token items' CTAs are the grid's last ones
-  x.base = token ? (int)(G - cb) : 0;
-  x.ctas = (int)(token ? cb : ca);
-  const long long c = (long long)blockIdx.x - x.base;
-  if (c < 0 || c >= x.ctas) {
-    x.u0 = x.count = 0;
-  } else {
-    x.u0 = x.U * c / x.ctas;
-    x.count = x.U * (c + 1) / x.ctas - x.u0;
-  }
-  x.phase = x.r = x.hk = x.t = x.j = 0;
-  if (x.count > 0) {
-    const long long pre = prefix_units(g, token);
-    if (x.u0 < pre) {
-      if (tid == 0) {
-        const long long head = pre / g.kv_heads, off = x.u0 % head;
-        const int tiles = prefix_part(g, token);
-        x.hk = (int)(x.u0 / head);
-        const long long pairs = token ? tiles : (long long)g.full * tiles;
-        x.t = off < pairs ? (int)(off / tiles) : g.full;
-        x.j = (int)(off < pairs ? off % tiles : off - pairs);
-        *run = x;
-      }
-    } else {
-      long long target = x.u0 - pre;
-      for (int r0 = 0; r0 < R; r0 += kThreads) {
-        units_of(r0 + tid, mine_a, mine_b);
-        const long long mine = token ? mine_b : mine_a;
-        long long total;
-        const long long before = cta_scan(mine, scratch, total);
-        if (before <= target && target < before + mine) {
-          const Request q = load_request(p, r0 + tid);
-          const Items it(g, q, token);
-          const int ptiles = g.concat ? prefix_part(g, token) : 0;
-          long long off = target - before;
-          x.phase = 1;
-          x.r = r0 + tid;
-          x.hk = (int)(off / (mine / g.kv_heads));
-          off -= x.hk * (mine / g.kv_heads);
-          for (;; ++x.t) {
-            const int u = it.units(x.t, it.tiles(g, q, token, x.t, ptiles));
-            if (off < u) break;
-            off -= u;
-          }
-          x.j = (int)off;
-          *run = x;
-        }
-        if (target < total) break;  // the same for all threads
-        target -= total;
-      }
+  // as many workers as units at most, so that none between two others is without any
+  x.workers = (int)min(x.U, (long long)(token ? (G - ca) * g.teams : ca));
+  const int own_runs = token ? g.teams : 1, self0 = token ? (int)(blockIdx.x - ca) * g.teams : (int)blockIdx.x;
+  const int items = token ? g.groups : g.kv_heads;  // of a request (for each pair of row tiles)
+  const long long pre = token ? pre_b : pre_a;
+  auto run_of = [&](int w) {  // the run without its start
+    Run y = x;
+    y.self = self0 + w;
+    if (y.self < x.workers) {
+      y.u0 = mul_div(x.U, y.self, x.workers);
+      y.count = mul_div(x.U, y.self + 1, x.workers) - y.u0;
     }
-  } else if (tid == 0) {
-    *run = x;
+    return y;
+  };
+  if (tid < own_runs) {
+    Run y = run_of(tid);
+    if (y.count > 0 && y.u0 < pre) {
+      const long long head = pre / items;
+      const int each = prefix_part(g, token) + (token ? g.token_item : g.tile_item);
+      y.hk = (int)mul_div(y.u0, 1, head);
+      const long long off = y.u0 - y.hk * head, pairs = token ? each : (long long)g.full * each;
+      y.t = off < pairs ? (int)mul_div(off, 1, each) : g.full;
+      y.j = (int)(off < pairs ? off - (long long)y.t * each : off - pairs);
+    }
+    runs[tid] = y;
+  }
+  __syncthreads();
+  long long base = pre;
+  for (int r0 = 0; r0 < R; r0 += kThreads) {
+    if (R > kThreads) {  // (else this is what was summed above)
+      mine = weights(r0 + tid);
+      before = cta_scan(mine, scratch, total);
+    }
+    const long long head = token ? mine.b : mine.a, from = base + (token ? before.b : before.a) * items;
+    for (int w = 0; head > 0 && w < own_runs; ++w) {
+      const long long u0 = runs[w].u0;
+      if (runs[w].count == 0 || u0 < from || u0 >= from + head * items) continue;
+      const Request q = load_request(p, r0 + tid);
+      const Items it(g, q, token);
+      const int ptiles = g.concat ? prefix_part(g, token) : 0;
+      Run y = runs[w];
+      y.phase = 1;
+      y.r = r0 + tid;
+      y.hk = (int)mul_div(u0 - from, 1, head);
+      long long off = u0 - from - y.hk * head;
+      for (y.t = 0;; ++y.t) {
+        const int u = it.weight(y.t, it.tiles(g, q, token, y.t, ptiles), g, token);
+        if (off < u) break;
+        off -= u;
+      }
+      y.j = (int)off;
+      runs[w] = y;
+    }
+    base += (token ? total.b : total.a) * items;
   }
   __syncthreads();
 }
 
-// Walks the segments (one item each) of a run.
-struct PrefixWalk {
-  const PrefixAttnParams& p;
-  const PrefixGeom& g;
-  bool token;
-  int phase, r, hk, t;
-  long long left, at;  // units left; the sequence's unit that the segment starts with
-  Request q;
-  Items it;
-  int ptiles;
-  int seg, tiles, units, j0, j1;
-  bool lone;
-  __device__ __forceinline__ PrefixWalk(const PrefixAttnParams& p_, const PrefixGeom& g_, const Run& x)
-      : p(p_), g(g_), token(x.token), phase(x.phase), r(x.r), hk(x.hk), t(x.t), left(x.count), at(x.u0), seg(-1), j0(0), j1(x.j) {
-    if (left > 0) set_request();
-  }
-  __device__ __forceinline__ void set_request() {
-    if (phase == 0) {
-      q.q0 = 0, q.n = p.tokens, q.own = 0;
-    } else {
-      q = load_request(p, r);
-    }
-    it = Items(g, q, token);
-    ptiles = phase == 0 || g.concat ? prefix_part(g, token) : 0;
-  }
-  __device__ __forceinline__ bool next() {
-    const int from = j0;
-    j0 = seg < 0 ? j1 : 0;
-    if (left <= 0) return false;
-    if (seg >= 0) {
-      at += j1 - from;
-      if (++t == it.full + it.lone) {
-        t = 0;
-        if (++hk == g.kv_heads) {
-          hk = 0;
-          if (phase == 0) phase = 1, r = -1;
-          for (;;) {
-            if (++r >= p.requests) return false;  // not reached while units are left
-            set_request();
-            if (q.n > 0 && is_token(g, q) == token) break;
-          }
-        }
-      }
-    }
-    ++seg;
-    tiles = it.tiles(g, q, token, t, ptiles);
-    lone = t == it.full;
-    units = it.units(t, tiles);
-    j1 = (int)min((long long)units, j0 + left);
-    left -= j1 - j0;
-    return true;
-  }
+// The worker that weight u falls to.
+__device__ __forceinline__ int worker_of(long long u, const Run& run) {
+  return (int)(((u + 1) * run.workers - 1) / run.U);
+}
+
+// One segment of a run: an item, or the part [j0, j1) of its units.
+struct Segment {
+  int q0, n, own;             // the request's first row, rows, own tokens (phase 0: all rows, none)
+  int r, hk, phase;           // (token items: hk the group of key heads)
+  int ptiles, tiles, units;   // K/V tiles of the prefix, K/V tiles and units in all
+  int j0, j1;
+  int lone, tile0, n_tiles;   // tile items: row tile(s) tile0, tile0 + 1 of n_tiles along the tokens
+  int code;                   // see below
+  int last;                   // 1: no segment, the run's end
   __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == units; }
-  // tile role: K/V tile of row tile w in unit j, and whether it has one
+  // own tokens that row i sees
+  __device__ __forceinline__ int limit(int i) const { return Request{q0, n, own}.limit(i); }
+  // tile items: K/V tile of row tile w in unit j, and whether it has one
   __device__ __forceinline__ int kv_tile(int w, int j) const { return lone ? 2 * j + w : j; }
   __device__ __forceinline__ bool uses(int w, int j) const { return kv_tile(w, j) < tiles; }
   // first token (of the item's rows) and head of row tile w
-  __device__ __forceinline__ void origin(int w, int& n0, int& g0) const {
-    const int tile = lone ? 2 * it.full : 2 * t + w, gi = tile / it.n_tiles;
-    n0 = (tile - gi * it.n_tiles) * g.nt;
+  __device__ __forceinline__ void origin(const PrefixGeom& g, int w, int& n0, int& g0) const {
+    const int tile = tile0 + (lone ? 0 : w), gi = tile / n_tiles;
+    n0 = (tile - gi * n_tiles) * g.nt;
     g0 = gi * g.gt;
   }
-  // Where the parts of the segment's item are: the CTA that starts it writes this for each row.  Bits: the row of
-  // a slot, the first CTA, how many CTAs follow it (0: one had it whole).
-  __device__ __forceinline__ int code(const Run& x, int row) const {
-    if (j1 == units) return row;
-    const long long last = at + units - 1;
-    const int c0 = (int)blockIdx.x, c1 = x.base + (int)(((last + 1) * x.ctas - 1) / x.U);
-    return row | c0 << 8 | (c1 - c0) << 20;
+  // A partial result's slot of this worker
+  __device__ __forceinline__ float* tile_slot(const PrefixGeom& g, const Run& run) const {
+    return g.tile_slots + (size_t)(2 * run.self + (j0 > 0)) * g.tile_rows * g.ld;
   }
-  // A part of the item: its slot in this CTA
-  __device__ __forceinline__ float* slot(const PrefixGeom& gg) const {
-    return gg.slots + (size_t)(2 * blockIdx.x + (j0 > 0)) * gg.slot_rows * gg.ld;
+  __device__ __forceinline__ float* token_slot(const PrefixGeom& g, const Run& run, int h) const {
+    return g.token_slots + (size_t)((2 * run.self + (j0 > 0)) * g.heads + h) * g.token_rows * g.ld;
+  }
+};
+static_assert(sizeof(Segment) == 64, "");
+
+// Where the parts of an item are, written for each of its rows by the worker that starts it.  Bits: the row of a
+// slot (added by the writer), << 8 the first worker (those of tile items from kTileWorkers on), << 20 how many
+// workers follow it (0: one had it whole).
+constexpr int kTileWorkers = 2048;
+
+// Walks the segments of a run.
+struct ItemWalk {
+  const PrefixAttnParams& p;
+  const PrefixGeom& g;
+  const Run& run;
+  int phase, r, hk, t, j, ptiles;
+  long long at, end;
+  Request q, ahead;  // this item's request, and the next one (asked for before it is needed)
+  Items it;
+  __device__ __forceinline__ ItemWalk(const PrefixAttnParams& p_, const PrefixGeom& g_, const Run& x)
+      : p(p_), g(g_), run(x), phase(x.phase), r(x.r), hk(x.hk), t(x.t), j(x.j), at(x.u0), end(x.u0 + x.count) {
+    if (at >= end) return;
+    if (phase == 1) ask(r);
+    set_request();
+  }
+  __device__ __forceinline__ void ask(int i) {
+    if (i < p.requests) ahead = load_request(p, i);
+  }
+  __device__ __forceinline__ void set_request() {
+    const bool token = run.token;
+    if (phase == 0)
+      q.q0 = 0, q.n = p.tokens, q.own = 0;
+    else
+      q = ahead;
+    it = Items(g, q, token);
+    ptiles = phase == 0 || g.concat ? prefix_part(g, token) : 0;
+    ask(phase == 0 ? 0 : r + 1);
+  }
+  // The next segment (x.last: none)
+  __device__ __forceinline__ void next(Segment& x) {
+    const bool token = run.token;
+    for (;;) {
+      x.last = at >= end;
+      if (x.last) return;
+      x.q0 = q.q0, x.n = q.n, x.own = q.own;
+      x.r = r, x.hk = hk, x.phase = phase;
+      x.ptiles = ptiles;
+      x.tiles = it.tiles(g, q, token, t, ptiles);
+      x.units = it.units(t, x.tiles);
+      x.j0 = j;
+      x.j1 = (int)min((long long)x.units, j + (end - at));
+      x.lone = t == it.full;
+      x.tile0 = 2 * t;
+      x.n_tiles = it.n_tiles;
+      x.code = 0;
+      if (j == 0 && x.j1 < x.units) {
+        const int more = worker_of(at + x.units - 1, run) - run.self;
+        x.code = (run.self + (token ? 0 : kTileWorkers)) << 8 | more << 20;
+      }
+      at += it.weight(t, x.tiles, g, token) - j;
+      j = 0;
+      if (at < end && ++t == it.full + it.lone) {
+        t = 0;
+        if (++hk == (token ? g.groups : g.kv_heads)) {
+          hk = 0;
+          if (phase == 0) phase = 1, r = -1;
+          do {
+            if (++r >= p.requests) {  // not reached: weights are left
+              at = end;
+              break;
+            }
+            set_request();
+          } while (q.n == 0 || is_token(g, q) != token);
+        }
+      }
+      if (x.j0 < x.units) return;  // (a run that starts past an item's units has none of it)
+    }
+  }
+};
+
+// Tile items: the segments of a CTA's run in a ring in shared memory: one lane walks the items for all roles (in
+// registers of every role the walk spilled 470 bytes, and local memory has little L1 beside the tiles).
+constexpr int kRing = 4;
+struct SegmentRing {
+  Segment at[kRing];
+  uint64_t full[kRing], empty[kRing];
+  __device__ void init(int readers) {
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], readers);
+    }
+  }
+  // The s-th segment once it is there; a warp's lanes together, or one lane alone
+  __device__ __forceinline__ bool wait_warp(int s, volatile int* abort_flag) {
+    return mbar_wait_warp<false>(&full[s % kRing], s / kRing & 1, kErrTimeoutAttnQ, abort_flag);
+  }
+  __device__ __forceinline__ bool wait(int s, volatile int* abort_flag) {
+    return mbar_wait<false>(&full[s % kRing], s / kRing & 1, kErrTimeoutAttnQ, abort_flag);
+  }
+  // One lane: walks the run
+  __device__ void fill(const PrefixAttnParams& p, const PrefixGeom& g, const Run& run, volatile int* abort_flag) {
+    ItemWalk walk(p, g, run);
+    for (int s = 0;; ++s) {
+      Segment x;
+      walk.next(x);
+      if (!mbar_wait<false>(&empty[s % kRing], (s / kRing & 1) ^ 1, kErrTimeoutAttnQ, abort_flag)) return;
+      at[s % kRing] = x;
+      mbar_arrive(&full[s % kRing]);
+      if (x.last) return;
+    }
   }
 };
 
@@ -369,7 +456,8 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + 2 * C::kTile;
   uint8_t* sV = sK + C::kKSlots * C::kTile;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + C::kVSlots * C::kTile);
+  SegmentRing* ring = reinterpret_cast<SegmentRing*>(smem + C::kTiles);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + 1);
   uint64_t* q_full = bars;
   uint64_t* q_empty = bars + 1;
   uint64_t* s_full = bars + 2;    // [NB buffers]
@@ -387,6 +475,7 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile uint32_t* s_bad = tmem_slot + 2;                 // a bit a segment (mod 32): see warp 2
   float* s_ml = reinterpret_cast<float*>(tmem_slot + 4);    // [2 halves][ref, l][128]
+  static_assert(sizeof(SegmentRing) + (19 + 2 * C::kKSlots + 3 * C::kVSlots) * 8 + 16 + 2048 <= C::kTail, "");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -411,6 +500,7 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
       mbar_init(&v_ready[i], 1);
       mbar_init(&v_empty[i], 1);
     }
+    ring->init(8);  // the softmax warps, which are the last to need a segment
     *abort_flag = 0;
     *s_bad = 0;
     mbar_fence_init();
@@ -422,7 +512,7 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  PrefixWalk k(p, g, run);
+  int s = 0;  // every role walks the segments of the run
 
   if (warp < kSoftmaxWarp0) {
     warpgroup_reg_dec<kFewRegs>();
@@ -436,15 +526,16 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         // K/V tile `tile` of the current item: whole boxes of the prefix (its end is filled with zeros), of
         // the own tokens the boxes that hold any
         auto load_tile = [&](const CUtensorMap& pre, int pre_headed, const CUtensorMap& cache, int cache_headed, uint8_t* dst,
-                             uint64_t* bar, int tile) {
+                             uint64_t* bar, const Segment& k, int tile) {
           if (tile < k.ptiles) {
             mbar_arrive_expect_tx(bar, C::kTile);
             for (int h = 0; h < C::kHalves; ++h)
-              for (int b = 0; b < 2; ++b)
-                tma_load_4d(dst + h * kHalfBytes + b * 8192, &pre, bar, h * 64, tile * 128 + b * 64, k.hk * pre_headed, 0);
+              for (int b = 0; b < 128 / kTokenKeys; ++b)
+                tma_load_4d(dst + h * kHalfBytes + b * kTokenBox, &pre, bar, h * 64, tile * 128 + b * kTokenKeys,
+                            k.hk * pre_headed, 0);
             return;
           }
-          const int key0 = (tile - k.ptiles) * 128, boxes = min(128 / g.box, max(0, (k.q.own - key0 + g.box - 1) / g.box));
+          const int key0 = (tile - k.ptiles) * 128, boxes = min(128 / g.box, max(0, (k.own - key0 + g.box - 1) / g.box));
           mbar_arrive_expect_tx(bar, (uint32_t)(boxes * g.box) * 128u * C::kHalves);
           const int* row = p.table + k.r * p.table_stride;
           for (int b0 = 0; b0 < boxes; b0 += 4) {
@@ -461,16 +552,19 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
             }
           }
         };
-        while (ok && k.next()) {
+        for (; ok; ++s) {
+          if (!(ok = ring->wait(s, abort_flag))) break;
+          const Segment k = ring->at[s % kRing];
+          if (k.last) break;
           if (!(ok = mbar_wait<false>(q_empty, q_phase ^ 1, kErrTimeoutAttnQ, abort_flag))) break;
           q_phase ^= 1;
           const int nq = k.lone ? 1 : 2;
           mbar_arrive_expect_tx(q_full, nq * C::kHalves * (uint32_t)(g.gt * g.nt) * 128u);
           for (int w = 0; w < nq; ++w) {
             int n0, g0;
-            k.origin(w, n0, g0);
+            k.origin(g, w, n0, g0);
             for (int h = 0; h < C::kHalves; ++h)
-              tma_load_4d(sQ + w * C::kTile + h * kHalfBytes, &qmap, q_full, h * 64, g0, k.q.q0 + n0, k.hk);
+              tma_load_4d(sQ + w * C::kTile + h * kHalfBytes, &qmap, q_full, h * 64, g0, k.q0 + n0, k.hk);
           }
           const int streams = k.lone ? 2 : 1;  // K/V tiles of a unit
           // with three buffers S runs ahead of PV by up to two units, so K goes first
@@ -478,13 +572,15 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
           for (int i = k.j0; ok && i < k.j1 + kLead; ++i) {
             for (int w = 0; w < streams && i < k.j1 && k.uses(w, i); ++w) {
               if (!(ok = mbar_wait<false>(&k_empty[kp.slot], kp.phase ^ 1, kErrTimeoutAttnKV, abort_flag))) break;
-              load_tile(pkmap, g.pk_headed, kcmap, g.kc_headed, sK + kp.slot * C::kTile, &k_full[kp.slot], k.kv_tile(w, i));
+              load_tile(pkmap, g.pk_headed, kcmap, g.kc_headed, sK + kp.slot * C::kTile, &k_full[kp.slot], k,
+                        k.kv_tile(w, i));
               kp = kp.plus(1);
             }
             const int v = i - kLead;
             for (int w = 0; ok && w < streams && v >= k.j0 && k.uses(w, v); ++w) {
               if (!(ok = mbar_wait<false>(&v_empty[vp.slot], vp.phase ^ 1, kErrTimeoutAttnKV, abort_flag))) break;
-              load_tile(pvmap, g.pv_headed, vcmap, g.vc_headed, sV + vp.slot * C::kTile, &v_full[vp.slot], k.kv_tile(w, v));
+              load_tile(pvmap, g.pv_headed, vcmap, g.vc_headed, sV + vp.slot * C::kTile, &v_full[vp.slot], k,
+                        k.kv_tile(w, v));
               vp = vp.plus(1);
             }
           }
@@ -510,8 +606,11 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         uint32_t mine[2] = {0, 0}, pmine[2] = {0, 0};  // S and PV issued so far, per tile
         uint32_t seq = 0;           // position in the sequence of the segment's first step
         bool ok = true;
-        while (ok && k.next()) {
-          if (!mbar_wait<false>(q_full, k.seg & 1, kErrTimeoutAttnQ, abort_flag)) break;
+        for (; ok; ++s) {
+          if (!(ok = ring->wait(s, abort_flag))) break;
+          const Segment k = ring->at[s % kRing];
+          if (k.last) break;
+          if (!(ok = mbar_wait<false>(q_full, s & 1, kErrTimeoutAttnQ, abort_flag))) break;
           tc_fence_after();
           const int steps = k.j1 - k.j0;
           // steps of the second tile: all, but for a lone tile's last unit without a K/V tile for it
@@ -581,21 +680,24 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
       // ------------------------------------------------------------ rows that nobody sees, or not all
       VPos vp;
       bool ok = true;
-      while (ok && k.next()) {
+      for (; ok; ++s) {
+        if (!(ok = ring->wait_warp(s, abort_flag))) break;
+        const Segment k = ring->at[s % kRing];
+        if (k.last) break;
         const int streams = k.lone ? 2 : 1;
         uint32_t bad = 0;
         int n0, g0;
-        k.origin(0, n0, g0);
+        k.origin(g, 0, n0, g0);
         // own tokens that every row of the item sees (along the group's tiles the tokens start over)
-        const int common = k.q.limit(g.g_tiles > 1 ? 0 : n0);
-        if (lane == 0) *s_bad = *s_bad & ~(1u << ((k.seg + 16) & 31));  // read by all long ago
+        const int common = k.limit(g.g_tiles > 1 ? 0 : n0);
+        if (lane == 0) *s_bad = *s_bad & ~(1u << ((s + 16) & 31));  // read by all long ago
         for (int j = k.j0; ok && j < k.j1; ++j) {
           for (int w = 0; w < streams && k.uses(w, j); ++w) {
             if (!(ok = mbar_wait_warp<false>(&v_full[vp.slot], vp.phase, kErrTimeoutAttnKV, abort_flag))) break;
             const int tile = k.kv_tile(w, j);
             const bool pre = tile < k.ptiles;
             const int key0 = (pre ? tile : tile - k.ptiles) * 128;
-            const int khi = (pre ? p.prefix : k.q.own) - key0, klo = pre ? khi : common - key0;
+            const int khi = (pre ? p.prefix : k.own) - key0, klo = pre ? khi : common - key0;
             uint8_t* tile_at = sV + vp.slot * C::kTile;
             if (khi < 128) {
               // a lane's row, its pieces in an order that keeps the lanes on different banks
@@ -621,7 +723,7 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
               }
               if (__any_sync(0xffffffffu, found) && !bad) {
                 bad = 1;
-                if (lane == 0) *s_bad = *s_bad | 1u << (k.seg & 31);
+                if (lane == 0) *s_bad = *s_bad | 1u << (s & 31);
               }
             }
             if (lane == 0) mbar_arrive(&v_ready[vp.slot]);
@@ -629,6 +731,8 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
           }
         }
       }
+    } else if (lane == 0) {
+      ring->fill(p, g, run, abort_flag);
     }
   } else {
     warpgroup_reg_inc<kSoftmaxRegs>();
@@ -641,13 +745,16 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
     uint32_t mine = 0, seq = 0;  // this tile's steps so far; sequence position of the segment
     uint32_t meets = 0;
     bool ok = true;
-    while (ok && k.next()) {
+    for (;; ++s) {
+      if (!ring->wait_warp(s, abort_flag)) break;
+      const Segment& k = ring->at[s % kRing];
+      if (k.last) break;
       int n0, g0;
-      k.origin(w, n0, g0);
+      k.origin(g, w, n0, g0);
       const int rn = row / g.gt, n = n0 + rn, head = g0 + row - rn * g.gt;
-      const bool valid = rn < g.nt && n < k.q.n && head < g.group;
+      const bool valid = rn < g.nt && n < k.n && head < g.group;
       const bool warp_active = __any_sync(0xffffffffu, valid);
-      const int limit = valid ? k.q.limit(n) : k.q.own;  // own tokens that the row sees
+      const int limit = valid ? k.limit(n) : k.own;  // own tokens that the row sees
       float ref = 0.f, l = 0.f;
       bool have = false;  // the reference is set
       const int all_steps = k.j1 - k.j0, steps1 = k.uses(1, k.j1 - 1) ? all_steps : all_steps - 1;
@@ -732,9 +839,9 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
       }
       if (!ok) break;
       seq += (uint32_t)(all_steps + steps1);
-      if (!mbar_wait_warp<false>(&o_done[w], k.seg & 1, kErrTimeoutAttnO, abort_flag)) break;
+      if (!mbar_wait_warp<false>(&o_done[w], s & 1, kErrTimeoutAttnO, abort_flag)) break;
       tc_fence_after();
-      const bool bad = *s_bad >> (k.seg & 31) & 1;
+      const bool bad = *s_bad >> (s & 31) & 1;
       // a lone tile: the two halves meet, weigh each other in and write half the columns each
       float a0 = 1.f, a1 = 0.f;
       int c_lo = 0, c_hi = p.head_dim;
@@ -774,12 +881,12 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
       const float inv = finish ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
       const float f0 = a0 * inv, f1 = a1 * inv;
       if (warp_active) {
-        const size_t grow = (size_t)(k.q.q0 + n) * p.q.heads + (size_t)(k.hk * g.group + head);
+        const size_t grow = (size_t)(k.q0 + n) * p.q.heads + (size_t)(k.hk * g.group + head);
         const size_t plane = (size_t)p.tokens * p.q.heads * k.phase;
-        T* out = static_cast<T*>(p.out.data) + (k.q.q0 + n) * p.out.seq_stride +
+        T* out = static_cast<T*>(p.out.data) + (k.q0 + n) * p.out.seq_stride +
                  (long long)(k.hk * g.group + head) * p.out.head_stride;
         const int at = (k.lone ? 0 : w * 128) + row;
-        float* po = whole ? g.whole + (plane + grow) * g.ld : k.slot(g) + (size_t)at * g.ld;
+        float* po = whole ? g.whole + (plane + grow) * g.ld : k.tile_slot(g, run) + (size_t)at * g.ld;
         for (int c0 = c_lo; c0 < c_hi; c0 += 16) {
           uint32_t r0[16], r1[16];
           tmem_ld16(src0 + c0, r0);
@@ -807,7 +914,7 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         }
         if (valid && (!k.lone || w == 0)) {
           if (!finish) *reinterpret_cast<float4*>(po + p.head_dim) = make_float4(ref, l, bad ? 1.f : 0.f, 0.f);
-          if (k.j0 == 0) g.where[plane + grow] = finish && bad ? kRecompute : k.code(run, at);
+          if (k.j0 == 0) g.where[plane + grow] = finish && bad ? kRecompute : k.code | at;
         }
       }
       tc_fence_before();
@@ -818,6 +925,8 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         if (!mbar_wait_warp<false>(&meet[q], meets & 1, kErrTimeoutAttnO, abort_flag)) break;
         ++meets;
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring->empty[s % kRing]);
     }
   }
 
@@ -829,172 +938,209 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
 }
 
 // ------------------------------------------------------------------------------- token items
-// 16-byte piece `chunk` (8 columns) of key `row` in a 128B-swizzled tile of 64-column boxes
-__device__ __forceinline__ uint32_t token_piece(uint32_t tile, int row, int chunk) {
-  return tile + (uint32_t)((chunk >> 3) * kTokenBox + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+// A team takes up to 8 key heads of a request as one item, a warp a head: K and V of 32 keys of all its heads
+// come by one TMA box (64 columns x 32 keys x heads), so that what lies side by side in the cache is read together,
+// and each warp multiplies them by its head's 16 rows and writes its parts from its registers; no warp waits for
+// another.  With fewer key heads a CTA has up to four teams with runs of their own.  A warp a team
+// brings the tiles, K and V in turn through one ring.
+// Measured on the way (64 requests of up to 1024 own tokens, 8 key heads of 128, without a prefix): tiles of one
+// head shared out over eight warps that met at each item's end, 42 us; a run for each warp, which asked for
+// its own tiles, 62.
+// 16-byte piece `chunk` (8 columns) of row `row` in a 128B-swizzled tile of 64-column boxes of `box` bytes
+__device__ __forceinline__ uint32_t token_piece(uint32_t tile, uint32_t box, int row, int chunk) {
+  return tile + (uint32_t)(chunk >> 3) * box + (uint32_t)(row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
+struct Team {  // in shared memory
+  Segment seg[2];
+  uint64_t seg_full[2], seg_empty[2], full[kMostEntries], empty[kMostEntries], q_full[2], q_empty[2];
+  int abort, pad;
+};
+
 template <typename T, int DP>
-__device__ void token_role(uint8_t* smem, const CUtensorMap& pkmap, const CUtensorMap& pvmap, const CUtensorMap& kcmap,
-                           const CUtensorMap& vcmap, const PrefixAttnParams& p, const PrefixGeom& g, const Run& run) {
+__device__ void token_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensorMap& pkmap, const CUtensorMap& pvmap,
+                           const CUtensorMap& kcmap, const CUtensorMap& vcmap, const PrefixAttnParams& p,
+                           const PrefixGeom& g, const Run* runs) {
   using C = PCfg<DP>;
   constexpr int kHalves = C::kHalves;
-  constexpr uint32_t kStage = C::kStage;
-  const int stages = g.stages;
-  float* s_o = reinterpret_cast<float*>(smem + (size_t)stages * kStage);  // [warps][rows][DP]
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kSmem - C::kTail);
-  uint64_t* empty = full + kMaxStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kMaxStages);
-  int* s_stop = const_cast<int*>(abort_flag) + 1;
-  volatile int* s_bad = abort_flag + 2;  // [2]: by the parity of the segment
-  float(*s_m)[16] = reinterpret_cast<float(*)[16]>(const_cast<int*>(abort_flag) + 4);
-  float(*s_l)[16] = s_m + kTokenWarps;
-
+  static_assert(kMostTeams * sizeof(Team) <= C::kTail, "");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < stages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 4);
+  const int team = warp < kTokenWarps ? warp / g.heads : warp - kTokenWarps, h = warp - team * g.heads;
+  Team* tm = reinterpret_cast<Team*>(smem + C::kTiles) + team;
+  volatile int* abort_flag = &tm->abort;
+  Run run{};
+  if (team < g.teams) run = runs[team];
+  __syncthreads();  // the runs have been read
+  if (threadIdx.x < g.teams) {
+    Team* x = reinterpret_cast<Team*>(smem + C::kTiles) + threadIdx.x;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&x->seg_full[i], 1);
+      mbar_init(&x->seg_empty[i], g.heads);
+      mbar_init(&x->q_full[i], 1);
+      mbar_init(&x->q_empty[i], g.heads);
     }
-    *abort_flag = 0;
-    s_bad[0] = s_bad[1] = 0;
+    for (int i = 0; i < g.entries; ++i) {
+      mbar_init(&x->full[i], 1);
+      mbar_init(&x->empty[i], g.heads);
+    }
+    x->abort = 0;
     mbar_fence_init();
   }
   __syncthreads();
-  if (warp > kTokenWarps) return;
-  PrefixWalk k(p, g, run);
+  if (team >= g.teams || run.count == 0) return;
+  const uint32_t entry_bytes = (uint32_t)g.heads * C::kEntry, half_bytes = (uint32_t)g.heads * kTokenBox;
+  const uint32_t q_half = (uint32_t)(g.heads * g.q_rows) * 128u;
+  uint8_t* tiles = smem + (size_t)team * g.entries * entry_bytes;
+  uint8_t* sQ = smem + (size_t)g.teams * g.entries * entry_bytes + (size_t)team * g.q_slots * kHalves * q_half;
 
-  if (warp == kTokenWarps) {
-    if (lane == 0) {
-      int st = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      // pages of tile j's boxes, asked for a tile ahead
-      auto pages_of = [&](int j, int (&page)[4]) {
-        const int key0 = (j - k.ptiles) * kTokenKeys;
-        const int* row = p.table + k.r * p.table_stride;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          page[i] = key0 >= 0 && i * g.box < kTokenKeys && key0 + i * g.box < k.q.own
-                        ? __ldg(row + ((key0 + i * g.box) >> p.page_shift))
-                        : 0;
-      };
-      while (ok && k.next()) {
-        int page[4], ahead[4];
-        pages_of(k.j0, page);
-        for (int j = k.j0; j < k.j1; ++j) {
-          pages_of(j + 1, ahead);
-          if (!mbar_wait<false>(&empty[st], phase ^ 1, kErrTimeoutAttnKV, abort_flag)) {
-            ok = false;
-            break;
+  if (warp >= kTokenWarps) {
+    // ------------------------------------------------------------ the team's tiles
+    ItemWalk walk(p, g, run);
+    int s = 0, e = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (;; ++s) {
+      Segment x;
+      walk.next(x);
+      if (!(ok = mbar_wait_warp<false>(&tm->seg_empty[s & 1], (s >> 1 & 1) ^ 1, kErrTimeoutAttnQ, abort_flag))) break;
+      if (lane == 0) {
+        tm->seg[s & 1] = x;
+        mbar_arrive(&tm->seg_full[s & 1]);
+      }
+      if (x.last) break;
+      const int head0 = x.hk * g.heads, qs = s % g.q_slots, q_use = s / g.q_slots;
+      if (!(ok = mbar_wait_warp<false>(&tm->q_empty[qs], (q_use & 1) ^ 1, kErrTimeoutAttnQ, abort_flag))) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&tm->q_full[qs], (uint32_t)(g.heads * (g.q_rows / g.group) * g.group) * 128u * kHalves);
+        for (int i = 0; i < kHalves; ++i)
+          tma_load_4d(sQ + (qs * kHalves + i) * q_half, &qmap, &tm->q_full[qs], i * 64, 0, x.q0, head0);
+      }
+      int table0 = -32, pages = 0;  // of the request's block table: entries [table0, table0 + 32), a lane each
+      for (int j = x.j0; ok && j < x.j1; ++j) {
+        int first = 0, second = 0, boxes = 1, at = 0;
+        if (j >= x.ptiles) {
+          const int key0 = (j - x.ptiles) * kTokenKeys, left = x.own - key0, block = key0 >> p.page_shift;
+          if (block + (kTokenKeys >> 4) > table0 + 32) {
+            table0 = block;
+            pages = block + lane < p.blocks ? __ldg(p.table + x.r * p.table_stride + block + lane) : 0;
           }
-          uint8_t* dst = smem + (size_t)st * kStage;
-          if (j < k.ptiles) {
-            mbar_arrive_expect_tx(&full[st], kStage);
-            for (int h = 0; h < kHalves; ++h) {
-              tma_load_4d(dst + h * kTokenBox, &pkmap, &full[st], h * 64, j * kTokenKeys, k.hk * g.pk_headed, 0);
-              tma_load_4d(dst + (kHalves + h) * kTokenBox, &pvmap, &full[st], h * 64, j * kTokenKeys, k.hk * g.pv_headed, 0);
-            }
-          } else {
-            const int key0 = (j - k.ptiles) * kTokenKeys;
-            const int boxes = min(kTokenKeys / g.box, max(0, (k.q.own - key0 + g.box - 1) / g.box));
-            mbar_arrive_expect_tx(&full[st], (uint32_t)(boxes * g.box) * 128u * 2 * kHalves);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (i >= boxes) break;
-              const int at = (key0 + i * g.box) & ((1 << p.page_shift) - 1), id = checked_page(p, page[i]);
-              uint8_t* to = dst + i * g.box * 128;
-              for (int h = 0; h < kHalves; ++h) {
-                tma_load_4d(to + h * kTokenBox, &kcmap, &full[st], h * 64, at, k.hk * g.kc_headed, id);
-                tma_load_4d(to + (kHalves + h) * kTokenBox, &vcmap, &full[st], h * 64, at, k.hk * g.vc_headed, id);
+          first = __shfl_sync(0xffffffffu, pages, block - table0);
+          second = __shfl_sync(0xffffffffu, pages, block + 1 - table0);  // (of a tile of two pages)
+          boxes = left <= 0 ? 0 : (left > g.box ? kTokenKeys / g.box : 1);
+          at = key0 & ((1 << p.page_shift) - 1);
+        }
+        for (int v = 0; v < 2; ++v) {
+          if (!(ok = mbar_wait_warp<false>(&tm->empty[e], phase ^ 1, kErrTimeoutAttnKV, abort_flag))) break;
+          if (lane == 0) {
+            uint64_t* bar = &tm->full[e];
+            uint8_t* dst = tiles + e * entry_bytes;
+            if (j < x.ptiles) {
+              mbar_arrive_expect_tx(bar, entry_bytes);
+              for (int i = 0; i < kHalves; ++i)
+                tma_load_4d(dst + i * half_bytes, v ? &pvmap : &pkmap, bar, i * 64, j * kTokenKeys,
+                            head0 * (v ? g.pv_headed : g.pk_headed), 0);
+            } else if (boxes == 0) {
+              mbar_arrive(bar);
+            } else {
+              // (a page of 16 keys is a box of its own, heads side by side in each: see the row that a key has)
+              mbar_arrive_expect_tx(bar, (uint32_t)(boxes * g.box * g.heads) * 128u * kHalves);
+              for (int b = 0; b < boxes; ++b) {
+                const int id = checked_page(p, b ? second : first);
+                for (int i = 0; i < kHalves; ++i)
+                  tma_load_4d(dst + i * half_bytes + b * g.box * g.heads * 128, v ? &vcmap : &kcmap, bar, i * 64, at,
+                              head0 * (v ? g.vc_headed : g.kc_headed), id);
               }
             }
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) page[i] = ahead[i];
-          if (++st == stages) st = 0, phase ^= 1;
+          __syncwarp();
+          if (++e == g.entries) e = 0, phase ^= 1;
         }
       }
-      mbar_drain_ring(full, stages, st, phase);
+      if (!ok) break;
+    }
+    if (!ok && lane == 0) {  // nothing is given up under copies in flight
+      mbar_drain_ring(tm->full, g.entries, e, phase);
+      mbar_drain_ring(tm->q_full, g.q_slots, s % g.q_slots, s / g.q_slots & 1);
     }
     return;
   }
 
-  const int set = warp >> 2, wk = warp & 3;  // tiles of this parity; 16 keys of each
-  const int qr = lane >> 2, qc = lane & 3;   // fragment row (and row + 8) and column pair
+  const int qr = lane >> 2, qc = lane & 3;  // fragment row (and row + 8) and column pair
   const float c = p.scale_log2;
-  const uint32_t base = smem_u32(smem);
-  // ldmatrix row addresses: K wants (keys 0-7, 8 columns), (keys 0-7, next 8), (keys 8-15, ..) x 2;
-  // V (transposed) wants (keys 0-7), (keys 8-15) of 8 columns, then of the next 8
-  const int krow = wk * 16 + (lane & 7) + ((lane >> 4) << 3), kchunk = (lane >> 3) & 1;
-  const int vrow = wk * 16 + (lane & 15), vchunk = lane >> 4;
-  int st = 0;
+  const uint32_t base = smem_u32(tiles), base_q = smem_u32(sQ);
+  // ldmatrix row addresses: Q wants (rows 0-7, 8 columns), (rows 8-15, ..), then the next 8 columns of both; K
+  // (keys 0-7, 8 columns), (keys 0-7, next 8), (keys 8-15, ..) x 2; V (transposed) (keys 0-7), (keys 8-15)
+  // of 8 columns, then of the next 8
+  const int krow = (lane & 7) + ((lane >> 4) << 3), kchunk = (lane >> 3) & 1;
+  const int vrow = lane & 15, vchunk = lane >> 4;
+  const int q_box = g.q_rows / g.group * g.group;  // rows of a head
+  int at = 0;  // the entry to wait for and the parity of its use
   uint32_t phase = 0;
   bool ok = true;
-  while (ok && k.next()) {
-    const int rows = k.q.n * g.group;
-    // Q fragments of the rows r = n * group + head of the group, from global memory
+  for (int s = 0; ok; ++s) {
+    if (!mbar_wait_warp<false>(&tm->seg_full[s & 1], s >> 1 & 1, kErrTimeoutAttnQ, abort_flag)) break;
+    const Segment& k = tm->seg[s & 1];
+    if (k.last) break;
     uint32_t qa[DP / 16][4];
-    int limit[2];  // own tokens that the fragment's two rows see
-    {
-      const T* qp = static_cast<const T*>(p.q.data) + k.q.q0 * p.q.seq_stride +
-                    (long long)k.hk * g.group * p.q.head_stride;
+    const int qs = s % g.q_slots;
+    if (!mbar_wait_warp<false>(&tm->q_full[qs], s / g.q_slots & 1, kErrTimeoutAttnQ, abort_flag)) break;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = qr + 8 * half, n = r / g.group, h = r - n * g.group;
-        const T* row = qp + (long long)n * p.q.seq_stride + (long long)h * p.q.head_stride;
-        limit[half] = r < rows ? k.q.limit(n) : k.q.own;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-          const int c0 = s * 16 + qc * 2;
-          qa[s][half] = r < rows && c0 < p.head_dim ? *reinterpret_cast<const uint32_t*>(row + c0) : 0u;
-          qa[s][2 + half] = r < rows && c0 + 8 < p.head_dim ? *reinterpret_cast<const uint32_t*>(row + c0 + 8) : 0u;
-        }
-      }
-    }
+    for (int i = 0; i < DP / 16; ++i)  // (rows past the head's are another's, whose results nobody reads)
+      ldmatrix4(token_piece(base_q + qs * kHalves * q_half, q_half, h * q_box + (vrow & (g.q_rows - 1)), 2 * i + vchunk), qa[i]);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tm->q_empty[qs]);
+    const int rows = k.n * g.group, j1 = k.j1, ptiles = k.ptiles, own = k.own;
+    // own tokens that the fragment's two rows see, and that every row sees
+    const int limit[2] = {qr < rows ? k.limit(qr / g.group) : own, qr + 8 < rows ? k.limit((qr + 8) / g.group) : own};
+    const int common = k.limit(0);
     float o[DP / 8][4];
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const int common = k.q.limit(0);
     bool bad = false;
-    for (int jj = k.j0; jj < k.j1; ++jj) {
-      const int stage = st;
-      const uint32_t par = phase;
-      if (++st == stages) st = 0, phase ^= 1;
-      if ((stage & 1) != set) continue;
-      if (!mbar_wait_warp<false>(&full[stage], par, kErrTimeoutAttnKV, abort_flag)) {
-        ok = false;
-        break;
-      }
-      const uint32_t kt = base + (uint32_t)stage * kStage, vt = kt + kHalves * kTokenBox;
-      // S: two column tiles of 8 keys; even and odd k-steps in accumulators of their own
-      float sc[2][2][4];
+    for (int jj = k.j0; jj < j1; ++jj) {
+      if (!(ok = mbar_wait_warp<false>(&tm->full[at], phase, kErrTimeoutAttnKV, abort_flag))) break;
+      const bool pre = jj < ptiles;
+      // Where a key's row is: in a box of 32 keys, head by head, or (16 keys a page) in two of 16, head by head in each
+      const bool split = !pre && g.box < kTokenKeys;
+      const int row0 = split ? h * 16 : h * 32, row16 = split ? g.heads * 16 : 16;
+      const uint32_t kt = base + at * entry_bytes;
+      float sc[4][4];  // four column tiles of 8 keys
 #pragma unroll
-      for (int i = 0; i < 16; ++i) (&sc[0][0][0])[i] = 0.f;
+      for (int i = 0; i < 16; ++i) (&sc[0][0])[i] = 0.f;
 #pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        uint32_t b[4];
-        ldmatrix4(token_piece(kt, krow, 2 * s + kchunk), b);
-        mma16816<T>(sc[s & 1][0], qa[s], b[0], b[1]);
-        mma16816<T>(sc[s & 1][1], qa[s], b[2], b[3]);
-      }
-      // of this warp's 16 keys: the first khi are there, the first klo are seen by every row
-      const bool pre = jj < k.ptiles;
-      const int key0 = (pre ? jj : jj - k.ptiles) * kTokenKeys + wk * 16;
-      const int khi = (pre ? p.prefix : k.q.own) - key0, klo = pre ? khi : common - key0;
-      const bool all = klo >= 16;
-      const int lim[2] = {pre ? khi : limit[0] - key0, pre ? khi : limit[1] - key0};
-      float e[2][4];
-      float mx[2] = {-INFINITY, -INFINITY};
+      for (int x = 0; x < DP / 16; ++x) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // i: row half * 2 + key of the pair
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const float x = (sc[0][t][i] + sc[1][t][i]) * c;
-          e[t][i] = all || 8 * t + qc * 2 + (i & 1) < lim[i >> 1] ? x : -INFINITY;
-          mx[i >> 1] = fmaxf(mx[i >> 1], e[t][i]);
+        for (int y = 0; y < 2; ++y) {
+          uint32_t b[4];
+          ldmatrix4(token_piece(kt, half_bytes, row0 + y * row16 + krow, 2 * x + kchunk), b);
+          mma16816<T>(sc[2 * y], qa[x], b[0], b[1]);
+          mma16816<T>(sc[2 * y + 1], qa[x], b[2], b[3]);
         }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tm->empty[at]);
+      if (++at == g.entries) at = 0, phase ^= 1;
+      // of the tile's 32 keys: the first khi are there, the first klo are seen by every row
+      const int key0 = (pre ? jj : jj - ptiles) * kTokenKeys;
+      const int khi = (pre ? p.prefix : own) - key0, klo = pre ? khi : common - key0;
+      const bool all = klo >= kTokenKeys;
+      float mx[2] = {-INFINITY, -INFINITY};
+      if (!all) {
+        const int lim[2] = {(pre ? khi : limit[0] - key0) - qc * 2, (pre ? khi : limit[1] - key0) - qc * 2};
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)  // i: row half * 2 + key of the pair
+            sc[t][i] = 8 * t + (i & 1) < lim[i >> 1] ? sc[t][i] * c : -INFINITY;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) (&sc[0][0])[i] *= c;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[h] = fmax3(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]),
+                      fmax3(sc[2][2 * h], sc[2][2 * h + 1], fmaxf(sc[3][2 * h], sc[3][2 * h + 1])));
       }
       float alpha[2], ref[2];
       bool moved = false;
@@ -1005,14 +1151,10 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& pkmap, const CUtens
         const float mn = fmaxf(m[h], mx[h]);
         ref[h] = mn == -INFINITY ? 0.f : mn;  // no kept key yet: exponentials of -inf stay 0
         alpha[h] = fast_exp2(m[h] - ref[h]);
+        ref[h] -= kLift<T>;
         moved |= mn > m[h];
         m[h] = mn;
       }
-      uint32_t pa[4];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[t][i] = fast_exp2(e[t][i] - (ref[i >> 1] - kLift<T>));
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) l[h] *= alpha[h];
@@ -1024,119 +1166,107 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& pkmap, const CUtens
           o[i][3] *= alpha[1];
         }
       }
+      uint32_t pa[2][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) l[h] += (e[0][2 * h] + e[0][2 * h + 1]) + (e[1][2 * h] + e[1][2 * h + 1]);
-      pa[0] = pack2<T>(e[0][0], e[0][1]);
-      pa[1] = pack2<T>(e[0][2], e[0][3]);
-      pa[2] = pack2<T>(e[1][0], e[1][1]);
-      pa[3] = pack2<T>(e[1][2], e[1][3]);
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[t][i] = fast_exp2(sc[t][i] - ref[i >> 1]);
+        pa[t >> 1][2 * (t & 1)] = pack2<T>(sc[t][0], sc[t][1]);
+        pa[t >> 1][2 * (t & 1) + 1] = pack2<T>(sc[t][2], sc[t][3]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        l[h] += ((sc[0][2 * h] + sc[0][2 * h + 1]) + (sc[1][2 * h] + sc[1][2 * h + 1])) +
+                ((sc[2][2 * h] + sc[2][2 * h + 1]) + (sc[3][2 * h] + sc[3][2 * h + 1]));
       // keys that are not there: their V is taken as zero (0 * NaN would reach the sum)
-      const int k0 = qc * 2;
-      const uint32_t v0 = (k0 < khi ? 0xffffu : 0u) | (k0 + 1 < khi ? 0xffff0000u : 0u);
-      const uint32_t v1 = (k0 + 8 < khi ? 0xffffu : 0u) | (k0 + 9 < khi ? 0xffff0000u : 0u);
-      const bool ask = klo < min(khi, 16);  // keys that some rows see and others do not
+      uint32_t keep[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        keep[i] = (8 * i + qc * 2 < khi ? 0xffffu : 0u) | (8 * i + qc * 2 + 1 < khi ? 0xffff0000u : 0u);
+      const bool some = klo < min(khi, kTokenKeys);  // keys that some rows see and others do not
+      if (!(ok = mbar_wait_warp<false>(&tm->full[at], phase, kErrTimeoutAttnKV, abort_flag))) break;
+      const uint32_t vt = base + at * entry_bytes;
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
-        uint32_t b[4];
-        ldmatrix4_trans(token_piece(vt, vrow, 2 * i + vchunk), b);
-        if (!all) {
-          b[0] &= v0;
-          b[1] &= v1;
-          b[2] &= v0;
-          b[3] &= v1;
-          if (ask)
-            bad |= any_non_finite<T>(b[0]) || any_non_finite<T>(b[1]) || any_non_finite<T>(b[2]) || any_non_finite<T>(b[3]);
-        }
         // a tile's products in accumulators of their own, added in fp32 (see cross_token.cu)
         float d[2][4] = {};
-        mma16816<T>(d[0], pa, b[0], b[1]);
-        mma16816<T>(d[1], pa, b[2], b[3]);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          uint32_t b[4];
+          ldmatrix4_trans(token_piece(vt, half_bytes, row0 + y * row16 + vrow, 2 * i + vchunk), b);
+          if (!all) {
+            b[0] &= keep[2 * y];
+            b[1] &= keep[2 * y + 1];
+            b[2] &= keep[2 * y];
+            b[3] &= keep[2 * y + 1];
+            if (some)
+              bad |= any_non_finite<T>(b[0]) || any_non_finite<T>(b[1]) || any_non_finite<T>(b[2]) || any_non_finite<T>(b[3]);
+          }
+          mma16816<T>(d[0], pa[y], b[0], b[1]);
+          mma16816<T>(d[1], pa[y], b[2], b[3]);
+        }
 #pragma unroll
         for (int x = 0; x < 8; ++x) o[2 * i + (x >> 2)][x & 3] += d[x >> 2][x & 3];
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[stage]);
+      if (lane == 0) mbar_arrive(&tm->empty[at]);
+      if (++at == g.entries) at = 0, phase ^= 1;
     }
-    if (!ok) *abort_flag = 1;
-    if (bad) s_bad[k.seg & 1] = 1;
-    // join the eight warps
+    if (!ok) break;
+    bad = __any_sync(0xffffffffu, bad);
+    const bool whole = k.j0 == 0 && j1 == k.units, finish = whole && g.concat;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      const int r = qr + 8 * h;
-      if (r < rows) {
-        if (qc == 0) {
-          s_m[warp][r] = m[h];
-          s_l[warp][r] = l[h];
-        }
-        float* so = s_o + ((size_t)warp * rows + r) * DP + qc * 2;
+    for (int half = 0; half < 2; ++half) {
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+      const int r = qr + 8 * half;
+      if (r >= rows) continue;
+      const int n = r / g.group, head = (k.hk * g.heads + h) * g.group + r - n * g.group;
+      const size_t grow = (size_t)p.tokens * p.q.heads * k.phase + (size_t)(k.q0 + n) * p.q.heads + head;
+      if (finish) {
+        const float inv = l[half] > 0.f ? 1.f / l[half] : (l[half] == 0.f ? 0.f : l[half]);
+        T* out = static_cast<T*>(p.out.data) + (k.q0 + n) * p.out.seq_stride + (long long)head * p.out.head_stride + qc * 2;
 #pragma unroll
         for (int i = 0; i < DP / 8; ++i)
-          *reinterpret_cast<float2*>(so + i * 8) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
-      }
-    }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    // one reading for all: the producer may set the flag while they read it
-    if (threadIdx.x == 0) *s_stop = *abort_flag;
-    const bool item_bad = s_bad[k.seg & 1] != 0;
-    if (threadIdx.x == 0) s_bad[(k.seg + 1) & 1] = 0;
-    const bool whole = k.whole(), finish = whole && g.concat;
-    for (int x = threadIdx.x; x < rows * (p.head_dim / 4); x += 256) {
-      const int r = x / (p.head_dim / 4), col = (x - r * (p.head_dim / 4)) * 4;
-      float mm = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kTokenWarps; ++i) mm = fmaxf(mm, s_m[i][r]);
-      float ls = 0.f;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < kTokenWarps; ++i) {
-        if (s_l[i][r] == 0.f) continue;
-        const float f = fast_exp2(s_m[i][r] - mm);
-        const float4 v = *reinterpret_cast<const float4*>(s_o + ((size_t)i * rows + r) * DP + col);
-        ls += s_l[i][r] * f;
-        sum = make_float4(sum.x + v.x * f, sum.y + v.y * f, sum.z + v.z * f, sum.w + v.w * f);
-      }
-      const int n = r / g.group, h = k.hk * g.group + r - n * g.group;
-      const size_t grow = (size_t)p.tokens * p.q.heads * k.phase + (size_t)(k.q.q0 + n) * p.q.heads + h;
-      if (finish) {
-        const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);
-        T* out = static_cast<T*>(p.out.data) + (k.q.q0 + n) * p.out.seq_stride + (long long)h * p.out.head_stride + col;
-        *reinterpret_cast<uint2*>(out) =
-            make_uint2(pack2<T>(sum.x * inv, sum.y * inv), pack2<T>(sum.z * inv, sum.w * inv));
+          if (8 * i < p.head_dim) *reinterpret_cast<uint32_t*>(out + 8 * i) = pack2<T>(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
       } else {
-        float* po = whole ? g.whole + grow * g.ld : k.slot(g) + (size_t)r * g.ld;
-        *reinterpret_cast<float4*>(po + col) = sum;
+        float* po = whole ? g.whole + grow * g.ld : k.token_slot(g, run, h) + (size_t)r * g.ld;
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i)
+          if (8 * i < p.head_dim) *reinterpret_cast<float2*>(po + 8 * i + qc * 2) = make_float2(o[i][2 * half], o[i][2 * half + 1]);
         // the sums are taken against the maximum less kLift
-        if (col == 0)
-          *reinterpret_cast<float4*>(po + p.head_dim) = make_float4(mm - kLift<T>, ls, item_bad ? 1.f : 0.f, 0.f);
+        if (qc == 0)
+          *reinterpret_cast<float4*>(po + p.head_dim) = make_float4(m[half] - kLift<T>, l[half], bad ? 1.f : 0.f, 0.f);
       }
-      if (col == 0 && k.j0 == 0) g.where[grow] = finish && item_bad ? kRecompute : k.code(run, r);
+      if (qc == 0 && k.j0 == 0) g.where[grow] = finish && bad ? kRecompute : k.code | r;
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    ok = *s_stop == 0;  // not written again before all have been at the next item's first barrier
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tm->seg_empty[s & 1]);
   }
 }
 
+// Tensor maps: of the tile items' query rows, K and V of one head; of the token items', of a team's heads.
+struct Maps {
+  CUtensorMap q, pk, pv, kc, vc;
+};
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-    prefix_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap pkmap,
-                            const __grid_constant__ CUtensorMap pvmap, const __grid_constant__ CUtensorMap kcmap,
-                            const __grid_constant__ CUtensorMap vcmap, const __grid_constant__ PrefixAttnParams p,
-                            const __grid_constant__ PrefixGeom g) {
+    prefix_attention_kernel(const __grid_constant__ Maps tile, const __grid_constant__ Maps token,
+                            const __grid_constant__ PrefixAttnParams p, const __grid_constant__ PrefixGeom g) {
   extern __shared__ __align__(1024) uint8_t smem[];  // the swizzled tiles start on 1024 bytes
-  // the run is found in memory that the roles take over
-  long long* scratch = reinterpret_cast<long long*>(smem);
-  Run* s_run = reinterpret_cast<Run*>(smem + 1024);
-  find_run(p, g, s_run, scratch);
-  const Run run = *s_run;
-  __syncthreads();
+  // the runs are found in memory that the roles take over
+  Two* scratch = reinterpret_cast<Two*>(smem);
+  Run* runs = reinterpret_cast<Run*>(smem + 1024);
+  find_runs(p, g, runs, scratch);
   dependents_may_start();
-  if (run.count == 0) return;
-  if (run.token)
-    token_role<T, DP>(smem, pkmap, pvmap, kcmap, vcmap, p, g, run);
-  else
-    tile_role<T, DP>(smem, qmap, pkmap, pvmap, kcmap, vcmap, p, g, run);
+  if (runs[0].token) {
+    token_role<T, DP>(smem, token.q, token.pk, token.pv, token.kc, token.vc, p, g, runs);
+  } else {
+    const Run run = runs[0];
+    __syncthreads();
+    if (run.count > 0) tile_role<T, DP>(smem, tile.q, tile.pk, tile.pv, tile.kc, tile.vc, p, g, run);
+  }
 }
 
 // ------------------------------------------------------------------------------- joining
@@ -1197,81 +1327,120 @@ __device__ __forceinline__ int request_of(const PrefixAttnParams& p, int token) 
   return lo < p.requests && first_row(p, lo) <= token ? lo : -1;
 }
 
-// Adds up the parts of each row, in the order of its keys: the prefix's and the own ones (kRows = 1, a warp a
-// row), or, of one sequence of both, those of the rows that a run cut (kRows = 32 rows a warp are looked
-// through; the others are done).  4 columns a lane, up to kAhead parts in flight.
+// What a row's parts have added up to: reference, sum and 4 columns a lane.
+struct Sum {
+  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float pm, float pl, const float4& x) {
+    if (pl == 0.f) return;  // no key of that part is seen
+    const float mn = fmaxf(m, pm), a = fast_exp2(m - mn), e = fast_exp2(pm - mn);
+    l = l * a + pl * e;
+    m = mn;
+    o[0] = o[0] * a + x.x * e;
+    o[1] = o[1] * a + x.y * e;
+    o[2] = o[2] * a + x.z * e;
+    o[3] = o[3] * a + x.w * e;
+  }
+};
+
+// Adds up the parts of each row, in a fixed order: the prefix's and the own ones, or, of one sequence of both,
+// those of the rows that a run cut (the others are done).  A block looks through `span` rows and its warps
+// share out those that need it; kWide (few rows, whose parts may be many): all eight take one row's parts in turn.
+// 4 columns a lane, kAhead parts in flight.
 // Bound: latency.
 constexpr int kAhead = 4;
+constexpr int kMostSpan = 64;
 
-template <typename T, int kRows>
+template <typename T, bool kWide>
 __global__ void __launch_bounds__(256)
-    prefix_join_kernel(const __grid_constant__ PrefixAttnParams p, const __grid_constant__ PrefixGeom g, int ctas) {
-  const int lane = threadIdx.x & 31;
-  const long long rows = (long long)p.tokens * p.q.heads;
-  const long long row0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kRows;
-  if (row0 >= rows) return;
+    prefix_join_kernel(const __grid_constant__ PrefixAttnParams p, const __grid_constant__ PrefixGeom g, int ctas,
+                       int span) {
+  __shared__ int s_rows[kMostSpan], s_count;
+  __shared__ float4 s_o[kWide ? 8 : 1][32];
+  __shared__ float s_m[8], s_l[8];
+  __shared__ int s_again[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long rows = (long long)p.tokens * p.q.heads, row0 = (long long)blockIdx.x * span;
+  if (threadIdx.x == 0) s_count = 0;
+  __syncthreads();
   wait_for_previous();
-  uint32_t todo = 1;
-  if (kRows > 1) {
-    const long long row = row0 + lane;
-    bool need = false;
-    if (row < rows && request_of(p, (int)(row / p.q.heads)) >= 0) {
+  if (threadIdx.x < span && row0 + threadIdx.x < rows) {
+    const long long row = row0 + threadIdx.x;
+    bool need = request_of(p, (int)(row / p.q.heads)) >= 0;
+    if (need && g.concat) {
       const int code = g.where[rows + row];
       need = code < 0 || code >> 20;
     }
-    todo = __ballot_sync(0xffffffffu, need);
+    if (need) s_rows[atomicAdd(&s_count, 1)] = threadIdx.x;
   }
-  while (todo) {
-    const long long row = row0 + __ffs(todo) - 1;
-    todo &= todo - 1;
+  __syncthreads();
+  const int count = s_count;
+  for (int x = kWide ? 0 : warp; x < count; x += kWide ? 1 : 8) {
+    const long long row = row0 + s_rows[x];
     const int token = (int)(row / p.q.heads), head = (int)(row - (long long)token * p.q.heads);
-    const int r = request_of(p, token);
-    if (r < 0) continue;
     const int d = p.head_dim, col = lane * 4;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    Sum sum;
     bool again = false;
-    for (int phase = kRows > 1 ? 1 : 0; phase < 2; ++phase) {
+    for (int phase = g.concat ? 1 : 0; phase < 2; ++phase) {
       const int code = g.where[rows * phase + row];
       if (code < 0) {
         again = true;
         break;
       }
       const int at = code & 255, c0 = code >> 8 & 0xfff, more = code >> 20;
+      const bool tile = c0 >= kTileWorkers;
+      const int first = tile ? c0 - kTileWorkers : c0, last = tile ? ctas - 1 : ctas * g.teams - 1;
+      // (of a team's slot: its head's rows)
+      const int slot_rows = tile ? g.tile_rows : g.heads * g.token_rows;
+      const int place = tile ? at : head / g.group % g.heads * g.token_rows + min(at, g.token_rows - 1);
+      const float* slots = (tile ? g.tile_slots : g.token_slots) + (size_t)place * g.ld;
       auto part = [&](int i) -> const float* {
         if (more == 0) return g.whole + (size_t)(rows * phase + row) * g.ld;
-        return g.slots + ((size_t)(2 * min(c0 + i, ctas - 1) + (i > 0)) * g.slot_rows + at) * g.ld;
+        return slots + (size_t)(2 * min(first + i, last) + (i > 0)) * slot_rows * g.ld;
       };
-      for (int i0 = 0; i0 <= more; i0 += kAhead) {
-        float4 head4[kAhead], x[kAhead];
+      constexpr int kStep = kWide ? 8 : 1;
+      for (int i0 = kWide ? warp : 0; i0 <= more; i0 += kAhead * kStep) {
+        float4 h[kAhead], v[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          head4[i] = x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (i0 + i > more) continue;
-          const float* f = part(i0 + i);
-          head4[i] = __ldcg(reinterpret_cast<const float4*>(f + d));
-          if (col < d) x[i] = __ldcg(reinterpret_cast<const float4*>(f + col));
+          h[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i0 + i * kStep > more) continue;
+          const float* f = part(i0 + i * kStep);
+          h[i] = __ldcg(reinterpret_cast<const float4*>(f + d));
+          if (col < d) v[i] = __ldcg(reinterpret_cast<const float4*>(f + col));
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          again |= head4[i].z != 0.f;
-          if (head4[i].y == 0.f) continue;  // no key of that part is seen
-          const float mn = fmaxf(m, head4[i].x), a = fast_exp2(m - mn), e = fast_exp2(head4[i].x - mn);
-          l = l * a + head4[i].y * e;
-          m = mn;
-          o[0] = o[0] * a + x[i].x * e;
-          o[1] = o[1] * a + x[i].y * e;
-          o[2] = o[2] * a + x[i].z * e;
-          o[3] = o[3] * a + x[i].w * e;
+          again |= h[i].z != 0.f;
+          sum.add(h[i].x, h[i].y, v[i]);
         }
       }
     }
+    if constexpr (kWide) {
+      if (x > 0) __syncthreads();  // the last row's have been read
+      s_o[warp][lane] = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+      if (lane == 0) {
+        s_m[warp] = sum.m;
+        s_l[warp] = sum.l;
+        s_again[warp] = again;
+      }
+      __syncthreads();
+      if (warp > 0) continue;
+      sum = Sum();
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        sum.add(s_m[w], s_l[w], s_o[w][lane]);
+        again |= s_again[w] != 0;
+      }
+    }
     if (again) {
+      const int r = request_of(p, token);
       const Request q = load_request(p, r);
       attend_row<T>(p, r, token, head, q.limit(token - q.q0), lane);
     } else if (col < d) {
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const float inv = sum.l > 0.f ? 1.f / sum.l : (sum.l == 0.f ? 0.f : sum.l);
       T* out = static_cast<T*>(p.out.data) + token * p.out.seq_stride + head * p.out.head_stride + col;
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(pack2<T>(sum.o[0] * inv, sum.o[1] * inv), pack2<T>(sum.o[2] * inv, sum.o[3] * inv));
     }
   }
 }
@@ -1280,7 +1449,7 @@ __global__ void __launch_bounds__(256)
 // Sizes of a launch, and where the parts of its workspace lie (bytes).
 struct Layout {
   PrefixGeom g;
-  long long where, slots, whole, bytes;
+  long long where, tile_slots, token_slots, whole, bytes;
 };
 
 Layout make_layout(int tokens, int requests, int prefix, int q_heads, int kv_heads, int head_dim, int num_sms) {
@@ -1297,28 +1466,42 @@ Layout make_layout(int tokens, int requests, int prefix, int q_heads, int kv_hea
   g.concat = prefix == 0 || rows >= 256LL * requests;
   g.prefix_token = rows <= kTokenRows;
   g.prefix_tiles = (int)(((long long)prefix + 127) >> 7);
-  g.prefix_tiles64 = (int)(((long long)prefix + 63) >> 6);
+  g.prefix_tiles32 = (int)(((long long)prefix + kTokenKeys - 1) >> kTokenShift);
   g.n_tiles = (tokens + g.nt - 1) / g.nt;
   const int tiles = g.n_tiles * g.g_tiles;
   g.full = tiles / 2;
   g.lone = tiles & 1;
-  g.slot_rows = g.prefix_token ? kTokenRows : 256;
+  for (g.heads = std::min(kv_heads, kTokenWarps); kv_heads % g.heads; --g.heads) {
+  }
+  g.groups = kv_heads / g.heads;
+  g.teams = std::min(kMostTeams, kTokenWarps / g.heads);
+  g.tile_rows = g.prefix_token ? 0 : 256;
+  g.token_rows = (int)std::min<long long>(rows, kTokenRows);
   g.ld = head_dim + 8;
   const long long n = (long long)tokens * q_heads;
   auto up = [](long long b) { return (b + 255) & ~255LL; };
-  x.slots = up(2 * n * 4);
-  x.whole = up(x.slots + 2LL * num_sms * g.slot_rows * g.ld * 4);
+  x.tile_slots = up(2 * n * 4);
+  x.token_slots = up(x.tile_slots + 2LL * num_sms * g.tile_rows * g.ld * 4);
+  x.whole = up(x.token_slots + 2LL * num_sms * g.teams * g.heads * g.token_rows * g.ld * 4);
   x.bytes = x.whole + (g.concat ? 0 : 2 * n * g.ld * 4);
   return x;
 }
 
-CUtensorMap prefix_query_map(const PrefixAttnParams& p, const PrefixGeom& g) {
-  // {d, group, tokens, key heads} in boxes of 64 x gt x nt; a stride that is never walked only has to be a legal one
-  auto st = [](long long s) { return (uint64_t)(s ? s * 2 : 16); };
+// {d, group, tokens, key heads} in boxes of 64 x group_box x tokens x heads; a stride that is never walked only has
+// to be a legal one
+uint64_t legal(long long stride) { return (uint64_t)(stride ? stride * 2 : 16); }
+CUtensorMap prefix_query_map(const PrefixAttnParams& p, const PrefixGeom& g, int group_box, int tokens, int heads) {
   const uint64_t dims[4] = {(uint64_t)p.head_dim, (uint64_t)g.group, (uint64_t)p.tokens, (uint64_t)g.kv_heads};
-  const uint64_t str[3] = {st(p.q.head_stride), st(p.q.seq_stride), st(p.q.head_stride * g.group)};
-  const uint32_t box[4] = {64, (uint32_t)g.gt, (uint32_t)g.nt, 1};
+  const uint64_t str[3] = {legal(p.q.head_stride), legal(p.q.seq_stride), legal(p.q.head_stride * g.group)};
+  const uint32_t box[4] = {64, (uint32_t)group_box, (uint32_t)tokens, (uint32_t)heads};
   return make_tensor_map(p.q.data, 4, dims, str, box);
+}
+// {d, keys, key heads, pages} in boxes of 64 x rows x heads; heads with stride 0 are one
+CUtensorMap prefix_kv_map(const HeadsView& v, int pages, int keys, int d, int rows, int heads) {
+  const uint64_t dims[4] = {(uint64_t)d, (uint64_t)keys, v.head_stride ? (uint64_t)v.heads : 1, (uint64_t)pages};
+  const uint64_t str[3] = {legal(v.seq_stride), legal(v.head_stride), legal(v.batch_stride)};
+  const uint32_t box[4] = {64, (uint32_t)rows, (uint32_t)heads, 1};
+  return make_tensor_map(v.data, 4, dims, str, box);
 }
 
 template <typename T, int DP>
@@ -1327,36 +1510,60 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   static std::atomic<unsigned long long> configured;
   cudaError_t e = ensure_smem_limit(prefix_attention_kernel<T, DP>, (int)C::kSmem, configured);
   if (e != cudaSuccess) return e;
-  // the ring of the token role: what the joined rows of its largest item leave
-  const long long rows = (long long)p.tokens * g.group;
-  const long long most = p.q_starts || (g.prefix_token && !g.concat) ? rows : g.group;
-  const size_t join = (size_t)kTokenWarps * std::min<long long>(most, kTokenRows) * DP * sizeof(float);
-  g.stages = std::min<int>(kMaxStages, (int)((C::kSmem - C::kTail - join) / C::kStage)) & ~1;
-  g.tile_cost = 20;
-  g.token_cost = DP == 128 ? 8 : 5;
-  g.box = std::min(1 << p.page_shift, kTokenKeys);
-  const CUtensorMap mq = prefix_query_map(p, g);
-  int batched;
-  const CUtensorMap mkc =
-      cross_kv_map(p.k_cache, p.pages, 1 << p.page_shift, p.head_dim, g.box, batched, g.kc_headed);
-  const CUtensorMap mvc =
-      cross_kv_map(p.v_cache, p.pages, 1 << p.page_shift, p.head_dim, g.box, batched, g.vc_headed);
-  const CUtensorMap mpk = p.prefix ? cross_kv_map(p.prefix_k, 1, p.prefix, p.head_dim, 64, batched, g.pk_headed) : mkc;
-  const CUtensorMap mpv = p.prefix ? cross_kv_map(p.prefix_v, 1, p.prefix, p.head_dim, 64, batched, g.pv_headed) : mvc;
+  g.pk_headed = p.prefix_k.head_stride != 0;
+  g.pv_headed = p.prefix_v.head_stride != 0;
+  g.kc_headed = p.k_cache.head_stride != 0;
+  g.vc_headed = p.v_cache.head_stride != 0;
+  if (g.kv_heads > 1 && !(g.kc_headed && g.vc_headed && (!p.prefix || (g.pk_headed && g.pv_headed)))) {
+    // heads that share one have no box of several
+    g.heads = 1;
+    g.groups = g.kv_heads;
+    g.teams = kMostTeams;
+  }
+  // a team's rings: query rows for one segment, for two where 8 rows a head are enough, tiles in the rest
+  const long long most_rows = p.q_starts || (g.prefix_token && !g.concat) ? (long long)p.tokens * g.group : g.group;
+  g.q_rows = most_rows <= 8 ? 8 : 16;
+  g.q_slots = most_rows <= 8 ? 2 : 1;
+  const int team_bytes = (int)C::kTiles / g.teams - g.q_slots * g.heads * g.q_rows * 128 * C::kHalves;
+  g.entries = std::min(kMostEntries, team_bytes / (g.heads * (int)C::kEntry));
+  // measured: microseconds of an SM in units of 10 ns
+  g.tile_cost = 215;
+  g.token_cost = g.heads * (DP == 128 ? 30 : 20);
+  g.tile_item = 1;
+  g.token_item = 1;
+  const int page = 1 << p.page_shift;
+  g.box = std::min(page, kTokenKeys);
+  auto maps = [&](const CUtensorMap& q, int heads) {
+    Maps m;
+    m.q = q;
+    m.kc = prefix_kv_map(p.k_cache, p.pages, page, p.head_dim, g.box, heads);
+    m.vc = prefix_kv_map(p.v_cache, p.pages, page, p.head_dim, g.box, heads);
+    m.pk = p.prefix ? prefix_kv_map(p.prefix_k, 1, p.prefix, p.head_dim, kTokenKeys, heads) : m.kc;
+    m.pv = p.prefix ? prefix_kv_map(p.prefix_v, 1, p.prefix, p.head_dim, kTokenKeys, heads) : m.vc;
+    return m;
+  };
+  const Maps tile = maps(prefix_query_map(p, g, g.gt, g.nt, 1), 1);
+  const Maps token = g.group <= kTokenRows
+                         ? maps(prefix_query_map(p, g, g.group, std::max(1, g.q_rows / g.group), g.heads), g.heads)
+                         : tile;
   const double values = (double)p.tokens * p.q.heads * p.head_dim;
   {
     // (the own tokens are counted on the GPU)
     LaunchScope scope("prefix_attention", 4.0 * values * p.prefix,
                       4.0 * values + 4.0 * p.prefix * g.kv_heads * p.head_dim, s);
-    prefix_attention_kernel<T, DP><<<num_sms, kThreads, C::kSmem, s>>>(mq, mpk, mpv, mkc, mvc, p, g);
+    prefix_attention_kernel<T, DP><<<num_sms, kThreads, C::kSmem, s>>>(tile, token, p, g);
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return e;
-  const long long n = (long long)p.tokens * p.q.heads, a_block = 8 * (g.concat ? 32 : 1);
+  // one row a warp, unless there are far more rows than the GPU has warps and only some of them need it, or so few
+  // that all warps of a block can share one
+  const long long n = (long long)p.tokens * p.q.heads;
+  const bool wide = n <= 8LL * num_sms;
+  const int span = wide ? 1 : (g.concat && n > 16384 ? kMostSpan : 8);
   LaunchScope scope("prefix_join", 0.0, 0.0, s);
-  DependentLaunch l(dim3((unsigned)((n + a_block - 1) / a_block)), 256, 0, s);
-  return g.concat ? cudaLaunchKernelEx(&l.cfg, prefix_join_kernel<T, 32>, p, g, num_sms)
-                  : cudaLaunchKernelEx(&l.cfg, prefix_join_kernel<T, 1>, p, g, num_sms);
+  DependentLaunch l(dim3((unsigned)((n + span - 1) / span)), 256, 0, s);
+  return wide ? cudaLaunchKernelEx(&l.cfg, prefix_join_kernel<T, true>, p, g, num_sms, span)
+              : cudaLaunchKernelEx(&l.cfg, prefix_join_kernel<T, false>, p, g, num_sms, span);
 }
 
 template <typename T>
@@ -1364,13 +1571,14 @@ cudaError_t launch_t(const PrefixAttnParams& p, int num_sms, cudaStream_t s) {
   Layout x = make_layout(p.tokens, p.requests, p.prefix, p.q.heads, p.k_cache.heads, p.head_dim, num_sms);
   char* ws = reinterpret_cast<char*>(p.ws);
   x.g.where = reinterpret_cast<int*>(ws);
-  x.g.slots = reinterpret_cast<float*>(ws + x.slots);
+  x.g.tile_slots = reinterpret_cast<float*>(ws + x.tile_slots);
+  x.g.token_slots = reinterpret_cast<float*>(ws + x.token_slots);
   x.g.whole = reinterpret_cast<float*>(ws + x.whole);
   return p.head_dim <= 64 ? launch_k<T, 64>(p, x.g, num_sms, s) : launch_k<T, 128>(p, x.g, num_sms, s);
 }
 
 // CTAs of a launch: one an SM, as many as a row's code can name.
-int ctas_of(int num_sms) { return std::min(num_sms, 2047); }
+int ctas_of(int num_sms) { return std::min(num_sms, kTileWorkers / kMostTeams); }
 
 }  // namespace
 
