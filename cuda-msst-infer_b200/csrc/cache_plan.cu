@@ -9,6 +9,8 @@
 // token can be placed by any thread; what is read is written only past the cluster's barrier.
 //
 // Bound: latency (two scans and a chain of three loads).
+#include <algorithm>
+
 #include "cache_ops.cuh"
 #include "common.cuh"
 #include "runtime.h"
@@ -17,27 +19,41 @@ namespace msst {
 
 namespace {
 
-constexpr int kMostThreads = 1024;
+constexpr int kMostThreads = 1024, kCtas = 8;
 
-// Exclusive sum over the block's threads, and the total.
-__device__ long long block_scan(long long v, long long* s_warp, long long& total) {
+// Exclusive sums over the block's threads of N values at once, and the totals.
+template <int N>
+__device__ __forceinline__ void block_scan(long long (&v)[N], long long (*s_warp)[2], long long (&total)[N]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  long long incl = v;
+  long long incl[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) incl[i] = v[i];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const long long x = __shfl_up_sync(0xffffffffu, incl[i], o);
+      if (lane >= o) incl[i] += x;
+    }
   }
-  __syncthreads();  // the last scan's sums have been read
-  if (lane == 31) s_warp[warp] = incl;
+  if (lane == 31) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s_warp[warp][i] = incl[i];
+  }
   __syncthreads();
-  long long before = 0;
-  total = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w < warp) before += s_warp[w];
-    total += s_warp[w];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    // the warps' sums, one a lane, summed by every warp for itself
+    long long x = lane < warps ? s_warp[lane][i] : 0;
+    const long long own = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    total[i] = __shfl_sync(0xffffffffu, x, 31);
+    v[i] = incl[i] - v[i] + __shfl_sync(0xffffffffu, x - own, warp);
   }
-  return before + incl - v;
 }
 
 // The last i of [0, n) with a[i] <= x (a[0] <= x).
@@ -60,7 +76,7 @@ __global__ void __launch_bounds__(kMostThreads) cache_plan_kernel(const __grid_c
   int* s_back = s_start + R + 1;    // [R + 1] pages given back before
   int* s_need = s_back + R + 1;     // [R + 1] pages taken before
   int* s_kept = s_need + R + 1;     // [R] tokens there already, negative (~) where the request is refused
-  __shared__ long long s_warp[32];
+  __shared__ long long s_warp[2][32][2];
   __shared__ int s_got, s_refused;
   const int tid = threadIdx.x, per = (R + blockDim.x - 1) / blockDim.x;
   const int r0 = min(R, tid * per), r1 = min(R, r0 + per);
@@ -69,48 +85,48 @@ __global__ void __launch_bounds__(kMostThreads) cache_plan_kernel(const __grid_c
   if (tid == 0) s_got = s_refused = 0;
 
   const int count = min(max(*p.free_count, 0), p.pages);
-  long long grow = 0, back = 0;
+  long long sums[2] = {0, 0};  // pages given back, new rows
   for (int r = r0; r < r1; ++r) {
     const int n = p.new_tokens[r], len = min(max(p.lens[r], 0), most);
     s_kept[r] = n < 0 ? 0 : len;
     s_back[r] = n < 0 ? (int)(((long long)len + page - 1) >> p.page_shift) : 0;
     s_start[r] = max(n, 0);
-    back += s_back[r];
-    grow += max(n, 0);
+    sums[0] += s_back[r];
+    sums[1] += max(n, 0);
   }
-  long long all_back, all_grow, all_need, need = 0;
-  back = block_scan(back, s_warp, all_back);
-  grow = block_scan(grow, s_warp, all_grow);
+  long long all[2], need[1] = {0}, all_need[1];
+  block_scan<2>(sums, s_warp[0], all);
   for (int r = r0; r < r1; ++r) {
     const int n = s_start[r], kept = s_kept[r], b = s_back[r];
     const long long after = (long long)kept + n;
-    const bool wide = after > most || grow + n > p.tokens;
+    const bool wide = after > most || sums[1] + n > p.tokens;
     s_need[r] = wide ? -1 : (int)(((after + page - 1) >> p.page_shift) - (((long long)kept + page - 1) >> p.page_shift));
-    need += max(s_need[r], 0);
-    s_start[r] = (int)min(grow, (long long)p.tokens);
-    s_back[r] = clamp_int(back);
-    grow += n;
-    back += b;
+    need[0] += max(s_need[r], 0);
+    s_start[r] = (int)min(sums[1], (long long)p.tokens);
+    s_back[r] = clamp_int(sums[0]);
+    sums[1] += n;
+    sums[0] += b;
   }
+  const long long all_back = all[0];
   if (tid == 0) {
-    s_start[R] = (int)min(all_grow, (long long)p.tokens);
+    s_start[R] = (int)min(all[1], (long long)p.tokens);
     s_back[R] = clamp_int(all_back);
   }
-  need = block_scan(need, s_warp, all_need);
+  block_scan<1>(need, s_warp[1], all_need);
   const int top = (int)min(count + all_back, (long long)p.pages);
   for (int r = r0; r < r1; ++r) {
     const int n = s_need[r];
-    const bool fits = n == 0 || (n > 0 && need + n <= top);
-    s_need[r] = clamp_int(need);
-    need += max(n, 0);
+    const bool fits = n == 0 || (n > 0 && need[0] + n <= top);
+    s_need[r] = clamp_int(need[0]);
+    need[0] += max(n, 0);
     if (!fits) {
       s_kept[r] = ~s_kept[r];
       s_refused = 1;
     } else if (n > 0) {
-      atomicMax(&s_got, (int)need);
+      atomicMax(&s_got, (int)need[0]);
     }
   }
-  if (tid == 0) s_need[R] = clamp_int(all_need);
+  if (tid == 0) s_need[R] = clamp_int(all_need[0]);
   __syncthreads();
   // pages of ended requests go on top of the stack
   for (long long i = first; i < s_back[R] && count + i < p.pages; i += stride) {
@@ -161,7 +177,10 @@ cudaError_t launch_cache_plan(const CachePlanParams& p, cudaStream_t stream) {
   constexpr int most = (4 * kMostPlanRequests + 3) * (int)sizeof(int);
   cudaError_t e = ensure_smem_limit(cache_plan_kernel, most, configured);
   if (e != cudaSuccess) return e;
-  const int threads = kMostThreads, ctas = p.tokens > 4096 ? 8 : 1;
+  // a thread a request or row, while there are few; one CTA's barrier is the cheaper one
+  const int ctas = p.tokens > 4096 ? kCtas : 1;
+  const int wanted = std::max(p.requests, std::min(p.tokens / ctas, kMostThreads));
+  const int threads = std::min(kMostThreads, std::max(128, (wanted + 31) & ~31));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = ctas;
   cfg.blockDim = threads;
@@ -171,7 +190,7 @@ cudaError_t launch_cache_plan(const CachePlanParams& p, cudaStream_t stream) {
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim = {(unsigned)ctas, 1, 1};
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
   LaunchScope scope("cache_plan", 0.0, 20.0 * p.requests + 8.0 * p.tokens, stream);
   return cudaLaunchKernelEx(&cfg, cache_plan_kernel, p);
 }

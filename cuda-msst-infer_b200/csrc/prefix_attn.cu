@@ -44,7 +44,7 @@ constexpr int kTokenKeys = 32, kTokenShift = 5;   // a token item's K/V tile
 constexpr uint32_t kTokenBox = kTokenKeys * 128;  // 32 keys x 64 columns
 constexpr int kTokenWarps = 8;                    // that multiply; the other four bring tiles, one a team
 constexpr int kMostTeams = 4, kMostEntries = 12;
-constexpr int kRecompute = -1;
+constexpr int kRecompute = -1;                     // less the worker's place
 
 template <int DP>
 struct PCfg {
@@ -79,7 +79,9 @@ struct PrefixGeom {
   int* where;                 // [phase][tokens * q_heads] which partial results a row has
   float* tile_slots;          // [CTA][begins, ends][tile_rows][ld]
   float* token_slots;         // [CTA * teams][begins, ends][heads][token_rows][ld]
-  float* whole;               // [phase][tokens * q_heads][ld] results of items that one CTA had whole
+  float* whole;               // [phase][tokens * q_heads][ld] results of items that one worker had whole
+  struct Segment* cuts;       // [CTA][teams] the item that the worker started and did not end (code 0: none)
+  int* bad;                   // [CTA][teams] whether one of the worker's rows has to be computed again
 };
 
 struct Request {
@@ -148,11 +150,11 @@ __device__ __forceinline__ long long prefix_weight(const PrefixGeom& g, bool tok
                                   g.lone * (((prefix_part(g, false) + 1) >> 1) + g.tile_item));
 }
 
-// The run of a CTA (tile items) or of a team of its warps (token items): weights [u0, u0 + count) of the U of its sequence,
+// The run of a worker, a CTA (tile items) or a team of its warps (token items): weights [u0, u0 + count) of the U of its sequence,
 // worker `self` of `workers`; where it starts.
 struct Run {
   long long u0, count, U;
-  int token, self, workers;
+  int token, self, workers, place;  // place: among the teams of all CTAs, the tile items' as team 0
   int phase, r, hk, t, j;
 };
 
@@ -227,6 +229,7 @@ __device__ void find_runs(const PrefixAttnParams& p, const PrefixGeom& g, Run* r
   auto run_of = [&](int w) {  // the run without its start
     Run y = x;
     y.self = self0 + w;
+    y.place = (int)blockIdx.x * g.teams + w;
     if (y.self < x.workers) {
       y.u0 = mul_div(x.U, y.self, x.workers);
       y.count = mul_div(x.U, y.self + 1, x.workers) - y.u0;
@@ -289,8 +292,8 @@ struct Segment {
   int ptiles, tiles, units;   // K/V tiles of the prefix, K/V tiles and units in all
   int j0, j1;
   int lone, tile0, n_tiles;   // tile items: row tile(s) tile0, tile0 + 1 of n_tiles along the tokens
-  int code;                   // see below
   int last;                   // 1: no segment, the run's end
+  int code;                   // see below
   __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == units; }
   // own tokens that row i sees
   __device__ __forceinline__ int limit(int i) const { return Request{q0, n, own}.limit(i); }
@@ -417,6 +420,7 @@ struct SegmentRing {
       at[s % kRing] = x;
       mbar_arrive(&full[s % kRing]);
       if (x.last) return;
+      if (x.code) g.cuts[run.place] = x;
     }
   }
 };
@@ -914,7 +918,8 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         }
         if (valid && (!k.lone || w == 0)) {
           if (!finish) *reinterpret_cast<float4*>(po + p.head_dim) = make_float4(ref, l, bad ? 1.f : 0.f, 0.f);
-          if (k.j0 == 0) g.where[plane + grow] = finish && bad ? kRecompute : k.code | at;
+          if (finish && bad) g.bad[run.place] = 1;
+          if (k.j0 == 0) g.where[plane + grow] = finish && bad ? kRecompute - run.place : k.code | at;
         }
       }
       tc_fence_before();
@@ -1006,6 +1011,7 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& qmap, const CUtenso
       if (lane == 0) {
         tm->seg[s & 1] = x;
         mbar_arrive(&tm->seg_full[s & 1]);
+        if (!x.last && x.code) g.cuts[run.place] = tm->seg[s & 1];
       }
       if (x.last) break;
       const int head0 = x.hk * g.heads, qs = s % g.q_slots, q_use = s / g.q_slots;
@@ -1238,7 +1244,8 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& qmap, const CUtenso
         if (qc == 0)
           *reinterpret_cast<float4*>(po + p.head_dim) = make_float4(m[half] - kLift<T>, l[half], bad ? 1.f : 0.f, 0.f);
       }
-      if (qc == 0 && k.j0 == 0) g.where[grow] = finish && bad ? kRecompute : k.code | r;
+      if (qc == 0 && finish && bad) g.bad[run.place] = 1;
+      if (qc == 0 && k.j0 == 0) g.where[grow] = finish && bad ? kRecompute - run.place : k.code | r;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&tm->seg_empty[s & 1]);
@@ -1258,6 +1265,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the runs are found in memory that the roles take over
   Two* scratch = reinterpret_cast<Two*>(smem);
   Run* runs = reinterpret_cast<Run*>(smem + 1024);
+  if (threadIdx.x < 10) {
+    const Maps& m = threadIdx.x < 5 ? tile : token;
+    tma_prefetch_desc(&m.q + threadIdx.x % 5);  // (the members in their order)
+  }
+  if (threadIdx.x < g.teams) {
+    const int place = (int)blockIdx.x * g.teams + threadIdx.x;
+    g.cuts[place].code = 0;
+    g.bad[place] = 0;
+  }
   find_runs(p, g, runs, scratch);
   dependents_may_start();
   if (runs[0].token) {
@@ -1342,106 +1358,154 @@ struct Sum {
   }
 };
 
-// Adds up the parts of each row, in a fixed order: the prefix's and the own ones, or, of one sequence of both,
-// those of the rows that a run cut (the others are done).  A block looks through `span` rows and its warps
-// share out those that need it; kWide (few rows, whose parts may be many): all eight take one row's parts in turn.
-// 4 columns a lane, kAhead parts in flight.
-// Bound: latency.
-constexpr int kAhead = 4;
-constexpr int kMostSpan = 64;
+// The parts of a row for one phase: their number, where the first one is and how far apart the others.
+struct Parts {
+  const float* base = nullptr;
+  size_t stride = 0;
+  int count = 0;
+  __device__ __forceinline__ void find(const PrefixGeom& g, int code, int place_in_slot, const float* whole, int ctas) {
+    const int c0 = code >> 8 & 0xfff, more = code >> 20;
+    const bool tile = c0 >= kTileWorkers;
+    const int first = tile ? c0 - kTileWorkers : c0, last = tile ? ctas - 1 : ctas * g.teams - 1;
+    const size_t slot = (size_t)(tile ? g.tile_rows : g.heads * g.token_rows) * g.ld;
+    // the first part ends its worker's run, the others begin theirs
+    base = more == 0 ? whole
+                     : (tile ? g.tile_slots : g.token_slots) + 2 * min(first, last) * slot + (size_t)place_in_slot * g.ld;
+    stride = 2 * slot;
+    count = 1 + min(more, max(last - first, 0));
+  }
+  __device__ __forceinline__ const float* at(int i) const { return base + i * stride + (i > 0 ? stride >> 1 : 0); }
+};
 
+// Parts first, first + step, ... of two lists one behind the other (kAhead in flight) into the sum.
+template <int kAhead>
+__device__ __forceinline__ void add_parts(const Parts& a, const Parts& b, int first, int step, int d, int col, Sum& sum,
+                                          bool& again) {
+  const int n = a.count + b.count;
+  for (int i0 = first; i0 < n; i0 += kAhead * step) {
+    float4 h[kAhead], v[kAhead];
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      h[y] = v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int i = i0 + y * step;
+      if (i >= n) continue;
+      const float* f = i < a.count ? a.at(i) : b.at(i - a.count);
+      h[y] = __ldcg(reinterpret_cast<const float4*>(f + d));
+      if (col < d) v[y] = __ldcg(reinterpret_cast<const float4*>(f + col));
+    }
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      again |= h[y].z != 0.f;
+      sum.add(h[y].x, h[y].y, v[y]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void finish_row(const PrefixAttnParams& p, int token, int head, const Sum& sum, bool again,
+                                           int lane) {
+  if (again) {
+    const int r = request_of(p, token);
+    const Request q = load_request(p, r);
+    attend_row<T>(p, r, token, head, q.limit(token - q.q0), lane);
+  } else if (4 * lane < p.head_dim) {
+    const float inv = sum.l > 0.f ? 1.f / sum.l : (sum.l == 0.f ? 0.f : sum.l);
+    T* out = static_cast<T*>(p.out.data) + token * p.out.seq_stride + head * p.out.head_stride + 4 * lane;
+    *reinterpret_cast<uint2*>(out) =
+        make_uint2(pack2<T>(sum.o[0] * inv, sum.o[1] * inv), pack2<T>(sum.o[2] * inv, sum.o[3] * inv));
+  }
+}
+
+// Adds up the parts of each row, in a fixed order: the prefix's and the own ones, or, of one sequence of both,
+// those of the rows that a run cut (the others are done).  4 columns a lane; a warp a row, kWide (few rows, whose
+// parts may be many): a block a row, its warps taking parts in turn.
+// Bound: latency, three loads one behind the other.
 template <typename T, bool kWide>
-__global__ void __launch_bounds__(256)
-    prefix_join_kernel(const __grid_constant__ PrefixAttnParams p, const __grid_constant__ PrefixGeom g, int ctas,
-                       int span) {
-  __shared__ int s_rows[kMostSpan], s_count;
+__global__ void __launch_bounds__(256, 2)
+    prefix_join_kernel(const __grid_constant__ PrefixAttnParams p, const __grid_constant__ PrefixGeom g, int ctas) {
   __shared__ float4 s_o[kWide ? 8 : 1][32];
   __shared__ float s_m[8], s_l[8];
   __shared__ int s_again[8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long rows = (long long)p.tokens * p.q.heads, row0 = (long long)blockIdx.x * span;
-  if (threadIdx.x == 0) s_count = 0;
-  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = p.head_dim;
+  const long long rows = (long long)p.tokens * p.q.heads, row = kWide ? blockIdx.x : (long long)blockIdx.x * 8 + warp;
+  if (row >= rows) return;
+  const int token = (int)(row / p.q.heads), head = (int)(row - (long long)token * p.q.heads);
   wait_for_previous();
-  if (threadIdx.x < span && row0 + threadIdx.x < rows) {
-    const long long row = row0 + threadIdx.x;
-    bool need = request_of(p, (int)(row / p.q.heads)) >= 0;
-    if (need && g.concat) {
-      const int code = g.where[rows + row];
-      need = code < 0 || code >> 20;
-    }
-    if (need) s_rows[atomicAdd(&s_count, 1)] = threadIdx.x;
+  const int code0 = g.concat ? 0 : g.where[row], code1 = g.where[rows + row];
+  if (g.concat && code1 >= 0 && code1 >> 20 == 0) return;
+  if (request_of(p, token) < 0) return;
+  bool again = code0 < 0 || code1 < 0;
+  Sum sum;
+  if (!again) {
+    const int h = head / g.group % g.heads;
+    auto place = [&](int code) {  // (of a team's slot: its head's rows)
+      const int at = code & 255;
+      return (code >> 8 & 0xfff) >= kTileWorkers ? at : h * g.token_rows + min(at, g.token_rows - 1);
+    };
+    Parts a, b;
+    if (!g.concat) a.find(g, code0, place(code0), g.whole + (size_t)row * g.ld, ctas);
+    b.find(g, code1, place(code1), g.whole + (size_t)(rows + row) * g.ld, ctas);
+    add_parts<kWide ? 4 : 8>(a, b, kWide ? warp : 0, kWide ? 8 : 1, d, lane * 4, sum, again);
   }
-  __syncthreads();
-  const int count = s_count;
-  for (int x = kWide ? 0 : warp; x < count; x += kWide ? 1 : 8) {
-    const long long row = row0 + s_rows[x];
-    const int token = (int)(row / p.q.heads), head = (int)(row - (long long)token * p.q.heads);
-    const int d = p.head_dim, col = lane * 4;
-    Sum sum;
-    bool again = false;
-    for (int phase = g.concat ? 1 : 0; phase < 2; ++phase) {
-      const int code = g.where[rows * phase + row];
-      if (code < 0) {
-        again = true;
-        break;
-      }
-      const int at = code & 255, c0 = code >> 8 & 0xfff, more = code >> 20;
-      const bool tile = c0 >= kTileWorkers;
-      const int first = tile ? c0 - kTileWorkers : c0, last = tile ? ctas - 1 : ctas * g.teams - 1;
-      // (of a team's slot: its head's rows)
-      const int slot_rows = tile ? g.tile_rows : g.heads * g.token_rows;
-      const int place = tile ? at : head / g.group % g.heads * g.token_rows + min(at, g.token_rows - 1);
-      const float* slots = (tile ? g.tile_slots : g.token_slots) + (size_t)place * g.ld;
-      auto part = [&](int i) -> const float* {
-        if (more == 0) return g.whole + (size_t)(rows * phase + row) * g.ld;
-        return slots + (size_t)(2 * min(first + i, last) + (i > 0)) * slot_rows * g.ld;
-      };
-      constexpr int kStep = kWide ? 8 : 1;
-      for (int i0 = kWide ? warp : 0; i0 <= more; i0 += kAhead * kStep) {
-        float4 h[kAhead], v[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          h[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (i0 + i * kStep > more) continue;
-          const float* f = part(i0 + i * kStep);
-          h[i] = __ldcg(reinterpret_cast<const float4*>(f + d));
-          if (col < d) v[i] = __ldcg(reinterpret_cast<const float4*>(f + col));
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          again |= h[i].z != 0.f;
-          sum.add(h[i].x, h[i].y, v[i]);
-        }
-      }
+  if constexpr (kWide) {
+    s_o[warp][lane] = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+    if (lane == 0) {
+      s_m[warp] = sum.m;
+      s_l[warp] = sum.l;
+      s_again[warp] = again;
     }
-    if constexpr (kWide) {
-      if (x > 0) __syncthreads();  // the last row's have been read
-      s_o[warp][lane] = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
-      if (lane == 0) {
-        s_m[warp] = sum.m;
-        s_l[warp] = sum.l;
-        s_again[warp] = again;
-      }
-      __syncthreads();
-      if (warp > 0) continue;
-      sum = Sum();
+    __syncthreads();
+    if (warp > 0) return;
+    sum = Sum();
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        sum.add(s_m[w], s_l[w], s_o[w][lane]);
-        again |= s_again[w] != 0;
-      }
+    for (int w = 0; w < 8; ++w) {
+      sum.add(s_m[w], s_l[w], s_o[w][lane]);
+      again |= s_again[w] != 0;
     }
-    if (again) {
-      const int r = request_of(p, token);
-      const Request q = load_request(p, r);
-      attend_row<T>(p, r, token, head, q.limit(token - q.q0), lane);
-    } else if (col < d) {
-      const float inv = sum.l > 0.f ? 1.f / sum.l : (sum.l == 0.f ? 0.f : sum.l);
-      T* out = static_cast<T*>(p.out.data) + token * p.out.seq_stride + head * p.out.head_stride + col;
-      *reinterpret_cast<uint2*>(out) =
-          make_uint2(pack2<T>(sum.o[0] * inv, sum.o[1] * inv), pack2<T>(sum.o[2] * inv, sum.o[3] * inv));
+  }
+  finish_row<T>(p, token, head, sum, again, lane);
+}
+
+// The same for many rows of one sequence of prefix and own keys, most of which are done: block (x, y) takes rows
+// [8 y, 8 y + 8) of the item that worker x started and did not end (4096 rows of 32 heads, 37,000 of them cut: by the
+// kernel above, which looks at all, 26 us).
+template <typename T>
+__global__ void __launch_bounds__(256, 4)
+    prefix_join_cuts_kernel(const __grid_constant__ PrefixAttnParams p, const __grid_constant__ PrefixGeom g, int ctas) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, x = blockIdx.y * 8 + warp;
+  wait_for_previous();
+  const Segment k = g.cuts[blockIdx.x];
+  if (k.code > 0) {
+    int n, head;
+    bool valid;
+    if ((k.code >> 8 & 0xfff) >= kTileWorkers) {
+      int n0, g0;
+      k.origin(g, x >> 7, n0, g0);
+      const int row = x & 127, rn = row / g.gt;
+      n = n0 + rn;
+      head = g0 + row - rn * g.gt;
+      valid = rn < g.nt && n < k.n && head < g.group && !(k.lone && x >= 128);
+      head += k.hk * g.group;
+    } else {
+      const int h = x / g.token_rows, r = x - h * g.token_rows;
+      n = r / g.group;
+      head = (k.hk * g.heads + h) * g.group + r - n * g.group;
+      valid = h < g.heads && n < k.n;
     }
+    if (valid) {
+      Parts none, parts;
+      parts.find(g, k.code, x, nullptr, ctas);
+      Sum sum;
+      bool again = false;
+      add_parts<4>(none, parts, 0, 1, p.head_dim, lane * 4, sum, again);
+      finish_row<T>(p, k.q0 + n, head, sum, again, lane);
+    }
+  }
+  if (g.bad[blockIdx.x]) {  // rows to be computed again
+    const long long rows = (long long)p.tokens * p.q.heads;
+    for (long long row = x; row < rows; row += gridDim.y * 8)
+      if (g.where[rows + row] == kRecompute - (int)blockIdx.x && request_of(p, (int)(row / p.q.heads)) >= 0)
+        finish_row<T>(p, (int)(row / p.q.heads), (int)(row % p.q.heads), Sum(), true, lane);
   }
 }
 
@@ -1449,7 +1513,7 @@ __global__ void __launch_bounds__(256)
 // Sizes of a launch, and where the parts of its workspace lie (bytes).
 struct Layout {
   PrefixGeom g;
-  long long where, tile_slots, token_slots, whole, bytes;
+  long long where, cuts, tile_slots, token_slots, whole, bytes;
 };
 
 Layout make_layout(int tokens, int requests, int prefix, int q_heads, int kv_heads, int head_dim, int num_sms) {
@@ -1480,7 +1544,8 @@ Layout make_layout(int tokens, int requests, int prefix, int q_heads, int kv_hea
   g.ld = head_dim + 8;
   const long long n = (long long)tokens * q_heads;
   auto up = [](long long b) { return (b + 255) & ~255LL; };
-  x.tile_slots = up(2 * n * 4);
+  x.cuts = up(2 * n * 4);
+  x.tile_slots = up(x.cuts + (long long)num_sms * kMostTeams * (sizeof(Segment) + sizeof(int)));
   x.token_slots = up(x.tile_slots + 2LL * num_sms * g.tile_rows * g.ld * 4);
   x.whole = up(x.token_slots + 2LL * num_sms * g.teams * g.heads * g.token_rows * g.ld * 4);
   x.bytes = x.whole + (g.concat ? 0 : 2 * n * g.ld * 4);
@@ -1528,7 +1593,7 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   g.entries = std::min(kMostEntries, team_bytes / (g.heads * (int)C::kEntry));
   // measured: microseconds of an SM in units of 10 ns
   g.tile_cost = 215;
-  g.token_cost = g.heads * (DP == 128 ? 30 : 20);
+  g.token_cost = g.heads * (DP == 128 ? 22 : 15);
   g.tile_item = 1;
   g.token_item = 1;
   const int page = 1 << p.page_shift;
@@ -1555,15 +1620,17 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return e;
-  // one row a warp, unless there are far more rows than the GPU has warps and only some of them need it, or so few
-  // that all warps of a block can share one
   const long long n = (long long)p.tokens * p.q.heads;
-  const bool wide = n <= 8LL * num_sms;
-  const int span = wide ? 1 : (g.concat && n > 16384 ? kMostSpan : 8);
   LaunchScope scope("prefix_join", 0.0, 0.0, s);
-  DependentLaunch l(dim3((unsigned)((n + span - 1) / span)), 256, 0, s);
-  return wide ? cudaLaunchKernelEx(&l.cfg, prefix_join_kernel<T, true>, p, g, num_sms, span)
-              : cudaLaunchKernelEx(&l.cfg, prefix_join_kernel<T, false>, p, g, num_sms, span);
+  if (g.concat && n > 16384) {
+    DependentLaunch l(dim3(num_sms * g.teams, 256 / 8), 256, 0, s);
+    return cudaLaunchKernelEx(&l.cfg, prefix_join_cuts_kernel<T>, p, g, num_sms);
+  }
+  // so few rows that all warps of a block can share one, or a row a warp
+  const bool wide = n <= 4LL * num_sms;
+  DependentLaunch l(dim3((unsigned)(wide ? n : (n + 7) / 8)), 256, 0, s);
+  return wide ? cudaLaunchKernelEx(&l.cfg, prefix_join_kernel<T, true>, p, g, num_sms)
+              : cudaLaunchKernelEx(&l.cfg, prefix_join_kernel<T, false>, p, g, num_sms);
 }
 
 template <typename T>
@@ -1571,6 +1638,8 @@ cudaError_t launch_t(const PrefixAttnParams& p, int num_sms, cudaStream_t s) {
   Layout x = make_layout(p.tokens, p.requests, p.prefix, p.q.heads, p.k_cache.heads, p.head_dim, num_sms);
   char* ws = reinterpret_cast<char*>(p.ws);
   x.g.where = reinterpret_cast<int*>(ws);
+  x.g.cuts = reinterpret_cast<Segment*>(ws + x.cuts);
+  x.g.bad = reinterpret_cast<int*>(x.g.cuts + num_sms * kMostTeams);
   x.g.tile_slots = reinterpret_cast<float*>(ws + x.tile_slots);
   x.g.token_slots = reinterpret_cast<float*>(ws + x.token_slots);
   x.g.whole = reinterpret_cast<float*>(ws + x.whole);

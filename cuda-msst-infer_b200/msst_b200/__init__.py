@@ -599,25 +599,28 @@ class ops:
         slot -1, and device_error() returns 16.  Returns (q_starts [R + 1], slots [tokens],
         positions [tokens], lens [R], free_count [1]), the last two in out_lens / out_free_count
         where given (lens / free_count themselves allowed)."""
-        torch = _torch()
+        _torch()
         dev, shape = new_tokens.get_device(), new_tokens.shape
         _need(len(shape) == 1 and free_pages.dim() == 1, "new_tokens and free_pages must have one dimension")
         R = shape[0]
         new, old = _int32(new_tokens, shape, dev, "new_tokens"), _int32(lens, shape, dev, "lens")
         table, blocks, stride = _table(block_table, R, dev)
         free, count = _int32(free_pages, free_pages.shape, dev, "free_pages"), _int32(free_count, (1,), dev, "free_count")
-        if out_lens is None:
-            out_lens = torch.empty_like(lens)
-        if out_free_count is None:
-            out_free_count = torch.empty_like(free_count)
         _need(tokens >= 0, "tokens must be >= 0")
-        made = new_tokens.new_empty(R + 1 + 2 * tokens)
-        q_starts, slots, positions = made[:R + 1], made[R + 1:R + 1 + tokens], made[R + 1 + tokens:]
+        made = new_tokens.new_empty(2 * R + 2 + 2 * tokens)
+        q_starts, slots, positions, new_lens, new_count = made.split((R + 1, tokens, tokens, R, 1))
         at = made.data_ptr()
-        check(lib().msst_cache_plan(
-            new, old, R, table, blocks, stride, free, free_pages.shape[0], count, page_size, start, tokens,
-            _int32(out_lens, shape, dev, "out_lens"), _int32(out_free_count, (1,), dev, "out_free_count"), at,
-            at + 4 * (R + 1), at + 4 * (R + 1 + tokens), _current_stream(dev)))
+        if out_lens is None:
+            out_lens, to_lens = new_lens, at + 4 * (R + 1 + 2 * tokens)
+        else:
+            to_lens = _int32(out_lens, shape, dev, "out_lens")
+        if out_free_count is None:
+            out_free_count, to_count = new_count, at + 4 * (2 * R + 1 + 2 * tokens)
+        else:
+            to_count = _int32(out_free_count, (1,), dev, "out_free_count")
+        check(lib().msst_cache_plan(new, old, R, table, blocks, stride, free, free_pages.shape[0], count, page_size, start,
+                                    tokens, to_lens, to_count, at, at + 4 * (R + 1), at + 4 * (R + 1 + tokens),
+                                    _current_stream(dev)))
         return q_starts, slots, positions, out_lens, out_free_count
 
     @staticmethod

@@ -381,6 +381,8 @@ ATTEND_CASES = [
     ([700, 64, 257], [701, 64, 900], 130, 6, 2, 96, 32, "plain"),
     ([40, 3], [10, 2], 20, 2, 1, 48, 16, "plain"),              # fewer own tokens than new ones: the first rows see none
     ([1000], [1200], 1500, 8, 1, 40, 256, "plain"),
+    ([900, 1, 1300, 3], [900, 70, 1500, 40], 600, 8, 4, 64, 32, "plain"),       # many rows, most of them of one worker
+    ([2, 1, 1], [3000, 5000, 10], 0, 3, 3, 48, 16, "strided"),
 ]
 
 
@@ -415,7 +417,7 @@ def test_prefix_attention(cuda, case, prec):
 
 
 @pytest.mark.parametrize("prec", ["fp16", "bf16"])
-@pytest.mark.parametrize("counts", [[4] * 6, [40, 9], [300, 5]], ids=str)
+@pytest.mark.parametrize("counts", [[4] * 6, [40, 9], [300, 5], [4200, 9]], ids=str)
 def test_prefix_attention_values_of_later_tokens(cuda, counts, prec):
     """What a new token holds, infinities and NaN included, does not reach the rows before it."""
     torch = cuda
