@@ -122,7 +122,8 @@ struct Items {
     int end = q.n;
     if (!token) {
       const int a = 2 * t, b = t < full ? a + 1 : a;
-      end = min((max(a % n_tiles, b % n_tiles) + 1) * g.nt, q.n);
+      const int last = g.g_tiles == 1 ? b : max(a % n_tiles, b % n_tiles);  // (along the group the tokens start over)
+      end = min((last + 1) * g.nt, q.n);
     }
     const int keys = q.own ? q.limit(end - 1) : 0, shift = token ? kTokenShift : 7;
     return max(1, ptiles + ((keys + (1 << shift) - 1) >> shift));
@@ -1598,19 +1599,25 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   g.token_item = 1;
   const int page = 1 << p.page_shift;
   g.box = std::min(page, kTokenKeys);
-  auto maps = [&](const CUtensorMap& q, int heads) {
-    Maps m;
-    m.q = q;
-    m.kc = prefix_kv_map(p.k_cache, p.pages, page, p.head_dim, g.box, heads);
-    m.vc = prefix_kv_map(p.v_cache, p.pages, page, p.head_dim, g.box, heads);
-    m.pk = p.prefix ? prefix_kv_map(p.prefix_k, 1, p.prefix, p.head_dim, kTokenKeys, heads) : m.kc;
-    m.pv = p.prefix ? prefix_kv_map(p.prefix_v, 1, p.prefix, p.head_dim, kTokenKeys, heads) : m.vc;
-    return m;
+  // What a launch cannot come to needs no map (0.25 us each): without q_starts every request is of one kind, and the
+  // prefix has items of one kind alone unless they are part of the requests'.
+  const bool own_tile = p.q_starts || g.group > kTokenRows, own_token = g.group <= kTokenRows;
+  Maps tile, token;
+  tile.q = prefix_query_map(p, g, g.gt, g.nt, 1);
+  token.q = own_token ? prefix_query_map(p, g, g.group, g.q_rows / g.group, g.heads) : tile.q;
+  auto fill = [&](Maps& m, bool own, bool pre, int heads) {
+    m.pk = m.pv = m.kc = m.vc = m.q;
+    if (own) {
+      m.kc = prefix_kv_map(p.k_cache, p.pages, page, p.head_dim, g.box, heads);
+      m.vc = prefix_kv_map(p.v_cache, p.pages, page, p.head_dim, g.box, heads);
+    }
+    if (p.prefix && (g.concat ? own : pre)) {
+      m.pk = prefix_kv_map(p.prefix_k, 1, p.prefix, p.head_dim, kTokenKeys, heads);
+      m.pv = prefix_kv_map(p.prefix_v, 1, p.prefix, p.head_dim, kTokenKeys, heads);
+    }
   };
-  const Maps tile = maps(prefix_query_map(p, g, g.gt, g.nt, 1), 1);
-  const Maps token = g.group <= kTokenRows
-                         ? maps(prefix_query_map(p, g, g.group, std::max(1, g.q_rows / g.group), g.heads), g.heads)
-                         : tile;
+  fill(tile, own_tile, !g.prefix_token, 1);
+  fill(token, own_token, g.prefix_token, g.heads);
   const double values = (double)p.tokens * p.q.heads * p.head_dim;
   {
     // (the own tokens are counted on the GPU)

@@ -302,30 +302,32 @@ def _int32(t, shape, device, what):
 
 def _table(t, requests, device):
     """(address, blocks, row stride) of a block table [requests, blocks]."""
-    if (t.dtype is not _torch_module.int32 or t.get_device() != device or t.dim() != 2 or t.shape[0] != requests
-            or (t.stride(1) != 1 and t.shape[1] > 1)):
+    sh, st = t.shape, t.stride()
+    if (len(sh) != 2 or sh[0] != requests or t.dtype is not _torch_module.int32 or t.get_device() != device
+            or (st[1] != 1 and sh[1] > 1)):
         raise ValueError("block_table must be int32 [requests, blocks] on the operands' device, unit last stride")
-    return t.data_ptr(), t.shape[1], t.stride(0)
+    return t.data_ptr(), sh[1], st[0]
 
 
-def _flat_heads(t, keep):
+def _flat_heads(t, shape, keep):
     """The msst_heads of a [tokens, heads, head_dim] tensor; one that 16-byte loads cannot walk is
     copied first (kept alive in `keep`)."""
-    n, h, d = t.shape
-    st = t.stride()
-    if ((st[2] != 1 and d > 1) or t.data_ptr() & 15 or ((st[0] & 7 or not st[0]) and n > 1)
-            or ((st[1] & 7 or not st[1]) and h > 1)):
+    n, h, d = shape
+    s0, s1, s2 = t.stride()
+    p = t.data_ptr()
+    if (s2 != 1 and d > 1) or p & 15 or ((s0 & 7 or not s0) and n > 1) or ((s1 & 7 or not s1) and h > 1):
         t = t.clone(memory_format=_torch_module.contiguous_format)
         keep.append(t)
-        st = t.stride()
-    return _HEADS(t.data_ptr(), h, 0, st[0], st[1])
+        s0, s1, _ = t.stride()
+        p = t.data_ptr()
+    return _HEADS(p, h, 0, s0, s1)
 
 
 def _cache_heads(t, dt, dev, what):
     """The msst_heads of a cache [pages, page_size, heads, head_dim] (never a copy)."""
-    if t.dim() != 4 or t.dtype is not dt or t.get_device() != dev or (t.stride(3) != 1 and t.shape[3] > 1):
-        raise ValueError(f"{what} must be [pages, page_size, heads, head_dim] with q's type and device, unit last stride")
     st = t.stride()
+    if len(st) != 4 or t.dtype is not dt or t.get_device() != dev or (st[3] != 1 and t.shape[3] > 1):
+        raise ValueError(f"{what} must be [pages, page_size, heads, head_dim] with q's type and device, unit last stride")
     return _HEADS(t.data_ptr(), t.shape[2], st[0], st[1], st[2])
 
 
@@ -608,7 +610,7 @@ class ops:
         free, count = _int32(free_pages, free_pages.shape, dev, "free_pages"), _int32(free_count, (1,), dev, "free_count")
         _need(tokens >= 0, "tokens must be >= 0")
         made = new_tokens.new_empty(2 * R + 2 + 2 * tokens)
-        q_starts, slots, positions, new_lens, new_count = made.split((R + 1, tokens, tokens, R, 1))
+        q_starts, slots, positions, new_lens, new_count = made.unsafe_split_with_sizes((R + 1, tokens, tokens, R, 1))
         at = made.data_ptr()
         if out_lens is None:
             out_lens, to_lens = new_lens, at + 4 * (R + 1 + 2 * tokens)
@@ -657,7 +659,7 @@ class ops:
                   (out_q.stride(2) == 1 or d < 2), "out_q must have q's shape, type and device, and unit last stride")
         ost = out_q.stride()
         check(lib().msst_rope_append(
-            _flat_heads(q, keep), _flat_heads(k, keep), _flat_heads(v, keep), T, d, pos,
+            _flat_heads(q, shape, keep), _flat_heads(k, ks, keep), _flat_heads(v, ks, keep), T, d, pos,
             _int32(slots, (T,), dev, "slots"), freq, 2 * half, amplitude, PAIRING[pairing], hk, hv, k_cache.shape[0],
             k_cache.shape[1], code, _HEADS(out_q.data_ptr(), Hq, 0, ost[0], ost[1]), _current_stream(dev)))
         return out_q
@@ -692,7 +694,7 @@ class ops:
                   prefix_v.get_device() == dev, "q and the prefix must share one 16-bit dtype and one device")
             P = ps[0]
             if P:
-                pk, pv = _flat_heads(prefix_k, keep), _flat_heads(prefix_v, keep)
+                pk, pv = _flat_heads(prefix_k, ps, keep), _flat_heads(prefix_v, ps, keep)
         _need(lens.dim() == 1, "lens must be int32 [requests]")
         R = lens.shape[0]
         table, blocks, stride = _table(block_table, R, dev)
@@ -710,7 +712,7 @@ class ops:
             space = q.new_empty(need // 2)  # 16-bit values; sizes are whole floats
             ws = space.data_ptr()
         check(lib().msst_prefix_attention(
-            _flat_heads(q, keep), T, starts, R, pk, pv, P, hk, hv, cs[0], cs[1], table, blocks, stride, own, d, scale,
+            _flat_heads(q, shape, keep), T, starts, R, pk, pv, P, hk, hv, cs[0], cs[1], table, blocks, stride, own, d, scale,
             code, _HEADS(out.data_ptr(), Hq, 0, so[0], so[1]), ws, need, _current_stream(dev)))
         return out
 

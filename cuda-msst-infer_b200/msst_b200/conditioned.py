@@ -10,7 +10,8 @@ ops.cross_attention.  The reference has no counterpart; its closest relative is 
 cross transformer (src/model_htdemucs.cu:600-664), whose cross attention has neither
 grouped heads, ragged encoder lengths nor adapters.
 
-    python -m msst_b200.conditioned          # one block on random data, prompt and single-token form
+    python -m msst_b200.conditioned          # one block on random data, prompt and single-token form, then tokens
+                                             # one by one behind a shared prefix (msst_b200.cached)
 """
 from __future__ import annotations
 
@@ -109,6 +110,31 @@ def main():
     print(f"prompt {tuple(y.shape)}, its last token alone differs by at most "
           f"{float((token - y[:, -1:]).abs().max()):.2g} (one bf16 step at the output's size: "
           f"{float(2.0 ** -8 * y[:, -1:].abs().max()):.2g})")
+    generate(block, k, v, who, lens)
+
+
+def generate(block, k, v, who, key_lens, prefix=300, steps=20):
+    """Rows one by one through a layer of both blocks: a CachedBlock over a shared prefix and each request's own
+    rows, then `block` over the encoder's states, each row the next one's input."""
+    from .cached import TokenCache, random_cached_block
+
+    torch = _torch()
+    layer = random_cached_block(dim=block.w["q"].shape[1], dtype=block.w["q"].dtype)
+    R = who.numel()
+    _, prefix_k, prefix_v = layer.prefill(torch.randn(prefix, block.w["q"].shape[1], device="cuda").to(block.w["q"].dtype))
+    cache = TokenCache(R, -(-steps // 16), layer.kv_heads, layer.head_dim, page_size=16, dtype=block.w["q"].dtype)
+    x = torch.randn(R, block.w["q"].shape[1], device="cuda").to(block.w["q"].dtype)
+    one = torch.ones_like(who)
+    for _ in range(steps):
+        step = cache.plan(one, R, start=prefix)
+        h = layer(x, prefix_k, prefix_v, cache, step, who, single=True)
+        y = block(h[:, None], k, v, who, positions=step.positions[:, None], key_lens=key_lens)[:, 0]
+        x = y / y.float().square().mean(-1, keepdim=True).sqrt().to(y.dtype)
+    cache.plan(-one, 0)  # all requests have ended
+    torch.cuda.synchronize()
+    print(f"{steps} tokens of {R} requests behind a prefix of {prefix}; {int(cache.free_count)} of "
+          f"{cache.free_pages.numel()} pages free at the end")
+    return x
 
 
 if __name__ == "__main__":

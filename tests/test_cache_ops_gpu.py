@@ -530,3 +530,110 @@ def test_far_slots_of_a_large_cache(cuda):
         torch.cat([_own_keys(torch, vc, table, i, n) for i, n in enumerate(lens)]), v)
     _attend_check(torch, y, *args, d ** -0.5, "bf16")
     _attend_check(torch, z, q2[last], *args[1:7], torch.arange(3), d ** -0.5, "bf16")
+
+
+# ------------------------------------------------------------------ together
+def _plain_block(torch, block, x, adapter):
+    """64-bit form of a CachedBlock on one request's whole sequence [N, dim] (adapter None: none), with the
+    16-bit roundings of what it stores: heads, rotated heads, attention, result."""
+    dt, d, Hq, Hk = x.dtype, block.head_dim, block.q_heads, block.kv_heads
+
+    def project(name, y):
+        z = y.double() @ block.w[name].double().T
+        if adapter is not None:
+            for rows, a in adapter:
+                if a >= 0:
+                    la, lb, sc = block.adapters[name]
+                    z[rows] += float(sc[a]) * (y[rows].double() @ la[a].double().T @ lb[a].double().T)
+        return z.to(dt)
+
+    qkv = project("qkv", x).view(x.shape[0], -1, d)
+    at = torch.arange(x.shape[0], device="cuda")
+    rot = [_rotate_ref(torch, y, at, block.inv_freq, block.amplitude, block.pairing)[0].to(dt).double()
+           for y in (qkv[:, :Hq], qkv[:, Hq:Hq + Hk])]
+    v = qkv[:, Hq + Hk:].double()
+    o = torch.empty(x.shape[0], Hq, d, dtype=torch.float64, device="cuda")
+    late = at > at[:, None]
+    for h in range(Hq):
+        s = (rot[0][:, h] @ rot[1][:, h * Hk // Hq].T * d ** -0.5).masked_fill(late, -torch.inf)
+        o[:, h] = torch.softmax(s, -1) @ v[:, h * Hk // Hq]
+    return x.double() + project("o", o.to(dt).view(x.shape[0], -1)).double()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("prec", ["fp16", "bf16"])
+def test_blocks_over_many_steps(cuda, prec, graph):
+    """A prefix, ragged prompts, single tokens (in a captured graph or not) and draft tokens through
+    plan, append, attention and projections, against each request's whole sequence at once.
+
+    The two sides round the same stored values to 16 bits and differ by fp32 sums before that, so a
+    value is off by a rounding here and there: heads, weights, attention and result, four of at most one
+    step of their size (2 u), which the next product averages; 8 u of the largest value covers them."""
+    torch = cuda
+    from msst_b200 import device_error
+    from msst_b200.cached import TokenCache, random_cached_block
+
+    block = random_cached_block(dim=256, q_heads=8, kv_heads=2, head_dim=64, dtype=_dt(torch, prec), seed=3,
+                                scaling="parts", factor=4.0, original=64)
+    P, prompts, singles, drafts = 150, [40, 1, 9, 17], 9, 3
+    R = len(prompts)
+    g = _gen(torch, 31)
+    rows = lambda n: torch.randn(n, 256, generator=g, device="cuda").to(_dt(torch, prec))  # noqa: E731
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    prefix, own = rows(P), [rows(n + singles + drafts) for n in prompts]
+    adapters = [0, -1, 2, 1]
+    y0, pk, pv = block.prefill(prefix)
+    u = U[prec]
+    want = _plain_block(torch, block, prefix, None)
+    _within(y0, want, 8 * u * want.abs().max() + 0 * want, "prefix")
+    cache = TokenCache(R, 5, 2, 64, page_size=16, dtype=_dt(torch, prec))
+    got = [[] for _ in range(R)]
+
+    def feed(new, single=False):
+        """The next new[r] rows of each request through the block."""
+        x = torch.cat([own[r][sum(map(len, got[r])):][:n] for r, n in enumerate(new)])
+        step = cache.plan(ints(new), sum(new), start=P)
+        who = ints(adapters).repeat_interleave(ints(new))
+        y = block(x, pk, pv, cache, step, who, single=single)
+        for r, n in enumerate(new):
+            got[r].append(y[sum(new[:r]):sum(new[:r + 1])])
+
+    feed(prompts)
+    if graph:
+        x, one, who = torch.empty(R, 256, dtype=_dt(torch, prec), device="cuda"), ints([1] * R), ints(adapters)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        saved = [t.clone() for t in (cache.lens, cache.block_table, cache.free_pages, cache.free_count)]
+        with torch.cuda.stream(side):
+            block(x, pk, pv, cache, cache.plan(one, R, start=P), who, single=True)  # (warm up)
+        side.synchronize()
+        for t, old in zip((cache.lens, cache.block_table, cache.free_pages, cache.free_count), saved):
+            t.copy_(old)
+        torch.cuda.synchronize()
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured, stream=side):
+            y = block(x, pk, pv, cache, cache.plan(one, R, start=P), who, single=True)
+        for i in range(singles):
+            x.copy_(torch.stack([own[r][prompts[r] + i] for r in range(R)]))
+            captured.replay()
+            for r in range(R):
+                got[r].append(y[r:r + 1].clone())
+    else:
+        for _ in range(singles):
+            feed([1] * R, single=True)
+    feed([drafts] * R)
+    assert device_error(True) == 0 and cache.lens.tolist() == [n + singles + drafts for n in prompts]
+    for r in range(R):
+        whole = torch.cat((prefix, own[r]))
+        want = _plain_block(torch, block, whole, [(slice(P, None), adapters[r])])[P:]
+        y = torch.cat(got[r])
+        _within(y, want, 8 * u * want.abs().max() + 0 * want, f"request {r}")
+    cache.plan(ints([-1] * R), 0)
+    assert int(cache.free_count) == cache.free_pages.numel() and cache.lens.tolist() == [0] * R
+
+
+def test_example_runs(cuda, capsys):
+    from msst_b200 import conditioned, device_error
+
+    conditioned.main()
+    assert "8 of 8 pages free" in capsys.readouterr().out and device_error(True) == 0
