@@ -137,3 +137,57 @@ def test_python_argument_checks():
         for bad in bads:
             with pytest.raises(ValueError):
                 op(**{**good, **bad})
+
+
+def _source(name):
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "cuda-msst-infer_b200", "csrc", name)) as f:
+        return f.read()
+
+
+@pytest.mark.parametrize("begin, end", [
+    ("// ------------------------------------------------------------ softmax + epilogue", "  __syncthreads();\n  if (warp == 1) {"),
+    ("// ------------------------------------------------------------ rows that nobody sees", "} else if (lane == 0) {"),
+    ("// ------------------------------------------------------------ the team's tiles", "if (!ok && lane == 0) {"),
+    ("  const int q_box =", "__global__"),
+])
+def test_whole_warp_roles_wait_together(begin, end):
+    """Where a wait gives up, lanes of a warp must not part (full-mask instructions follow): a wait cannot be made
+    to run out from outside, so the source is read."""
+    text = _source("prefix_attn.cu")
+    assert text.count(begin) == 1
+    role = text[text.index(begin):]
+    role = role[:role.index(end)]
+    assert "mbar_wait_warp" in role and "mbar_wait<" not in role and "ring->wait(" not in role
+
+
+def test_roles_end_after_their_own_copies():
+    text = _source("prefix_attn.cu")
+    assert text.count("mbar_drain_ring(") == 4  # K and V of the tile role, tiles and query rows of the token role
+    assert text.count("umma_commit(mma_end)") == text.count("mbar_drain(mma_end, 0)") == 1
+
+
+def test_rope_frequencies():
+    import math
+
+    import torch
+    from msst_b200 import rope_frequencies
+
+    plain, one = rope_frequencies(64, 10000.0)
+    assert plain.dtype == torch.float64 and plain.shape == (32,) and one == 1.0
+    assert torch.allclose(plain, 10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32), rtol=1e-14)
+    assert torch.equal(rope_frequencies(64, scaling="linear", factor=4.0)[0], plain / 4)
+    wide, _ = rope_frequencies(64, scaling="base", factor=4.0)
+    assert abs(float(wide[0] - plain[0])) < 1e-15 and abs(float(wide[-1] / plain[-1]) - 0.25) < 1e-12
+    parts, amplitude = rope_frequencies(64, scaling="parts", factor=8.0, original=4096)
+    turns = plain * 4096 / (2 * math.pi)
+    assert torch.equal(parts[turns > 32], plain[turns > 32]) and amplitude == 1 + 0.1 * math.log(8.0)
+    assert torch.allclose(parts[turns < 1], plain[turns < 1] / 8, rtol=1e-14)
+    between = (turns >= 1) & (turns <= 32)
+    assert bool((parts[between] <= plain[between]).all()) and bool((parts[between] >= plain[between] / 8).all())
+    for bad in (dict(rot_dim=3), dict(rot_dim=0), dict(base=0.0), dict(scaling="ntk"), dict(factor=-1.0),
+                dict(scaling="parts", slow=4.0, fast=2.0)):
+        with pytest.raises(ValueError):
+            rope_frequencies(**{"rot_dim": 64, **bad})
