@@ -1592,10 +1592,13 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   g.q_slots = most_rows <= 8 ? 2 : 1;
   const int team_bytes = (int)C::kTiles / g.teams - g.q_slots * g.heads * g.q_rows * 128 * C::kHalves;
   g.entries = std::min(kMostEntries, team_bytes / (g.heads * (int)C::kEntry));
-  // measured: microseconds of an SM in units of 10 ns
+  // What a unit takes of an SM in units of 10 ns: a tile unit 2.1 us of the chain; a token unit what its bytes take.  An
+  // item's start and end is as long as four tile units (its query rows, the first scores, the last product, the rows written):
+  // with 1, 2 and 3 a prompt of 4096 tokens, 32/8 heads of 128, took 224, 210 and 194 us, with 4 and 6 190; 64 single
+  // tokens behind 8192 keys 57, 51, 51 and 51, 50.  Token units at 18 and 30: 51 and 55.
   g.tile_cost = 215;
-  g.token_cost = g.heads * (DP == 128 ? 22 : 15);
-  g.tile_item = 1;
+  g.token_cost = g.heads * (DP == 128 ? 22 : 16);
+  g.tile_item = 4;
   g.token_item = 1;
   const int page = 1 << p.page_shift;
   g.box = std::min(page, kTokenKeys);
