@@ -441,12 +441,20 @@ __device__ __forceinline__ void store8(float* to, const float* v) {
                : "memory");
 }
 
-// Whether one of the 16-bit values in w is an infinity or NaN.
-template <typename T>
-__device__ __forceinline__ bool any_non_finite(uint32_t w) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || (w >> 16 & e) == e;
-}
+// Infinities and NaN among 16-bit values: the largest magnitudes so far, for the even and the odd ones, as whole
+// numbers; theirs are the largest of all.
+struct Magnitude {
+  uint32_t top = 0;
+  __device__ __forceinline__ void add(const uint4& v) {
+    top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu));
+    top = __vmaxu2(top, v.w & 0x7fff7fffu);
+  }
+  template <typename T>
+  __device__ __forceinline__ bool finite() const {
+    constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    return (top & 0xffffu) < e && top >> 16 < e;
+  }
+};
 
 // ------------------------------------------------------------------------------- tile items
 template <typename T, int DP>
@@ -717,16 +725,15 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
             }
             if (klo < min(khi, 128)) {
               // rows that some see and others do not: 0 * NaN would reach the others
-              bool found = false;
+              Magnitude seen;
               for (int row = max(klo, 0) + lane; row < min(khi, 128); row += 32) {
 #pragma unroll
                 for (int x = 0; x < 8 * C::kHalves; ++x) {
-                  const uint4 v = *reinterpret_cast<const uint4*>(tile_at + row * 128 + (x >> 3) * kHalfBytes +
-                                                                  (((x + lane) & 7) << 4));
-                  found |= any_non_finite<T>(v.x) || any_non_finite<T>(v.y) || any_non_finite<T>(v.z) || any_non_finite<T>(v.w);
+                  seen.add(*reinterpret_cast<const uint4*>(tile_at + row * 128 + (x >> 3) * kHalfBytes +
+                                                           (((x + lane) & 7) << 4)));
                 }
               }
-              if (__any_sync(0xffffffffu, found) && !bad) {
+              if (__any_sync(0xffffffffu, !seen.finite<T>()) && !bad) {
                 bad = 1;
                 if (lane == 0) *s_bad = *s_bad | 1u << (s & 31);
               }
@@ -957,6 +964,29 @@ __device__ __forceinline__ uint32_t token_piece(uint32_t tile, uint32_t box, int
   return tile + (uint32_t)(chunk >> 3) * box + (uint32_t)(row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
+// The V rows of a tile that not all rows see, a lane a key: zeroed from key khi on, which is not there (0 * NaN would
+// reach the sum); whether one of the others from klo on, which some see and others do not, holds an infinity or NaN.
+// (Out of the loop's way: its instructions are fetched again and again, and masks on every fragment were a third of them.)
+template <typename T, int kHalves>
+__device__ __noinline__ bool clear_keys(uint8_t* tile, uint32_t half_bytes, int row0, int row16, int klo, int khi, int lane) {
+  uint8_t* row = tile + (lane < 16 ? row0 + lane : row0 + row16 + lane - 16) * 128;
+  Magnitude seen;
+  if (lane >= klo) {
+#pragma unroll 1
+    for (int x = 0; x < 8 * kHalves; ++x) {
+      uint4* piece = reinterpret_cast<uint4*>(row + (x >> 3) * half_bytes + (((x + lane) & 7) << 4));
+      if (lane >= khi) {
+        *piece = make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        seen.add(*piece);
+      }
+    }
+  }
+  fence_proxy_async_smem();  // the tile's place is given back to TMA after these writes
+  __syncwarp();
+  return !seen.finite<T>();
+}
+
 struct Team {  // in shared memory
   Segment seg[2];
   uint64_t seg_full[2], seg_empty[2], full[kMostEntries], empty[kMostEntries], q_full[2], q_empty[2];
@@ -1185,14 +1215,9 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& qmap, const CUtenso
       for (int h = 0; h < 2; ++h)
         l[h] += ((sc[0][2 * h] + sc[0][2 * h + 1]) + (sc[1][2 * h] + sc[1][2 * h + 1])) +
                 ((sc[2][2 * h] + sc[2][2 * h + 1]) + (sc[3][2 * h] + sc[3][2 * h + 1]));
-      // keys that are not there: their V is taken as zero (0 * NaN would reach the sum)
-      uint32_t keep[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        keep[i] = (8 * i + qc * 2 < khi ? 0xffffu : 0u) | (8 * i + qc * 2 + 1 < khi ? 0xffff0000u : 0u);
-      const bool some = klo < min(khi, kTokenKeys);  // keys that some rows see and others do not
       if (!(ok = mbar_wait_warp<false>(&tm->full[at], phase, kErrTimeoutAttnKV, abort_flag))) break;
       const uint32_t vt = base + at * entry_bytes;
+      if (!all) bad |= clear_keys<T, kHalves>(tiles + at * entry_bytes, half_bytes, row0, row16, klo, khi, lane);
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         // a tile's products in accumulators of their own, added in fp32 (see cross_token.cu)
@@ -1201,14 +1226,6 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& qmap, const CUtenso
         for (int y = 0; y < 2; ++y) {
           uint32_t b[4];
           ldmatrix4_trans(token_piece(vt, half_bytes, row0 + y * row16 + vrow, 2 * i + vchunk), b);
-          if (!all) {
-            b[0] &= keep[2 * y];
-            b[1] &= keep[2 * y + 1];
-            b[2] &= keep[2 * y];
-            b[3] &= keep[2 * y + 1];
-            if (some)
-              bad |= any_non_finite<T>(b[0]) || any_non_finite<T>(b[1]) || any_non_finite<T>(b[2]) || any_non_finite<T>(b[3]);
-          }
           mma16816<T>(d[0], pa[y], b[0], b[1]);
           mma16816<T>(d[1], pa[y], b[2], b[3]);
         }
@@ -1432,9 +1449,10 @@ __global__ void __launch_bounds__(256, 2)
   if (row >= rows) return;
   const int token = (int)(row / p.q.heads), head = (int)(row - (long long)token * p.q.heads);
   wait_for_previous();
+  const bool of_a_request = !p.q_starts || (token >= first_row(p, 0) && token < first_row(p, p.requests));
   const int code0 = g.concat ? 0 : g.where[row], code1 = g.where[rows + row];
   if (g.concat && code1 >= 0 && code1 >> 20 == 0) return;
-  if (request_of(p, token) < 0) return;
+  if (!of_a_request) return;
   bool again = code0 < 0 || code1 < 0;
   Sum sum;
   if (!again) {
@@ -1446,7 +1464,7 @@ __global__ void __launch_bounds__(256, 2)
     Parts a, b;
     if (!g.concat) a.find(g, code0, place(code0), g.whole + (size_t)row * g.ld, ctas);
     b.find(g, code1, place(code1), g.whole + (size_t)(rows + row) * g.ld, ctas);
-    add_parts<kWide ? 4 : 8>(a, b, kWide ? warp : 0, kWide ? 8 : 1, d, lane * 4, sum, again);
+    add_parts<8>(a, b, kWide ? warp : 0, kWide ? 8 : 1, d, lane * 4, sum, again);
   }
   if constexpr (kWide) {
     s_o[warp][lane] = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
