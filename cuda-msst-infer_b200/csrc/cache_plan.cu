@@ -6,9 +6,11 @@
 //   free[count + back(r) + b] = table[r][b]              of an ended request,
 //   table[r][have(r) + b] = free[top - 1 - need(r) - b]  of one that grows.
 // Every CTA of a cluster scans all requests for itself (a few KB), so that a page or a
-// token can be placed by any thread; what is read is written only past the cluster's barrier.
+// token can be placed by any thread; lengths and count, which may be updated in place, are written only past the
+// cluster's barrier.
 //
-// Bound: latency (two scans and a chain of three loads).
+// Bound: latency (two scans and a chain of three loads): 64 requests of one token 3.8 us, 1024 requests 7.6, prompts of
+// 48060 tokens (384 KB written) on eight CTAs 9.8.  With three scans of 1024 threads for whatever sizes: 8.5, 11.0, 12.4.
 #include <algorithm>
 
 #include "cache_ops.cuh"

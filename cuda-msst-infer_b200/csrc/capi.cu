@@ -749,6 +749,78 @@ int msst_prefix_attention(const msst_heads* q, int tokens, const int* q_starts, 
   });
 }
 
+int msst_call(int op, const msst_word* args) {
+  if (!args || op < MSST_CALL_CACHE_PLAN || op > MSST_CALL_PREFIX_ATTENTION)
+    return guarded([] { MSST_REQUIRE(false, "msst_call: unknown operation or no arguments"); });
+  const msst_word* a = args;
+  auto i64 = [&] { return (a++)->i; };
+  auto i32 = [&] { return (int)std::min(std::max((a++)->i, -0x80000000LL), 0x7fffffffLL); };
+  auto f32 = [&] { return (float)(a++)->f; };
+  auto ptr = [&] { return (a++)->p; };
+  auto ints = [&] { return static_cast<int*>((a++)->p); };
+  auto heads = [&] {
+    msst_heads h;
+    h.data = ptr();
+    h.heads = i32();
+    h.batch_stride = i64();
+    h.seq_stride = i64();
+    h.head_stride = i64();
+    return h;
+  };
+  auto or_null = [](const msst_heads& h) { return h.heads ? &h : nullptr; };
+  // (one by one: the order of a call's arguments is not that of their evaluation)
+  if (op == MSST_CALL_CACHE_PLAN) {
+    const int *new_tokens = ints(), *lens = ints();
+    const int requests = i32();
+    int* table = ints();
+    const int blocks = i32();
+    const long long stride = i64();
+    int* free_pages = ints();
+    const int pages = i32();
+    const int* free_count = ints();
+    const int page_size = i32(), start = i32(), tokens = i32();
+    int *out_lens = ints(), *out_count = ints(), *q_starts = ints(), *slots = ints(), *positions = ints();
+    return msst_cache_plan(new_tokens, lens, requests, table, blocks, stride, free_pages, pages, free_count, page_size, start,
+                           tokens, out_lens, out_count, q_starts, slots, positions, ptr());
+  }
+  if (op == MSST_CALL_ROPE_APPEND) {
+    const msst_heads q = heads(), k = heads(), v = heads();
+    const int tokens = i32(), head_dim = i32();
+    const int *positions = ints(), *slots = ints();
+    const double* inv_freq = static_cast<double*>(ptr());
+    const int rot_dim = i32();
+    const float amplitude = f32();
+    const int pairing = i32();
+    const msst_heads k_cache = heads(), v_cache = heads();
+    const int pages = i32(), page_size = i32(), dtype = i32();
+    const msst_heads q_out = heads();
+    return msst_rope_append(or_null(q), or_null(k), or_null(v), tokens, head_dim, positions, slots, inv_freq, rot_dim,
+                            amplitude, pairing, or_null(k_cache), or_null(v_cache), pages, page_size, dtype, or_null(q_out),
+                            ptr());
+  }
+  const msst_heads q = heads();
+  const int tokens = i32();
+  const int* q_starts = ints();
+  const int requests = i32();
+  const msst_heads prefix_k = heads(), prefix_v = heads();
+  const int prefix_len = i32();
+  const msst_heads k_cache = heads(), v_cache = heads();
+  const int pages = i32(), page_size = i32();
+  const int* table = ints();
+  const int blocks = i32();
+  const long long stride = i64();
+  const int* lens = ints();
+  const int head_dim = i32();
+  const float scale = f32();
+  const int dtype = i32();
+  const msst_heads out = heads();
+  void* ws = ptr();
+  const long long ws_bytes = i64();
+  return msst_prefix_attention(or_null(q), tokens, q_starts, requests, or_null(prefix_k), or_null(prefix_v), prefix_len,
+                               or_null(k_cache), or_null(v_cache), pages, page_size, table, blocks, stride, lens, head_dim,
+                               scale, dtype, or_null(out), ws, ws_bytes, ptr());
+}
+
 int msst_grouped_gemm(int num_groups, const msst_gemm_group* groups, const void* x, long long x_rows, long long ldx,
                       const void* w, long long w_rows, long long ldw, int epilogue, int act, int dtype, void* out,
                       long long out_rows, long long ldo, void* stream) {

@@ -7,23 +7,33 @@
 // tiles and each K/V tile of the prefix is read for 256 rows, not for a request's few.  The own
 // part has an item for each request and key head.
 //
-// One launch does both.  Items are cut into units (a K/V tile of 128 keys for a pair of row tiles, two
-// for a lone one; 64 keys for up to 16 rows), in two sequences:
-//   tile items   more than 16 rows: tcgen05, 128-row tiles (tile_role, as cross_attn.cu)
-//   token items  up to 16 rows, a request's single token or a few: mma.sync (token_role, as
-//                cross_token.cu), bound by reading K and V
-// Every CTA sums the units of both from the lengths, shares the CTAs out by what a unit of each costs
-// and takes an equal contiguous run of its sequence.  The prefix's products and the reading of the
-// requests' own pages so overlap, and nothing is known on the host but the tensors' sizes.
-// prefix_join_kernel adds up the parts of a row in a fixed order.
+// One launch does both, with one CTA an SM.  Items are cut into units, in two sequences:
+//   tile items   more than 16 rows a key head: tcgen05, pairs of 128-row tiles of one key head (tile_role, as
+//                cross_attn.cu); a unit is a K/V tile of 128 keys for a pair, two for a lone tile
+//   token items  up to 16 rows, a request's single token or a few: mma.sync (token_role), up to eight key heads at a
+//                time; a unit is a K/V tile of 32 keys of these heads
+// Every CTA sums the units of both from the lengths (find_runs), shares the CTAs out by what a unit of each
+// costs and takes an equal contiguous run of its sequence.  The prefix's products and the reading of the
+// requests' own pages so overlap, and the host knows nothing but the tensors' sizes (a captured call may be
+// replayed with other lengths).  The parts of a row are joined by a second launch in a fixed order.
 //
 // Long prompts (256 rows a request and more) take prefix and own keys as one sequence instead: the rows of one
-// request fill the tiles, and only items that a CTA's run cuts are joined.
+// request fill the tiles, and only the items that the runs cut are joined.
 //
 // What a row does not see is selected away; V rows past a request's last token are zeroed in shared memory
-// before the MMA.  The V rows of new tokens cannot be, as later rows see them: where one of
+// before the product.  The V rows of new tokens cannot be, as later rows see them: where one of
 // those holds an infinity or NaN (0 * NaN would reach the rows before), the item's rows are computed again, key by
-// key, by the joining kernel.
+// key, by the joining launch.
+//
+// Measured (one B200, both launches, in a CUDA graph) and what bounds it:
+//   64 requests, one token each, 8192 keys of prefix, up to 1024 own, 32/8 heads of 128: 51 us.  Memory: 173 MB, most of
+//     them at 6 TB/s; 8 us before the first tiles, then CTAs of equal runs end between 31 and 48 us, as the SMs do
+//     not share the memory's rate equally (in whatever order the two kinds of CTA are put: taking turns over the grid, 63 us)
+//   16 tokens, 131072 keys of prefix: 107 us, 555 MB at 5.2 TB/s
+//   4096 tokens of six prompts, 4096 keys of prefix: 320 us, 1.0 PFLOP/s; tensor and XU pipe half busy each (the chain
+//     scores, softmax, product behind one buffer of scores a tile, as in cross_attn.cu)
+//   32 requests of 5 tokens, 3791 keys, 12/4 heads of 80: 26 us, all of it latency: 2.5 us to find the runs, 4 to the first
+//     tile, three or four units, 2 to the second launch and 5 in it
 #include <algorithm>
 
 #include "attn_steps.cuh"
@@ -151,8 +161,8 @@ __device__ __forceinline__ long long prefix_weight(const PrefixGeom& g, bool tok
                                   g.lone * (((prefix_part(g, false) + 1) >> 1) + g.tile_item));
 }
 
-// The run of a worker, a CTA (tile items) or a team of its warps (token items): weights [u0, u0 + count) of the U of its sequence,
-// worker `self` of `workers`; where it starts.
+// The run of a worker, a CTA (tile items) or a team of its warps (token items): weights [u0, u0 + count) of the U of
+// its sequence, worker `self` of `workers`; where it starts.
 struct Run {
   long long u0, count, U;
   int token, self, workers, place;  // place: among the teams of all CTAs, the tile items' as team 0
@@ -956,9 +966,10 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
 // and each warp multiplies them by its head's 16 rows and writes its parts from its registers; no warp waits for
 // another.  With fewer key heads a CTA has up to four teams with runs of their own.  A warp a team
 // brings the tiles, K and V in turn through one ring.
-// Measured on the way (64 requests of up to 1024 own tokens, 8 key heads of 128, without a prefix): tiles of one
-// head shared out over eight warps that met at each item's end, 42 us; a run for each warp, which asked for
-// its own tiles, 62.
+// Bound: memory, 64 requests of up to 1024 own tokens, 8 key heads of 128, without a prefix: 135 MB in 31 us.  On the way
+// to it: tiles of one head shared out over eight warps that met at each item's end, 37 us; a run for
+// each warp, which asked for its own tiles, 57 (its warps stood still while the TMA unit was busy, and the parts of a
+// cache line were asked for at different times).
 // 16-byte piece `chunk` (8 columns) of row `row` in a 128B-swizzled tile of 64-column boxes of `box` bytes
 __device__ __forceinline__ uint32_t token_piece(uint32_t tile, uint32_t box, int row, int chunk) {
   return tile + (uint32_t)(chunk >> 3) * box + (uint32_t)(row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
@@ -1486,8 +1497,8 @@ __global__ void __launch_bounds__(256, 2)
 }
 
 // The same for many rows of one sequence of prefix and own keys, most of which are done: block (x, y) takes rows
-// [8 y, 8 y + 8) of the item that worker x started and did not end (4096 rows of 32 heads, 37,000 of them cut: by the
-// kernel above, which looks at all, 26 us).
+// [8 y, 8 y + 8) of the item that worker x started and did not end.  (4096 tokens of 32 heads, 37,000 rows of them cut:
+// about 10 us; looking through all rows, 26.)
 template <typename T>
 __global__ void __launch_bounds__(256, 4)
     prefix_join_cuts_kernel(const __grid_constant__ PrefixAttnParams p, const __grid_constant__ PrefixGeom g, int ctas) {
@@ -1611,9 +1622,9 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   const int team_bytes = (int)C::kTiles / g.teams - g.q_slots * g.heads * g.q_rows * 128 * C::kHalves;
   g.entries = std::min(kMostEntries, team_bytes / (g.heads * (int)C::kEntry));
   // What a unit takes of an SM in units of 10 ns: a tile unit 2.1 us of the chain; a token unit what its bytes take.  An
-  // item's start and end is as long as four tile units (its query rows, the first scores, the last product, the rows written):
-  // with 1, 2 and 3 a prompt of 4096 tokens, 32/8 heads of 128, took 224, 210 and 194 us, with 4 and 6 190; 64 single
-  // tokens behind 8192 keys 57, 51, 51 and 51, 50.  Token units at 18 and 30: 51 and 55.
+  // item's start and end is as long as three or four tile units (its query rows, the first scores, the last product, the
+  // rows written): with 2, 3 and 4 a prompt of 4096 tokens, 32/8 heads of 128, takes 186, 179 and 180 us and 64 single
+  // tokens behind 8192 keys 53, 51 and 51.  Token units at 18, 26 and 30: 51, 53 and 55.
   g.tile_cost = 215;
   g.token_cost = g.heads * (DP == 128 ? 22 : 16);
   g.tile_item = 4;

@@ -9,7 +9,8 @@
 //
 // 8 columns a lane, a group of lanes (the power of two that covers head_dim / 8) takes four heads of a
 // token, so a lane's four angles serve four heads.
-// Bound: HBM, from a few thousand tokens; launch latency below.
+// Bound: HBM: 403 MB (16384 tokens, 32 + 8 + 8 heads of 128) in 62 us, 6.5 TB/s, with loads and stores marked as streaming
+// above L2's size; 5685 tokens of 8 + 8 + 8 heads of 48 6.6 us (4.0 TB/s), one token of 64 requests 2.7 us.
 #include "cache_ops.cuh"
 #include "common.cuh"
 #include "runtime.h"

@@ -33,7 +33,7 @@ EXPORTS = [
     "msst_kernel_timing_report", "msst_rmsnorm", "msst_gemm", "msst_gemm_qkv_rope",
     "msst_attention", "msst_layernorm", "msst_sdpa", "msst_qk_norm_rope", "msst_cross_attention_workspace",
     "msst_cross_attention", "msst_adapter_gemm_workspace", "msst_adapter_gemm", "msst_cache_plan", "msst_rope_append",
-    "msst_prefix_attention_workspace", "msst_prefix_attention", "msst_grouped_gemm", "msst_band_gather", "msst_mask_apply", "msst_model_band_tables",
+    "msst_prefix_attention_workspace", "msst_prefix_attention", "msst_call", "msst_grouped_gemm", "msst_band_gather", "msst_mask_apply", "msst_model_band_tables",
     "msst_roformer_attn_block", "msst_roformer_ffn_block", "msst_model_load", "msst_model_free", "msst_model_get_info", "msst_model_forward",
     "msst_model_masks", "msst_model_transformer", "msst_model_transformer_noalloc", "msst_model_separate", "msst_model_separate_host",
     "msst_model_chunk_plan", "msst_model_forward_chunks", "msst_model_stitch",
@@ -112,6 +112,7 @@ def lib():
     L.msst_prefix_attention_workspace.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int, pi64]
     L.msst_prefix_attention.argtypes = [vp, c_int, vp, c_int, vp, vp, c_int, vp, vp, c_int, c_int, vp, c_int, i64, vp,
                                         c_int, c_float, c_int, vp, vp, i64, vp]
+    L.msst_call.argtypes = [c_int, vp]
     L.msst_grouped_gemm.argtypes = [c_int, ctypes.POINTER(GemmGroupC), vp, i64, i64, vp, i64, i64, c_int, c_int,
                                     c_int, vp, i64, i64, vp]
     L.msst_band_gather.argtypes = [vp, c_int, c_int, ctypes.POINTER(BandTables), c_int, vp, i64, vp]
@@ -309,8 +310,15 @@ def _table(t, requests, device):
     return t.data_ptr(), sh[1], st[0]
 
 
+# arguments of msst_call: words in the calls' order, five for a msst_heads
+_PLAN = struct.Struct("18q").pack
+_APPEND = struct.Struct("21qd20q").pack
+_ATTEND = struct.Struct("36qd9q").pack
+_NO_HEADS = (0, 0, 0, 0, 0)
+
+
 def _flat_heads(t, shape, keep):
-    """The msst_heads of a [tokens, heads, head_dim] tensor; one that 16-byte loads cannot walk is
+    """The five words of a [tokens, heads, head_dim] tensor; one that 16-byte loads cannot walk is
     copied first (kept alive in `keep`)."""
     n, h, d = shape
     s0, s1, s2 = t.stride()
@@ -320,15 +328,15 @@ def _flat_heads(t, shape, keep):
         keep.append(t)
         s0, s1, _ = t.stride()
         p = t.data_ptr()
-    return _HEADS(p, h, 0, s0, s1)
+    return p, h, 0, s0, s1
 
 
 def _cache_heads(t, dt, dev, what):
-    """The msst_heads of a cache [pages, page_size, heads, head_dim] (never a copy)."""
+    """The five words of a cache [pages, page_size, heads, head_dim] (never a copy)."""
     st = t.stride()
     if len(st) != 4 or t.dtype is not dt or t.get_device() != dev or (st[3] != 1 and t.shape[3] > 1):
         raise ValueError(f"{what} must be [pages, page_size, heads, head_dim] with q's type and device, unit last stride")
-    return _HEADS(t.data_ptr(), t.shape[2], st[0], st[1], st[2])
+    return t.data_ptr(), t.shape[2], st[0], st[1], st[2]
 
 
 def rope_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, original=8192, slow=1.0, fast=32.0, device=None):
@@ -620,9 +628,9 @@ class ops:
             out_free_count, to_count = new_count, at + 4 * (2 * R + 1 + 2 * tokens)
         else:
             to_count = _int32(out_free_count, (1,), dev, "out_free_count")
-        check(lib().msst_cache_plan(new, old, R, table, blocks, stride, free, free_pages.shape[0], count, page_size, start,
-                                    tokens, to_lens, to_count, at, at + 4 * (R + 1), at + 4 * (R + 1 + tokens),
-                                    _current_stream(dev)))
+        check(lib().msst_call(0, _PLAN(new, old, R, table, blocks, stride, free, free_pages.shape[0], count, page_size, start,
+                                       tokens, to_lens, to_count, at, at + 4 * (R + 1), at + 4 * (R + 1 + tokens),
+                                       _current_stream(dev))))
         return q_starts, slots, positions, out_lens, out_free_count
 
     @staticmethod
@@ -646,7 +654,7 @@ class ops:
         T, Hq, d = shape
         hk, hv = _cache_heads(k_cache, dt, dev, "k_cache"), _cache_heads(v_cache, dt, dev, "v_cache")
         _need(k_cache.shape == v_cache.shape and k_cache.shape[2:] == ks[1:], "the caches must have k's heads and head_dim")
-        half, freq, pos = 0, None, None
+        half, freq, pos = 0, 0, 0
         if inv_freq is not None:
             _need(inv_freq.dtype is torch.float64 and inv_freq.dim() == 1 and inv_freq.get_device() == dev,
                   "inv_freq must be float64 [rot / 2] on q's device")
@@ -658,10 +666,10 @@ class ops:
             _need(out_q.shape == shape and out_q.dtype is dt and out_q.get_device() == dev and
                   (out_q.stride(2) == 1 or d < 2), "out_q must have q's shape, type and device, and unit last stride")
         ost = out_q.stride()
-        check(lib().msst_rope_append(
-            _flat_heads(q, shape, keep), _flat_heads(k, ks, keep), _flat_heads(v, ks, keep), T, d, pos,
-            _int32(slots, (T,), dev, "slots"), freq, 2 * half, amplitude, PAIRING[pairing], hk, hv, k_cache.shape[0],
-            k_cache.shape[1], code, _HEADS(out_q.data_ptr(), Hq, 0, ost[0], ost[1]), _current_stream(dev)))
+        check(lib().msst_call(1, _APPEND(
+            *_flat_heads(q, shape, keep), *_flat_heads(k, ks, keep), *_flat_heads(v, ks, keep), T, d, pos,
+            _int32(slots, (T,), dev, "slots"), freq, 2 * half, amplitude, PAIRING[pairing], *hk, *hv, k_cache.shape[0],
+            k_cache.shape[1], code, out_q.data_ptr(), Hq, 0, ost[0], ost[1], _current_stream(dev))))
         return out_q
 
     @staticmethod
@@ -685,7 +693,7 @@ class ops:
         _need(Hk > 0 and Hq > 0 and Hq % Hk == 0, "q must have a multiple of the caches' heads")
         hk, hv = _cache_heads(k_cache, dt, dev, "k_cache"), _cache_heads(v_cache, dt, dev, "v_cache")
         _need((prefix_k is None) == (prefix_v is None), "prefix_k and prefix_v go together")
-        P, pk, pv = 0, None, None
+        P, pk, pv = 0, _NO_HEADS, _NO_HEADS
         if prefix_k is not None:
             ps = prefix_k.shape
             _need(len(ps) == 3 and ps[1] == Hk and ps[2] == d and prefix_v.shape == ps,
@@ -698,7 +706,7 @@ class ops:
         _need(lens.dim() == 1, "lens must be int32 [requests]")
         R = lens.shape[0]
         table, blocks, stride = _table(block_table, R, dev)
-        own, starts = _int32(lens, (R,), dev, "lens"), None
+        own, starts = _int32(lens, (R,), dev, "lens"), 0
         if q_starts is not None:
             starts = _int32(q_starts, (R + 1,), dev, "q_starts")
         if out is None:
@@ -707,13 +715,13 @@ class ops:
             _need(out.shape == shape and out.dtype is dt and out.get_device() == dev and (out.stride(2) == 1 or d < 2),
                   "out must have q's shape, type and device, and unit last stride")
         so = out.stride()
-        need, ws = _workspace("prefix_attention", dev, T, R, P, Hq, Hk, d), None
+        need, ws = _workspace("prefix_attention", dev, T, R, P, Hq, Hk, d), 0
         if need:
             space = q.new_empty(need // 2)  # 16-bit values; sizes are whole floats
             ws = space.data_ptr()
-        check(lib().msst_prefix_attention(
-            _flat_heads(q, shape, keep), T, starts, R, pk, pv, P, hk, hv, cs[0], cs[1], table, blocks, stride, own, d, scale,
-            code, _HEADS(out.data_ptr(), Hq, 0, so[0], so[1]), ws, need, _current_stream(dev)))
+        check(lib().msst_call(2, _ATTEND(
+            *_flat_heads(q, shape, keep), T, starts, R, *pk, *pv, P, *hk, *hv, cs[0], cs[1], table, blocks, stride, own, d,
+            scale, code, out.data_ptr(), Hq, 0, so[0], so[1], ws, need, _current_stream(dev))))
         return out
 
     @staticmethod

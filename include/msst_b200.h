@@ -294,6 +294,20 @@ int msst_prefix_attention(const msst_heads* q, int tokens, const int* q_starts, 
                           float scale, int dtype, const msst_heads* out, void* workspace, long long workspace_bytes,
                           void* stream);
 
+/* The three calls above with their arguments in one array, in their order, each an integer, a pointer or (float)
+ * a double in 64 bits, a msst_heads as its five members (a NULL one: data NULL and 0 heads); integers beyond 32
+ * bits count as the largest or smallest int.  For hosts whose foreign calls cost by the argument (Python's ctypes: 4.5 us for
+ * 18, 1.2 for two). */
+typedef union msst_word {
+  long long i;
+  double f;
+  void* p;
+} msst_word;
+#define MSST_CALL_CACHE_PLAN 0
+#define MSST_CALL_ROPE_APPEND 1
+#define MSST_CALL_PREFIX_ATTENTION 2
+int msst_call(int op, const msst_word* args);
+
 /* One problem of msst_grouped_gemm: rows [a_row0, a_row0 + m) and columns
  * [a_col0, a_col0 + k) of x times rows [b_row0, b_row0 + n) (same k columns from
  * b_col0) of W, written to out rows out_row0.. and columns out_col0.. (for

@@ -102,6 +102,47 @@ def test_workspace_refuses_heads(q_heads, kv_heads, head_dim):
     assert n.value == -1
 
 
+def test_calls_by_words():
+    """msst_call hands each argument on to its place: the refusals of the calls themselves, one argument wrong at a time."""
+    from msst_b200 import MSST_ERR_INVALID, MSST_OK, lib
+
+    L, big = lib(), 1 << 40
+
+    def call(op, form, words):
+        return L.msst_call(op, struct.pack(form, *words))
+
+    heads = [16, 2, 2048, 128, 64]
+    plan = [16, 16, 4, 16, 8, 8, 16, 64, 16, 16, 0, 4, 16, 16, 16, 16, 16, 0]
+    append = heads * 3 + [0, 64, 16, 16, 16, 64, 1.0, 0] + heads * 2 + [4, 16, 0] + heads + [0]
+    attend = heads + [0, 16, 2] + heads * 2 + [8] + heads * 2 + [4, 16, 16, 2, 2, 16, 64, 0.0, 0] + heads + [0, 0, 0]
+    for op, form, good, bads in (
+        (0, "18q", plan, ((0, 0, "null"), (1, 0, "null"), (2, 9000, "requests"), (3, 0, "block_table"), (4, big, "blocks"),
+                          (5, 7, "overlap"), (6, 0, "null"), (7, 0, "pages"), (8, 0, "null"), (9, 48, "page_size"),
+                          (10, -1, "positions"), (11, big, "tokens"), (11, -big, "tokens"), (12, 0, "null"), (13, 0, "null"),
+                          (14, 0, "null"), (15, 0, "null"), (16, 0, "null"))),
+        (1, "21qd20q", append, ((0, 24, "q must be"), (1, 0, "q needs"), (3, 132, "q needs strides"), (6, 0, "k needs"),
+                                (9, 60, "k needs strides"), (10, 8, "v must be"), (15, -1, "tokens"), (16, 60, "head_dim"),
+                                (20, 72, "rot_dim"), (21, float("nan"), "amplitude"), (22, 2, "pairing"), (24, 1, "same number"),
+                                (25, 0, "k_cache is written"), (30, -8, "v_cache has a negative"), (33, 0, "pages"),
+                                (34, 17, "page_size"), (35, 3, "dtype"), (37, 3, "q's heads"))),
+        (2, "36qd9q", attend, ((1, 3, "q's heads"), (5, -1, "shape"), (7, -1, "requests"), (8, 8, "prefix_k must be"),
+                               (9, 0, "prefix_k needs"), (14, 1, "caches' heads"), (18, -1, "shape"), (20, 0, "k_cache needs"),
+                               (25, 1, "same number"), (29, 0, "pages"), (30, 12, "page_size"), (31, 0, "block_table"),
+                               (32, -1, "blocks"), (33, 1, "overlap"), (35, 12, "head_dim"), (36, float("inf"), "scale"),
+                               (37, 2, "dtype"), (39, 4, "q's heads"))),
+    ):
+        if op:
+            assert call(op, form, good) == MSST_OK  # (no row: nothing is launched)
+        for at, value, word in bads:
+            wrong = list(good)
+            if op:
+                wrong[{1: 15, 2: 5}[op]] = 4  # rows, for which strides and pointers have to be right
+            wrong[at] = value
+            assert call(op, form, wrong) == MSST_ERR_INVALID, (op, at)
+            assert word in L.msst_last_error().decode(), (op, at, L.msst_last_error())
+    assert L.msst_call(3, struct.pack("q", 0)) == MSST_ERR_INVALID and L.msst_call(0, None) == MSST_ERR_INVALID
+
+
 def test_empty_calls_need_no_device():
     from msst_b200 import MSST_OK
 

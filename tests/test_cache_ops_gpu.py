@@ -469,7 +469,7 @@ def test_prefix_attention_rows_of_nobody(cuda):
         lens = [n + 20 for n in counts]
         q, pk, pv, kc, vc, table, own, starts = _attend_inputs(torch, counts, lens, 200, Hq, 2, 64, 16, "fp16", 13)
         y = ops.prefix_attention(q, pk, pv, kc, vc, table, own, q_starts=starts)
-        padded = torch.nn.functional.pad(q, (0, 0, 0, 0, 2, 37))
+        padded = torch.nn.functional.pad(q, (0, 0, 0, 0, 2, 37), value=float("nan"))
         wide = torch.full((padded.shape[0], Hq, 72), 5.0, dtype=q.dtype, device="cuda")
         out = wide[..., :64]
         ops.prefix_attention(padded, pk, pv, kc, vc, table, own, q_starts=starts + 2, out=out)
