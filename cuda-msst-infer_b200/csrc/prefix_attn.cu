@@ -786,73 +786,90 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         const uint32_t sAddr = tmem + lane_off + b.buf * 128;
         const int tile = k.kv_tile(w, k.j0 + t);
         const int khi = tile < k.ptiles ? p.prefix - tile * 128 : limit - (tile - k.ptiles) * 128;
-        const bool all = __all_sync(0xffffffffu, khi >= 128), any = __any_sync(0xffffffffu, khi > 0);
+        const bool all = __all_sync(0xffffffffu, khi >= 128);
         if (!mbar_wait_warp<false>(&s_full[b.buf], b.parity, kErrTimeoutAttnS, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
         if (warp_active) {
-          uint32_t words[4];
-#pragma unroll
-          for (int ch = 0; ch < 4; ++ch) words[ch] = len_word(khi, ch);
-          uint32_t pk[64];
-          if (any) {
+          bool done = false;
+          if (all) {
+            // every key is seen: one pass without a maximum, against the reference (at first that of 32 scores)
+            constexpr uint32_t kAllWords[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
             if (!have) {
               uint32_t r[32];
               tmem_ld32(sAddr, r);
               tmem_ld_wait(r);
-              // -inf for a row that sees none of these keys or whose scores are -inf: no reference yet, and
-              // sums against it are not finite, which sends every step through the exact passes until one finds a score
-              ref = chunk_max(r, words[0], c) - kRefShift<T>;
+              // (-inf where these scores are: sums against it are not finite)
+              ref = chunk_max(r, 0xffffffffu, c) - kRefShift<T>;
               have = true;
             }
-            float sum = all ? row_exp<T, true>(sAddr, words, c, ref, pk) : row_exp<T, false>(sAddr, words, c, ref, pk);
-            if (__any_sync(0xffffffffu, valid && !(sum <= kSumLimit<T>))) {
-              // exact passes: the reference moves to the row's maximum, O and l with it
-              float m = -INFINITY;
-#pragma unroll 1
-              for (int ch = 0; ch < 4; ++ch) {
-                uint32_t r[32], word = words[0];
-#pragma unroll
-                for (int i = 1; i < 4; ++i)
-                  if (i == ch) word = words[i];
-                tmem_ld32(sAddr + ch * 32, r);
-                tmem_ld_wait(r);
-                m = fmaxf(m, chunk_max(r, word, c));
-              }
-              const float moved = fmaxf(ref, m - kRefShift<T>), base = moved == -INFINITY ? 0.f : moved;
-              const float alpha = fast_exp2(ref - base);
-              if (t > 0) {
-                // O holds the previous steps once the last PV is through (the one before it was
-                // when this step's S was issued, so the parity is the right phase's)
-                if (!mbar_wait_warp<false>(&pv_done[w], (mine - 1) & 1, kErrTimeoutAttnO, abort_flag)) {
-                  ok = false;
-                  break;
-                }
-                tc_fence_after();
-#pragma unroll 1
-                for (int h = 0; h < DP / 32; ++h) {
-                  uint32_t r[32];
-                  tmem_ld32(oAddr + h * 32, r);
-                  tmem_ld_wait(r);
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-                  tmem_st32(oAddr + h * 32, r);
-                }
-                tmem_st_wait();
-              }
-              l *= alpha;
-              ref = moved;
-              sum = row_exp<T, false>(sAddr, words, c, base, pk);
+            uint32_t pk[64];
+            const float sum = row_exp<T, true>(sAddr, kAllWords, c, ref, pk);
+            done = __all_sync(0xffffffffu, !valid || sum <= kSumLimit<T>);
+            if (done) {
+              l += sum;
+              tmem_st32(sAddr, *reinterpret_cast<const uint32_t(*)[32]>(pk));
+              tmem_st32(sAddr + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
             }
-            l += sum;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) pk[i] = 0u;
           }
-          tmem_st32(sAddr, *reinterpret_cast<const uint32_t(*)[32]>(pk));
-          tmem_st32(sAddr + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
+          if (!done) {
+            // Some keys are not seen, or a sum has grown too large or is not finite: the reference moves to the row's
+            // maximum where that is above it, O and l with it, in two passes chunk by chunk.  (Rolled up, with one form for all
+            // masks: code that a short run meets once is fetched while it waits.)
+            float m = -INFINITY;
+#pragma unroll 1
+            for (int ch = 0; ch < 4; ++ch) {
+              uint32_t r[32];
+              tmem_ld32(sAddr + ch * 32, r);
+              tmem_ld_wait(r);
+              m = fmaxf(m, chunk_max(r, len_word(khi, ch), c));
+            }
+            if (!have) ref = -INFINITY;
+            have = true;
+            const float moved = fmaxf(ref, m - kRefShift<T>), base = moved == -INFINITY ? 0.f : moved;
+            const float alpha = fast_exp2(ref - base);
+            if (t > 0 && __any_sync(0xffffffffu, moved > ref)) {
+              // O holds the previous steps once the last PV is through (the one before it was
+              // when this step's S was issued, so the parity is the right phase's)
+              if (!mbar_wait_warp<false>(&pv_done[w], (mine - 1) & 1, kErrTimeoutAttnO, abort_flag)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+#pragma unroll 1
+              for (int h = 0; h < DP / 32; ++h) {
+                uint32_t r[32];
+                tmem_ld32(oAddr + h * 32, r);
+                tmem_ld_wait(r);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                tmem_st32(oAddr + h * 32, r);
+              }
+              tmem_st_wait();
+            }
+            l *= moved > ref ? alpha : 1.f;
+            ref = moved;
+            // P of chunk ch goes over scores of chunks that have been read
+#pragma unroll 1
+            for (int ch = 0; ch < 4; ++ch) {
+              uint32_t r[32], pk[16];
+              tmem_ld32(sAddr + ch * 32, r);
+              tmem_ld_wait(r);
+              const uint32_t word = len_word(khi, ch);
+              float sum = 0.f;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float e0 = word >> (2 * i) & 1 ? fast_exp2(__uint_as_float(r[2 * i]) * c - base) : 0.f;
+                const float e1 = word >> (2 * i + 1) & 1 ? fast_exp2(__uint_as_float(r[2 * i + 1]) * c - base) : 0.f;
+                sum += e0 + e1;
+                pk[i] = pack2<T>(e0, e1);
+              }
+              l += sum;
+              tmem_st16(sAddr + ch * 16, pk);
+            }
+          }
           tmem_st_wait();
         }
         // (a barrier a buffer: the tile's other warps may be a step ahead)
