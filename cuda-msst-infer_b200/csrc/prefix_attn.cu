@@ -622,12 +622,10 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         const uint64_t dv0 = sw128_desc(smem_u32(sV), kHalfBytes, 1024);
         constexpr uint32_t kTileDesc = C::kTile >> 4;
         const int ksteps = g.ksteps;
-        KPos kp;                    // next K slot to wait for
+        KPos kp;  // next K and V slots to wait for
         VPos vp;
-        uint32_t kc[2] = {0, 0};    // slots in use
-        uint32_t vc[2] = {0, 0};
-        uint32_t mine[2] = {0, 0}, pmine[2] = {0, 0};  // S and PV issued so far, per tile
-        uint32_t seq = 0;           // position in the sequence of the segment's first step
+        uint32_t kslot = 0, vslot = 0, turns = 0;  // slots in use; parity of each tile's steps (two buffers)
+        uint32_t seq = 0;  // position in the sequence of the segment's first step
         bool ok = true;
         for (; ok; ++s) {
           if (!(ok = ring->wait(s, abort_flag))) break;
@@ -639,59 +637,51 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
           // steps of the second tile: all, but for a lone tile's last unit without a K/V tile for it
           const int steps1 = k.uses(1, k.j1 - 1) ? steps : steps - 1;
           const bool lone = k.lone;
-          // S of step t of tile w
-          auto do_s = [&](const int w, const int t) -> bool {
-            if (t >= (w ? steps1 : steps)) return true;
-            if (w == 0 || lone) {
-              if (!mbar_wait<false>(&k_full[kp.slot], kp.phase, kErrTimeoutAttnKV, abort_flag)) return false;
-              kc[w] = kp.slot;
-              kp = kp.plus(1);
+          // Step n of the segment is step n / 2 of tile n % 2.  PV(n), and S(n + NB) behind it: NB scores ahead.
+          // (One copy of either, as all of this is fetched while the first tile waits.)
+#pragma unroll 1
+          for (int n = -NB; n < 2 * steps; ++n) {
+            if (n >= 0 && (n >> 1) < (n & 1 ? steps1 : steps)) {
+              const int w = n & 1, t = n >> 1;
+              if (w == 0 || lone) {
+                if (!(ok = mbar_wait<false>(&v_ready[vp.slot], vp.phase, kErrTimeoutAttnKV, abort_flag))) break;
+                vslot = vp.slot;
+                vp = vp.plus(1);
+              }
+              const StepBuf<NB> b(w, turns >> w, seq + n);
+              turns ^= 1u << w;
+              if (!(ok = mbar_wait<false>(&p_full[b.buf], b.parity, kErrTimeoutAttnP, abort_flag))) break;
               tc_fence_after();
-            }
-            const uint32_t slot = lone ? kc[w] : kc[0];
-            const StepBuf<NB> b(w, mine[w]++, seq + 2 * t + w);
-            const uint64_t dq = dq0 + (uint64_t)((lone ? 0 : w) * kTileDesc);
-            const uint64_t dk = dk0 + (uint64_t)(slot * kTileDesc);
-            const uint32_t dS = tmem + b.buf * 128;
+              const uint64_t dv = dv0 + (uint64_t)(vslot * kTileDesc);
+              const uint32_t pa = tmem + b.buf * 128, dO = tmem + C::kColO + (uint32_t)(w * DP);
+              umma_f16_ts(dO, pa, dv, idesc_o, t > 0);
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
-              if (kk >= ksteps) break;
-              const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
-              umma_f16_ss(dS, dq + off, dk + off, idesc_s, kk != 0);
+              for (int kk = 1; kk < 8; ++kk) umma_f16_ts(dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
+              umma_commit(&pv_done[w]);
+              if (w == 1 || lone) umma_commit(&v_empty[vslot]);
             }
-            umma_commit(&s_full[b.buf]);
-            if (w == 1 || lone) umma_commit(&k_empty[slot]);
-            return true;
-          };
-          // PV of step t of tile w
-          auto do_pv = [&](const int w, const int t) -> bool {
-            if (t >= (w ? steps1 : steps)) return true;
-            if (w == 0 || lone) {
-              if (!mbar_wait<false>(&v_ready[vp.slot], vp.phase, kErrTimeoutAttnKV, abort_flag)) return false;
-              vc[w] = vp.slot;
-              vp = vp.plus(1);
-            }
-            const uint32_t slot = lone ? vc[w] : vc[0];
-            const StepBuf<NB> b(w, pmine[w]++, seq + 2 * t + w);
-            if (!mbar_wait<false>(&p_full[b.buf], b.parity, kErrTimeoutAttnP, abort_flag)) return false;
-            tc_fence_after();
-            const uint64_t dv = dv0 + (uint64_t)(slot * kTileDesc);
-            const uint32_t pa = tmem + b.buf * 128, dO = tmem + C::kColO + (uint32_t)(w * DP);
-            umma_f16_ts(dO, pa, dv, idesc_o, t > 0);
+            if (n == 2 * steps - 2) umma_commit(&o_done[0]);
+            const int n2 = n + NB, w = n2 & 1;
+            if ((n2 >> 1) < (w ? steps1 : steps)) {
+              if (w == 0 || lone) {
+                if (!(ok = mbar_wait<false>(&k_full[kp.slot], kp.phase, kErrTimeoutAttnKV, abort_flag))) break;
+                kslot = kp.slot;
+                kp = kp.plus(1);
+                tc_fence_after();
+              }
+              const uint32_t dS = tmem + StepBuf<NB>(w, 0, seq + n2).buf * 128;
+              const uint64_t dq = dq0 + (uint64_t)((lone ? 0 : w) * kTileDesc);
+              const uint64_t dk = dk0 + (uint64_t)(kslot * kTileDesc);
 #pragma unroll
-            for (int kk = 1; kk < 8; ++kk) umma_f16_ts(dO, pa + (uint32_t)(kk * 8), dv + 128 * kk, idesc_o, 1u);
-            umma_commit(&pv_done[w]);
-            if (w == 1 || lone) umma_commit(&v_empty[slot]);
-            return true;
-          };
-          // S(s + NB) behind PV(s)
-          if (!(ok = do_s(0, 0) && do_s(1, 0) && (NB == 2 || do_s(0, 1)))) break;
-          for (int t = 0; t < steps; ++t) {
-            if (!(ok = do_pv(0, t))) break;
-            if (t == steps - 1) umma_commit(&o_done[0]);
-            if (!(ok = NB == 3 ? do_s(1, t + 1) : do_s(0, t + 1))) break;
-            if (!(ok = do_pv(1, t) && (NB == 3 ? do_s(0, t + 2) : do_s(1, t + 1)))) break;
-            if (t == (steps > 1 ? steps - 2 : 0)) umma_commit(q_empty);  // every S has been issued
+              for (int kk = 0; kk < DP / 16; ++kk) {
+                if (kk >= ksteps) break;
+                const uint64_t off = (uint64_t)((kk >> 2) * (kHalfBytes >> 4) + (kk & 3) * 2);
+                umma_f16_ss(dS, dq + off, dk + off, idesc_s, kk != 0);
+              }
+              umma_commit(&s_full[StepBuf<NB>(w, 0, seq + n2).buf]);
+              if (w == 1 || lone) umma_commit(&k_empty[kslot]);
+            }
+            if (n2 == 2 * steps - 1) umma_commit(q_empty);  // every S has been issued
           }
           if (ok) umma_commit(&o_done[1]);
           seq += (uint32_t)(steps + steps1);
@@ -1190,17 +1180,16 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& qmap, const CUtenso
       const int key0 = (pre ? jj : jj - ptiles) * kTokenKeys;
       const int khi = (pre ? p.prefix : own) - key0, klo = pre ? khi : common - key0;
       const bool all = klo >= kTokenKeys;
-      float mx[2] = {-INFINITY, -INFINITY};
+      float mx[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) (&sc[0][0])[i] *= c;
       if (!all) {
         const int lim[2] = {(pre ? khi : limit[0] - key0) - qc * 2, (pre ? khi : limit[1] - key0) - qc * 2};
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i)  // i: row half * 2 + key of the pair
-            sc[t][i] = 8 * t + (i & 1) < lim[i >> 1] ? sc[t][i] * c : -INFINITY;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) (&sc[0][0])[i] *= c;
+            if (8 * t + (i & 1) >= lim[i >> 1]) sc[t][i] = -INFINITY;
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
