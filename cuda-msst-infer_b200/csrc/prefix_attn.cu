@@ -35,6 +35,7 @@
 //   32 requests of 5 tokens, 3791 keys, 12/4 heads of 80: 26 us, all of it latency: 2.5 us to find the runs, 4 to the first
 //     tile, three or four units, 2 to the second launch and 5 in it
 #include <algorithm>
+#include <cstddef>
 
 #include "attn_steps.cuh"
 #include "cache_ops.cuh"
@@ -408,11 +409,8 @@ constexpr int kRing = 4;
 struct SegmentRing {
   Segment at[kRing];
   uint64_t full[kRing], empty[kRing];
-  __device__ void init(int readers) {
-    for (int i = 0; i < kRing; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], readers);
-    }
+  __device__ __forceinline__ void init(int readers, int lane) {
+    if (lane < 2 * kRing) mbar_init(&full[lane], lane < kRing ? 1 : readers);
   }
   // The s-th segment once it is there; a warp's lanes together, or one lane alone
   __device__ __forceinline__ bool wait_warp(int s, volatile int* abort_flag) {
@@ -501,31 +499,15 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
   static_assert(sizeof(SegmentRing) + (19 + 2 * C::kKSlots + 3 * C::kVSlots) * 8 + 16 + 2048 <= C::kTail, "");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
-    for (int i = 0; i < NB; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+  if (warp == 0) {
+    // a lane a barrier: softmax warps' 128 threads arrive at p_full, the two halves at meet, one thread elsewhere
+    constexpr int kBars = 19 + 2 * C::kKSlots + 3 * C::kVSlots;
+    for (int i = lane; i < kBars; i += 32) mbar_init(&bars[i], i >= 6 && i < 10 ? 128 : (i >= 14 && i < 18 ? 2 : 1));
+    ring->init(8, lane);  // the softmax warps are the last to need a segment
+    if (lane == 0) {
+      *abort_flag = 0;
+      *s_bad = 0;
     }
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(&pv_done[w], 1);
-      mbar_init(&o_done[w], 1);
-    }
-    for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
-    mbar_init(mma_end, 1);
-    for (int i = 0; i < C::kKSlots; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
-    }
-    for (int i = 0; i < C::kVSlots; ++i) {
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_ready[i], 1);
-      mbar_init(&v_empty[i], 1);
-    }
-    ring->init(8);  // the softmax warps, which are the last to need a segment
-    *abort_flag = 0;
-    *s_bad = 0;
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -1025,19 +1007,12 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& qmap, const CUtenso
   Run run{};
   if (team < g.teams) run = runs[team];
   __syncthreads();  // the runs have been read
-  if (threadIdx.x < g.teams) {
-    Team* x = reinterpret_cast<Team*>(smem + C::kTiles) + threadIdx.x;
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&x->seg_full[i], 1);
-      mbar_init(&x->seg_empty[i], g.heads);
-      mbar_init(&x->q_full[i], 1);
-      mbar_init(&x->q_empty[i], g.heads);
-    }
-    for (int i = 0; i < g.entries; ++i) {
-      mbar_init(&x->full[i], 1);
-      mbar_init(&x->empty[i], g.heads);
-    }
-    x->abort = 0;
+  if (warp < g.teams) {  // a lane a barrier: the team's warps arrive where something is given back
+    Team* x = reinterpret_cast<Team*>(smem + C::kTiles) + warp;
+    static_assert(offsetof(Team, abort) - offsetof(Team, seg_full) == 32 * sizeof(uint64_t), "");
+    const bool given_back = (lane >= 2 && lane < 4) || (lane >= 16 && lane < 28) || lane >= 30;
+    mbar_init(&x->seg_full[lane], given_back ? g.heads : 1);
+    if (lane == 0) x->abort = 0;
     mbar_fence_init();
   }
   __syncthreads();
