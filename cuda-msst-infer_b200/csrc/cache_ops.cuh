@@ -51,6 +51,7 @@ struct PrefixAttnParams {
   const int* table;             // [requests, blocks], row stride table_stride
   long long table_stride;
   int tokens, requests, prefix, pages, page_shift, blocks, head_dim;
+  int zero_rest;                // rows of no request: 0 left as they were, 1 zeroed
   float scale_log2;             // softmax scale * log2(e)
   float* ws;                    // prefix_attention_workspace() bytes
 };

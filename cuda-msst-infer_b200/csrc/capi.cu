@@ -695,8 +695,8 @@ int msst_prefix_attention(const msst_heads* q, int tokens, const int* q_starts, 
                           const msst_heads* prefix_k, const msst_heads* prefix_v, int prefix_len,
                           const msst_heads* k_cache, const msst_heads* v_cache, int pages, int page_size,
                           const int* block_table, int blocks, long long table_stride, const int* lens, int head_dim,
-                          float scale, int dtype, const msst_heads* out, void* workspace, long long workspace_bytes,
-                          void* stream) {
+                          float scale, int dtype, const msst_heads* out, int zero_rest, void* workspace,
+                          long long workspace_bytes, void* stream) {
   return guarded([&] {
     check_dtype(dtype);
     msst::PrefixAttnParams p{};
@@ -738,6 +738,7 @@ int msst_prefix_attention(const msst_heads* q, int tokens, const int* q_starts, 
     p.pages = pages;
     p.blocks = blocks;
     p.head_dim = head_dim;
+    p.zero_rest = zero_rest != 0;
     const float s = scale == 0.f ? 1.0f / std::sqrt((float)head_dim) : scale;
     p.scale_log2 = s * 1.4426950408889634f;
     DeviceScope dev_scope(device_of(q->data));
@@ -814,11 +815,12 @@ int msst_call(int op, const msst_word* args) {
   const float scale = f32();
   const int dtype = i32();
   const msst_heads out = heads();
+  const int zero_rest = i32();
   void* ws = ptr();
   const long long ws_bytes = i64();
   return msst_prefix_attention(or_null(q), tokens, q_starts, requests, or_null(prefix_k), or_null(prefix_v), prefix_len,
                                or_null(k_cache), or_null(v_cache), pages, page_size, table, blocks, stride, lens, head_dim,
-                               scale, dtype, or_null(out), ws, ws_bytes, ptr());
+                               scale, dtype, or_null(out), zero_rest, ws, ws_bytes, ptr());
 }
 
 int msst_grouped_gemm(int num_groups, const msst_gemm_group* groups, const void* x, long long x_rows, long long ldx,

@@ -1443,8 +1443,11 @@ __global__ void __launch_bounds__(256, 2)
   wait_for_previous();
   const bool of_a_request = !p.q_starts || (token >= first_row(p, 0) && token < first_row(p, p.requests));
   const int code0 = g.concat ? 0 : g.where[row], code1 = g.where[rows + row];
+  if (!of_a_request) {
+    if (p.zero_rest) finish_row<T>(p, token, head, Sum(), false, lane);
+    return;
+  }
   if (g.concat && code1 >= 0 && code1 >> 20 == 0) return;
-  if (!of_a_request) return;
   bool again = code0 < 0 || code1 < 0;
   Sum sum;
   if (!again) {
@@ -1510,6 +1513,14 @@ __global__ void __launch_bounds__(256, 4)
       bool again = false;
       add_parts<4>(none, parts, 0, 1, p.head_dim, lane * 4, sum, again);
       finish_row<T>(p, k.q0 + n, head, sum, again, lane);
+    }
+  }
+  if (p.zero_rest && p.q_starts) {
+    const int before = first_row(p, 0), behind = first_row(p, p.requests);
+    const long long rest = ((long long)before + max(p.tokens - behind, 0)) * p.q.heads;
+    for (long long i = (long long)blockIdx.x * gridDim.y * 8 + x; i < rest; i += (long long)gridDim.x * gridDim.y * 8) {
+      const int token = (int)(i / p.q.heads);
+      finish_row<T>(p, token < before ? token : behind + token - before, (int)(i % p.q.heads), Sum(), false, lane);
     }
   }
   if (g.bad[blockIdx.x]) {  // rows to be computed again

@@ -111,7 +111,7 @@ def lib():
                                    c_int, vp, vp]
     L.msst_prefix_attention_workspace.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int, pi64]
     L.msst_prefix_attention.argtypes = [vp, c_int, vp, c_int, vp, vp, c_int, vp, vp, c_int, c_int, vp, c_int, i64, vp,
-                                        c_int, c_float, c_int, vp, vp, i64, vp]
+                                        c_int, c_float, c_int, vp, c_int, vp, i64, vp]
     L.msst_call.argtypes = [c_int, vp]
     L.msst_grouped_gemm.argtypes = [c_int, ctypes.POINTER(GemmGroupC), vp, i64, i64, vp, i64, i64, c_int, c_int,
                                     c_int, vp, i64, i64, vp]
@@ -313,7 +313,7 @@ def _table(t, requests, device):
 # arguments of msst_call: words in the calls' order, five for a msst_heads
 _PLAN = struct.Struct("18q").pack
 _APPEND = struct.Struct("21qd20q").pack
-_ATTEND = struct.Struct("36qd9q").pack
+_ATTEND = struct.Struct("36qd10q").pack
 _NO_HEADS = (0, 0, 0, 0, 0)
 
 
@@ -683,45 +683,50 @@ class ops:
         rows q_starts[r] to q_starts[r + 1] (int32 [R + 1]; None: one row each, T = R).  Rows that
         see no key give zeros; rows of no request are left as they were in `out`, zeros without
         one.  Returns [T, Hq, d]."""
-        torch = _torch()
+        _torch()
         dt, dev, shape, cs, keep = q.dtype, q.get_device(), q.shape, k_cache.shape, []
         code = _dtype_code(dt)
-        _need(len(shape) == 3 and len(cs) == 4 and cs[3] == shape[2] and v_cache.shape == cs,
-              "q must be [T, heads, head_dim], the caches [pages, page_size, heads, head_dim]")
+        if len(shape) != 3 or len(cs) != 4 or cs[3] != shape[2] or v_cache.shape != cs:
+            raise ValueError("q must be [T, heads, head_dim], the caches [pages, page_size, heads, head_dim]")
         T, Hq, d = shape
-        Hk = cs[2]
-        _need(Hk > 0 and Hq > 0 and Hq % Hk == 0, "q must have a multiple of the caches' heads")
+        pages, page, Hk, _ = cs
+        if Hk < 1 or Hq < 1 or Hq % Hk:
+            raise ValueError("q must have a multiple of the caches' heads")
         hk, hv = _cache_heads(k_cache, dt, dev, "k_cache"), _cache_heads(v_cache, dt, dev, "v_cache")
-        _need((prefix_k is None) == (prefix_v is None), "prefix_k and prefix_v go together")
         P, pk, pv = 0, _NO_HEADS, _NO_HEADS
-        if prefix_k is not None:
+        if prefix_k is not None and prefix_v is not None:
             ps = prefix_k.shape
-            _need(len(ps) == 3 and ps[1] == Hk and ps[2] == d and prefix_v.shape == ps,
-                  "prefix_k and prefix_v must be [P, heads, head_dim] with the caches' heads and head_dim")
-            _need(prefix_k.dtype is dt and prefix_v.dtype is dt and prefix_k.get_device() == dev and
-                  prefix_v.get_device() == dev, "q and the prefix must share one 16-bit dtype and one device")
+            if len(ps) != 3 or ps[1] != Hk or ps[2] != d or prefix_v.shape != ps:
+                raise ValueError("prefix_k and prefix_v must be [P, heads, head_dim] with the caches' heads and head_dim")
+            if (prefix_k.dtype is not dt or prefix_v.dtype is not dt or prefix_k.get_device() != dev
+                    or prefix_v.get_device() != dev):
+                raise ValueError("q and the prefix must share one 16-bit dtype and one device")
             P = ps[0]
             if P:
                 pk, pv = _flat_heads(prefix_k, ps, keep), _flat_heads(prefix_v, ps, keep)
-        _need(lens.dim() == 1, "lens must be int32 [requests]")
-        R = lens.shape[0]
-        table, blocks, stride = _table(block_table, R, dev)
+        elif prefix_k is not prefix_v:
+            raise ValueError("prefix_k and prefix_v go together")
+        R = lens.shape[0] if lens.dim() == 1 else -1
         own, starts = _int32(lens, (R,), dev, "lens"), 0
+        table, blocks, stride = _table(block_table, R, dev)
         if q_starts is not None:
             starts = _int32(q_starts, (R + 1,), dev, "q_starts")
+        zero_rest = 0
         if out is None:
-            out = q.new_empty(shape) if q_starts is None else q.new_zeros(shape)
+            zero_rest = 1
+            out = q.new_empty(shape) if R else q.new_zeros(shape)
+            s0, s1 = Hq * d, d
         else:
-            _need(out.shape == shape and out.dtype is dt and out.get_device() == dev and (out.stride(2) == 1 or d < 2),
-                  "out must have q's shape, type and device, and unit last stride")
-        so = out.stride()
+            s0, s1, s2 = out.stride() if out.dim() == 3 else (0, 0, 0)
+            if out.shape != shape or out.dtype is not dt or out.get_device() != dev or (s2 != 1 and d > 1):
+                raise ValueError("out must have q's shape, type and device, and unit last stride")
         need, ws = _workspace("prefix_attention", dev, T, R, P, Hq, Hk, d), 0
         if need:
             space = q.new_empty(need // 2)  # 16-bit values; sizes are whole floats
             ws = space.data_ptr()
         check(lib().msst_call(2, _ATTEND(
-            *_flat_heads(q, shape, keep), T, starts, R, *pk, *pv, P, *hk, *hv, cs[0], cs[1], table, blocks, stride, own, d,
-            scale, code, out.data_ptr(), Hq, 0, so[0], so[1], ws, need, _current_stream(dev))))
+            *_flat_heads(q, shape, keep), T, starts, R, *pk, *pv, P, *hk, *hv, pages, page, table, blocks, stride, own, d,
+            scale, code, out.data_ptr(), Hq, 0, s0, s1, zero_rest, ws, need, _current_stream(dev))))
         return out
 
     @staticmethod

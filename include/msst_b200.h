@@ -280,8 +280,8 @@ int msst_rope_append(const msst_heads* q, const msst_heads* k, const msst_heads*
  * the last of its lens[r] own ones: the i-th of n sees the first lens[r] - n + i + 1 of them (not below 0).
  * q.heads is a multiple of the caches' heads, head_dim a multiple of 8 and <= 128,
  * scale 0 selects 1/sqrt(head_dim).  What a row does not see, the rest of a page
- * included, has no influence on it, whatever it holds.  A row that sees no key gives zeros; rows of no request are left as
- * they were.  A page outside the caches reads as zeros, and
+ * included, has no influence on it, whatever it holds.  A row that sees no key gives zeros; rows of no request (before
+ * the first or behind the last) are left as they were, or zeroed with zero_rest != 0.  A page outside the caches reads as zeros, and
  * msst_device_error reports 18.  lens is taken into [0, blocks * page_size].  out must
  * not overlap the inputs.  Precision, alignment and workspace as in msst_cross_attention
  * (head strides of the prefix and the caches may be 0). */
@@ -291,8 +291,8 @@ int msst_prefix_attention(const msst_heads* q, int tokens, const int* q_starts, 
                           const msst_heads* prefix_k, const msst_heads* prefix_v, int prefix_len,
                           const msst_heads* k_cache, const msst_heads* v_cache, int pages, int page_size,
                           const int* block_table, int blocks, long long table_stride, const int* lens, int head_dim,
-                          float scale, int dtype, const msst_heads* out, void* workspace, long long workspace_bytes,
-                          void* stream);
+                          float scale, int dtype, const msst_heads* out, int zero_rest, void* workspace,
+                          long long workspace_bytes, void* stream);
 
 /* The three calls above with their arguments in one array, in their order, each an integer, a pointer or (float)
  * a double in 64 bits, a msst_heads as its five members (a NULL one: data NULL and 0 heads); integers beyond 32

@@ -68,7 +68,7 @@ def _attention(**kw):
     from msst_b200 import lib
 
     a = dict(q=_heads(), tokens=4, starts=16, requests=2, pk=_heads(), pv=_heads(), prefix=8, kc=_heads(), vc=_heads(),
-             pages=4, page=16, table=16, blocks=2, stride=2, lens=16, d=64, scale=0.0, dtype=0, out=_heads(), ws=None,
+             pages=4, page=16, table=16, blocks=2, stride=2, lens=16, d=64, scale=0.0, dtype=0, out=_heads(), rest=0, ws=None,
              wsb=0)
     a.update(kw)
     return lib().msst_prefix_attention(*a.values(), None)
@@ -114,7 +114,7 @@ def test_calls_by_words():
     heads = [16, 2, 2048, 128, 64]
     plan = [16, 16, 4, 16, 8, 8, 16, 64, 16, 16, 0, 4, 16, 16, 16, 16, 16, 0]
     append = heads * 3 + [0, 64, 16, 16, 16, 64, 1.0, 0] + heads * 2 + [4, 16, 0] + heads + [0]
-    attend = heads + [0, 16, 2] + heads * 2 + [8] + heads * 2 + [4, 16, 16, 2, 2, 16, 64, 0.0, 0] + heads + [0, 0, 0]
+    attend = heads + [0, 16, 2] + heads * 2 + [8] + heads * 2 + [4, 16, 16, 2, 2, 16, 64, 0.0, 0] + heads + [0, 0, 0, 0]
     for op, form, good, bads in (
         (0, "18q", plan, ((0, 0, "null"), (1, 0, "null"), (2, 9000, "requests"), (3, 0, "block_table"), (4, big, "blocks"),
                           (5, 7, "overlap"), (6, 0, "null"), (7, 0, "pages"), (8, 0, "null"), (9, 48, "page_size"),
@@ -125,7 +125,7 @@ def test_calls_by_words():
                                 (20, 72, "rot_dim"), (21, float("nan"), "amplitude"), (22, 2, "pairing"), (24, 1, "same number"),
                                 (25, 0, "k_cache is written"), (30, -8, "v_cache has a negative"), (33, 0, "pages"),
                                 (34, 17, "page_size"), (35, 3, "dtype"), (37, 3, "q's heads"))),
-        (2, "36qd9q", attend, ((1, 3, "q's heads"), (5, -1, "shape"), (7, -1, "requests"), (8, 8, "prefix_k must be"),
+        (2, "36qd10q", attend, ((1, 3, "q's heads"), (5, -1, "shape"), (7, -1, "requests"), (8, 8, "prefix_k must be"),
                                (9, 0, "prefix_k needs"), (14, 1, "caches' heads"), (18, -1, "shape"), (20, 0, "k_cache needs"),
                                (25, 1, "same number"), (29, 0, "pages"), (30, 12, "page_size"), (31, 0, "block_table"),
                                (32, -1, "blocks"), (33, 1, "overlap"), (35, 12, "head_dim"), (36, float("inf"), "scale"),

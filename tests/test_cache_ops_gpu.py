@@ -465,7 +465,7 @@ def test_prefix_attention_rows_of_nobody(cuda):
     torch = cuda
     from msst_b200 import ops
 
-    for counts, Hq in (([1] * 30, 8), ([50, 90], 4), ([3, 2], 2)):
+    for counts, Hq in (([1] * 30, 8), ([50, 90], 4), ([3, 2], 2), ([2500, 1700], 4)):
         lens = [n + 20 for n in counts]
         q, pk, pv, kc, vc, table, own, starts = _attend_inputs(torch, counts, lens, 200, Hq, 2, 64, 16, "fp16", 13)
         y = ops.prefix_attention(q, pk, pv, kc, vc, table, own, q_starts=starts)
