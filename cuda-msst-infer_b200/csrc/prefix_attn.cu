@@ -26,14 +26,15 @@
 // key, by the joining launch.
 //
 // Measured (one B200, both launches, in a CUDA graph) and what bounds it:
-//   64 requests, one token each, 8192 keys of prefix, up to 1024 own, 32/8 heads of 128: 51 us.  Memory: 173 MB, most of
-//     them at 6 TB/s; 8 us before the first tiles, then CTAs of equal runs end between 31 and 48 us, as the SMs do
-//     not share the memory's rate equally (in whatever order the two kinds of CTA are put: taking turns over the grid, 63 us)
-//   16 tokens, 131072 keys of prefix: 107 us, 555 MB at 5.2 TB/s
-//   4096 tokens of six prompts, 4096 keys of prefix: 320 us, 1.0 PFLOP/s; tensor and XU pipe half busy each (the chain
+//   64 requests, one token each, 8192 keys of prefix, up to 1024 own, 32/8 heads of 128: 47 us.  Memory: 173 MB, most of
+//     them at 6 TB/s; 8 us before the first tiles, then CTAs of equal runs end between 29 and 41 us, as the SMs do
+//     not share the memory's rate equally (with the two kinds of CTA taking turns over the grid, 6 us more)
+//   16 tokens, 131072 keys of prefix: 104 us, 555 MB at 5.4 TB/s
+//   4096 tokens of six prompts, 4096 keys of prefix: 291 us, 1.1 PFLOP/s; tensor and XU pipe 58 % busy each (the chain
 //     scores, softmax, product behind one buffer of scores a tile, as in cross_attn.cu)
-//   32 requests of 5 tokens, 3791 keys, 12/4 heads of 80: 26 us, all of it latency: 2.5 us to find the runs, 4 to the first
-//     tile, three or four units, 2 to the second launch and 5 in it
+//   32 requests of 5 tokens, 3791 keys, 12/4 heads of 80: 25 us, all of it latency: 2.5 us to find the runs, 4 to the first
+//     tile, three or four units, 2 to the second launch and 5 in it.  Code counts here: "no instruction" is the warps' first
+//     stall, and forms that are written once and rolled up (the product's issue, the exact passes, barriers) are the faster ones
 #include <algorithm>
 #include <cstddef>
 
@@ -1481,8 +1482,8 @@ __global__ void __launch_bounds__(256, 2)
 }
 
 // The same for many rows of one sequence of prefix and own keys, most of which are done: block (x, y) takes rows
-// [8 y, 8 y + 8) of the item that worker x started and did not end.  (4096 tokens of 32 heads, 37,000 rows of them cut:
-// about 10 us; looking through all rows, 26.)
+// [8 y, 8 y + 8) of both tiles of the item that worker x started and did not end, a warp one of each, whose parts come
+// together.  (4096 tokens of 32 heads, 37,000 rows of them cut: 9 us; a row a warp, 15; looking through all rows, 26.)
 template <typename T>
 __global__ void __launch_bounds__(256, 4)
     prefix_join_cuts_kernel(const __grid_constant__ PrefixAttnParams p, const __grid_constant__ PrefixGeom g, int ctas) {
@@ -1490,30 +1491,56 @@ __global__ void __launch_bounds__(256, 4)
   wait_for_previous();
   const Segment k = g.cuts[blockIdx.x];
   if (k.code > 0) {
-    int n, head;
-    bool valid;
+    int n[2], head[2];
+    bool valid[2];
     if ((k.code >> 8 & 0xfff) >= kTileWorkers) {
-      int n0, g0;
-      k.origin(g, x >> 7, n0, g0);
-      const int row = x & 127, rn = row / g.gt;
-      n = n0 + rn;
-      head = g0 + row - rn * g.gt;
-      valid = rn < g.nt && n < k.n && head < g.group && !(k.lone && x >= 128);
-      head += k.hk * g.group;
-    } else {
+      const int rn = x / g.gt;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        int n0, g0;
+        k.origin(g, u, n0, g0);
+        n[u] = n0 + rn;
+        head[u] = g0 + x - rn * g.gt;
+        valid[u] = rn < g.nt && n[u] < k.n && head[u] < g.group && !(k.lone && u);
+        head[u] += k.hk * g.group;
+      }
+    } else {  // (up to 128 rows)
       const int h = x / g.token_rows, r = x - h * g.token_rows;
-      n = r / g.group;
-      head = (k.hk * g.heads + h) * g.group + r - n * g.group;
-      valid = h < g.heads && n < k.n;
+      n[0] = r / g.group;
+      head[0] = (k.hk * g.heads + h) * g.group + r - n[0] * g.group;
+      valid[0] = h < g.heads && n[0] < k.n;
+      n[1] = head[1] = 0;
+      valid[1] = false;
     }
-    if (valid) {
-      Parts none, parts;
-      parts.find(g, k.code, x, nullptr, ctas);
-      Sum sum;
-      bool again = false;
-      add_parts<4>(none, parts, 0, 1, p.head_dim, lane * 4, sum, again);
-      finish_row<T>(p, k.q0 + n, head, sum, again, lane);
+    Parts parts;
+    parts.find(g, k.code, x, nullptr, ctas);
+    const int d = p.head_dim, col = lane * 4;
+    Sum sum[2];
+    bool again[2] = {false, false};
+    for (int i0 = 0; i0 < parts.count; i0 += 2) {
+      float4 h[2][2], v[2][2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          h[y][u] = v[y][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i0 + y >= parts.count || !valid[u]) continue;
+          const float* f = parts.at(i0 + y) + (size_t)u * 128 * g.ld;
+          h[y][u] = __ldcg(reinterpret_cast<const float4*>(f + d));
+          if (col < d) v[y][u] = __ldcg(reinterpret_cast<const float4*>(f + col));
+        }
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          again[u] |= h[y][u].z != 0.f;
+          sum[u].add(h[y][u].x, h[y][u].y, v[y][u]);
+        }
     }
+#pragma unroll 1
+    for (int u = 0; u < 2; ++u)
+      if (u ? valid[1] : valid[0])
+        finish_row<T>(p, k.q0 + (u ? n[1] : n[0]), u ? head[1] : head[0], u ? sum[1] : sum[0], u ? again[1] : again[0], lane);
   }
   if (p.zero_rest && p.q_starts) {
     const int before = first_row(p, 0), behind = first_row(p, p.requests);
@@ -1613,10 +1640,11 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   g.q_slots = most_rows <= 8 ? 2 : 1;
   const int team_bytes = (int)C::kTiles / g.teams - g.q_slots * g.heads * g.q_rows * 128 * C::kHalves;
   g.entries = std::min(kMostEntries, team_bytes / (g.heads * (int)C::kEntry));
-  // What a unit takes of an SM in units of 10 ns: a tile unit 2.1 us of the chain; a token unit what its bytes take.  An
+  // What a unit takes of an SM in units of 10 ns: a tile unit 2 us of the chain; a token unit what its bytes take.  An
   // item's start and end is as long as three or four tile units (its query rows, the first scores, the last product, the
-  // rows written): with 2, 3 and 4 a prompt of 4096 tokens, 32/8 heads of 128, takes 186, 179 and 180 us and 64 single
-  // tokens behind 8192 keys 53, 51 and 51.  Token units at 18, 26 and 30: 51, 53 and 55.
+  // rows written): with 2, 3 and 4 a prompt of 4096 tokens, 32/8 heads of 128, took 186, 179 and 180 us (155 with later
+  // steps) and 64 single tokens behind 8192 keys 53, 51 and 51 (47).  Tile units at 170, 190 and 235: 51, 49 and 48; token
+  // units at 18, 26 and 30: 51, 53 and 55 (before those steps).
   g.tile_cost = 215;
   g.token_cost = g.heads * (DP == 128 ? 22 : 16);
   g.tile_item = 4;
@@ -1654,7 +1682,7 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   const long long n = (long long)p.tokens * p.q.heads;
   LaunchScope scope("prefix_join", 0.0, 0.0, s);
   if (g.concat && n > 16384) {
-    DependentLaunch l(dim3(num_sms * g.teams, 256 / 8), 256, 0, s);
+    DependentLaunch l(dim3(num_sms * g.teams, 128 / 8), 256, 0, s);
     return cudaLaunchKernelEx(&l.cfg, prefix_join_cuts_kernel<T>, p, g, num_sms);
   }
   // so few rows that all warps of a block can share one, or a row a warp
