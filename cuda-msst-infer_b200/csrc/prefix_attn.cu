@@ -64,7 +64,7 @@ struct PCfg {
   static constexpr uint32_t kTile = kHalves * kHalfBytes;  // one Q, K or V tile
   static constexpr int kKSlots = DP == 128 ? 3 : 5, kVSlots = DP == 128 ? 2 : 5;
   static constexpr uint32_t kTiles = (2 + kKSlots + kVSlots) * kTile;
-  static constexpr uint32_t kTail = 3072;  // segments, barriers and exchange of either role
+  static constexpr uint32_t kTail = 3 * 1024;  // segments, barriers and exchange of either role
   static constexpr size_t kSmem = kTiles + kTail;
   static_assert(kSmem <= 227 * 1024, "");
   static constexpr uint32_t kEntry = kHalves * kTokenBox;  // token role: K or V of one head and tile
@@ -853,7 +853,6 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
       seq += (uint32_t)(all_steps + steps1);
       if (!mbar_wait_warp<false>(&o_done[w], s & 1, kErrTimeoutAttnO, abort_flag)) break;
       tc_fence_after();
-      const bool bad = *s_bad >> (s & 31) & 1;
       // a lone tile: the two halves meet, weigh each other in and write half the columns each
       float a0 = 1.f, a1 = 0.f;
       int c_lo = 0, c_hi = p.head_dim;
@@ -889,6 +888,8 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         else
           c_lo = min(mid, p.head_dim);
       }
+      // (past the meeting: a lone tile's other half may have multiplied the last V tile)
+      const bool bad = *s_bad >> (s & 31) & 1;
       const bool whole = k.whole(), finish = whole && g.concat;
       const float inv = finish ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
       const float f0 = a0 * inv, f1 = a1 * inv;

@@ -108,6 +108,33 @@ def test_lengths(cuda, counts, lens, prefix, prec):
         _attend_check(torch, y, *args, d ** -0.5, prec)
 
 
+@pytest.mark.parametrize("prec", ["fp16", "bf16"])
+@pytest.mark.parametrize("counts, lens, prefix", [
+    ([4] * 20, [130 + 97 * i for i in range(20)], 127),         # lone tiles, the last keys with either half
+    ([1, 9, 5, 16], [700, 2003, 129, 385], 0),
+    ([600], [600], 32),
+    ([250, 183, 260, 831], [250, 879, 287, 1526], 0),
+], ids=["few", "ragged", "prompt", "prompts"])
+def test_last_token_not_finite(cuda, counts, lens, prefix, prec):
+    """The V row of a request's last token, which its last row alone sees, holds infinities and NaN."""
+    torch = cuda
+    from msst_b200 import ops
+
+    for value in (float("nan"), -float("inf")):
+        q, pk, pv, kc, vc, table, own, starts = _attend_inputs(torch, counts, lens, prefix, 16, 2, 64, 32, prec, 61)
+        upto, keep, early = [0], [], own.clone()
+        for r, (n, m) in enumerate(zip(counts, lens)):
+            vc[table[r, (m - 1) // 32].long(), (m - 1) % 32] = value
+            early[r] -= 1
+            keep += range(int(starts[r]), int(starts[r + 1]) - 1)
+            upto.append(len(keep))
+        for _ in range(3):
+            z = ops.prefix_attention(q, pk, pv, kc, vc, table, own, q_starts=starts)
+            last = (starts[1:] - 1).long()
+            assert not bool(z[last].isfinite().any())
+            _attend_check(torch, z[keep], q[keep], pk, pv, kc, vc, table, early, torch.tensor(upto), 0.125, prec)
+
+
 def test_lengths_outside_their_range(cuda):
     """Lengths below 0 count as 0, those past the table's row as the row's."""
     torch = cuda
