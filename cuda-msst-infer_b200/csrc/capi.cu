@@ -199,11 +199,11 @@ int check_pages(int pages, int page_size) {
   return shift;
 }
 
-// A block table [requests, blocks] whose rows count their tokens in 32 bits.
+// A block table [requests, blocks] whose rows count their tokens in 32 bits, rounded up to a tile too.
 void check_table(const int* table, int requests, int blocks, long long stride, int page_size) {
   MSST_REQUIRE(requests >= 0 && requests <= msst::kMostPlanRequests,
                "at most " + std::to_string(msst::kMostPlanRequests) + " requests");
-  MSST_REQUIRE(blocks >= 0 && (long long)blocks * page_size < (1LL << 31), "bad number of blocks");
+  MSST_REQUIRE(blocks >= 0 && (long long)blocks * page_size <= kMostRows, "bad number of blocks");
   MSST_REQUIRE(requests < 2 || stride >= blocks, "the block table's rows overlap");
   MSST_REQUIRE(table || blocks == 0 || requests == 0, "block_table is null");
 }

@@ -232,3 +232,12 @@ def test_rope_frequencies():
                 dict(scaling="parts", slow=4.0, fast=2.0)):
         with pytest.raises(ValueError):
             rope_frequencies(**{"rot_dim": 64, **bad})
+
+
+def test_tokens_of_a_request_within_a_tile_of_32_bits_are_refused():
+    """Rounded up to a tile of keys they would pass 2^31 - 1 and count as none."""
+    from msst_b200 import MSST_ERR_INVALID, lib
+
+    most = dict(blocks=(1 << 27) - 1, stride=1 << 27)  # of 16 tokens
+    for call in (_plan, _attention):
+        assert call(**most) == MSST_ERR_INVALID and "blocks" in lib().msst_last_error().decode()
