@@ -1643,9 +1643,10 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   g.entries = std::min(kMostEntries, team_bytes / (g.heads * (int)C::kEntry));
   // What a unit takes of an SM in units of 10 ns: a tile unit 2 us of the chain; a token unit what its bytes take.  An
   // item's start and end is as long as four tile units (its query rows, the first scores, the last product, the rows
-  // written).  64 single tokens behind 8192 keys, 32/8 heads of 128, take 47.6 us with these; with tile units at 170, 190
-  // and 245 50.3, 48.5 and 48.2, with items of 3 and 5 tile units 48.6 and 47.1 (but 60 requests of 8 tokens 27.5 with 5,
-  // 26.6 with 3), with token items of 2 units 48.4, with token units at 18, 26 and 30 3 to 6 us more.
+  // written).  64 single tokens behind 8192 keys, 32/8 heads of 128, take 47.6 us with these (four inputs in turn); with
+  // tile units at 170, 190 and 245 50.3, 48.5 and 48.2, with items of 3 and 5 tile units 48.6 and 47.1, with token items of
+  // 2 units 48.4; 60 requests of 8 tokens 27.4, 26.6 with 3 and 27.5 with 5; a prompt of 4096 tokens was slowest with 2
+  // and alike with 3 and 4.  Token units at 18, 26 and 30, before the last steps: 51, 53 and 55 us, 51 with 22.
   g.tile_cost = 215;
   g.token_cost = g.heads * (DP == 128 ? 22 : 16);
   g.tile_item = 4;
