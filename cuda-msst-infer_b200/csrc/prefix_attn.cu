@@ -1560,6 +1560,9 @@ __global__ void __launch_bounds__(256, 4)
 }
 
 // ------------------------------------------------------------------------------- host
+// Bytes of a workspace that it may take to reach the next multiple of 32 (see store8).
+constexpr int kSpare = 16;
+
 // Sizes of a launch, and where the parts of its workspace lie (bytes).
 struct Layout {
   PrefixGeom g;
@@ -1697,7 +1700,8 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
 template <typename T>
 cudaError_t launch_t(const PrefixAttnParams& p, int num_sms, cudaStream_t s) {
   Layout x = make_layout(p.tokens, p.requests, p.prefix, p.q.heads, p.k_cache.heads, p.head_dim, num_sms);
-  char* ws = reinterpret_cast<char*>(p.ws);
+  // (the caller's workspace starts on 16 bytes, the parts are written 32 at a time)
+  char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p.ws) + kSpare + 15) & ~(uintptr_t)(kSpare + 15));
   x.g.where = reinterpret_cast<int*>(ws);
   x.g.cuts = reinterpret_cast<Segment*>(ws + x.cuts);
   x.g.bad = reinterpret_cast<int*>(x.g.cuts + num_sms * kMostTeams);
@@ -1715,7 +1719,7 @@ int ctas_of(int num_sms) { return std::min(num_sms, kTileWorkers / kMostTeams); 
 long long prefix_attention_workspace(int tokens, int requests, int prefix, int q_heads, int kv_heads, int head_dim,
                                      int num_sms) {
   if (tokens == 0 || requests == 0) return 0;
-  return make_layout(tokens, requests, prefix, q_heads, kv_heads, head_dim, ctas_of(num_sms)).bytes;
+  return make_layout(tokens, requests, prefix, q_heads, kv_heads, head_dim, ctas_of(num_sms)).bytes + kSpare;
 }
 
 cudaError_t launch_prefix_attention(const PrefixAttnParams& p, int bf16, int num_sms, cudaStream_t stream) {

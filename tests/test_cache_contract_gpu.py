@@ -1,0 +1,64 @@
+"""GPU tests of what the header promises of the paged-cache operators beyond the Python entry points' own use
+of them.  Forms and tolerances as in test_cache_ops_gpu.py."""
+from __future__ import annotations
+
+import ctypes
+import struct
+
+import pytest
+
+from test_cache_ops_gpu import _attend_check, _attend_inputs, _dt
+
+pytestmark = pytest.mark.gpu
+
+
+def _view(t):
+    """The msst_heads of a [.., heads, head_dim] tensor of three or four dimensions."""
+    st = t.stride()
+    return struct.pack("Pi4xqqq", t.data_ptr(), t.shape[-2], st[0] if t.dim() == 4 else 0, st[-3], st[-2])
+
+
+def _workspace_bytes(T, R, P, Hq, Hk, d):
+    from msst_b200 import check, lib
+
+    n = ctypes.c_longlong()
+    check(lib().msst_prefix_attention_workspace(T, R, P, Hq, Hk, d, ctypes.byref(n)))
+    return n.value
+
+
+def _attend_c(torch, q, pk, pv, kc, vc, table, own, starts, out, rest, ws, ws_bytes):
+    """msst_prefix_attention by its C signature."""
+    from msst_b200 import check, lib
+
+    check(lib().msst_prefix_attention(
+        _view(q), q.shape[0], starts.data_ptr(), own.numel(), _view(pk), _view(pv), pk.shape[0], _view(kc), _view(vc),
+        kc.shape[0], kc.shape[1], table.data_ptr(), table.shape[1], table.stride(0), own.data_ptr(), q.shape[2], 0.0,
+        1 if q.dtype is torch.bfloat16 else 0, _view(out), rest, ws, ws_bytes, torch.cuda.current_stream().cuda_stream))
+
+
+@pytest.mark.parametrize("counts, lens", [
+    ([1] * 30, [5 * i for i in range(30)]),       # tile items of the prefix, whole and cut, token items of the requests
+    ([40, 3], [90, 200]),
+    ([700, 300], [700, 900]),                     # prefix and own keys as one sequence
+    ([2], [70]),
+], ids=["single", "few", "prompts", "one"])
+@pytest.mark.parametrize("d, prec", [(64, "fp16"), (128, "bf16"), (40, "bf16")])
+def test_workspace_on_any_16_bytes(cuda, counts, lens, d, prec):
+    """A workspace of just the size asked for at any multiple of 16 bytes, and nothing written around it."""
+    torch = cuda
+    from msst_b200 import device_error
+
+    args = _attend_inputs(torch, counts, lens, 900, 8, 2, d, 16, prec, 83)
+    q, pk, pv, kc, vc, table, own, starts = args
+    need = _workspace_bytes(q.shape[0], len(counts), 900, 8, 2, d)
+    results = []
+    for off in (0, 16, 32, 48, 112, 240):
+        space = torch.full((need + 512,), 0x5a, dtype=torch.uint8, device="cuda")
+        out = torch.zeros_like(q)
+        assert space.data_ptr() % 256 == 0
+        _attend_c(torch, q, pk, pv, kc, vc, table, own, starts, out, 0, space.data_ptr() + off, need)
+        assert bool((space[:off] == 0x5a).all()) and bool((space[off + need:] == 0x5a).all())
+        results.append(out)
+    assert device_error(True) == 0
+    _attend_check(torch, results[0], *args, d ** -0.5, prec)
+    assert all(torch.equal(results[0], r) for r in results[1:])
