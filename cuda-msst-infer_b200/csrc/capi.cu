@@ -722,8 +722,8 @@ int msst_prefix_attention(const msst_heads* q, int tokens, const int* q_starts, 
       MSST_REQUIRE(prefix_len == 1 || (p.prefix_k.seq_stride > 0 && p.prefix_v.seq_stride > 0),
                    "the prefix's sequence strides must not be 0");
     }
-    if (tokens == 0 || requests == 0) return;
-    MSST_REQUIRE(lens, "lens is null");
+    if (tokens == 0 || (requests == 0 && !zero_rest)) return;
+    MSST_REQUIRE(lens || requests == 0, "lens is null");
     MSST_REQUIRE((tokens == 1 || p.q.seq_stride > 0) && (p.q.heads == 1 || p.q.head_stride > 0) &&
                      p.k_cache.seq_stride > 0 && p.v_cache.seq_stride > 0 &&
                      (pages == 1 || (p.k_cache.batch_stride > 0 && p.v_cache.batch_stride > 0)),

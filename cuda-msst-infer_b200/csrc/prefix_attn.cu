@@ -1559,6 +1559,19 @@ __global__ void __launch_bounds__(256, 4)
   }
 }
 
+// Without a request every row is one of nobody: zeroed, 8 columns a thread.
+__global__ void __launch_bounds__(256) prefix_zero_kernel(const __grid_constant__ PrefixAttnParams p) {
+  const unsigned pieces = (unsigned)p.head_dim >> 3;
+  const long long all = (long long)p.tokens * p.out.heads * pieces;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+    const long long row = i / pieces, token = row / p.out.heads;
+    // (16-bit values of either type)
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out.data) + token * p.out.seq_stride +
+                              (row - token * p.out.heads) * p.out.head_stride + 8 * (i - row * pieces)) =
+        make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 // ------------------------------------------------------------------------------- host
 // Bytes of a workspace that it may take to reach the next multiple of 32 (see store8).
 constexpr int kSpare = 16;
@@ -1723,6 +1736,12 @@ long long prefix_attention_workspace(int tokens, int requests, int prefix, int q
 }
 
 cudaError_t launch_prefix_attention(const PrefixAttnParams& p, int bf16, int num_sms, cudaStream_t stream) {
+  if (p.requests == 0) {
+    const long long pieces = (long long)p.tokens * p.out.heads * (p.head_dim / 8);
+    LaunchScope scope("prefix_zero", 0.0, 16.0 * pieces, stream);
+    prefix_zero_kernel<<<(unsigned)std::min((pieces + 255) / 256, 8LL * num_sms), 256, 0, stream>>>(p);
+    return cudaGetLastError();
+  }
   return bf16 ? launch_t<__nv_bfloat16>(p, ctas_of(num_sms), stream) : launch_t<__half>(p, ctas_of(num_sms), stream);
 }
 

@@ -714,7 +714,7 @@ class ops:
         zero_rest = 0
         if out is None:
             zero_rest = 1
-            out = _torch_module.empty_like(q, memory_format=_torch_module.contiguous_format) if R else q.new_zeros(shape)
+            out = _torch_module.empty_like(q, memory_format=_torch_module.contiguous_format)
             s0, s1 = Hq * d, d
         else:
             s0, s1, s2 = out.stride() if out.dim() == 3 else (0, 0, 0)

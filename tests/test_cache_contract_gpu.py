@@ -62,3 +62,25 @@ def test_workspace_on_any_16_bytes(cuda, counts, lens, d, prec):
     assert device_error(True) == 0
     _attend_check(torch, results[0], *args, d ** -0.5, prec)
     assert all(torch.equal(results[0], r) for r in results[1:])
+
+
+@pytest.mark.parametrize("T, Hq, d", [(1, 1, 8), (7, 4, 64), (300, 6, 40), (20000, 32, 128)])
+def test_rows_without_a_request(cuda, T, Hq, d):
+    """No request at all: every row of `out` is zeroed with zero_rest, and left as it was without."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    q, pk, pv, kc, vc, table, own, starts = _attend_inputs(torch, [T], [3], 5, Hq, 1, d, 16, "fp16", 89)
+    table, own, starts = table[:0], own[:0], starts[:1]
+    wide = torch.full((T, Hq + 2, d + 8), float("nan"), dtype=q.dtype, device="cuda")
+    out = wide[:, 1:-1, :d]
+    _attend_c(torch, q, pk, pv, kc, vc, table, own, starts, out, 0, None, 0)
+    assert bool(wide.isnan().all())
+    assert _workspace_bytes(T, 0, 5, Hq, 1, d) == 0
+    _attend_c(torch, q, pk, pv, kc, vc, table, own, starts, out, 1, None, 0)
+    assert bool((out == 0).all()) and int(wide.isnan().sum()) == wide.numel() - out.numel()
+    y = ops.prefix_attention(q, pk, pv, kc, vc, table, own, q_starts=starts)
+    assert y.shape == q.shape and bool((y == 0).all())
+    left = torch.full_like(q, 3.0)
+    assert ops.prefix_attention(q, pk, pv, kc, vc, table, own, q_starts=starts, out=left) is left and bool((left == 3).all())
+    assert device_error(True) == 0
