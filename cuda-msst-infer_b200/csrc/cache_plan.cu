@@ -158,9 +158,12 @@ __global__ void __launch_bounds__(kMostThreads) cache_plan_kernel(const __grid_c
     int slot = -1, position = 0;
     if (t < s_start[R]) {
       const int r = last_at_most(s_start, R + 1, t);
-      const int kept = s_kept[r], at = (kept < 0 ? ~kept : kept) + t - s_start[r];
-      position = p.start + at;
+      const int kept = s_kept[r];
+      // (a refused request's rows may pass what the host has checked the sum of start and a row of the table for)
+      const long long place = (long long)(kept < 0 ? ~kept : kept) + (t - s_start[r]);
+      position = clamp_int(p.start + place);
       if (kept >= 0) {
+        const int at = (int)place;
         const int have = (int)(((long long)kept + page - 1) >> p.page_shift), b = at >> p.page_shift;
         const int at_page = b < have ? p.table[r * p.table_stride + b]
                                      : __ldcg(p.free_pages + top - 1 - (s_need[r] + b - have));

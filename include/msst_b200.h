@@ -246,8 +246,8 @@ int msst_adapter_gemm(const void* x, long long rows, int K, long long ldx, const
  * Written: out_lens [requests] and *out_free_count (which may be lens and free_count
  * themselves), block_table and free_pages in place; q_starts [requests + 1], the first
  * row of each request among the call's new tokens, and for each of the `tokens` rows its
- * slot and its position start + place in the request (rows behind the last request: -1
- * and 0).  With outputs of their own a call may be repeated with the same result.
+ * slot and its position start + place in the request (2^31 - 1 where a refused request's is
+ * more; rows behind the last request: -1 and 0).  With outputs of their own a call may be repeated with the same result.
  * Lengths are taken into [0, blocks * page_size], the count into [0, pages]. */
 int msst_cache_plan(const int* new_tokens, const int* lens, int requests, int* block_table, int blocks,
                     long long table_stride, int* free_pages, int pages, const int* free_count, int page_size, int start,

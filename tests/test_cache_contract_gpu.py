@@ -84,3 +84,19 @@ def test_rows_without_a_request(cuda, T, Hq, d):
     left = torch.full_like(q, 3.0)
     assert ops.prefix_attention(q, pk, pv, kc, vc, table, own, q_starts=starts, out=left) is left and bool((left == 3).all())
     assert device_error(True) == 0
+
+
+@pytest.mark.parametrize("tokens", [60, 5000])  # one CTA, a cluster
+def test_positions_of_a_refused_request_end_at_the_largest(cuda, tokens):
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    start, n = 2 ** 31 - 1 - 32, tokens - 11
+    starts, slots, positions, lens, count = ops.cache_plan(ints([3, n, 2]), ints([5, 30, 0]), ints([[4, 9], [7, 2], [0, 0]]),
+                                                           ints([1, 3, 5]), ints([3]), 16, tokens, start=start)
+    assert device_error(True) == 16 and starts.tolist() == [0, 3, 3 + n, 5 + n]
+    assert lens.tolist() == [8, 30, 2] and count.tolist() == [2]
+    assert slots.tolist() == [69, 70, 71] + [-1] * n + [80, 81] + [-1] * 6
+    want = [start + 5 + i for i in range(3)] + [min(start + 30 + i, 2 ** 31 - 1) for i in range(n)] + [start, start + 1] + [0] * 6
+    assert positions.tolist() == want
