@@ -19,7 +19,10 @@ from . import _need, _torch, ops
 
 
 class Step(NamedTuple):
-    """A plan's rows: first row of each request, slot and position of each row, lengths after it."""
+    """A plan's rows: first row of each request, slot and position of each row, lengths after it.
+
+    It stays as it is while the next step is planned ahead; its layers have to be launched before the
+    next step's, and before the plan behind that (which may fill an ended request's row of the block table)."""
     q_starts: object
     slots: object
     positions: object
@@ -31,8 +34,8 @@ class TokenCache:
 
     `layers` layers share the block table and slots; `blocks` pages of page_size tokens are the most
     that a request may hold, `pages` the most of all together (None: enough for all).  A plan is
-    made once a step, for all layers, on the current stream; lengths, table and free pages are
-    updated in place, so a captured step may be replayed."""
+    made once a step, for all layers, on the current stream; the cache's lengths, table and free pages
+    are updated in place, so a captured step may be replayed."""
 
     def __init__(self, requests, blocks, kv_heads, head_dim, layers=1, page_size=64, pages=None, dtype=None, device=None):
         torch = _torch()
@@ -54,7 +57,8 @@ class TokenCache:
         ended and its pages are free), `tokens` rows in all, positions from `start` (the prefix's length)."""
         q_starts, slots, positions, lens, _ = ops.cache_plan(
             new_tokens, self.lens, self.block_table, self.free_pages, self.free_count, self.page_size, tokens, start=start,
-            out_lens=self.lens, out_free_count=self.free_count)
+            out_free_count=self.free_count)
+        self.lens.copy_(lens)  # (the step keeps its own)
         return Step(q_starts, slots, positions, lens)
 
 

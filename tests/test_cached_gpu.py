@@ -1,0 +1,40 @@
+"""GPU tests of TokenCache and CachedBlock beyond the steps of test_cache_ops_gpu.py."""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _ints(torch, x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _steps(torch, ahead):
+    """Outputs of a few steps, each planned just before its layer or one step ahead."""
+    from msst_b200 import device_error
+    from msst_b200.cached import TokenCache, random_cached_block
+
+    block = random_cached_block(dim=128, q_heads=4, kv_heads=2, head_dim=64, seed=5)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    rows = lambda n: torch.randn(n, 128, generator=g, device="cuda").bfloat16()  # noqa: E731
+    P, new = 40, [[30, 3, 17, 1], [1, 1, 1, 1], [1, 16, -1, 1], [2, 1, 0, -1], [1, 1, 1, 5]]
+    _, pk, pv = block.prefill(rows(P))
+    cache = TokenCache(4, 6, 2, 64, page_size=16)
+    plan = lambda i: cache.plan(_ints(torch, new[i]), sum(max(n, 0) for n in new[i]), start=P)  # noqa: E731
+    out, step = [], plan(0)
+    for i in range(len(new)):
+        later = plan(i + 1) if ahead and i + 1 < len(new) else None
+        x = rows(sum(max(n, 0) for n in new[i]))
+        out.append(block(x, pk, pv, cache, step, _ints(torch, [-1] * x.shape[0])))
+        if i + 1 < len(new):
+            step = later if ahead else plan(i + 1)
+    assert cache.lens.tolist() == [35, 22, 1, 5] and device_error(True) == 0
+    return out
+
+
+def test_steps_planned_ahead(cuda):
+    """A step's lengths are its own: the next one's plan does not show its rows keys that are not there yet."""
+    for a, b in zip(_steps(cuda, False), _steps(cuda, True)):
+        assert cuda.equal(a, b)
