@@ -86,7 +86,7 @@ class CachedBlock:
         return ops.adapter_gemm(x, w, *none, row_adapter.new_full(row_adapter.shape, -1))
 
     def _heads(self, x, row_adapter):
-        qkv = self._project("qkv", x, row_adapter).view(x.shape[0], -1, self.head_dim)
+        qkv = self._project("qkv", x, row_adapter).view(x.shape[0], self.q_heads + 2 * self.kv_heads, self.head_dim)
         return qkv[:, :self.q_heads], qkv[:, self.q_heads:-self.kv_heads], qkv[:, -self.kv_heads:]
 
     def _append(self, x, positions, slots, row_adapter, k_cache, v_cache):
@@ -99,13 +99,13 @@ class CachedBlock:
         torch = _torch()
         P = x.shape[0]
         page = 256
-        room = x.new_zeros(2, -(-P // page), page, self.kv_heads, self.head_dim)
+        room = x.new_zeros(2, max(1, -(-P // page)), page, self.kv_heads, self.head_dim)
         at = torch.arange(P, dtype=torch.int32, device=x.device)
         q = self._append(x, at, at, at.new_full((P,), -1), room[0], room[1])
-        pages = at[:room.shape[1]].view(1, -1)
+        pages = at[:-(-P // page)].view(1, -(-P // page))
         o = ops.prefix_attention(q, None, None, room[0], room[1], pages, at.new_full((1,), P),
                                  q_starts=torch.tensor([0, P], dtype=torch.int32, device=x.device))
-        y = x + self._project("o", o.view(P, -1), at.new_full((P,), -1))
+        y = x + self._project("o", o.flatten(1), at.new_full((P,), -1))
         return y, room[0].view(-1, self.kv_heads, self.head_dim)[:P], room[1].view(-1, self.kv_heads, self.head_dim)[:P]
 
     def __call__(self, x, prefix_k, prefix_v, cache: TokenCache, step: Step, row_adapter, layer=0, single=False):
@@ -115,7 +115,7 @@ class CachedBlock:
         q = self._append(x, step.positions, step.slots, row_adapter, k_cache, v_cache)
         o = ops.prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache.block_table, step.lens,
                                  q_starts=None if single else step.q_starts)
-        return x + self._project("o", o.view(x.shape[0], -1), row_adapter)
+        return x + self._project("o", o.flatten(1), row_adapter)
 
 
 def random_cached_block(dim=512, q_heads=8, kv_heads=2, head_dim=64, count=3, rank=16, dtype=None, seed=0, **scaling):

@@ -38,3 +38,26 @@ def test_steps_planned_ahead(cuda):
     """A step's lengths are its own: the next one's plan does not show its rows keys that are not there yet."""
     for a, b in zip(_steps(cuda, False), _steps(cuda, True)):
         assert cuda.equal(a, b)
+
+
+def test_steps_without_a_row(cuda):
+    """A prefix of no token, and a step in which no request has a new one."""
+    torch = cuda
+    from msst_b200 import device_error
+    from msst_b200.cached import TokenCache, random_cached_block
+
+    block = random_cached_block(dim=128, q_heads=4, kv_heads=2, head_dim=64, seed=5)
+    nothing = torch.empty(0, 128, dtype=torch.bfloat16, device="cuda")
+    y, pk, pv = block.prefill(nothing)
+    assert y.shape == (0, 128) and pk.shape == pv.shape == (0, 2, 64)
+    cache = TokenCache(3, 2, 2, 64, page_size=16)
+    x = torch.randn(6, 128, device="cuda").bfloat16()
+    who = _ints(torch, [0, -1, 2] * 2)
+    outs = []
+    for k, v in ((pk, pv), (None, None)):
+        step = cache.plan(_ints(torch, [2, 3, 1]), 6)
+        outs.append(block(x, k, v, cache, step, who))
+        step = cache.plan(_ints(torch, [0, 0, 0]), 0)
+        assert block(nothing, k, v, cache, step, who[:0]).shape == (0, 128) and step.lens.tolist() == [2, 3, 1]
+        cache.plan(_ints(torch, [-1, -1, -1]), 0)
+    assert torch.equal(*outs) and device_error(True) == 0
