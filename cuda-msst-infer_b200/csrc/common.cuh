@@ -158,7 +158,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // the CTA already gave up (*abort != 0).
 template <bool kSuspend = true>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned code,
-                                          volatile int* abort) {
+                                          volatile int* abort, unsigned long long limit_ns = kWaitLimitNs) {
   const uint32_t a = smem_u32(bar);
   if (mbar_try_wait<kSuspend>(a, parity)) return true;
   const unsigned long long t0 = global_timer_ns();
@@ -166,7 +166,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
     if (mbar_try_wait<kSuspend>(a, parity)) return true;
     if ((spins & 15u) == 0u) {
       if (*abort) return false;
-      if (global_timer_ns() - t0 > kWaitLimitNs) {
+      if (global_timer_ns() - t0 > limit_ns) {
         record_error(code);
         *abort = 1;
         return false;

@@ -414,6 +414,7 @@ struct ItemWalk {
 // Tile items: the segments of a CTA's run in a ring in shared memory: one lane walks the items for all roles (in
 // registers of every role the walk spilled 470 bytes, and local memory has little L1 beside the tiles).
 constexpr int kRing = 4;
+constexpr unsigned long long kUnitLimitNs = 20000;  // ten times what a unit takes
 struct SegmentRing {
   Segment at[kRing];
   uint64_t full[kRing], empty[kRing];
@@ -433,7 +434,11 @@ struct SegmentRing {
     for (int s = 0;; ++s) {
       Segment x;
       walk.next(x);
-      if (!mbar_wait<false>(&empty[s % kRing], (s / kRing & 1) ^ 1, kErrTimeoutAttnQ, abort_flag)) return;
+      // The place is free when the segment kRing before has ended: no step of a chain but all of its units
+      const Segment& before = at[s % kRing];
+      const unsigned long long more = s < kRing ? 0 : (unsigned long long)(before.j1 - before.j0) * kUnitLimitNs;
+      if (!mbar_wait<false>(&empty[s % kRing], (s / kRing & 1) ^ 1, kErrTimeoutAttnQ, abort_flag, kWaitLimitNs + more))
+        return;
       at[s % kRing] = x;
       mbar_arrive(&full[s % kRing]);
       if (x.last) return;

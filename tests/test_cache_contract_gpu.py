@@ -100,3 +100,24 @@ def test_positions_of_a_refused_request_end_at_the_largest(cuda, tokens):
     assert slots.tolist() == [69, 70, 71] + [-1] * n + [80, 81] + [-1] * 6
     want = [start + 5 + i for i in range(3)] + [min(start + 30 + i, 2 ** 31 - 1) for i in range(n)] + [start, start + 1] + [0] * 6
     assert positions.tolist() == want
+
+
+def test_a_run_that_lasts_longer_than_a_wait_may(cuda):
+    """Items of seconds (a prefix of 2^28 tokens for 37 thousand rows) with short ones behind them: nothing gives up.
+
+    All weights are 1 (q is 0) and all values too: a bf16 row's sums are whole numbers that fp32 holds, a multiple of 128
+    up to 2^28, and the requests' own tokens behind them 2^-24 of the whole."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    R, n, P = 1900, 5, 1 << 28
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("12 GB of GPU memory")
+    ones = torch.ones(P, 1, 8, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros(R * n, 4, 8, dtype=torch.bfloat16, device="cuda")
+    cache = torch.ones(R, 16, 1, 8, dtype=torch.bfloat16, device="cuda")
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    y = ops.prefix_attention(q, ones, ones, cache, cache, ints([[r] for r in range(R)]), ints([n] * R),
+                             q_starts=ints([n * r for r in range(R + 1)]))
+    assert device_error(True) == 0
+    assert float((y.double() - 1).abs().max()) <= 2.0 ** -8
