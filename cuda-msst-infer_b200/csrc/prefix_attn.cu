@@ -22,8 +22,8 @@
 //
 // What a row does not see is selected away; V rows past a request's last token are zeroed in shared memory
 // before the product.  The V rows of new tokens cannot be, as later rows see them: where one of
-// those holds an infinity or NaN (0 * NaN would reach the rows before), the item's rows are computed again, key by
-// key, by the joining launch.
+// those holds infinities or NaN (0 * NaN would reach the rows before), these values alone are zeroed, and the joining
+// launch adds them to the rows that see them (a weight is above 0, so that it does not matter to an infinity or NaN).
 //
 // Measured (one B200, both launches, in a CUDA graph) and what bounds it:
 //   64 requests, one token each, 8192 keys of prefix, up to 1024 own, 32/8 heads of 128: 47 us.  Memory: 173 MB, most of
@@ -63,7 +63,7 @@ constexpr int kMostTeams = 4, kMostEntries = 12;
 // so, 9.1 with every 8192 keys.)
 template <typename T>
 constexpr int kSumSteps = std::is_same<T, __half>::value ? 128 : 512;
-constexpr int kRecompute = -1;                     // less the worker's place
+constexpr int kLeftOut = -1;                       // less the worker's place: infinities and NaN are yet to be added
 
 template <int DP>
 struct PCfg {
@@ -100,7 +100,7 @@ struct PrefixGeom {
   float* token_slots;         // [CTA * teams][begins, ends][heads][token_rows][ld]
   float* whole;               // [phase][tokens * q_heads][ld] results of items that one worker had whole
   struct Segment* cuts;       // [CTA][teams] the item that the worker started and did not end (code 0: none)
-  int* bad;                   // [CTA][teams] whether one of the worker's rows has to be computed again
+  int* bad;                   // [CTA][teams] whether values have been left out of one of the worker's whole items
 };
 
 struct Request {
@@ -476,6 +476,15 @@ struct Magnitude {
     return (top & 0xffffu) < e && top >> 16 < e;
   }
 };
+// Those of eight values that are neither.
+template <typename T>
+__device__ __forceinline__ uint4 finite_ones(uint4 v) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  auto pair = [](uint32_t x) {
+    return ((x & 0x7fffu) < e ? x & 0xffffu : 0u) | ((x >> 16 & 0x7fffu) < e ? x & 0xffff0000u : 0u);
+  };
+  return make_uint4(pair(v.x), pair(v.y), pair(v.z), pair(v.w));
+}
 
 // ------------------------------------------------------------------------------- tile items
 // O of a row (null: none that counts) after kSumSteps<T> steps: stored, or added to what is there times beta.  A warp's
@@ -758,9 +767,19 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
                                                            (((x + lane) & 7) << 4)));
                 }
               }
-              if (__any_sync(0xffffffffu, !seen.finite<T>()) && !bad) {
+              if (__any_sync(0xffffffffu, !seen.finite<T>())) {
+                if (!bad && lane == 0) *s_bad = *s_bad | 1u << (s & 31);
                 bad = 1;
-                if (lane == 0) *s_bad = *s_bad | 1u << (s & 31);
+                for (int row = max(klo, 0) + lane; row < min(khi, 128); row += 32) {
+#pragma unroll 1
+                  for (int x = 0; x < 8 * C::kHalves; ++x) {
+                    uint4* piece = reinterpret_cast<uint4*>(tile_at + row * 128 + (x >> 3) * kHalfBytes +
+                                                            (((x + lane) & 7) << 4));
+                    *piece = finite_ones<T>(*piece);
+                  }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
               }
             }
             if (lane == 0) mbar_arrive(&v_ready[vp.slot]);
@@ -1003,7 +1022,7 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         if (valid && (!k.lone || w == 0)) {
           if (!finish) *reinterpret_cast<float4*>(po + p.head_dim) = make_float4(ref, l, bad ? 1.f : 0.f, 0.f);
           if (finish && bad) g.bad[run.place] = 1;
-          if (k.j0 == 0) g.where[plane + grow] = finish && bad ? kRecompute - run.place : k.code | at;
+          if (k.j0 == 0) g.where[plane + grow] = finish && bad ? kLeftOut - run.place : k.code | at;
         }
       }
       tc_fence_before();
@@ -1042,7 +1061,8 @@ __device__ __forceinline__ uint32_t token_piece(uint32_t tile, uint32_t box, int
 }
 
 // The V rows of a tile that not all rows see, a lane a key: zeroed from key khi on, which is not there (0 * NaN would
-// reach the sum); whether one of the others from klo on, which some see and others do not, holds an infinity or NaN.
+// reach the sum); of the others from klo on, which some see and others do not, infinities and NaN alone, and whether there
+// were any.
 // (Out of the loop's way: its instructions are fetched again and again, and masks on every fragment were a third of them.)
 template <typename T, int kHalves>
 __device__ __noinline__ bool clear_keys(uint8_t* tile, uint32_t half_bytes, int row0, int row16, int klo, int khi, int lane) {
@@ -1056,6 +1076,13 @@ __device__ __noinline__ bool clear_keys(uint8_t* tile, uint32_t half_bytes, int 
         *piece = make_uint4(0u, 0u, 0u, 0u);
       } else {
         seen.add(*piece);
+      }
+    }
+    if (!seen.finite<T>()) {
+#pragma unroll 1
+      for (int x = 0; x < 8 * kHalves; ++x) {
+        uint4* piece = reinterpret_cast<uint4*>(row + (x >> 3) * half_bytes + (((x + lane) & 7) << 4));
+        *piece = finite_ones<T>(*piece);
       }
     }
   }
@@ -1332,7 +1359,7 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& qmap, const CUtenso
           *reinterpret_cast<float4*>(po + p.head_dim) = make_float4(m[half] - kLift<T>, l[half], bad ? 1.f : 0.f, 0.f);
       }
       if (qc == 0 && finish && bad) g.bad[run.place] = 1;
-      if (qc == 0 && k.j0 == 0) g.where[grow] = finish && bad ? kRecompute - run.place : k.code | r;
+      if (qc == 0 && k.j0 == 0) g.where[grow] = finish && bad ? kLeftOut - run.place : k.code | r;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&tm->seg_empty[s & 1]);
@@ -1373,51 +1400,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------------------- joining
-// One query row by one warp, key by key, 4 columns a lane.
-template <typename T>
-__device__ void attend_row(const PrefixAttnParams& p, int r, int token, int head, int limit, int lane) {
-  const int hk = head / (p.q.heads / p.k_cache.heads);
-  const bool active = 4 * lane < p.head_dim;
-  auto load4 = [&](const T* x, float (&v)[4]) {
-    v[0] = v[1] = v[2] = v[3] = 0.f;
-    if (!active) return;
-    const uint2 w = *reinterpret_cast<const uint2*>(x + 4 * lane);
-    unpack2<T>(w.x, v[0], v[1]);
-    unpack2<T>(w.y, v[2], v[3]);
-  };
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  load4(static_cast<const T*>(p.q.data) + token * p.q.seq_stride + head * p.q.head_stride, q);
-  for (long long j = 0; j < (long long)p.prefix + limit; ++j) {
-    const HeadsView& kv = j < p.prefix ? p.prefix_k : p.k_cache;
-    const HeadsView& vv = j < p.prefix ? p.prefix_v : p.v_cache;
-    float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-    long long page = 0, at = j;
-    if (j >= p.prefix) {
-      const int i = (int)(j - p.prefix);
-      page = checked_page(p, __ldg(p.table + r * p.table_stride + (i >> p.page_shift)));
-      at = i & ((1 << p.page_shift) - 1);
-    }
-    if (page < p.pages) {
-      load4(static_cast<const T*>(kv.data) + page * kv.batch_stride + at * kv.seq_stride + hk * kv.head_stride, k);
-      load4(static_cast<const T*>(vv.data) + page * vv.batch_stride + at * vv.seq_stride + hk * vv.head_stride, v);
-    }
-    float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= p.scale_log2;
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-    const float a = fast_exp2(m - base), e = fast_exp2(s - base);
-    m = mn;
-    l = l * a + e;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) o[x] = o[x] * a + e * v[x];
-  }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  if (!active) return;
-  T* out = static_cast<T*>(p.out.data) + token * p.out.seq_stride + head * p.out.head_stride + 4 * lane;
-  *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
-}
-
 // The request of a token, or -1.
 __device__ __forceinline__ int request_of(const PrefixAttnParams& p, int token) {
   if (!p.q_starts) return token;
@@ -1428,6 +1410,36 @@ __device__ __forceinline__ int request_of(const PrefixAttnParams& p, int token) 
     len -= half;
   }
   return lo < p.requests && first_row(p, lo) <= token ? lo : -1;
+}
+
+// Adds the infinities and NaN of the V rows that a query row sees and that its item left out of the product, 4 columns
+// a lane.  Left out are those of keys that not all of the item's rows see (see `common`), of tokens no further back than a
+// pair of row tiles reaches; where others had their part in the product, they are in v already and change nothing.
+template <typename T>
+__device__ void add_left_out(const PrefixAttnParams& p, const PrefixGeom& g, int token, int head, int lane, float (&v)[4]) {
+  const int r = request_of(p, token);
+  if (r < 0) return;
+  const Request q = load_request(p, r);
+  const int limit = q.limit(token - q.q0), from = g.g_tiles == 1 ? max(limit - 2 * g.nt, 0) : min(q.limit(0), limit);
+  const T* x = static_cast<const T*>(p.v_cache.data) + (head / g.group) * p.v_cache.head_stride + 4 * lane;
+  const int* row = p.table + r * p.table_stride;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = from; i < limit; ++i) {
+    const int page = checked_page(p, __ldg(row + (i >> p.page_shift)));
+    if (4 * lane >= p.head_dim || page >= p.pages) continue;
+    const uint2 w = *reinterpret_cast<const uint2*>(x + page * p.v_cache.batch_stride +
+                                                    (i & ((1 << p.page_shift) - 1)) * p.v_cache.seq_stride);
+    float f[4];
+    unpack2<T>(w.x, f[0], f[1]);
+    unpack2<T>(w.y, f[2], f[3]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (!isfinite(f[c])) sum[c] += f[c];
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (!isfinite(sum[c])) v[c] += sum[c];
 }
 
 // What a row's parts have added up to: reference, sum and 4 columns a lane.
@@ -1488,19 +1500,31 @@ __device__ __forceinline__ void add_parts(const Parts& a, const Parts& b, int fi
   }
 }
 
+// Writes a row; again: its item has left values out.
 template <typename T>
-__device__ __forceinline__ void finish_row(const PrefixAttnParams& p, int token, int head, const Sum& sum, bool again,
-                                           int lane) {
-  if (again) {
-    const int r = request_of(p, token);
-    const Request q = load_request(p, r);
-    attend_row<T>(p, r, token, head, q.limit(token - q.q0), lane);
-  } else if (4 * lane < p.head_dim) {
-    const float inv = sum.l > 0.f ? 1.f / sum.l : (sum.l == 0.f ? 0.f : sum.l);
-    T* out = static_cast<T*>(p.out.data) + token * p.out.seq_stride + head * p.out.head_stride + 4 * lane;
-    *reinterpret_cast<uint2*>(out) =
-        make_uint2(pack2<T>(sum.o[0] * inv, sum.o[1] * inv), pack2<T>(sum.o[2] * inv, sum.o[3] * inv));
+__device__ __forceinline__ void finish_row(const PrefixAttnParams& p, const PrefixGeom& g, int token, int head, const Sum& sum,
+                                           bool again, int lane) {
+  const float inv = sum.l > 0.f ? 1.f / sum.l : (sum.l == 0.f ? 0.f : sum.l);
+  float v[4] = {sum.o[0] * inv, sum.o[1] * inv, sum.o[2] * inv, sum.o[3] * inv};
+  if (again) add_left_out<T>(p, g, token, head, lane, v);
+  if (4 * lane >= p.head_dim) return;
+  T* out = static_cast<T*>(p.out.data) + token * p.out.seq_stride + head * p.out.head_stride + 4 * lane;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+}
+
+// The same for a row that has been written without them.
+template <typename T>
+__device__ __forceinline__ void complete_row(const PrefixAttnParams& p, const PrefixGeom& g, int token, int head, int lane) {
+  T* out = static_cast<T*>(p.out.data) + token * p.out.seq_stride + head * p.out.head_stride + 4 * lane;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool active = 4 * lane < p.head_dim;
+  if (active) {
+    const uint2 w = *reinterpret_cast<const uint2*>(out);
+    unpack2<T>(w.x, v[0], v[1]);
+    unpack2<T>(w.y, v[2], v[3]);
   }
+  add_left_out<T>(p, g, token, head, lane, v);
+  if (active) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
 }
 
 // Adds up the parts of each row, in a fixed order: the prefix's and the own ones, or, of one sequence of both,
@@ -1521,13 +1545,17 @@ __global__ void __launch_bounds__(256, 2)
   const bool of_a_request = !p.q_starts || (token >= first_row(p, 0) && token < first_row(p, p.requests));
   const int code0 = g.concat ? 0 : g.where[row], code1 = g.where[rows + row];
   if (!of_a_request) {
-    if (p.zero_rest) finish_row<T>(p, token, head, Sum(), false, lane);
+    if (p.zero_rest) finish_row<T>(p, g, token, head, Sum(), false, lane);
     return;
   }
-  if (g.concat && code1 >= 0 && code1 >> 20 == 0) return;
-  bool again = code0 < 0 || code1 < 0;
+  if (code0 < 0 || code1 < 0) {
+    if (!kWide || warp == 0) complete_row<T>(p, g, token, head, lane);
+    return;
+  }
+  if (g.concat && code1 >> 20 == 0) return;
+  bool again = false;
   Sum sum;
-  if (!again) {
+  {
     const int h = head / g.group % g.heads;
     auto place = [&](int code) {  // (of a team's slot: its head's rows)
       const int at = code & 255;
@@ -1554,7 +1582,7 @@ __global__ void __launch_bounds__(256, 2)
       again |= s_again[w] != 0;
     }
   }
-  finish_row<T>(p, token, head, sum, again, lane);
+  finish_row<T>(p, g, token, head, sum, again, lane);
 }
 
 // The same for many rows of one sequence of prefix and own keys, most of which are done: block (x, y) takes rows
@@ -1616,21 +1644,25 @@ __global__ void __launch_bounds__(256, 4)
 #pragma unroll 1
     for (int u = 0; u < 2; ++u)
       if (u ? valid[1] : valid[0])
-        finish_row<T>(p, k.q0 + (u ? n[1] : n[0]), u ? head[1] : head[0], u ? sum[1] : sum[0], u ? again[1] : again[0], lane);
+        finish_row<T>(p, g, k.q0 + (u ? n[1] : n[0]), u ? head[1] : head[0], u ? sum[1] : sum[0], u ? again[1] : again[0], lane);
   }
   if (p.zero_rest && p.q_starts) {
     const int before = first_row(p, 0), behind = first_row(p, p.requests);
     const long long rest = ((long long)before + max(p.tokens - behind, 0)) * p.q.heads;
     for (long long i = (long long)blockIdx.x * gridDim.y * 8 + x; i < rest; i += (long long)gridDim.x * gridDim.y * 8) {
       const int token = (int)(i / p.q.heads);
-      finish_row<T>(p, token < before ? token : behind + token - before, (int)(i % p.q.heads), Sum(), false, lane);
+      finish_row<T>(p, g, token < before ? token : behind + token - before, (int)(i % p.q.heads), Sum(), false, lane);
     }
   }
-  if (g.bad[blockIdx.x]) {  // rows to be computed again
+  if (g.bad[blockIdx.x]) {  // whole items that have left values out
     const long long rows = (long long)p.tokens * p.q.heads;
-    for (long long row = x; row < rows; row += gridDim.y * 8)
-      if (g.where[rows + row] == kRecompute - (int)blockIdx.x && request_of(p, (int)(row / p.q.heads)) >= 0)
-        finish_row<T>(p, (int)(row / p.q.heads), (int)(row % p.q.heads), Sum(), true, lane);
+    for (long long row0 = 32LL * x; row0 < rows; row0 += 32LL * gridDim.y * 8) {
+      const bool hit = row0 + lane < rows && g.where[rows + row0 + lane] == kLeftOut - (int)blockIdx.x;
+      for (uint32_t some = __ballot_sync(0xffffffffu, hit); some; some &= some - 1) {
+        const long long row = row0 + __ffs(some) - 1;
+        complete_row<T>(p, g, (int)(row / p.q.heads), (int)(row % p.q.heads), lane);
+      }
+    }
   }
 }
 
