@@ -487,34 +487,54 @@ __device__ __forceinline__ uint4 finite_ones(uint4 v) {
 }
 
 // ------------------------------------------------------------------------------- tile items
-// O of a row (null: none that counts) after kSumSteps<T> steps: stored, or added to what is there times beta.  A warp's
-// lanes together.  (Out of the loop's way, as clear_keys below.)
-__device__ __noinline__ void put_away(uint32_t o, float* to, int d, bool first, float beta) {
-  const bool scaled = __any_sync(0xffffffffu, to && beta != 1.f);
+// Rows [lo, hi) of a V tile: infinities and NaN become zeros.  (Rare: out of the loop's way, as clear_keys below.)
+template <typename T, int kHalves>
+__device__ __noinline__ void leave_out(uint8_t* tile, int lo, int hi, int lane) {
+#pragma unroll 1
+  for (int row = lo + lane; row < hi; row += 32) {
+#pragma unroll 1
+    for (int x = 0; x < 8 * kHalves; ++x) {
+      uint4* piece = reinterpret_cast<uint4*>(tile + row * 128 + (x >> 3) * kHalfBytes + (((x + lane) & 7) << 4));
+      *piece = finite_ones<T>(*piece);
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// O of a row (mem null: none that counts) after kSumSteps<T> steps: stored in memory, or added to what is there times
+// beta; kBack: what is there times beta added to O.  A warp's lanes together.  (Out of the loop's way, as clear_keys below.)
+enum Away { kStore, kAdd, kBack };
+__device__ __noinline__ void put_away(uint32_t o, float* mem, int d, Away how, float beta) {
+  const bool scaled = __any_sync(0xffffffffu, mem && beta != 1.f);
 #pragma unroll 1
   for (int c0 = 0; c0 < d; c0 += 32) {
     uint32_t r[32];
     tmem_ld32(o + c0, r);
     tmem_ld_wait(r);
-    if (!to) continue;
 #pragma unroll
     for (int u = 0; u < 32; u += 4) {
-      if (c0 + u >= d) break;
-      float* at = to + c0 + u;
+      if (!mem || c0 + u >= d) break;
+      float* at = mem + c0 + u;
       float4 v = make_float4(__uint_as_float(r[u]), __uint_as_float(r[u + 1]), __uint_as_float(r[u + 2]),
                              __uint_as_float(r[u + 3]));
-      if (!first && !scaled) {  // (the row's thread alone adds here: in the order of its steps)
+      if (how == kAdd && !scaled) {  // (the row's thread alone adds here: in the order of its steps)
         asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                      : "memory");
         continue;
       }
-      if (!first) {
+      if (how != kStore) {
         const float4 x = __ldcg(reinterpret_cast<const float4*>(at));
         v.x += beta * x.x, v.y += beta * x.y, v.z += beta * x.z, v.w += beta * x.w;
       }
-      __stcg(reinterpret_cast<float4*>(at), v);
+      if (how != kBack) __stcg(reinterpret_cast<float4*>(at), v);
+      r[u] = __float_as_uint(v.x), r[u + 1] = __float_as_uint(v.y);
+      r[u + 2] = __float_as_uint(v.z), r[u + 3] = __float_as_uint(v.w);
     }
+    __syncwarp();
+    if (how == kBack) tmem_st32(o + c0, r);
   }
+  if (how == kBack) tmem_st_wait();
 }
 
 template <typename T, int DP>
@@ -770,16 +790,7 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
               if (__any_sync(0xffffffffu, !seen.finite<T>())) {
                 if (!bad && lane == 0) *s_bad = *s_bad | 1u << (s & 31);
                 bad = 1;
-                for (int row = max(klo, 0) + lane; row < min(khi, 128); row += 32) {
-#pragma unroll 1
-                  for (int x = 0; x < 8 * C::kHalves; ++x) {
-                    uint4* piece = reinterpret_cast<uint4*>(tile_at + row * 128 + (x >> 3) * kHalfBytes +
-                                                            (((x + lane) & 7) << 4));
-                    *piece = finite_ones<T>(*piece);
-                  }
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
+                leave_out<T, C::kHalves>(tile_at, max(klo, 0), min(khi, 128), lane);
               }
             }
             if (lane == 0) mbar_arrive(&v_ready[vp.slot]);
@@ -815,7 +826,6 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
       bool have = false;  // the reference is set
       const int all_steps = k.j1 - k.j0, steps1 = k.uses(1, k.j1 - 1) ? all_steps : all_steps - 1;
       const int steps = w ? steps1 : all_steps;
-      const bool many = all_steps > kSumSteps<T>;
       float away_ref = 0.f;  // reference of what has been put away, in the worker's slot
       float* const away = valid ? k.tile_slot(g, run) + (size_t)(w * 128 + row) * g.ld : nullptr;
       for (int t = 0; t < steps; ++t, ++mine) {
@@ -823,23 +833,14 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         const uint32_t sAddr = tmem + lane_off + b.buf * 128;
         const int tile = k.kv_tile(w, k.j0 + t);
         const int khi = tile < k.ptiles ? p.prefix - tile * 128 : limit - (tile - k.ptiles) * 128;
-        const bool all = __all_sync(0xffffffffu, khi >= 128);
+        const bool put = t > 0 && (t & (kSumSteps<T> - 1)) == 0;  // O is put away, and starts anew
+        const bool all = __all_sync(0xffffffffu, khi >= 128) && !put;
         if (!mbar_wait_warp<false>(&s_full[b.buf], b.parity, kErrTimeoutAttnS, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
         if (warp_active) {
-          if (t > 0 && (t & (kSumSteps<T> - 1)) == 0) {
-            // (as for a reference that moves, below)
-            if (!mbar_wait_warp<false>(&pv_done[w], (mine - 1) & 1, kErrTimeoutAttnO, abort_flag)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            put_away(oAddr, away, p.head_dim, t == kSumSteps<T>, away_ref == ref ? 1.f : fast_exp2(away_ref - ref));
-            away_ref = ref;
-          }
           bool done = false;
           if (all) {
             // every key is seen: one pass without a maximum, against the reference (at first that of 32 scores)
@@ -862,9 +863,9 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
             }
           }
           if (!done) {
-            // Some keys are not seen, or a sum has grown too large or is not finite: the reference moves to the row's
-            // maximum where that is above it, O and l with it, in two passes chunk by chunk.  (Rolled up, with one form for all
-            // masks: code that a short run meets once is fetched while it waits.)
+            // Some keys are not seen, or a sum has grown too large or is not finite, or O is put away: the reference moves
+            // to the row's maximum where that is above it, O and l with it, in two passes chunk by chunk.  (Rolled up, with
+            // one form for all masks: code that a short run meets once is fetched while it waits.)
             float m = -INFINITY;
 #pragma unroll 1
             for (int ch = 0; ch < 4; ++ch) {
@@ -877,7 +878,7 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
             have = true;
             const float moved = fmaxf(ref, m - kRefShift<T>), base = moved == -INFINITY ? 0.f : moved;
             const float alpha = fast_exp2(ref - base);
-            if ((t & (kSumSteps<T> - 1)) != 0 && __any_sync(0xffffffffu, moved > ref)) {
+            if (put || (t > 0 && __any_sync(0xffffffffu, moved > ref))) {
               // O holds the previous steps once the last PV is through (the one before it was
               // when this step's S was issued, so the parity is the right phase's)
               if (!mbar_wait_warp<false>(&pv_done[w], (mine - 1) & 1, kErrTimeoutAttnO, abort_flag)) {
@@ -885,14 +886,20 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
                 break;
               }
               tc_fence_after();
+              if (put) {
+                put_away(oAddr, away, p.head_dim, t == kSumSteps<T> ? kStore : kAdd,
+                         away_ref == ref ? 1.f : fast_exp2(away_ref - ref));
+                away_ref = ref;
+              } else {
 #pragma unroll 1
-              for (int h = 0; h < DP / 32; ++h) {
-                uint32_t r[32];
-                tmem_ld32(oAddr + h * 32, r);
-                tmem_ld_wait(r);
+                for (int h = 0; h < DP / 32; ++h) {
+                  uint32_t r[32];
+                  tmem_ld32(oAddr + h * 32, r);
+                  tmem_ld_wait(r);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-                tmem_st32(oAddr + h * 32, r);
+                  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                  tmem_st32(oAddr + h * 32, r);
+                }
               }
               tmem_st_wait();
             }
@@ -927,13 +934,12 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
       seq += (uint32_t)(all_steps + steps1);
       if (!mbar_wait_warp<false>(&o_done[w], s & 1, kErrTimeoutAttnO, abort_flag)) break;
       tc_fence_after();
-      if (many && warp_active)  // all of O is taken from memory then
-        put_away(oAddr, away, p.head_dim, steps <= kSumSteps<T>, away_ref == ref ? 1.f : fast_exp2(away_ref - ref));
+      if (steps > kSumSteps<T> && warp_active)
+        put_away(oAddr, away, p.head_dim, kBack, away_ref == ref ? 1.f : fast_exp2(away_ref - ref));
       // a lone tile: the two halves meet, weigh each other in and write half the columns each
       float a0 = 1.f, a1 = 0.f;
       int c_lo = 0, c_hi = p.head_dim;
       uint32_t src0 = oAddr, src1 = oAddr;
-      const float *away0 = away, *away1 = away;
       if (k.lone) {
         float* ml = s_ml;
         ml[w * 256 + row] = ref;
@@ -958,10 +964,6 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         }
         src0 = tmem + lane_off + C::kColO;
         src1 = has1 ? src0 + DP : src0;
-        if (valid) {
-          away0 = away - w * 128 * g.ld;
-          away1 = away0 + (has1 ? 128 * g.ld : 0);
-        }
         // 16-column pieces, the first half of them to w = 0
         const int mid = ((p.head_dim + 31) >> 5) * 16;
         if (w == 0)
@@ -983,22 +985,9 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
         float* po = whole ? g.whole + (plane + grow) * g.ld : k.tile_slot(g, run) + (size_t)at * g.ld;
         for (int c0 = c_lo; c0 < c_hi; c0 += 16) {
           uint32_t r0[16], r1[16];
-          if (!many) {
-            tmem_ld16(src0 + c0, r0);
-            tmem_ld16(src1 + c0, r1);
-            tmem_ld_wait(r0, r1);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
-              if (valid && c0 + i < c_hi) {
-                x = __ldcg(reinterpret_cast<const uint4*>(away0 + c0 + i));
-                y = __ldcg(reinterpret_cast<const uint4*>(away1 + c0 + i));
-              }
-              r0[i] = x.x, r0[i + 1] = x.y, r0[i + 2] = x.z, r0[i + 3] = x.w;
-              r1[i] = y.x, r1[i + 1] = y.y, r1[i + 2] = y.z, r1[i + 3] = y.w;
-            }
-          }
+          tmem_ld16(src0 + c0, r0);
+          tmem_ld16(src1 + c0, r1);
+          tmem_ld_wait(r0, r1);
           float v[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
