@@ -1741,7 +1741,8 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   g.pv_headed = p.prefix_v.head_stride != 0;
   g.kc_headed = p.k_cache.head_stride != 0;
   g.vc_headed = p.v_cache.head_stride != 0;
-  if (g.kv_heads > 1 && !(g.kc_headed && g.vc_headed && (!p.prefix || (g.pk_headed && g.pv_headed)))) {
+  const bool token_prefix = p.prefix && (g.concat || g.prefix_token);  // token items have a part of the prefix
+  if (g.kv_heads > 1 && !(g.kc_headed && g.vc_headed && (!token_prefix || (g.pk_headed && g.pv_headed)))) {
     // heads that share one have no box of several
     g.heads = 1;
     g.groups = g.kv_heads;

@@ -317,13 +317,13 @@ _ATTEND = struct.Struct("36qd10q").pack
 _NO_HEADS = (0, 0, 0, 0, 0)
 
 
-def _flat_heads(t, shape, keep):
+def _flat_heads(t, shape, keep, shared=False):
     """The five words of a [tokens, heads, head_dim] tensor; one that 16-byte loads cannot walk is
-    copied first (kept alive in `keep`)."""
+    copied first (kept alive in `keep`).  `shared`: heads may have stride 0 (an expanded one)."""
     n, h, d = shape
     s0, s1, s2 = t.stride()
     p = t.data_ptr()
-    if (s2 != 1 and d > 1) or p & 15 or ((s0 & 7 or not s0) and n > 1) or ((s1 & 7 or not s1) and h > 1):
+    if (s2 != 1 and d > 1) or p & 15 or ((s0 & 7 or not s0) and n > 1) or ((s1 & 7 or not (s1 or shared)) and h > 1):
         t = t.clone(memory_format=_torch_module.contiguous_format)
         keep.append(t)
         s0, s1, _ = t.stride()
@@ -703,7 +703,7 @@ class ops:
                 raise ValueError("q and the prefix must share one 16-bit dtype and one device")
             P = ps[0]
             if P:
-                pk, pv = _flat_heads(prefix_k, ps, keep), _flat_heads(prefix_v, ps, keep)
+                pk, pv = _flat_heads(prefix_k, ps, keep, True), _flat_heads(prefix_v, ps, keep, True)
         elif prefix_k is not prefix_v:
             raise ValueError("prefix_k and prefix_v go together")
         R = lens.shape[0] if lens.dim() == 1 else -1

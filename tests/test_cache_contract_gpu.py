@@ -121,3 +121,37 @@ def test_a_run_that_lasts_longer_than_a_wait_may(cuda):
                              q_starts=ints([n * r for r in range(R + 1)]))
     assert device_error(True) == 0
     assert float((y.double() - 1).abs().max()) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("which", ["k", "v", "kv"])
+@pytest.mark.parametrize("counts, lens, prefix", [
+    ([1] * 30, [3 + 5 * i for i in range(30)], 900),   # tile items of the prefix beside token items
+    ([1, 1], [40, 3], 1000),                           # token items of the prefix
+    ([300, 2], [310, 90], 500),                        # one sequence: tile items and token items
+], ids=["beside", "tokens", "one"])
+@pytest.mark.parametrize("d, prec", [(64, "fp16"), (128, "bf16")])
+def test_prefix_of_shared_heads(cuda, counts, lens, prefix, which, d, prec):
+    """A prefix whose heads are one expanded head, with caches that have heads of their own."""
+    torch = cuda
+    from msst_b200 import device_error, ops
+
+    q, pk, pv, kc, vc, table, own, starts = _attend_inputs(torch, counts, lens, prefix, 8, 4, d, 16, prec, 107)
+    pk, pv = (x[:, 1:2].expand(-1, 4, -1) if name in which else x for name, x in (("k", pk), ("v", pv)))
+    y = ops.prefix_attention(q, pk, pv, kc, vc, table, own, q_starts=starts)
+    assert device_error(True) == 0
+    _attend_check(torch, y, q, pk, pv, kc, vc, table, own, starts, d ** -0.5, prec)
+
+
+def test_prefix_of_shared_heads_is_not_copied(cuda):
+    torch = cuda
+    from msst_b200 import ops
+
+    q, _, _, kc, vc, table, own, starts = _attend_inputs(torch, [1] * 20, [9] * 20, 1, 16, 8, 128, 16, "bf16", 109)
+    pk, pv = (torch.zeros(100000, 1, 128, dtype=torch.bfloat16, device="cuda").expand(-1, 8, -1) for _ in range(2))
+    ops.prefix_attention(q, pk, pv, kc, vc, table, own)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.prefix_attention(q, pk, pv, kc, vc, table, own)
+    need = _workspace_bytes(20, 20, 100000, 16, 8, 128)
+    assert torch.cuda.max_memory_allocated() - before < need + (1 << 24) < pk.numel() * 2
