@@ -104,7 +104,7 @@ class CachedBlock:
         q = self._append(x, at, at, at.new_full((P,), -1), room[0], room[1])
         pages = at[:-(-P // page)].view(1, -(-P // page))
         o = ops.prefix_attention(q, None, None, room[0], room[1], pages, at.new_full((1,), P),
-                                 q_starts=torch.tensor([0, P], dtype=torch.int32, device=x.device))
+                                 q_starts=P * torch.arange(2, dtype=torch.int32, device=x.device))
         y = x + self._project("o", o.flatten(1), at.new_full((P,), -1))
         return y, room[0].view(-1, self.kv_heads, self.head_dim)[:P], room[1].view(-1, self.kv_heads, self.head_dim)[:P]
 

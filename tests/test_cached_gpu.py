@@ -61,3 +61,28 @@ def test_steps_without_a_row(cuda):
         assert block(nothing, k, v, cache, step, who[:0]).shape == (0, 128) and step.lens.tolist() == [2, 3, 1]
         cache.plan(_ints(torch, [-1, -1, -1]), 0)
     assert torch.equal(*outs) and device_error(True) == 0
+
+
+def test_prefill_in_a_graph(cuda):
+    """The prefix may be computed in a captured step: nothing in it comes from the host."""
+    torch = cuda
+    from msst_b200 import device_error
+    from msst_b200.cached import random_cached_block
+
+    block = random_cached_block(dim=128, q_heads=4, kv_heads=2, head_dim=64, seed=5)
+    x = torch.randn(300, 128, device="cuda").bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block.prefill(x)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = block.prefill(x)
+    x.copy_(torch.randn(300, 128, device="cuda").bfloat16())
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, block.prefill(x)):
+        assert torch.equal(a, b)
+    assert device_error(True) == 0
+    del graph
