@@ -17,8 +17,9 @@
 // requests' own pages so overlap, and the host knows nothing but the tensors' sizes (a captured call may be
 // replayed with other lengths).  The parts of a row are joined by a second launch in a fixed order.
 //
-// Long prompts (256 rows a request and more) take prefix and own keys as one sequence instead: the rows of one
-// request fill the tiles, and only the items that the runs cut are joined.
+// A call whose requests have 256 rows of a key head and more on average (all that the host knows) takes prefix and own keys
+// as one sequence instead: the rows of one request fill the tiles, and only the items that the runs cut are joined.
+// Each request then reads the prefix for its own rows, a single token among the prompts too.
 //
 // What a row does not see is selected away; V rows past a request's last token are zeroed in shared memory
 // before the product.  The V rows of new tokens cannot be, as later rows see them: where one of
@@ -26,13 +27,14 @@
 // launch adds them to the rows that see them (a weight is above 0, so that it does not matter to an infinity or NaN).
 //
 // Measured (one B200, both launches, in a CUDA graph) and what bounds it:
-//   64 requests, one token each, 8192 keys of prefix, up to 1024 own, 32/8 heads of 128: 47 us.  Memory: 173 MB, most of
+//   64 requests, one token each, 8192 keys of prefix, up to 1024 own, 32/8 heads of 128: 48 us.  Memory: 173 MB, most of
 //     them at 6 TB/s; 8 us before the first tiles, then CTAs of equal runs end between 29 and 41 us, as the SMs do
 //     not share the memory's rate equally (with the two kinds of CTA taking turns over the grid, 6 us more)
-//   16 tokens, 131072 keys of prefix: 104 us, 555 MB at 5.4 TB/s
-//   4096 tokens of six prompts, 4096 keys of prefix: 291 us, 1.1 PFLOP/s; tensor and XU pipe 58 % busy each (the chain
-//     scores, softmax, product behind one buffer of scores a tile, as in cross_attn.cu)
-//   32 requests of 5 tokens, 3791 keys, 12/4 heads of 80: 25 us, all of it latency: 2.5 us to find the runs, 4 to the first
+//   16 tokens, 131072 keys of prefix: 107 us, 555 MB at 5.2 TB/s
+//   4096 tokens of six prompts, 4096 keys of prefix: 332 us back to back (power-capped), 303 after a pause, 1.06 PFLOP/s;
+//     tensor and XU pipe 58 % busy each (the chain scores, softmax, product behind one buffer of scores a tile, as in
+//     cross_attn.cu)
+//   32 requests of 5 tokens, 3791 keys, 12/4 heads of 80: 25 to 28 us, all of it latency: 2.5 us to find the runs, 4 to the first
 //     tile, three or four units, 2 to the second launch and 5 in it.  Code counts here: "no instruction" is the warps' first
 //     stall, and forms that are written once and rolled up (the product's issue, the exact passes, barriers) are the faster ones
 #include <algorithm>
@@ -60,7 +62,7 @@ constexpr int kMostTeams = 4, kMostEntries = 12;
 // the sum so far, so that values of one sign lose 2^-27 of the sum with each key: 8e-4 of the result behind 131072 keys, 1.3 %
 // behind 2 million.  After 16384 keys (fp16) or 65536 (bf16), 2^-13 and 2^-11, O goes to memory, where it is added
 // in fp32, rounded to nearest.  (A prompt of 4096 tokens behind 131072 keys, bf16, 32/8 heads of 128: 8.6 ms without, 8.9
-// so, 9.1 with every 8192 keys.)
+// so, 9.1 with every 8192 keys.  A step that puts O away takes the exact passes, whose wait it needs.)
 template <typename T>
 constexpr int kSumSteps = std::is_same<T, __half>::value ? 128 : 512;
 constexpr int kLeftOut = -1;                       // less the worker's place: infinities and NaN are yet to be added
@@ -865,7 +867,8 @@ __device__ void tile_role(uint8_t* smem, const CUtensorMap& qmap, const CUtensor
           if (!done) {
             // Some keys are not seen, or a sum has grown too large or is not finite, or O is put away: the reference moves
             // to the row's maximum where that is above it, O and l with it, in two passes chunk by chunk.  (Rolled up, with
-            // one form for all masks: code that a short run meets once is fetched while it waits.)
+            // one form for all masks: code that a short run meets once is fetched while it waits.  P in 16 bits as in
+            // chunk_exp.)
             float m = -INFINITY;
 #pragma unroll 1
             for (int ch = 0; ch < 4; ++ch) {
@@ -1288,6 +1291,7 @@ __device__ void token_role(uint8_t* smem, const CUtensorMap& qmap, const CUtenso
           o[i][3] *= alpha[1];
         }
       }
+      // weights in the operands' 16 bits, which the product with V takes (l adds them up unrounded, in fp32)
       uint32_t pa[2][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -1754,12 +1758,14 @@ cudaError_t launch_k(const PrefixAttnParams& p, PrefixGeom g, int num_sms, cudaS
   g.q_slots = most_rows <= 8 ? 2 : 1;
   const int team_bytes = (int)C::kTiles / g.teams - g.q_slots * g.heads * g.q_rows * 128 * C::kHalves;
   g.entries = std::min(kMostEntries, team_bytes / (g.heads * (int)C::kEntry));
-  // What a unit takes of an SM in units of 10 ns: a tile unit 2 us of the chain; a token unit what its bytes take.  An
-  // item's start and end is as long as four tile units (its query rows, the first scores, the last product, the rows
-  // written).  64 single tokens behind 8192 keys, 32/8 heads of 128, take 47.6 us with these (four inputs in turn); with
-  // tile units at 170, 190 and 245 50.3, 48.5 and 48.2, with items of 3 and 5 tile units 48.6 and 47.1, with token items of
-  // 2 units 48.4; 60 requests of 8 tokens 27.4, 26.6 with 3 and 27.5 with 5; a prompt of 4096 tokens was slowest with 2
-  // and alike with 3 and 4.  Token units at 18, 26 and 30, before the last steps: 51, 53 and 55 us, 51 with 22.
+  // What a unit takes of an SM in units of 10 ns, as measured at head_dim 128 (and, token units, 64): a tile unit 2 us of the
+  // chain; a token unit what its boxes take, whole ones of 64 columns whatever head_dim fills of them.  (They share the CTAs
+  // out, and change no result but by the order of its sums; a sweep scatters by 2 %.)  An item's start and end is as long as
+  // four tile units (its query rows, the first scores, the last product, the rows written).  When they were chosen, 64 single
+  // tokens behind 8192 keys, 32/8 heads of 128, took 47.6 us (four inputs in turn); with tile units at 170, 190 and 245 50.3,
+  // 48.5 and 48.2, with items of 3 and 5 tile units 48.6 and 47.1, with token items of 2 units 48.4; 60 requests of 8 tokens
+  // 27.4, 26.6 with 3 and 27.5 with 5; a prompt of 4096 tokens was slowest with 2 and alike with 3 and 4.  Token units
+  // at 18, 26 and 30, some steps before: 51, 53 and 55 us, 51 with 22.
   g.tile_cost = 215;
   g.token_cost = g.heads * (DP == 128 ? 22 : 16);
   g.tile_item = 4;

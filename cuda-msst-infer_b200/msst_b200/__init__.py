@@ -674,8 +674,9 @@ class ops:
 
     @staticmethod
     def prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, block_table, lens, q_starts=None, scale=0.0, out=None):
-        """Attention of new tokens to a prefix that all requests share (read once for all of them) and
-        to each request's own tokens in a paged cache, causal among the new ones.
+        """Attention of new tokens to a prefix that all requests share and to each request's own tokens in a
+        paged cache, causal among the new ones.  The prefix is read once for all requests, except where these have 256
+        query rows of a key head and more on average: then each reads it for its own rows.
 
         q [T, Hq, d]; prefix_k / prefix_v [P, Hk, d] (None: no prefix); caches [pages, page_size,
         Hk, d]; one 16-bit type, Hq a multiple of Hk, d a multiple of 8 and <= 128.  block_table

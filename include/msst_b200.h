@@ -278,9 +278,12 @@ int msst_rope_append(const msst_heads* q, const msst_heads* k, const msst_heads*
  * caches.  q and out are [tokens, q.heads, head_dim], rows q_starts[r] to q_starts[r + 1]
  * (ascending, [requests + 1]; NULL: one row a request) request r's new tokens, which are
  * the last of its lens[r] own ones: the i-th of n sees the first lens[r] - n + i + 1 of them (not below 0).
+ * The prefix is read once for all requests where these have fewer than 256 rows (tokens * q.heads / heads) on
+ * average, and by each request for its own rows otherwise: a call of prompts had better not hold single tokens too.
  * q.heads is a multiple of the caches' heads, head_dim a multiple of 8 and <= 128,
  * scale 0 selects 1/sqrt(head_dim).  What a row does not see, the rest of a page
- * included, has no influence on it, whatever it holds.  A row that sees no key gives zeros; rows of no request (before
+ * included, has no influence on it, whatever it holds; an infinity or
+ * NaN in a v that it sees leaves that column infinite or NaN.  A row that sees no key gives zeros; rows of no request (before
  * the first or behind the last) are left as they were, or zeroed with zero_rest != 0.  A page outside the caches reads as zeros, and
  * msst_device_error reports 18.  lens is taken into [0, blocks * page_size].  out must
  * not overlap the inputs.  Precision, alignment and workspace as in msst_cross_attention
